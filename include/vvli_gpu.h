@@ -393,6 +393,148 @@ typedef struct vvli_gpu_linear_route {
 int vvli_gpu_test_linear_route(uint32_t M, uint32_t N, uint32_t K, uint32_t cus, uint32_t flags,
                                vvli_gpu_linear_route* out);
 
+/* ---------------------------------------------------------------------- */
+/* Ops for several requests over a paged cache (device pointers)            */
+/* ---------------------------------------------------------------------- */
+/* No counterpart in the reference, which runs one request over a cache of its
+ * own. These are for programs that keep their own loop around vvli_gpu_linear
+ * and serve several requests at once: one step assigns pages to the new rows
+ * (vvli_gpu_paged_assign), and in each layer normalises, rotates and appends
+ * them (vvli_gpu_norm_rope_append) and lets them attend
+ * (vvli_gpu_paged_attention); drafted tokens are checked at its end
+ * (vvli_gpu_verify_drafts), and the next assign gives back what was refused.
+ *
+ * Every pointer is device memory, aligned to its elements (where more is asked
+ * for, a call says so), of the current device, to which `stream` belongs
+ * (hipStream_t, NULL: the null stream). The calls are asynchronous, allocate
+ * nothing, keep nothing and may be captured. Lengths, tables and row numbers
+ * are read on the device, so a captured step serves any batch up to its sizes.
+ * Values there that fit no page, table or row are treated as each call says;
+ * none leads outside the buffers that the arguments describe. Sizes that a
+ * call does not take return VVLI_INVALID_CONFIG before any launch.
+ * Workspaces are the caller's: one belongs to one call at a time, so calls or
+ * replays that may overlap need one each. They are zeroed once, when they are
+ * allocated; a call leaves its counters zeroed. */
+
+/* Types of a paged cache. Activations are f32 as in vvli_gpu_linear; values
+ * are rounded to the cache's type once, to nearest even. */
+enum { VVLI_CACHE_F32 = 0, VVLI_CACHE_BF16 = 1, VVLI_CACHE_F16 = 2 };
+
+/* Keys and values of one layer: pages of page_size slots; slot s of k and of v
+ * holds kv_heads * head_dim values at element s * slot_stride. k and v at
+ * 16-byte addresses, a slot stride of whole 16-byte units that holds a slot
+ * (k and v may lie in one buffer), head_dim 32, 64 or 128, pages * page_size
+ * below 2^31. */
+typedef struct vvli_gpu_paged_cache {
+    void* k;
+    void* v;
+    uint32_t kind; /* VVLI_CACHE_* */
+    uint32_t kv_heads, head_dim, page_size, pages, reserved;
+    uint64_t slot_stride;
+} vvli_gpu_paged_cache;
+
+/* Which pages are whose: `table` ([requests][table_stride] page numbers, of a
+ * request's position p at p / page_size; -1 where there is none) and a stack
+ * of the free pages (`free_pages`, room for `pages` numbers, the top at
+ * free_count[0] - 1). table_stride * page_size, pages * page_size and
+ * requests * table_stride below 2^31. */
+typedef struct vvli_gpu_page_pool {
+    int32_t* free_pages;
+    int32_t* free_count;
+    int32_t* table;
+    uint32_t requests, table_stride, page_size, pages;
+} vvli_gpu_page_pool;
+
+/* Pages for one step: request r holds held[r] tokens, keeps the first keep[r]
+ * of them (all: keep = held; none: a request that has ended) and gets add[r]
+ * new ones behind those. Pages that it needs no longer go back on the stack
+ * and leave -1 in the table, missing ones are taken from its top: with L the
+ * given pages in the order of requests and positions, and behind them the
+ * stack from its top, the new pages in that order take L[0], L[1], ... (so a
+ * step that is given back leaves the pool as it was). A request whose pages L
+ * does not cover keeps what it holds and gets no rows, and so do all behind it
+ * that need pages; the same goes for one with add[r] < 0, keep[r] outside
+ * 0..held[r], more tokens than its row of the table has room for, or rows past
+ * `rows`.
+ * Outputs: len[r] = keep[r] + add[r] (or held[r], see above; may be `held`
+ * itself); row_start[0..requests]: new rows before request r (negative add
+ * counts 0, at most `rows`); start_pos[r] = keep[r], the position of its first
+ * new row (-add[r] for a request without pages, so that its rows have negative
+ * positions); for every new row its position row_pos[i] and cache slot
+ * slots[i] = table[r][p / page_size] * page_size + p % page_size (both -1
+ * without pages, the slot also where the page number is outside 0..pages - 1).
+ * row_pos and slots hold `rows` entries (0: both may be NULL); those behind the
+ * last new row stay as they are. `held` is what earlier calls returned: this
+ * one does not look for pages that two requests share. */
+int vvli_gpu_paged_assign(const vvli_gpu_page_pool* pool, const int32_t* held, const int32_t* keep, const int32_t* add,
+                          uint32_t rows, int32_t* len, int32_t* row_start, int32_t* start_pos, int32_t* row_pos,
+                          int64_t* slots, void* stream);
+
+/* RMS norm of every q and k head (weights q_norm / k_norm [head_dim] of type
+ * weight_kind, VVLI_WEIGHT_*; NULL: no norm), rotation of q and k by the angles
+ * pos[i] * inv_freq[0..head_dim/2-1] in rope_layout (VVLI_ROPE_*; angles are
+ * formed in 64 bits), and the append of k and v to the cache, in one pass. Row
+ * i of q, k and v is at i * ldq, i * ldk, i * ldv (elements; the three may lie
+ * in one stacked projection); q_out (row stride ldo; may be q itself with the
+ * same stride) receives the rotated heads * head_dim values. k and v go to slot
+ * slots[i]; a row whose slot is outside the cache is not appended, and two rows
+ * of one slot leave one of them. q, k, v and q_out at 16-byte addresses, their
+ * strides multiples of 4. */
+int vvli_gpu_norm_rope_append(const vvli_gpu_paged_cache* cache, const float* q, uint64_t ldq, const float* k,
+                              uint64_t ldk, const float* v, uint64_t ldv, uint32_t rows, uint32_t heads, float* q_out,
+                              uint64_t ldo, const float* inv_freq, const int32_t* pos, const int64_t* slots,
+                              uint32_t rope_layout, const void* q_norm, const void* k_norm, uint32_t weight_kind,
+                              float eps, void* stream);
+
+/* Attention of every request's new rows over its pages (kv_heads divides
+ * heads): request r has rows row_start[r] .. row_start[r + 1] - 1 (clamped to
+ * 0..rows) of q and out (row strides ldq, ldo; heads * head_dim values each);
+ * its row i stands at position p = start_pos[r] + i and sees the positions
+ * max(0, p - window + 1) .. p (window 0: all up to p). out = sum of
+ * softmax(scale * q . k) v over what a row sees; a row that sees nothing (a
+ * negative position) gets zeros. Positions behind the table's end, and those
+ * whose page number is outside 0..pages - 1, are not seen; keys and values that
+ * a row does not see do not reach it, whatever they are. Rows of no request
+ * stay as they are; row_start ascends (rows that it gives to several requests
+ * get one's output). Scores, sums and outputs are held in f32: an f32 q
+ * and the weights are split into terms of the cache's type so that the products
+ * keep f32 accuracy. Results do not change from run to run. q and out at
+ * 16-byte addresses, their strides multiples of 4, out not overlapping q.
+ * workspace: at least vvli_gpu_paged_attention_workspace bytes, at a 16-byte
+ * address. */
+int vvli_gpu_paged_attention(const vvli_gpu_paged_cache* cache, const int32_t* table, uint32_t table_stride,
+                             const int32_t* row_start, const int32_t* start_pos, uint32_t requests, const float* q,
+                             uint64_t ldq, float* out, uint64_t ldo, uint32_t rows, uint32_t heads, float scale,
+                             uint32_t window, void* workspace, size_t workspace_bytes, void* stream);
+/* Bytes of workspace that calls of up to these sizes need; 0 for sizes that a call refuses. */
+size_t vvli_gpu_paged_attention_workspace(uint32_t rows, uint32_t requests, uint32_t heads, uint32_t kv_heads,
+                                          uint32_t head_dim);
+
+/* Checks drafted tokens against the target's probabilities. Request r has rows
+ * row_start[r] .. row_start[r + 1] - 1 (clamped to 0..rows): the row of its
+ * last given token and one for each drafted token behind it. target row i
+ * (`vocab` probabilities, stride ldt) is what follows row i, draft row i
+ * (stride ldd) what token i + 1 was drawn from; draft NULL: the draft was
+ * certain of its tokens. Draft token x = tokens[i + 1] is accepted while
+ * u_accept[i] * draft[i][x] < target[i][x] (a token outside the vocabulary is
+ * refused). Behind the accepted[r] accepted ones one more token is drawn: at a
+ * refused draft from max(target - draft, 0) of that row (NULL: from target
+ * without x), else, or where that is zero throughout, from the target row: the
+ * lowest token whose running sum is over u_sample[r] * (sum of the row). Sums
+ * and comparisons are made in f64; values that are not finite and positive
+ * count 0. out[row_start[r] ..] receives the accepted tokens, the drawn one (-1
+ * if the whole row is 0) and -1 for the rest of the request's rows; a request
+ * without rows has accepted[r] = 0. Rows of no request stay as they are;
+ * row_start ascends (as above).
+ * target and draft may have any stride >= vocab; out is not tokens. workspace: at least
+ * vvli_gpu_verify_drafts_workspace bytes, at a 16-byte address. */
+int vvli_gpu_verify_drafts(const float* target, uint64_t ldt, const float* draft, uint64_t ldd, const int32_t* tokens,
+                           const int32_t* row_start, uint32_t requests, uint32_t rows, uint32_t vocab,
+                           const float* u_accept, const float* u_sample, int32_t* accepted, int32_t* out,
+                           void* workspace, size_t workspace_bytes, void* stream);
+/* Bytes of workspace that calls of up to these sizes need. */
+size_t vvli_gpu_verify_drafts_workspace(uint32_t requests, uint32_t vocab);
+
 #ifdef __cplusplus
 }
 #endif

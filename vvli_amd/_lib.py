@@ -102,6 +102,32 @@ class CLinearRoute(ctypes.Structure):
     ]
 
 
+class CPagedCache(ctypes.Structure):
+    _fields_ = [
+        ("k", c_void_p),
+        ("v", c_void_p),
+        ("kind", c_uint32),
+        ("kv_heads", c_uint32),
+        ("head_dim", c_uint32),
+        ("page_size", c_uint32),
+        ("pages", c_uint32),
+        ("reserved", c_uint32),
+        ("slot_stride", c_uint64),
+    ]
+
+
+class CPagePool(ctypes.Structure):
+    _fields_ = [
+        ("free_pages", c_void_p),
+        ("free_count", c_void_p),
+        ("table", c_void_p),
+        ("requests", c_uint32),
+        ("table_stride", c_uint32),
+        ("page_size", c_uint32),
+        ("pages", c_uint32),
+    ]
+
+
 # void (*)(void* user, size_t completed, size_t total, const char* name)
 PROGRESS_FN = ctypes.CFUNCTYPE(None, c_void_p, c_size_t, c_size_t, c_char_p)
 
@@ -159,6 +185,21 @@ PROTOTYPES = {
     "vvli_gpu_linear_noalloc": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_uint32, c_uint32, c_uint32,
                                         c_void_p]),
     "vvli_gpu_test_linear_route": (c_int, [c_uint32, c_uint32, c_uint32, c_uint32, c_uint32, POINTER(CLinearRoute)]),
+    "vvli_gpu_paged_assign": (
+        c_int, [POINTER(CPagePool), c_void_p, c_void_p, c_void_p, c_uint32, c_void_p, c_void_p, c_void_p, c_void_p,
+                c_void_p, c_void_p]),
+    "vvli_gpu_norm_rope_append": (
+        c_int, [POINTER(CPagedCache), c_void_p, c_uint64, c_void_p, c_uint64, c_void_p, c_uint64, c_uint32, c_uint32,
+                c_void_p, c_uint64, c_void_p, c_void_p, c_void_p, c_uint32, c_void_p, c_void_p, c_uint32, c_float,
+                c_void_p]),
+    "vvli_gpu_paged_attention": (
+        c_int, [POINTER(CPagedCache), c_void_p, c_uint32, c_void_p, c_void_p, c_uint32, c_void_p, c_uint64, c_void_p,
+                c_uint64, c_uint32, c_uint32, c_float, c_uint32, c_void_p, c_size_t, c_void_p]),
+    "vvli_gpu_paged_attention_workspace": (c_size_t, [c_uint32, c_uint32, c_uint32, c_uint32, c_uint32]),
+    "vvli_gpu_verify_drafts": (
+        c_int, [c_void_p, c_uint64, c_void_p, c_uint64, c_void_p, c_void_p, c_uint32, c_uint32, c_uint32, c_void_p,
+                c_void_p, c_void_p, c_void_p, c_void_p, c_size_t, c_void_p]),
+    "vvli_gpu_verify_drafts_workspace": (c_size_t, [c_uint32, c_uint32]),
     "vvli_host_fill_deterministic": (None, [c_void_p, c_size_t, c_uint32]),
     "vvli_host_fill_synthetic": (c_int, [POINTER(CConfig), c_uint64, c_float, c_void_p, c_size_t, c_uint32]),
     "vvli_host_synthetic_normal": (c_double, [c_uint64, c_uint64, c_uint64]),

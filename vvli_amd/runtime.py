@@ -429,3 +429,71 @@ def linear_noalloc(dW: int, dX: int, dY: int, M: int, N: int, K: int, dBias: int
     array (no allocation; at most VVLI_LINEAR_NOALLOC_SCRATCH_BYTES of split planes)."""
     _lib.check(_lib.lib().vvli_gpu_linear_noalloc(c_void_p(dW), c_void_p(dX), None if dBias is None else c_void_p(dBias),
                                                   c_void_p(dY), M, N, K, None if stream is None else c_void_p(stream)))
+
+
+# ---- ops for several requests over a paged cache (raw device pointers) ----
+CACHE_KINDS = {"f32": 0, "bf16": 1, "f16": 2}
+
+
+class PagedCache:
+    """vvli_gpu_paged_cache: one layer's keys and values in pages (raw device
+    pointers, which the caller keeps alive); ``kind`` is "f32", "bf16" or
+    "f16", ``slot_stride`` (elements) is kv_heads * head_dim unless given."""
+
+    def __init__(self, k: int, v: int, kind: str, kv_heads: int, head_dim: int, page_size: int, pages: int,
+                 slot_stride: int | None = None):
+        self._c = _lib.CPagedCache(k, v, CACHE_KINDS[kind], kv_heads, head_dim, page_size, pages, 0,
+                                   kv_heads * head_dim if slot_stride is None else slot_stride)
+        self._p = byref(self._c)
+
+
+class PagePool:
+    """vvli_gpu_page_pool: the page table of ``requests`` requests and the stack of free pages (raw device pointers)."""
+
+    def __init__(self, free_pages: int, free_count: int, table: int, requests: int, table_stride: int, page_size: int,
+                 pages: int):
+        self._c = _lib.CPagePool(free_pages, free_count, table, requests, table_stride, page_size, pages)
+        self._p = byref(self._c)
+
+
+def paged_assign(pool: PagePool, held: int, keep: int, add: int, rows: int, length: int, row_start: int, start_pos: int,
+                 row_pos: int | None, slots: int | None, stream: int | None = None) -> None:
+    """vvli_gpu_paged_assign: pages, positions and cache slots of one step's new rows."""
+    _lib.check(_lib.lib().vvli_gpu_paged_assign(pool._p, held, keep, add, rows, length, row_start, start_pos, row_pos, slots,
+                                                stream))
+
+
+def norm_rope_append(cache: PagedCache, q: int, ldq: int, k: int, ldk: int, v: int, ldv: int, rows: int, heads: int,
+                     q_out: int, ldo: int, inv_freq: int, pos: int, slots: int, rope_layout: str = "interleaved",
+                     q_norm: int | None = None, k_norm: int | None = None, eps: float = 1e-6, stream: int | None = None,
+                     weight_kind: int = WEIGHT_BF16) -> None:
+    """vvli_gpu_norm_rope_append: head norms, rotation and the append to the paged cache in one pass."""
+    _lib.check(_lib.lib().vvli_gpu_norm_rope_append(cache._p, q, ldq, k, ldk, v, ldv, rows, heads, q_out, ldo, inv_freq, pos,
+                                                    slots, {"interleaved": 0, "split_half": 1}[rope_layout], q_norm,
+                                                    k_norm, weight_kind, eps, stream))
+
+
+def paged_attention_workspace(rows: int, requests: int, heads: int, kv_heads: int, head_dim: int) -> int:
+    """Bytes of workspace (zeroed once) of ``paged_attention`` calls of up to these sizes."""
+    return _lib.lib().vvli_gpu_paged_attention_workspace(rows, requests, heads, kv_heads, head_dim)
+
+
+def paged_attention(cache: PagedCache, table: int, table_stride: int, row_start: int, start_pos: int, requests: int, q: int,
+                    ldq: int, out: int, ldo: int, rows: int, heads: int, scale: float, window: int, workspace: int,
+                    workspace_bytes: int, stream: int | None = None) -> None:
+    """vvli_gpu_paged_attention: every request's new rows over its pages."""
+    _lib.check(_lib.lib().vvli_gpu_paged_attention(cache._p, table, table_stride, row_start, start_pos, requests, q, ldq, out,
+                                                   ldo, rows, heads, scale, window, workspace, workspace_bytes, stream))
+
+
+def verify_drafts_workspace(requests: int, vocab: int) -> int:
+    """Bytes of workspace (zeroed once) of ``verify_drafts`` calls of up to these sizes."""
+    return _lib.lib().vvli_gpu_verify_drafts_workspace(requests, vocab)
+
+
+def verify_drafts(target: int, ldt: int, draft: int | None, ldd: int, tokens: int, row_start: int, requests: int, rows: int,
+                  vocab: int, u_accept: int, u_sample: int, accepted: int, out: int, workspace: int, workspace_bytes: int,
+                  stream: int | None = None) -> None:
+    """vvli_gpu_verify_drafts: drafted tokens against the target's probabilities."""
+    _lib.check(_lib.lib().vvli_gpu_verify_drafts(target, ldt, draft, ldd, tokens, row_start, requests, rows, vocab, u_accept,
+                                                 u_sample, accepted, out, workspace, workspace_bytes, stream))

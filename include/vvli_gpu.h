@@ -494,7 +494,9 @@ int vvli_gpu_norm_rope_append(const vvli_gpu_paged_cache* cache, const float* q,
  * softmax(scale * q . k) v over what a row sees; a row that sees nothing (a
  * negative position) gets zeros. Positions behind the table's end, and those
  * whose page number is outside 0..pages - 1, are not seen; keys and values that
- * a row does not see do not reach it, whatever they are. Rows of no request
+ * a row does not see do not reach it, whatever they are (of those that it sees,
+ * a value that is not finite reaches its dimension, and a key that is not finite
+ * makes NaN of the row in a 16-bit cache). Rows of no request
  * stay as they are; row_start ascends (rows that it gives to several requests
  * get one's output). Scores, sums and outputs are held in f32: an f32 q
  * and the weights are split into terms of the cache's type so that the products

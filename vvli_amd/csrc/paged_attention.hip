@@ -1,6 +1,24 @@
 // paged_attention.hip -- attention of the new rows of several requests over
 // their pages (vvli_gpu_paged_attention).
+//
+// For a row at position p, with j over the positions that it sees,
+//   o = sum_j e^(s_j) v_j / sum_j e^(s_j),   s_j = scale q . k_j,
+// in one pass over the keys: a running maximum m, the sum l of 2^(s_j - m)
+// (scores in base 2 for v_exp_f32) and the output so far, both rescaled where
+// m grows; parts over different keys join by the same rescaling.
+//
+// A vector is one (row, query head); the G vectors of a row that share a kv
+// head, and the rows behind one another, stand together so that a key is read
+// once for all of them. An item is up to M such vectors of one request and kv
+// head. Its keys are counted in units of UK positions from position 0, and the
+// units of all items, in the order (request, kv head, vectors, keys), are cut
+// into equal runs, one for each block: no batch, whatever its lengths, leaves
+// blocks with more to do than others. An item that a run's end cuts leaves its
+// parts in the workspace and a second kernel joins them in order of keys, so
+// results do not depend on timing.
 #include <hip/hip_fp16.h>
+
+#include <algorithm>
 
 #include "device_common.hpp"
 #include "paged.hpp"
@@ -9,80 +27,724 @@ using namespace vvli;
 
 namespace {
 
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+
+constexpr int kThreads = 256;
+constexpr uint32_t kFewestKeys = 256;  // a run shorter than this costs more at its ends than it saves
+
+// What a block leaves for the joining kernel about the item that its run's end cut.
+struct Cut {
+    uint32_t parts;  // 0: none; else of this block's second slot and the first slots of the blocks behind it
+    uint32_t first_row, m0, vecs, kvh, pad[3];
+};
+
 struct PagedAttnArgs {
     const void *k, *v;
     const int32_t *table, *row_start, *start_pos;
     const float* q;
     float* out;
+    Cut* cuts;
+    float* parts;  // two slots for each block: [M][HD] outputs, then [M] maxima and [M] sums
     uint64_t slot_stride, ldq, ldo;
-    uint32_t stride, requests, rows, heads, kv_heads, window, pages;
-    PageDiv ps;
+    uint32_t stride, requests, rows, kv_heads, window, pages, room;
+    PageDiv ps, group;
     float scale;
 };
 
-// One block per (row, head): each of its four waves takes every fourth key
-// with a running maximum and sum, and wave 0 joins them.
-template <int HD, typename T>
-__global__ __launch_bounds__(256) void paged_attn_kernel(PagedAttnArgs a) {
-    constexpr int E = (HD + 63) / 64;
-    __shared__ float part[4][HD + 2];
-    const uint32_t row = blockIdx.x, h = blockIdx.y, kvh = h / (a.heads / a.kv_heads);
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    uint32_t lo = 0, hi = a.requests;  // the request whose rows hold `row`
-    while (lo < hi) {
-        const uint32_t mid = (lo + hi) / 2;
-        if (a.row_start[mid + 1] > static_cast<int64_t>(row)) hi = mid;
-        else lo = mid + 1;
+// ---------------------------------------------------------------------------
+// Items and runs
+// ---------------------------------------------------------------------------
+struct Request {
+    uint32_t first, vecs;  // first row, vectors of one kv head
+    int64_t start;
+};
+
+__device__ __forceinline__ Request request_at(const PagedAttnArgs& a, uint32_t r) {
+    const RowSpan s = row_span(a.row_start[r], a.row_start[r + 1], a.rows);
+    return Request{s.first, s.count * a.group.d, a.start_pos[r]};
+}
+
+// The keys lo .. hi - 1 that some vector of m0 .. m0 + M - 1 sees (hi = 0:
+// none), and the units that they touch; an item without keys counts one, in
+// which its zeros are written.
+struct Units {
+    uint32_t lo, hi, first, count;
+};
+template <int M, int UK>
+__device__ __forceinline__ Units units_of(const PagedAttnArgs& a, const Request& q, uint32_t m0) {
+    const int64_t p0 = q.start + page_of(a.group, m0);
+    const int64_t p1 = q.start + page_of(a.group, min(m0 + M, q.vecs) - 1);
+    const int64_t hi = min(p1 + 1, static_cast<int64_t>(a.room));
+    const int64_t lo = a.window && p0 + 1 > a.window ? p0 + 1 - a.window : 0;
+    if (hi <= lo) return Units{0, 0, 0, 1};
+    Units u{static_cast<uint32_t>(lo), static_cast<uint32_t>(hi), static_cast<uint32_t>(lo) / UK, 0};
+    u.count = (u.hi + UK - 1) / UK - u.first;
+    return u;
+}
+
+__device__ __forceinline__ uint64_t wave_scan(uint64_t v) {
+    const int lane = threadIdx.x & 63;
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+        const uint64_t u = __shfl_up(v, o, 64);
+        if (lane >= o) v += u;
     }
-    if (lo == a.requests) return;
-    const RowSpan span = row_span(a.row_start[lo], a.row_start[lo + 1], a.rows);
-    if (row < span.first || row >= span.first + span.count) return;
-    const int32_t* table = a.table + static_cast<size_t>(lo) * a.stride;
-    const KeySpan keys = key_span(static_cast<int64_t>(a.start_pos[lo]) + (row - span.first), a.window, a.stride * a.ps.d);
-    const bool on = lane < HD;
-    float q[E], o[E], m = -INFINITY, l = 0;
-    for (int e = 0; e < E; ++e) q[e] = on ? a.q[row * a.ldq + static_cast<size_t>(h) * HD + lane + 64 * e] * a.scale : 0.f, o[e] = 0;
-    for (uint32_t j = keys.lo + wave; j < keys.hi; j += 4) {
-        const int32_t slot = page_slot(table, a.stride, a.pages, a.ps, j);
-        if (slot < 0) continue;
-        const uint64_t at = static_cast<uint64_t>(slot) * a.slot_stride + static_cast<size_t>(kvh) * HD + lane;
-        float s = 0;
-        for (int e = 0; e < E; ++e) s += on ? q[e] * static_cast<float>(static_cast<const T*>(a.k)[at + 64 * e]) : 0.f;
-        s = wave_sum(s);
-        const float m_new = fmaxf(m, s), base = m_new == -INFINITY ? 0.f : m_new;
-        const float c = expf(m - base), p = expf(s - base);
-        l = l * c + p;
-        for (int e = 0; e < E; ++e) o[e] = o[e] * c + (on ? p * static_cast<float>(static_cast<const T*>(a.v)[at + 64 * e]) : 0.f);
-        m = m_new;
+    return v;
+}
+
+// Units of one kv head of each lane's request, summed over its items: by the
+// lane itself where they are few, else by its wave.
+template <int M, int UK>
+__device__ __forceinline__ uint64_t request_units(const PagedAttnArgs& a, const Request& q) {
+    const uint32_t lane = threadIdx.x & 63, items = (q.vecs + M - 1) / M;
+    uint64_t sum = 0;
+    if (items <= 2)
+        for (uint32_t i = 0; i < items; ++i) sum += units_of<M, UK>(a, q, i * M).count;
+    for (uint64_t todo = __ballot(items > 2); todo; todo &= todo - 1) {
+        const int from = __builtin_ctzll(todo);
+        const Request f{static_cast<uint32_t>(__shfl(q.first, from, 64)), static_cast<uint32_t>(__shfl(q.vecs, from, 64)), __shfl(q.start, from, 64)};
+        uint64_t s = 0;
+        for (uint32_t i = lane; i < (f.vecs + M - 1) / M; i += 64) s += units_of<M, UK>(a, f, i * M).count;
+#pragma unroll
+        for (int o = 32; o; o >>= 1) s += __shfl_xor(s, o, 64);
+        if (static_cast<int>(lane) == from) sum = s;
     }
-    for (int e = 0; e < E; ++e)
-        if (on) part[wave][lane + 64 * e] = o[e];
-    if (lane == 0) part[wave][HD] = m, part[wave][HD + 1] = l;
+    return sum;
+}
+
+// Where a block's run starts: request, kv head, vector and unit of the item; units of the run.
+struct Run {
+    uint32_t r, kvh, m0, unit;
+    uint64_t left, per;
+};
+
+struct RunScratch {
+    uint64_t sums[kThreads / 64], found_rest, found_units;
+    uint32_t found_r;
+};
+
+template <int M, int UK>
+__device__ Run find_run(const PagedAttnArgs& a, uint32_t block, uint32_t blocks, RunScratch& sc) {
+    const uint32_t tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    const uint32_t chunks = (a.requests + kThreads - 1) / kThreads;
+    uint64_t mine = 0, end = 0, before = 0;
+    auto chunk = [&](uint32_t c) {  // this thread's request's units, and the sum up to it
+        const uint32_t r = c * kThreads + tid;
+        mine = request_units<M, UK>(a, r < a.requests ? request_at(a, r) : Request{0, 0, 0});
+        const uint64_t s = wave_scan(mine);
+        __syncthreads();
+        if (lane == 63) sc.sums[wave] = s;
+        __syncthreads();
+        end = before + s;
+        for (uint32_t w = 0; w < kThreads / 64; ++w) {
+            if (w < wave) end += sc.sums[w];
+            before += sc.sums[w];
+        }
+    };
+    for (uint32_t c = 0; c < chunks; ++c) chunk(c);
+    const uint64_t total = before * a.kv_heads;
+    Run run{};
+    run.per = max((total + blocks - 1) / blocks, static_cast<uint64_t>(kFewestKeys / UK));
+    const uint64_t from = run.per * block;
+    if (from >= total) return run;
+    run.left = min(run.per, total - from);
+    before = 0;
+    for (uint32_t c = 0; c < chunks; ++c) {
+        if (chunks > 1) chunk(c);
+        const uint64_t lo = (end - mine) * a.kv_heads;
+        if (mine && from >= lo && from < end * a.kv_heads) sc.found_r = c * kThreads + tid, sc.found_rest = from - lo, sc.found_units = mine;
+    }
     __syncthreads();
-    if (wave || !on) return;
-    float top = -INFINITY;
-    for (int w = 0; w < 4; ++w) top = fmaxf(top, part[w][HD]);
-    if (top == -INFINITY) top = 0;
-    float sum = 0;
-    for (int e = 0; e < E; ++e) o[e] = 0;
-    for (int w = 0; w < 4; ++w) {
-        const float c = expf(part[w][HD] - top);
-        sum += part[w][HD + 1] * c;
-        for (int e = 0; e < E; ++e) o[e] += part[w][lane + 64 * e] * c;
+    run.r = __builtin_amdgcn_readfirstlane(sc.found_r);
+    const uint64_t rest = sc.found_rest, units = sc.found_units;
+    run.kvh = __builtin_amdgcn_readfirstlane(static_cast<uint32_t>(rest / units));
+    uint64_t v = rest % units;
+    const Request q = request_at(a, run.r);
+    for (uint32_t i = 0;; i += 64) {  // every wave by itself: the item that holds unit v
+        const uint32_t m = (i + lane) * M;
+        const uint64_t s = wave_scan(m < q.vecs ? units_of<M, UK>(a, q, m).count : 0);
+        const uint64_t past = __ballot(s > v);
+        if (past || (i + 64) * M >= q.vecs) {
+            const int at = past ? __builtin_ctzll(past) : 0;
+            const uint64_t prev = __shfl(s, at ? at - 1 : 0, 64);
+            run.m0 = __builtin_amdgcn_readfirstlane((i + at) * M);
+            run.unit = __builtin_amdgcn_readfirstlane(static_cast<uint32_t>(at ? v - prev : v));
+            return run;
+        }
+        v -= __shfl(s, 63, 64);
     }
-    for (int e = 0; e < E; ++e) a.out[row * a.ldo + static_cast<size_t>(h) * HD + lane + 64 * e] = sum == 0 ? 0.f : o[e] / sum;
+}
+
+// ---------------------------------------------------------------------------
+// Cache types. 16-bit caches go through 16x16x32 products; an f32 operand is
+// split into TERMS values of the type whose sum is it: x = t0 + t1 + ..., each
+// the rounding of what is left. bf16 has 8 bits, so three terms hold 24; f16
+// has 11, so two hold 22 (the rest, 2^-22 of x at most and half of that on
+// average, is what rounding a product to f32 leaves too). f16 has few
+// exponents: q is scaled by a power of two to below 2^13 (and the scores back),
+// and p to 2^13 at most by the exponent of its own maximum, so that second
+// terms stay clear of the subnormals; 2^13 times f16's largest value times
+// the number of keys stays far below f32's end. An f32 cache goes through
+// 16x16x4 products of f32.
+// ---------------------------------------------------------------------------
+template <int KIND> struct Kind;
+template <> struct Kind<VVLI_CACHE_F32> {
+    static constexpr int TERMS = 1, BYTES = 4, U = 1;
+};
+template <> struct Kind<VVLI_CACHE_BF16> {
+    static constexpr int TERMS = 3, BYTES = 2, U = 2;
+    static constexpr float PBIAS = 0.f;
+    typedef __bf16 T;
+    typedef bf16x8 T8;
+    static __device__ __forceinline__ f32x4 mfma(T8 x, T8 y, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_bf16(x, y, c, 0, 0, 0); }
+};
+template <> struct Kind<VVLI_CACHE_F16> {
+    static constexpr int TERMS = 2, BYTES = 2, U = 2;
+    static constexpr float PBIAS = 13.f;
+    typedef _Float16 T;
+    typedef f16x8 T8;
+    static __device__ __forceinline__ f32x4 mfma(T8 x, T8 y, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_f16(x, y, c, 0, 0, 0); }
+};
+
+template <typename K>
+__device__ __forceinline__ void split(float x, int e, typename K::T8 (&t)[K::TERMS]) {
+#pragma unroll
+    for (int i = 0; i < K::TERMS; ++i) {
+        const typename K::T h = static_cast<typename K::T>(x);
+        t[i][e] = h;
+        x -= static_cast<float>(h);
+    }
+}
+
+// ---------------------------------------------------------------------------
+// Items of few vectors: 16 GI of them. The block's four waves take the keys in
+// turn, 16 U positions each, and join at the item's end. Nothing is shared
+// between waves on the way, so keys and values go from memory straight into
+// the registers that the products read, the next step's loads in flight while
+// one is computed:
+//   S^T = K Q^T  A: lane l has key l % 16, dims 32 s + 8 (l / 16) .. + 7 (16-bit)
+//                   or 16 s + 4 (l / 16) + e (f32); D: lane l has keys
+//                   4 (l / 16) + j of vector l % 16
+//   O^T += V^T P^T  B: a lane's own scores, keys 16 u + 4 (l / 16) + j as the
+//                   k index (u, j); A: row i of tile e is dim DV i + e, so that
+//                   a lane loads DV = HD / 16 adjacent dims of each of its
+//                   keys; 16-bit pairs of keys are put together by v_perm
+// ---------------------------------------------------------------------------
+template <int HD, int KIND, int GI>
+struct Few {
+    using K = Kind<KIND>;
+    static constexpr int M = 16 * GI, U = K::U, WK = 16 * U, UK = 4 * WK, DV = HD / 16;
+    static constexpr int KL = HD * K::BYTES / 64;   // 16-byte loads of a key row by a lane
+    static constexpr int VW = DV * K::BYTES / 4;    // 32-bit words of a value row in a lane
+    struct Step {
+        u32x4 k[U][KL];
+        uint32_t v[U][4][VW];
+    };
+    // What a block has of an item: [M][HD] outputs, [M] maxima, [M] sums; and
+    // what a wave leaves in LDS of it: the same with rows ROW apart, so that 16
+    // rows' 16-byte writes fall on different banks, or, on the way, one step's
+    // values and weights (values that are not finite).
+    static constexpr int kPart = M * (HD + 2), ROW = HD + 4;
+    static constexpr int kWave = std::max(M * (ROW + 2), WK * (HD * K::BYTES / 4 + M));
+};
+
+template <int W>
+__device__ __forceinline__ void load_words(uint32_t (&d)[W], const char* p) {
+    if constexpr (W == 1) d[0] = *as_global(reinterpret_cast<const uint32_t*>(p));
+    else if constexpr (W == 2) {
+        const vvli_u32x2 x = *as_global(reinterpret_cast<const vvli_u32x2*>(p));
+        d[0] = x.x, d[1] = x.y;
+    } else {
+#pragma unroll
+        for (int i = 0; i < W; i += 4) {
+            const vvli_u32x4 x = *as_global(reinterpret_cast<const vvli_u32x4*>(p + 4 * i));
+            d[i] = x.x, d[i + 1] = x.y, d[i + 2] = x.z, d[i + 3] = x.w;
+        }
+    }
+}
+
+template <int KIND>
+__device__ __forceinline__ bool word_not_finite(uint32_t w) {
+    if constexpr (KIND == VVLI_CACHE_F32) return (w & 0x7f800000u) == 0x7f800000u;
+    constexpr uint32_t e = KIND == VVLI_CACHE_BF16 ? 0x7f80u : 0x7c00u;
+    return (w & e) == e || (w & (e << 16)) == (e << 16);
+}
+template <int KIND>
+__device__ __forceinline__ uint32_t word_finite(uint32_t w) {  // values that are not finite become 0
+    if constexpr (KIND == VVLI_CACHE_F32) return (w & 0x7f800000u) == 0x7f800000u ? 0u : w;
+    constexpr uint32_t e = KIND == VVLI_CACHE_BF16 ? 0x7f80u : 0x7c00u;
+    const uint32_t lo = (w & e) == e ? 0u : w & 0xffffu, hi = (w & (e << 16)) == (e << 16) ? 0u : w & 0xffff0000u;
+    return lo | hi;
+}
+template <int KIND>
+__device__ __forceinline__ float value_at(const uint32_t* words, int i) {
+    if constexpr (KIND == VVLI_CACHE_F32) return __uint_as_float(words[i]);
+    const uint16_t h = reinterpret_cast<const uint16_t*>(words)[i];
+    if constexpr (KIND == VVLI_CACHE_BF16) return __uint_as_float(static_cast<uint32_t>(h) << 16);
+    else return static_cast<float>(__builtin_bit_cast(_Float16, h));
+}
+
+template <int HD, int KIND, int GI>
+__global__ __launch_bounds__(kThreads) void paged_few_kernel(PagedAttnArgs a) {
+    using F = Few<HD, KIND, GI>;
+    using K = Kind<KIND>;
+    constexpr int M = F::M, U = F::U, WK = F::WK, UK = F::UK, DV = F::DV, KL = F::KL, VW = F::VW;
+    constexpr bool F32 = KIND == VVLI_CACHE_F32;
+    __shared__ RunScratch sc;
+    __shared__ __attribute__((aligned(16))) float part[4][F::kWave];
+    constexpr int ROW = F::ROW;
+
+    const uint32_t blocks = gridDim.x;
+    // Neighbouring runs on one XCD (blocks go to the eight in turn): they share keys and table rows in its L2.
+    const uint32_t block = blocks % 8 == 0 ? blockIdx.x % 8 * (blocks / 8) + blockIdx.x / 8 : blockIdx.x;
+    Run run = find_run<M, UK>(a, block, blocks, sc);
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, fr = lane & 15, fq = lane >> 4;
+    uint32_t cut_parts = 0;
+    if (run.left == 0) {
+        if (tid == 0) a.cuts[block].parts = 0;
+        return;
+    }
+    const uint64_t row_bytes = a.slot_stride * K::BYTES;
+    Request req = request_at(a, run.r);
+    while (run.left) {
+        while (run.m0 >= req.vecs) {  // the next item
+            run.m0 = 0;
+            if (req.vecs == 0 || ++run.kvh == a.kv_heads) run.kvh = 0, req = request_at(a, ++run.r);
+        }
+        const Units un = units_of<M, UK>(a, req, run.m0);
+        const uint32_t t0 = run.unit, t1 = static_cast<uint32_t>(min(static_cast<uint64_t>(un.count), t0 + run.left));
+        const int32_t* table = a.table + static_cast<size_t>(run.r) * a.stride;
+        const char* kbase = static_cast<const char*>(a.k) + static_cast<size_t>(run.kvh) * HD * K::BYTES;
+        const char* vbase = static_cast<const char*>(a.v) + static_cast<size_t>(run.kvh) * HD * K::BYTES;
+
+        // The lane's vectors: their keys and q.
+        KeySpan see[GI];
+        float inv[GI];  // scores are this times the products (f16's power of two)
+        typename std::conditional<F32, f32x4, u32x4>::type qf[GI][KL][K::TERMS];
+#pragma unroll
+        for (int gi = 0; gi < GI; ++gi) {
+            const uint32_t m = run.m0 + 16 * gi + fr;
+            const bool there = m < req.vecs;
+            const uint32_t row = page_of(a.group, there ? m : 0), g = (there ? m : 0) - row * a.group.d;
+            see[gi] = there ? key_span(req.start + row, a.window, a.room) : KeySpan{0, 0};
+            const float* qp = a.q + (req.first + row) * a.ldq + (static_cast<size_t>(run.kvh) * a.group.d + g) * HD;
+            const float f = there ? a.scale * 1.44269504088896341f : 0.f;
+            inv[gi] = 1.f;
+            if constexpr (F32) {
+#pragma unroll
+                for (int s = 0; s < KL; ++s) {
+                    const float4 x = load_f32x4(qp + 16 * s + 4 * fq);
+                    qf[gi][s][0] = there ? f32x4{x.x * f, x.y * f, x.z * f, x.w * f} : f32x4{0, 0, 0, 0};
+                }
+            } else {
+                float x[KL][8];
+                float top = 0.f;
+#pragma unroll
+                for (int s = 0; s < KL; ++s) {
+                    const float4 x0 = load_f32x4(qp + 32 * s + 8 * fq), x1 = load_f32x4(qp + 32 * s + 8 * fq + 4);
+                    x[s][0] = x0.x, x[s][1] = x0.y, x[s][2] = x0.z, x[s][3] = x0.w, x[s][4] = x1.x, x[s][5] = x1.y, x[s][6] = x1.z, x[s][7] = x1.w;
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) x[s][e] = there ? x[s][e] * f : 0.f, top = fmaxf(top, fabsf(x[s][e]));
+                }
+                if constexpr (KIND == VVLI_CACHE_F16) {
+                    top = fmaxf(top, __shfl_xor(top, 16, 64));
+                    top = fmaxf(top, __shfl_xor(top, 32, 64));
+                    int ex = top > 0.f && top < INFINITY ? 13 - (ilogbf(top) + 1) : 0;
+                    ex = min(max(ex, -120), 120);
+                    const float up = ldexpf(1.f, ex);
+                    inv[gi] = ldexpf(1.f, -ex);
+#pragma unroll
+                    for (int s = 0; s < KL; ++s)
+#pragma unroll
+                        for (int e = 0; e < 8; ++e) x[s][e] *= up;
+                }
+#pragma unroll
+                for (int s = 0; s < KL; ++s) {
+                    typename K::T8 t[K::TERMS];
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) split<K>(x[s][e], e, t);
+#pragma unroll
+                    for (int i = 0; i < K::TERMS; ++i) qf[gi][s][i] = __builtin_bit_cast(u32x4, t[i]);
+                }
+            }
+        }
+        // Keys all_lo .. all_hi - 1 are seen by every vector of the item: no test needed there.
+        uint32_t all_lo, all_hi;
+        {
+            const uint32_t last = min(run.m0 + M, req.vecs) - 1;
+            const KeySpan s0 = key_span(req.start + page_of(a.group, run.m0), a.window, a.room);
+            const KeySpan s1 = key_span(req.start + page_of(a.group, last), a.window, a.room);
+            all_lo = s1.lo, all_hi = min(s0.hi, s1.hi);
+        }
+
+        f32x4 o[GI][DV];
+        float m_run[GI], l_run[GI];
+
+        // Slot of key 16 U w + lane of a unit's keys for this wave; -1 where no vector sees it.
+        auto slot_of = [&](uint32_t t) -> int32_t {
+            const uint32_t key = (un.first + t) * UK + wave * WK + (lane & (WK - 1));
+            return t < t1 && key >= un.lo && key < un.hi ? page_slot(table, a.stride, a.pages, a.ps, key) : -1;
+        };
+        auto load = [&](typename F::Step& st, int32_t slots) {
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                const int32_t s = __shfl(slots, 16 * u + fr, 64);
+                const char* p = kbase + static_cast<uint64_t>(static_cast<uint32_t>(s)) * row_bytes + 16 * fq;
+#pragma unroll
+                for (int i = 0; i < KL; ++i) {
+                    uint32_t w[4] = {0, 0, 0, 0};
+                    if (s >= 0) load_words<4>(w, p + 64 * i);
+                    st.k[u][i] = u32x4{w[0], w[1], w[2], w[3]};
+                }
+            }
+#pragma unroll
+            for (int u = 0; u < U; ++u)
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    const int32_t s = __shfl(slots, 16 * u + 4 * fq + j, 64);
+                    const char* p = vbase + static_cast<uint64_t>(static_cast<uint32_t>(s)) * row_bytes + fr * (4 * VW);
+#pragma unroll
+                    for (int i = 0; i < VW; ++i) st.v[u][j][i] = 0;
+                    if (s >= 0) load_words<VW>(st.v[u][j], p);
+                }
+        };
+        auto compute = [&](typename F::Step& st, uint32_t t, int32_t slots, bool careful) {
+            const uint32_t key0 = (un.first + t) * UK + wave * WK;
+            if (key0 >= un.hi || key0 + WK <= un.lo) return;
+            // Holes in the table and the ends of spans need the test.
+            const uint64_t none = __ballot(slots < 0);
+            const bool masked = key0 < all_lo || key0 + WK > all_hi || none;
+            f32x4 s[GI][U];
+#pragma unroll
+            for (int gi = 0; gi < GI; ++gi)
+#pragma unroll
+                for (int u = 0; u < U; ++u) s[gi][u] = f32x4{0, 0, 0, 0};
+#pragma unroll
+            for (int i = 0; i < KL; ++i)
+#pragma unroll
+                for (int u = 0; u < U; ++u)
+#pragma unroll
+                    for (int gi = 0; gi < GI; ++gi) {
+                        if constexpr (F32) {
+                            const f32x4 kf = __builtin_bit_cast(f32x4, st.k[u][i]);
+#pragma unroll
+                            for (int e = 0; e < 4; ++e) s[gi][u] = __builtin_amdgcn_mfma_f32_16x16x4f32(kf[e], qf[gi][i][0][e], s[gi][u], 0, 0, 0);
+                        } else {
+#pragma unroll
+                            for (int x = 0; x < K::TERMS; ++x)
+                                s[gi][u] = K::mfma(__builtin_bit_cast(typename K::T8, st.k[u][i]), __builtin_bit_cast(typename K::T8, qf[gi][i][x]), s[gi][u]);
+                        }
+                    }
+            if (masked) {
+#pragma unroll
+                for (int u = 0; u < U; ++u)
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        const uint32_t at = 16 * u + 4 * fq + j, key = key0 + at;
+                        const bool hole = none >> at & 1;
+#pragma unroll
+                        for (int gi = 0; gi < GI; ++gi)
+                            if (hole || key < see[gi].lo || key >= see[gi].hi) s[gi][u][j] = -INFINITY;
+                    }
+            }
+            typename std::conditional<F32, f32x4, u32x4>::type pf[GI][F32 ? U : K::TERMS];
+            float corr[GI];
+            bool grew = false;
+#pragma unroll
+            for (int gi = 0; gi < GI; ++gi) {
+                float mx = -INFINITY;
+#pragma unroll
+                for (int u = 0; u < U; ++u)
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) mx = fmaxf(mx, s[gi][u][j]);
+                mx = fmaxf(mx, __shfl_xor(mx, 16, 64));
+                mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
+                const float m_new = fmaxf(m_run[gi], mx * inv[gi]);
+                const float m_sub = m_new == -INFINITY ? 0.f : m_new;
+                grew |= m_new != m_run[gi];
+                corr[gi] = __builtin_amdgcn_exp2f(m_run[gi] - m_sub);
+                float sum = 0.f;
+                if constexpr (!F32) {
+                    typename K::T8 t8[K::TERMS];
+#pragma unroll
+                    for (int u = 0; u < U; ++u)
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) {
+                            const float p = __builtin_amdgcn_exp2f(fmaf(s[gi][u][j], inv[gi], K::PBIAS - m_sub));
+                            s[gi][u][j] = p;
+                            sum += p;
+                            split<K>(p, 4 * u + j, t8);
+                        }
+#pragma unroll
+                    for (int x = 0; x < K::TERMS; ++x) pf[gi][x] = __builtin_bit_cast(u32x4, t8[x]);
+                } else {
+#pragma unroll
+                    for (int u = 0; u < U; ++u)
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) {
+                            const float p = __builtin_amdgcn_exp2f(s[gi][u][j] - m_sub);
+                            pf[gi][u][j] = p;
+                            s[gi][u][j] = p;
+                            sum += p;
+                        }
+                }
+                l_run[gi] = l_run[gi] * corr[gi] + sum;
+                m_run[gi] = m_new;
+            }
+            if (__any(grew)) {
+#pragma unroll
+                for (int gi = 0; gi < GI; ++gi)
+#pragma unroll
+                    for (int e = 0; e < DV; ++e) o[gi][e] *= corr[gi];
+            }
+            if (careful) {
+                // Values that are not finite leave the products and are added for the vectors that see them.
+                uint32_t* odd_v = reinterpret_cast<uint32_t*>(part[wave]);  // [WK][HD * BYTES / 4]
+                float* odd_p = part[wave] + WK * (HD * K::BYTES / 4);       // [WK][M]
+#pragma unroll
+                for (int u = 0; u < U; ++u)
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        const int at = 16 * u + 4 * fq + j;
+#pragma unroll
+                        for (int i = 0; i < VW; ++i) odd_v[at * (HD * K::BYTES / 4) + fr * VW + i] = st.v[u][j][i], st.v[u][j][i] = word_finite<KIND>(st.v[u][j][i]);
+#pragma unroll
+                        for (int gi = 0; gi < GI; ++gi) odd_p[at * M + 16 * gi + fr] = s[gi][u][j];
+                    }
+                __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+                __builtin_amdgcn_wave_barrier();
+                __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+                for (int at = 0; at < WK; ++at) {
+                    if (none >> at & 1) continue;  // (no vector sees it)
+                    const uint32_t key = key0 + at;
+#pragma unroll
+                    for (int gi = 0; gi < GI; ++gi) {
+                        const bool sees = key >= see[gi].lo && key < see[gi].hi;
+                        const float p = odd_p[at * M + 16 * gi + fr];
+#pragma unroll
+                        for (int e = 0; e < DV; ++e)
+#pragma unroll
+                            for (int j = 0; j < 4; ++j) {
+                                const float x = value_at<KIND>(odd_v + at * (HD * K::BYTES / 4), DV * (4 * fq + j) + e);
+                                if (sees && !(fabsf(x) < INFINITY)) o[gi][e][j] += p * x;
+                            }
+                    }
+                }
+                __builtin_amdgcn_wave_barrier();
+            }
+#pragma unroll
+            for (int e = 0; e < DV; ++e) {
+                if constexpr (F32) {
+#pragma unroll
+                    for (int u = 0; u < U; ++u)
+#pragma unroll
+                        for (int j = 0; j < 4; ++j)
+#pragma unroll
+                            for (int gi = 0; gi < GI; ++gi)
+                                o[gi][e] = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(st.v[u][j][e]), pf[gi][u][j], o[gi][e], 0, 0, 0);
+                } else {
+                    u32x4 w;
+#pragma unroll
+                    for (int u = 0; u < U; ++u)
+#pragma unroll
+                        for (int jp = 0; jp < 2; ++jp)  // keys 2 jp and 2 jp + 1, dim e of the lane's
+                            w[2 * u + jp] = __builtin_amdgcn_perm(st.v[u][2 * jp + 1][e / 2], st.v[u][2 * jp][e / 2], e % 2 ? 0x07060302u : 0x05040100u);
+#pragma unroll
+                    for (int x = 0; x < K::TERMS; ++x)
+#pragma unroll
+                        for (int gi = 0; gi < GI; ++gi)
+                            o[gi][e] = K::mfma(__builtin_bit_cast(typename K::T8, w), __builtin_bit_cast(typename K::T8, pf[gi][x]), o[gi][e]);
+                }
+            }
+        };
+        // A value that is not finite spoils its dimension of every vector of the item, also of those that
+        // do not see its key (0 times it is NaN) and, through split terms of either sign, an infinity of
+        // those that do. That shows in the outputs, so no step looks for it: where outputs are not
+        // finite, the wave goes over its keys once more, with care.
+        for (int careful = 0; careful < 2; ++careful) {
+#pragma unroll
+            for (int gi = 0; gi < GI; ++gi) {
+                m_run[gi] = -INFINITY, l_run[gi] = 0.f;
+#pragma unroll
+                for (int e = 0; e < DV; ++e) o[gi][e] = f32x4{0, 0, 0, 0};
+            }
+            if (un.hi == 0) break;
+            typename F::Step st[2];
+            int32_t sl[2];
+            sl[0] = slot_of(t0);
+            sl[1] = slot_of(t0 + 1);
+            load(st[0], sl[0]);
+            for (uint32_t t = t0; t < t1; t += 2) {
+                load(st[1], sl[1]);
+                const int32_t n0 = slot_of(t + 2);
+                compute(st[0], t, sl[0], careful);
+                sl[0] = n0;
+                if (t + 1 >= t1) break;
+                load(st[0], sl[0]);
+                const int32_t n1 = slot_of(t + 3);
+                compute(st[1], t + 1, sl[1], careful);
+                sl[1] = n1;
+            }
+            float sum = 0.f;  // NaN if one of them is not finite
+#pragma unroll
+            for (int gi = 0; gi < GI; ++gi)
+#pragma unroll
+                for (int e = 0; e < DV; ++e)
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) sum = fmaf(o[gi][e][j], 0.f, sum);
+            if (!__any(sum != sum)) break;
+        }
+
+        // The waves' parts: outputs [M][HD], maxima, sums.
+        float* mine = part[wave];
+#pragma unroll
+        for (int gi = 0; gi < GI; ++gi) {
+            float l = l_run[gi];
+            l += __shfl_xor(l, 16, 64);
+            l += __shfl_xor(l, 32, 64);
+            if (fq == 0) mine[M * ROW + 16 * gi + fr] = m_run[gi], mine[M * ROW + M + 16 * gi + fr] = l;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                float* p = mine + (16 * gi + fr) * ROW + DV * (4 * fq + j);
+                if constexpr (DV >= 4) {
+#pragma unroll
+                    for (int e = 0; e < DV; e += 4)
+                        *reinterpret_cast<f32x4*>(p + e) = f32x4{o[gi][e][j], o[gi][e + 1][j], o[gi][e + 2][j], o[gi][e + 3][j]};
+                } else {
+                    p[0] = o[gi][0][j], p[1] = o[gi][1][j];
+                }
+            }
+        }
+        __syncthreads();
+        const bool whole = t0 == 0 && t1 == un.count;
+        float* slot = a.parts + (2 * static_cast<size_t>(block) + (t0 == 0)) * F::kPart;
+        for (int i = tid; i < M * HD / 4; i += kThreads) {
+            const int v = i / (HD / 4), d = i % (HD / 4) * 4;
+            float top = -INFINITY;
+#pragma unroll
+            for (int w = 0; w < 4; ++w) top = fmaxf(top, part[w][M * ROW + v]);
+            const float base = top == -INFINITY ? 0.f : top;
+            float l = 0.f;
+            f32x4 x = {0, 0, 0, 0};
+#pragma unroll
+            for (int w = 0; w < 4; ++w) {
+                const float c = __builtin_amdgcn_exp2f(part[w][M * ROW + v] - base);
+                l += part[w][M * ROW + M + v] * c;
+                x += *reinterpret_cast<const f32x4*>(&part[w][v * ROW + d]) * c;
+            }
+            if (whole) {
+                const uint32_t m = run.m0 + v;
+                if (m < req.vecs) {
+                    const uint32_t row = page_of(a.group, m), g = m - row * a.group.d;
+                    float* op = a.out + (req.first + row) * a.ldo + (static_cast<size_t>(run.kvh) * a.group.d + g) * HD + d;
+                    const float r = l == 0.f ? 0.f : 1.f / l;
+                    *reinterpret_cast<f32x4*>(op) = l == 0.f ? f32x4{0, 0, 0, 0} : x * r;
+                }
+            } else {
+                *reinterpret_cast<f32x4*>(slot + v * HD + d) = x;
+                if (d == 0) slot[M * HD + v] = top, slot[M * HD + M + v] = l;
+            }
+        }
+        __syncthreads();
+        run.left -= t1 - t0;
+        if (t1 < un.count) {  // the run ends inside the item
+            if (t0 == 0) {
+                cut_parts = 1 + static_cast<uint32_t>((un.count - t1 + run.per - 1) / run.per);
+                if (tid == 0) a.cuts[block] = Cut{cut_parts, req.first, run.m0, min(static_cast<uint32_t>(M), req.vecs - run.m0), run.kvh, {}};
+            }
+            break;
+        }
+        run.unit = 0;
+        run.m0 += M;
+    }
+    if (cut_parts == 0 && tid == 0) a.cuts[block].parts = 0;
+}
+
+// Joins the parts of the items that runs cut: block (b, y) takes four vectors
+// of the item that run b began and did not end. HD / 4 threads hold a vector's
+// dims, the others' groups take the parts in turn.
+template <int HD, int M>
+__global__ __launch_bounds__(kThreads) void paged_join_kernel(PagedAttnArgs a) {
+    constexpr int LANES = HD / 4, GROUPS = kThreads / LANES, V = 4, PART = M * (HD + 2);
+    __shared__ __attribute__((aligned(16))) float sum[GROUPS][V][HD + 4];
+    __shared__ float tops[V];
+    const uint32_t block = blockIdx.x, v0 = blockIdx.y * V, tid = threadIdx.x;
+    const Cut cut = a.cuts[block];
+    if (cut.parts == 0 || v0 >= cut.vecs) return;
+    const float* first = a.parts + (2 * static_cast<size_t>(block) + 1) * PART;  // then the first slots of the blocks behind
+    auto part_at = [&](uint32_t i) { return i == 0 ? first : first + (2 * static_cast<size_t>(i) - 1) * PART; };
+    const uint32_t wave = tid >> 6, lane = tid & 63;
+    {
+        float top = -INFINITY;  // wave w: vector v0 + w
+        for (uint32_t i = lane; i < cut.parts; i += 64) top = fmaxf(top, part_at(i)[M * HD + v0 + wave]);
+        top = wave_max(top);
+        if (lane == 0) tops[wave] = top == -INFINITY ? 0.f : top;
+    }
+    __syncthreads();
+    const uint32_t g = tid / LANES, d = tid % LANES * 4;
+    f32x4 x[V];
+    float l[V];
+#pragma unroll
+    for (int v = 0; v < V; ++v) x[v] = f32x4{0, 0, 0, 0}, l[v] = 0.f;
+    for (uint32_t i = g; i < cut.parts; i += GROUPS) {
+        const float* p = part_at(i);
+#pragma unroll
+        for (int v = 0; v < V; ++v) {
+            const float c = __builtin_amdgcn_exp2f(p[M * HD + v0 + v] - tops[v]);
+            l[v] += p[M * HD + M + v0 + v] * c;
+            x[v] += *reinterpret_cast<const f32x4*>(p + (v0 + v) * HD + d) * c;
+        }
+    }
+#pragma unroll
+    for (int v = 0; v < V; ++v) {
+        *reinterpret_cast<f32x4*>(&sum[g][v][d]) = x[v];
+        if (d == 0) sum[g][v][HD] = l[v];
+    }
+    __syncthreads();
+    for (uint32_t i = tid; i < V * LANES; i += kThreads) {
+        const uint32_t v = i / LANES, dd = i % LANES * 4, m = cut.m0 + v0 + v;
+        if (v0 + v >= cut.vecs) continue;
+        float lt = 0.f;
+        f32x4 xt = {0, 0, 0, 0};
+        for (int w = 0; w < GROUPS; ++w) lt += sum[w][v][HD], xt += *reinterpret_cast<const f32x4*>(&sum[w][v][dd]);
+        const uint32_t row = page_of(a.group, m), h = m - row * a.group.d;
+        float* op = a.out + (cut.first_row + row) * a.ldo + (static_cast<size_t>(cut.kvh) * a.group.d + h) * HD + dd;
+        *reinterpret_cast<f32x4*>(op) = lt == 0.f ? f32x4{0, 0, 0, 0} : xt * (1.f / lt);
+    }
+}
+
+// What a call runs: vectors of an item, blocks.
+struct Plan {
+    uint32_t m, blocks;
+};
+constexpr uint32_t kBlocksPerCu = 2;
+
+Plan plan_of(uint32_t rows, uint32_t requests, uint32_t group) {
+    const uint64_t vecs = (static_cast<uint64_t>(rows) * group + requests - 1) / requests;  // of an average request and kv head
+    return Plan{vecs <= 16 ? 16u : 32u, gemm_cus() * kBlocksPerCu};
+}
+
+size_t plan_bytes(uint32_t m, uint32_t blocks, uint32_t hd) { return blocks * (sizeof(Cut) + 2 * sizeof(float) * m * (hd + 2)); }
+
+bool sizes_ok(uint32_t rows, uint32_t requests, uint32_t heads, uint32_t kv_heads) {
+    return requests != 0 && heads != 0 && kv_heads != 0 && heads % kv_heads == 0 && heads <= 65535 &&
+           static_cast<uint64_t>(rows) * heads < kPagedMost;
+}
+
+template <int HD, int KIND>
+hipError_t launch(const PagedAttnArgs& a, const Plan& p, hipStream_t s) {
+    const dim3 grid(p.blocks), block(kThreads);
+    const hipError_t e = p.m == 16 ? vlaunch(paged_few_kernel<HD, KIND, 1>, grid, block, 0, s, a) : vlaunch(paged_few_kernel<HD, KIND, 2>, grid, block, 0, s, a);
+    if (e != hipSuccess) return e;
+    return p.m == 16 ? vlaunch(paged_join_kernel<HD, 16>, dim3(p.blocks, 4), block, 0, s, a) : vlaunch(paged_join_kernel<HD, 32>, dim3(p.blocks, 8), block, 0, s, a);
 }
 
 template <int HD>
-hipError_t launch(const PagedAttnArgs& a, uint32_t kind, hipStream_t s) {
-    const dim3 grid(a.rows, a.heads), block(256);
-    if (kind == VVLI_CACHE_F32) return vlaunch(paged_attn_kernel<HD, float>, grid, block, 0, s, a);
-    if (kind == VVLI_CACHE_BF16) return vlaunch(paged_attn_kernel<HD, __bf16>, grid, block, 0, s, a);
-    return vlaunch(paged_attn_kernel<HD, _Float16>, grid, block, 0, s, a);
-}
-
-bool sizes_ok(uint32_t rows, uint32_t requests, uint32_t heads, uint32_t kv_heads) {
-    return requests != 0 && heads != 0 && kv_heads != 0 && heads % kv_heads == 0 && heads <= 65535 && rows < kPagedMost;
+hipError_t launch(const PagedAttnArgs& a, uint32_t kind, const Plan& p, hipStream_t s) {
+    return kind == VVLI_CACHE_F32 ? launch<HD, VVLI_CACHE_F32>(a, p, s) : kind == VVLI_CACHE_BF16 ? launch<HD, VVLI_CACHE_BF16>(a, p, s) : launch<HD, VVLI_CACHE_F16>(a, p, s);
 }
 
 }  // namespace
@@ -92,7 +754,9 @@ extern "C" {
 size_t vvli_gpu_paged_attention_workspace(uint32_t rows, uint32_t requests, uint32_t heads, uint32_t kv_heads,
                                           uint32_t head_dim) {
     if (!sizes_ok(rows, requests, heads, kv_heads) || (head_dim != 32 && head_dim != 64 && head_dim != 128)) return 0;
-    return 16;
+    // (the largest form that so many rows reach, of however few requests)
+    const Plan p = plan_of(rows, 1, heads / kv_heads);
+    return plan_bytes(p.m, p.blocks, head_dim);
 }
 
 int vvli_gpu_paged_attention(const vvli_gpu_paged_cache* cache, const int32_t* table, uint32_t table_stride,
@@ -115,14 +779,20 @@ int vvli_gpu_paged_attention(const vvli_gpu_paged_cache* cache, const int32_t* t
         return set_error(VVLI_INVALID_CONFIG, "%s: workspace of %zu bytes", who, workspace_bytes);
     if (q == out) return set_error(VVLI_INVALID_CONFIG, "%s: out is q", who);
     if (rows == 0) return VVLI_OK;
-    PagedAttnArgs a{cache->k, cache->v, table,        row_start, start_pos, q,
-                    out,      cache->slot_stride,     ldq,       ldo,       table_stride,
-                    requests, rows,     heads,        cache->kv_heads, window, cache->pages,
-                    page_div(cache->page_size),       scale};
+    const uint32_t group = heads / cache->kv_heads;
+    const Plan p = plan_of(rows, requests, group);
+    PagedAttnArgs a{};
+    a.k = cache->k, a.v = cache->v, a.table = table, a.row_start = row_start, a.start_pos = start_pos, a.q = q, a.out = out;
+    a.cuts = static_cast<Cut*>(workspace);
+    a.parts = reinterpret_cast<float*>(static_cast<char*>(workspace) + p.blocks * sizeof(Cut));
+    a.slot_stride = cache->slot_stride, a.ldq = ldq, a.ldo = ldo;
+    a.stride = table_stride, a.requests = requests, a.rows = rows, a.kv_heads = cache->kv_heads, a.window = window;
+    a.pages = cache->pages, a.room = table_stride * cache->page_size, a.ps = page_div(cache->page_size), a.group = page_div(group);
+    a.scale = scale;
     const hipStream_t s = static_cast<hipStream_t>(stream);
-    PAGED_TRY(cache->head_dim == 128 ? launch<128>(a, cache->kind, s)
-              : cache->head_dim == 64 ? launch<64>(a, cache->kind, s)
-                                      : launch<32>(a, cache->kind, s));
+    PAGED_TRY(cache->head_dim == 128 ? launch<128>(a, cache->kind, p, s)
+              : cache->head_dim == 64 ? launch<64>(a, cache->kind, p, s)
+                                      : launch<32>(a, cache->kind, p, s));
     return VVLI_OK;
 }
 

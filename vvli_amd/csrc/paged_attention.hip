@@ -193,6 +193,7 @@ __device__ Run find_run(const PagedAttnArgs& a, uint32_t block, uint32_t blocks,
 template <int KIND> struct Kind;
 template <> struct Kind<VVLI_CACHE_F32> {
     static constexpr int TERMS = 1, BYTES = 4, U = 1;
+    static constexpr float PBIAS = 0.f;
 };
 template <> struct Kind<VVLI_CACHE_BF16> {
     static constexpr int TERMS = 3, BYTES = 2, U = 2;
@@ -220,11 +221,12 @@ __device__ __forceinline__ void split(float x, int e, typename K::T8 (&t)[K::TER
 }
 
 // ---------------------------------------------------------------------------
-// Items of few vectors: 16 GI of them. The block's four waves take the keys in
-// turn, 16 U positions each, and join at the item's end. Nothing is shared
-// between waves on the way, so keys and values go from memory straight into
-// the registers that the products read, the next step's loads in flight while
-// one is computed:
+// An item has M = 16 GI QW vectors: QW of the block's four waves hold 16 GI of
+// them each, and KS = 4 / QW groups of such waves take the item's keys in turn,
+// WK = 16 U positions each, and join at its end. Nothing is shared between
+// waves on the way, so keys and values go from memory (or the caches, where
+// waves read the same ones) straight into the registers that the products
+// read, the next step's keys and values in flight behind this one's:
 //   S^T = K Q^T  A: lane l has key l % 16, dims 32 s + 8 (l / 16) .. + 7 (16-bit)
 //                   or 16 s + 4 (l / 16) + e (f32); D: lane l has keys
 //                   4 (l / 16) + j of vector l % 16
@@ -232,11 +234,13 @@ __device__ __forceinline__ void split(float x, int e, typename K::T8 (&t)[K::TER
 //                   k index (u, j); A: row i of tile e is dim DV i + e, so that
 //                   a lane loads DV = HD / 16 adjacent dims of each of its
 //                   keys; 16-bit pairs of keys are put together by v_perm
+// The first term of q stays in registers, the others in LDS: two waves fit a
+// SIMD, one's products beside the other's exponentials.
 // ---------------------------------------------------------------------------
-template <int HD, int KIND, int GI>
-struct Few {
+template <int HD, int KIND, int GI, int QW>
+struct Form {
     using K = Kind<KIND>;
-    static constexpr int M = 16 * GI, U = K::U, WK = 16 * U, UK = 4 * WK, DV = HD / 16;
+    static constexpr int M = 16 * GI * QW, KS = 4 / QW, U = K::U, WK = 16 * U, UK = KS * WK, DV = HD / 16;
     static constexpr int KL = HD * K::BYTES / 64;   // 16-byte loads of a key row by a lane
     static constexpr int VW = DV * K::BYTES / 4;    // 32-bit words of a value row in a lane
     struct Step {
@@ -244,11 +248,14 @@ struct Few {
         uint32_t v[U][4][VW];
     };
     // What a block has of an item: [M][HD] outputs, [M] maxima, [M] sums; and
-    // what a wave leaves in LDS of it: the same with rows ROW apart, so that 16
-    // rows' 16-byte writes fall on different banks, or, on the way, one step's
-    // values and weights (values that are not finite).
-    static constexpr int kPart = M * (HD + 2), ROW = HD + 4;
-    static constexpr int kWave = std::max(M * (ROW + 2), WK * (HD * K::BYTES / 4 + M));
+    // what a wave leaves in LDS of it at its end, in the place of q's terms:
+    // the same with rows ROW apart, so that 16 rows' 16-byte writes fall on
+    // different banks.
+    static constexpr int kPart = M * (HD + 2), ROW = HD + 4, kWave = 16 * GI * (ROW + 2);
+    static constexpr int kQ = QW * GI * KL * (K::TERMS - 1) * 64;  // 16-byte units
+    static constexpr int kShared = std::max(4 * kWave, 4 * kQ);    // 32-bit words
+    // Four keys' values and weights of a wave (values that are not finite).
+    static constexpr int kOddV = HD * K::BYTES / 4, kOdd = 4 * (kOddV + 16 * GI);
 };
 
 template <int W>
@@ -267,12 +274,6 @@ __device__ __forceinline__ void load_words(uint32_t (&d)[W], const char* p) {
 }
 
 template <int KIND>
-__device__ __forceinline__ bool word_not_finite(uint32_t w) {
-    if constexpr (KIND == VVLI_CACHE_F32) return (w & 0x7f800000u) == 0x7f800000u;
-    constexpr uint32_t e = KIND == VVLI_CACHE_BF16 ? 0x7f80u : 0x7c00u;
-    return (w & e) == e || (w & (e << 16)) == (e << 16);
-}
-template <int KIND>
 __device__ __forceinline__ uint32_t word_finite(uint32_t w) {  // values that are not finite become 0
     if constexpr (KIND == VVLI_CACHE_F32) return (w & 0x7f800000u) == 0x7f800000u ? 0u : w;
     constexpr uint32_t e = KIND == VVLI_CACHE_BF16 ? 0x7f80u : 0x7c00u;
@@ -287,27 +288,38 @@ __device__ __forceinline__ float value_at(const uint32_t* words, int i) {
     else return static_cast<float>(__builtin_bit_cast(_Float16, h));
 }
 
-template <int HD, int KIND, int GI>
-__global__ __launch_bounds__(kThreads) void paged_few_kernel(PagedAttnArgs a) {
-    using F = Few<HD, KIND, GI>;
+// Maximum over the four lanes that hold a vector's scores (l % 16 alike).
+__device__ __forceinline__ float rows_max(float x) {
+    const auto a = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    const float y = fmaxf(__uint_as_float(a[0]), __uint_as_float(a[1]));
+    const auto b = __builtin_amdgcn_permlane32_swap(__float_as_uint(y), __float_as_uint(y), false, false);
+    return fmaxf(__uint_as_float(b[0]), __uint_as_float(b[1]));
+}
+
+template <int HD, int KIND, int GI, int QW>
+__global__ __launch_bounds__(kThreads, 2) void paged_attn_kernel(PagedAttnArgs a) {
+    using F = Form<HD, KIND, GI, QW>;
     using K = Kind<KIND>;
-    constexpr int M = F::M, U = F::U, WK = F::WK, UK = F::UK, DV = F::DV, KL = F::KL, VW = F::VW;
+    constexpr int M = F::M, KS = F::KS, U = F::U, WK = F::WK, UK = F::UK, DV = F::DV, KL = F::KL, VW = F::VW, ROW = F::ROW;
+    constexpr int WV = 16 * GI;  // vectors of a wave
     constexpr bool F32 = KIND == VVLI_CACHE_F32;
     __shared__ RunScratch sc;
-    __shared__ __attribute__((aligned(16))) float part[4][F::kWave];
-    constexpr int ROW = F::ROW;
+    __shared__ __attribute__((aligned(16))) float shared[F::kShared];
+    __shared__ uint32_t odd[4][F::kOdd];
 
     const uint32_t blocks = gridDim.x;
     // Neighbouring runs on one XCD (blocks go to the eight in turn): they share keys and table rows in its L2.
     const uint32_t block = blocks % 8 == 0 ? blockIdx.x % 8 * (blocks / 8) + blockIdx.x / 8 : blockIdx.x;
     Run run = find_run<M, UK>(a, block, blocks, sc);
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, fr = lane & 15, fq = lane >> 4;
+    const int tid = threadIdx.x, lane = tid & 63, fr = lane & 15, fq = lane >> 4;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), qw = wave % QW, ks = wave / QW;
     uint32_t cut_parts = 0;
     if (run.left == 0) {
         if (tid == 0) a.cuts[block].parts = 0;
         return;
     }
     const uint64_t row_bytes = a.slot_stride * K::BYTES;
+    u32x4* const q_mine = reinterpret_cast<u32x4*>(shared) + qw * (F::kQ / QW) + lane;  // (the key groups of one qw write the same values)
     Request req = request_at(a, run.r);
     while (run.left) {
         while (run.m0 >= req.vecs) {  // the next item
@@ -317,27 +329,28 @@ __global__ __launch_bounds__(kThreads) void paged_few_kernel(PagedAttnArgs a) {
         const Units un = units_of<M, UK>(a, req, run.m0);
         const uint32_t t0 = run.unit, t1 = static_cast<uint32_t>(min(static_cast<uint64_t>(un.count), t0 + run.left));
         const int32_t* table = a.table + static_cast<size_t>(run.r) * a.stride;
-        const char* kbase = static_cast<const char*>(a.k) + static_cast<size_t>(run.kvh) * HD * K::BYTES;
-        const char* vbase = static_cast<const char*>(a.v) + static_cast<size_t>(run.kvh) * HD * K::BYTES;
+        const char* kbase = static_cast<const char*>(a.k) + static_cast<size_t>(run.kvh) * HD * K::BYTES + 16 * fq;
+        const char* vbase = static_cast<const char*>(a.v) + static_cast<size_t>(run.kvh) * HD * K::BYTES + 4 * VW * fr;
 
         // The lane's vectors: their keys and q.
+        const uint32_t wm0 = run.m0 + qw * WV;  // the wave's first vector
         KeySpan see[GI];
         float inv[GI];  // scores are this times the products (f16's power of two)
-        typename std::conditional<F32, f32x4, u32x4>::type qf[GI][KL][K::TERMS];
+        u32x4 qf[GI][KL];
 #pragma unroll
         for (int gi = 0; gi < GI; ++gi) {
-            const uint32_t m = run.m0 + 16 * gi + fr;
+            const uint32_t m = wm0 + 16 * gi + fr;
             const bool there = m < req.vecs;
             const uint32_t row = page_of(a.group, there ? m : 0), g = (there ? m : 0) - row * a.group.d;
             see[gi] = there ? key_span(req.start + row, a.window, a.room) : KeySpan{0, 0};
             const float* qp = a.q + (req.first + row) * a.ldq + (static_cast<size_t>(run.kvh) * a.group.d + g) * HD;
-            const float f = there ? a.scale * 1.44269504088896341f : 0.f;
+            const float f = a.scale * 1.44269504088896341f;
             inv[gi] = 1.f;
             if constexpr (F32) {
 #pragma unroll
                 for (int s = 0; s < KL; ++s) {
                     const float4 x = load_f32x4(qp + 16 * s + 4 * fq);
-                    qf[gi][s][0] = there ? f32x4{x.x * f, x.y * f, x.z * f, x.w * f} : f32x4{0, 0, 0, 0};
+                    qf[gi][s] = __builtin_bit_cast(u32x4, f32x4{x.x * f, x.y * f, x.z * f, x.w * f});
                 }
             } else {
                 float x[KL][8];
@@ -347,11 +360,10 @@ __global__ __launch_bounds__(kThreads) void paged_few_kernel(PagedAttnArgs a) {
                     const float4 x0 = load_f32x4(qp + 32 * s + 8 * fq), x1 = load_f32x4(qp + 32 * s + 8 * fq + 4);
                     x[s][0] = x0.x, x[s][1] = x0.y, x[s][2] = x0.z, x[s][3] = x0.w, x[s][4] = x1.x, x[s][5] = x1.y, x[s][6] = x1.z, x[s][7] = x1.w;
 #pragma unroll
-                    for (int e = 0; e < 8; ++e) x[s][e] = there ? x[s][e] * f : 0.f, top = fmaxf(top, fabsf(x[s][e]));
+                    for (int e = 0; e < 8; ++e) x[s][e] *= f, top = fmaxf(top, fabsf(x[s][e]));
                 }
                 if constexpr (KIND == VVLI_CACHE_F16) {
-                    top = fmaxf(top, __shfl_xor(top, 16, 64));
-                    top = fmaxf(top, __shfl_xor(top, 32, 64));
+                    top = rows_max(top);
                     int ex = top > 0.f && top < INFINITY ? 13 - (ilogbf(top) + 1) : 0;
                     ex = min(max(ex, -120), 120);
                     const float up = ldexpf(1.f, ex);
@@ -366,199 +378,64 @@ __global__ __launch_bounds__(kThreads) void paged_few_kernel(PagedAttnArgs a) {
                     typename K::T8 t[K::TERMS];
 #pragma unroll
                     for (int e = 0; e < 8; ++e) split<K>(x[s][e], e, t);
+                    qf[gi][s] = __builtin_bit_cast(u32x4, t[0]);
 #pragma unroll
-                    for (int i = 0; i < K::TERMS; ++i) qf[gi][s][i] = __builtin_bit_cast(u32x4, t[i]);
+                    for (int i = 1; i < K::TERMS; ++i) q_mine[((gi * KL + s) * (K::TERMS - 1) + i - 1) * 64] = __builtin_bit_cast(u32x4, t[i]);
                 }
             }
         }
-        // Keys all_lo .. all_hi - 1 are seen by every vector of the item: no test needed there.
-        uint32_t all_lo, all_hi;
-        {
-            const uint32_t last = min(run.m0 + M, req.vecs) - 1;
-            const KeySpan s0 = key_span(req.start + page_of(a.group, run.m0), a.window, a.room);
-            const KeySpan s1 = key_span(req.start + page_of(a.group, last), a.window, a.room);
+        // Keys w_lo .. w_hi - 1 are seen by some vector of the wave, all_lo .. all_hi - 1 by
+        // every one of them (no test needed there).
+        uint32_t w_lo = 0, w_hi = 0, all_lo = 0, all_hi = 0;
+        if (wm0 < req.vecs) {
+            const int64_t p0 = req.start + page_of(a.group, wm0), p1 = req.start + page_of(a.group, min(wm0 + WV, req.vecs) - 1);
+            const KeySpan s0 = key_span(p0, a.window, a.room), s1 = key_span(p1, a.window, a.room);
+            w_lo = max(un.lo, a.window && p0 + 1 > a.window ? static_cast<uint32_t>(min(p0 + 1 - a.window, static_cast<int64_t>(a.room))) : 0);
+            w_hi = p1 < 0 ? 0 : static_cast<uint32_t>(min(p1 + 1, static_cast<int64_t>(a.room)));
             all_lo = s1.lo, all_hi = min(s0.hi, s1.hi);
         }
+        // The wave's steps: those units of the run whose WK keys from t * UK + ks * WK on meet w_lo .. w_hi - 1.
+        uint32_t ta = un.first + t0, tb = un.first + t1;
+        if (w_lo >= static_cast<uint32_t>((ks + 1) * WK)) ta = max(ta, (w_lo - (ks + 1) * WK) / UK + 1);
+        tb = w_lo < w_hi && w_hi > static_cast<uint32_t>(ks * WK) ? min(tb, (w_hi - ks * WK + UK - 1) / UK) : 0;
 
         f32x4 o[GI][DV];
         float m_run[GI], l_run[GI];
 
-        // Slot of key 16 U w + lane of a unit's keys for this wave; -1 where no vector sees it.
+        // Slot of key t * UK + ks * WK + lane (of WK lanes), -1 where no vector of the wave sees it.
         auto slot_of = [&](uint32_t t) -> int32_t {
-            const uint32_t key = (un.first + t) * UK + wave * WK + (lane & (WK - 1));
-            return t < t1 && key >= un.lo && key < un.hi ? page_slot(table, a.stride, a.pages, a.ps, key) : -1;
+            const uint32_t key = t * UK + ks * WK + (lane & (WK - 1));
+            return t < tb && key >= w_lo && key < w_hi ? page_slot(table, a.stride, a.pages, a.ps, key) : -1;
         };
-        auto load = [&](typename F::Step& st, int32_t slots) {
+        // Slots that there are none of read another key of the step, whose score is then not used: they
+        // need neither a test at every load nor memory of their own.
+        auto filled = [&](int32_t slot, uint64_t& none) -> uint32_t {
+            none = __ballot(slot < 0);
+            const int32_t other = ~none ? __builtin_amdgcn_readlane(slot, __builtin_ctzll(~none)) : 0;
+            return slot < 0 ? other : slot;
+        };
+        typename F::Step st;
+        auto load_k = [&](uint32_t slots) {
 #pragma unroll
             for (int u = 0; u < U; ++u) {
-                const int32_t s = __shfl(slots, 16 * u + fr, 64);
-                const char* p = kbase + static_cast<uint64_t>(static_cast<uint32_t>(s)) * row_bytes + 16 * fq;
+                const uint32_t s = __shfl(slots, 16 * u + fr, 64);
+                const char* p = kbase + s * row_bytes;
 #pragma unroll
                 for (int i = 0; i < KL; ++i) {
-                    uint32_t w[4] = {0, 0, 0, 0};
-                    if (s >= 0) load_words<4>(w, p + 64 * i);
+                    uint32_t w[4];
+                    load_words<4>(w, p + 64 * i);
                     st.k[u][i] = u32x4{w[0], w[1], w[2], w[3]};
                 }
             }
+        };
+        auto load_v = [&](uint32_t slots) {
 #pragma unroll
             for (int u = 0; u < U; ++u)
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {
-                    const int32_t s = __shfl(slots, 16 * u + 4 * fq + j, 64);
-                    const char* p = vbase + static_cast<uint64_t>(static_cast<uint32_t>(s)) * row_bytes + fr * (4 * VW);
-#pragma unroll
-                    for (int i = 0; i < VW; ++i) st.v[u][j][i] = 0;
-                    if (s >= 0) load_words<VW>(st.v[u][j], p);
+                    const uint32_t s = __shfl(slots, 16 * u + 4 * fq + j, 64);
+                    load_words<VW>(st.v[u][j], vbase + s * row_bytes);
                 }
-        };
-        auto compute = [&](typename F::Step& st, uint32_t t, int32_t slots, bool careful) {
-            const uint32_t key0 = (un.first + t) * UK + wave * WK;
-            if (key0 >= un.hi || key0 + WK <= un.lo) return;
-            // Holes in the table and the ends of spans need the test.
-            const uint64_t none = __ballot(slots < 0);
-            const bool masked = key0 < all_lo || key0 + WK > all_hi || none;
-            f32x4 s[GI][U];
-#pragma unroll
-            for (int gi = 0; gi < GI; ++gi)
-#pragma unroll
-                for (int u = 0; u < U; ++u) s[gi][u] = f32x4{0, 0, 0, 0};
-#pragma unroll
-            for (int i = 0; i < KL; ++i)
-#pragma unroll
-                for (int u = 0; u < U; ++u)
-#pragma unroll
-                    for (int gi = 0; gi < GI; ++gi) {
-                        if constexpr (F32) {
-                            const f32x4 kf = __builtin_bit_cast(f32x4, st.k[u][i]);
-#pragma unroll
-                            for (int e = 0; e < 4; ++e) s[gi][u] = __builtin_amdgcn_mfma_f32_16x16x4f32(kf[e], qf[gi][i][0][e], s[gi][u], 0, 0, 0);
-                        } else {
-#pragma unroll
-                            for (int x = 0; x < K::TERMS; ++x)
-                                s[gi][u] = K::mfma(__builtin_bit_cast(typename K::T8, st.k[u][i]), __builtin_bit_cast(typename K::T8, qf[gi][i][x]), s[gi][u]);
-                        }
-                    }
-            if (masked) {
-#pragma unroll
-                for (int u = 0; u < U; ++u)
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) {
-                        const uint32_t at = 16 * u + 4 * fq + j, key = key0 + at;
-                        const bool hole = none >> at & 1;
-#pragma unroll
-                        for (int gi = 0; gi < GI; ++gi)
-                            if (hole || key < see[gi].lo || key >= see[gi].hi) s[gi][u][j] = -INFINITY;
-                    }
-            }
-            typename std::conditional<F32, f32x4, u32x4>::type pf[GI][F32 ? U : K::TERMS];
-            float corr[GI];
-            bool grew = false;
-#pragma unroll
-            for (int gi = 0; gi < GI; ++gi) {
-                float mx = -INFINITY;
-#pragma unroll
-                for (int u = 0; u < U; ++u)
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) mx = fmaxf(mx, s[gi][u][j]);
-                mx = fmaxf(mx, __shfl_xor(mx, 16, 64));
-                mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
-                const float m_new = fmaxf(m_run[gi], mx * inv[gi]);
-                const float m_sub = m_new == -INFINITY ? 0.f : m_new;
-                grew |= m_new != m_run[gi];
-                corr[gi] = __builtin_amdgcn_exp2f(m_run[gi] - m_sub);
-                float sum = 0.f;
-                if constexpr (!F32) {
-                    typename K::T8 t8[K::TERMS];
-#pragma unroll
-                    for (int u = 0; u < U; ++u)
-#pragma unroll
-                        for (int j = 0; j < 4; ++j) {
-                            const float p = __builtin_amdgcn_exp2f(fmaf(s[gi][u][j], inv[gi], K::PBIAS - m_sub));
-                            s[gi][u][j] = p;
-                            sum += p;
-                            split<K>(p, 4 * u + j, t8);
-                        }
-#pragma unroll
-                    for (int x = 0; x < K::TERMS; ++x) pf[gi][x] = __builtin_bit_cast(u32x4, t8[x]);
-                } else {
-#pragma unroll
-                    for (int u = 0; u < U; ++u)
-#pragma unroll
-                        for (int j = 0; j < 4; ++j) {
-                            const float p = __builtin_amdgcn_exp2f(s[gi][u][j] - m_sub);
-                            pf[gi][u][j] = p;
-                            s[gi][u][j] = p;
-                            sum += p;
-                        }
-                }
-                l_run[gi] = l_run[gi] * corr[gi] + sum;
-                m_run[gi] = m_new;
-            }
-            if (__any(grew)) {
-#pragma unroll
-                for (int gi = 0; gi < GI; ++gi)
-#pragma unroll
-                    for (int e = 0; e < DV; ++e) o[gi][e] *= corr[gi];
-            }
-            if (careful) {
-                // Values that are not finite leave the products and are added for the vectors that see them.
-                uint32_t* odd_v = reinterpret_cast<uint32_t*>(part[wave]);  // [WK][HD * BYTES / 4]
-                float* odd_p = part[wave] + WK * (HD * K::BYTES / 4);       // [WK][M]
-#pragma unroll
-                for (int u = 0; u < U; ++u)
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) {
-                        const int at = 16 * u + 4 * fq + j;
-#pragma unroll
-                        for (int i = 0; i < VW; ++i) odd_v[at * (HD * K::BYTES / 4) + fr * VW + i] = st.v[u][j][i], st.v[u][j][i] = word_finite<KIND>(st.v[u][j][i]);
-#pragma unroll
-                        for (int gi = 0; gi < GI; ++gi) odd_p[at * M + 16 * gi + fr] = s[gi][u][j];
-                    }
-                __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
-                __builtin_amdgcn_wave_barrier();
-                __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
-                for (int at = 0; at < WK; ++at) {
-                    if (none >> at & 1) continue;  // (no vector sees it)
-                    const uint32_t key = key0 + at;
-#pragma unroll
-                    for (int gi = 0; gi < GI; ++gi) {
-                        const bool sees = key >= see[gi].lo && key < see[gi].hi;
-                        const float p = odd_p[at * M + 16 * gi + fr];
-#pragma unroll
-                        for (int e = 0; e < DV; ++e)
-#pragma unroll
-                            for (int j = 0; j < 4; ++j) {
-                                const float x = value_at<KIND>(odd_v + at * (HD * K::BYTES / 4), DV * (4 * fq + j) + e);
-                                if (sees && !(fabsf(x) < INFINITY)) o[gi][e][j] += p * x;
-                            }
-                    }
-                }
-                __builtin_amdgcn_wave_barrier();
-            }
-#pragma unroll
-            for (int e = 0; e < DV; ++e) {
-                if constexpr (F32) {
-#pragma unroll
-                    for (int u = 0; u < U; ++u)
-#pragma unroll
-                        for (int j = 0; j < 4; ++j)
-#pragma unroll
-                            for (int gi = 0; gi < GI; ++gi)
-                                o[gi][e] = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(st.v[u][j][e]), pf[gi][u][j], o[gi][e], 0, 0, 0);
-                } else {
-                    u32x4 w;
-#pragma unroll
-                    for (int u = 0; u < U; ++u)
-#pragma unroll
-                        for (int jp = 0; jp < 2; ++jp)  // keys 2 jp and 2 jp + 1, dim e of the lane's
-                            w[2 * u + jp] = __builtin_amdgcn_perm(st.v[u][2 * jp + 1][e / 2], st.v[u][2 * jp][e / 2], e % 2 ? 0x07060302u : 0x05040100u);
-#pragma unroll
-                    for (int x = 0; x < K::TERMS; ++x)
-#pragma unroll
-                        for (int gi = 0; gi < GI; ++gi)
-                            o[gi][e] = K::mfma(__builtin_bit_cast(typename K::T8, w), __builtin_bit_cast(typename K::T8, pf[gi][x]), o[gi][e]);
-                }
-            }
         };
         // A value that is not finite spoils its dimension of every vector of the item, also of those that
         // do not see its key (0 times it is NaN) and, through split terms of either sign, an infinity of
@@ -571,22 +448,166 @@ __global__ __launch_bounds__(kThreads) void paged_few_kernel(PagedAttnArgs a) {
 #pragma unroll
                 for (int e = 0; e < DV; ++e) o[gi][e] = f32x4{0, 0, 0, 0};
             }
-            if (un.hi == 0) break;
-            typename F::Step st[2];
-            int32_t sl[2];
-            sl[0] = slot_of(t0);
-            sl[1] = slot_of(t0 + 1);
-            load(st[0], sl[0]);
-            for (uint32_t t = t0; t < t1; t += 2) {
-                load(st[1], sl[1]);
-                const int32_t n0 = slot_of(t + 2);
-                compute(st[0], t, sl[0], careful);
-                sl[0] = n0;
-                if (t + 1 >= t1) break;
-                load(st[0], sl[0]);
-                const int32_t n1 = slot_of(t + 3);
-                compute(st[1], t + 1, sl[1], careful);
-                sl[1] = n1;
+            if (ta >= tb) break;
+            uint64_t none, none_next;
+            uint32_t slots = filled(slot_of(ta), none), slots_next;
+            int32_t ahead = slot_of(ta + 1);
+            load_k(slots);
+            load_v(slots);
+            for (uint32_t t = ta; t < tb; ++t) {
+                slots_next = filled(ahead, none_next);
+                ahead = slot_of(t + 2);
+                const uint32_t key0 = t * UK + ks * WK;
+                f32x4 s[GI][U];
+#pragma unroll
+                for (int gi = 0; gi < GI; ++gi)
+#pragma unroll
+                    for (int u = 0; u < U; ++u) s[gi][u] = f32x4{0, 0, 0, 0};
+#pragma unroll
+                for (int i = 0; i < KL; ++i) {
+                    if constexpr (F32) {
+#pragma unroll
+                        for (int e = 0; e < 4; ++e)
+#pragma unroll
+                            for (int u = 0; u < U; ++u)
+#pragma unroll
+                                for (int gi = 0; gi < GI; ++gi)
+                                    s[gi][u] = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(st.k[u][i][e]), __uint_as_float(qf[gi][i][e]), s[gi][u], 0, 0, 0);
+                    } else {
+#pragma unroll
+                        for (int x = 0; x < K::TERMS; ++x)
+#pragma unroll
+                            for (int gi = 0; gi < GI; ++gi) {
+                                const u32x4 qx = x == 0 ? qf[gi][i] : q_mine[((gi * KL + i) * (K::TERMS - 1) + x - 1) * 64];
+#pragma unroll
+                                for (int u = 0; u < U; ++u)
+                                    s[gi][u] = K::mfma(__builtin_bit_cast(typename K::T8, st.k[u][i]), __builtin_bit_cast(typename K::T8, qx), s[gi][u]);
+                            }
+                    }
+                }
+                if (t + 1 < tb) load_k(slots_next);
+                // Holes in the table and the ends of spans need the test.
+                if (key0 < all_lo || key0 + WK > all_hi || none) {
+#pragma unroll
+                    for (int u = 0; u < U; ++u)
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) {
+                            const uint32_t at = 16 * u + 4 * fq + j, key = key0 + at;
+                            const bool hole = none >> at & 1;
+#pragma unroll
+                            for (int gi = 0; gi < GI; ++gi)
+                                if (hole || key < see[gi].lo || key >= see[gi].hi) s[gi][u][j] = -INFINITY;
+                        }
+                }
+                u32x4 pf[GI][F32 ? U : K::TERMS];
+                float corr[GI];
+                bool grew = false;
+#pragma unroll
+                for (int gi = 0; gi < GI; ++gi) {
+                    float mx = -INFINITY;
+#pragma unroll
+                    for (int u = 0; u < U; ++u)
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) mx = fmaxf(mx, s[gi][u][j]);
+                    const float m_new = fmaxf(m_run[gi], rows_max(mx) * inv[gi]);
+                    const float m_sub = m_new == -INFINITY ? 0.f : m_new;
+                    grew |= m_new != m_run[gi];
+                    corr[gi] = __builtin_amdgcn_exp2f(m_run[gi] - m_sub);
+                    float sum = 0.f;
+#pragma unroll
+                    for (int u = 0; u < U; ++u)
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) {
+                            const float p = __builtin_amdgcn_exp2f(fmaf(s[gi][u][j], inv[gi], K::PBIAS - m_sub));
+                            s[gi][u][j] = p;
+                            sum += p;
+                        }
+                    if constexpr (F32) {
+#pragma unroll
+                        for (int u = 0; u < U; ++u) pf[gi][u] = __builtin_bit_cast(u32x4, s[gi][u]);
+                    } else {
+                        typename K::T8 t8[K::TERMS];
+#pragma unroll
+                        for (int u = 0; u < U; ++u)
+#pragma unroll
+                            for (int j = 0; j < 4; ++j) split<K>(s[gi][u][j], 4 * u + j, t8);
+#pragma unroll
+                        for (int x = 0; x < K::TERMS; ++x) pf[gi][x] = __builtin_bit_cast(u32x4, t8[x]);
+                    }
+                    l_run[gi] = l_run[gi] * corr[gi] + sum;
+                    m_run[gi] = m_new;
+                }
+                if (__any(grew)) {
+#pragma unroll
+                    for (int gi = 0; gi < GI; ++gi)
+#pragma unroll
+                        for (int e = 0; e < DV; ++e) o[gi][e] *= corr[gi];
+                }
+                if (careful) {
+                    // Values that are not finite leave the products and are added for the vectors that
+                    // see them, the four keys 16 u + 4 (l / 16) + j of the lanes at a time.
+                    uint32_t* odd_v = odd[wave];
+                    float* odd_p = reinterpret_cast<float*>(odd[wave] + 4 * F::kOddV);
+#pragma unroll
+                    for (int u = 0; u < U; ++u)
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) {
+#pragma unroll
+                            for (int i = 0; i < VW; ++i)
+                                odd_v[fq * F::kOddV + fr * VW + i] = st.v[u][j][i], st.v[u][j][i] = word_finite<KIND>(st.v[u][j][i]);
+#pragma unroll
+                            for (int gi = 0; gi < GI; ++gi) odd_p[fq * WV + 16 * gi + fr] = s[gi][u][j];
+                            __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup");
+                            __builtin_amdgcn_wave_barrier();
+                            __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup");
+                            for (int f = 0; f < 4; ++f) {
+                                const int at = 16 * u + 4 * f + j;
+                                if (none >> at & 1) continue;  // (no vector sees it)
+                                const uint32_t key = key0 + at;
+#pragma unroll
+                                for (int gi = 0; gi < GI; ++gi) {
+                                    const bool sees = key >= see[gi].lo && key < see[gi].hi;
+                                    const float p = odd_p[f * WV + 16 * gi + fr];
+#pragma unroll
+                                    for (int e = 0; e < DV; ++e)
+#pragma unroll
+                                        for (int i = 0; i < 4; ++i) {
+                                            const float x = value_at<KIND>(odd_v + f * F::kOddV, DV * (4 * fq + i) + e);
+                                            if (sees && !(fabsf(x) < INFINITY)) o[gi][e][i] += p * x;
+                                        }
+                                }
+                            }
+                            __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup");
+                            __builtin_amdgcn_wave_barrier();
+                            __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup");
+                        }
+                }
+#pragma unroll
+                for (int e = 0; e < DV; ++e) {
+                    if constexpr (F32) {
+#pragma unroll
+                        for (int u = 0; u < U; ++u)
+#pragma unroll
+                            for (int j = 0; j < 4; ++j)
+#pragma unroll
+                                for (int gi = 0; gi < GI; ++gi)
+                                    o[gi][e] = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(st.v[u][j][e]), __uint_as_float(pf[gi][u][j]), o[gi][e], 0, 0, 0);
+                    } else {
+                        u32x4 w;
+#pragma unroll
+                        for (int u = 0; u < U; ++u)
+#pragma unroll
+                            for (int jp = 0; jp < 2; ++jp)  // keys 2 jp and 2 jp + 1, dim e of the lane's
+                                w[2 * u + jp] = __builtin_amdgcn_perm(st.v[u][2 * jp + 1][e / 2], st.v[u][2 * jp][e / 2], e % 2 ? 0x07060302u : 0x05040100u);
+#pragma unroll
+                        for (int x = 0; x < K::TERMS; ++x)
+#pragma unroll
+                            for (int gi = 0; gi < GI; ++gi)
+                                o[gi][e] = K::mfma(__builtin_bit_cast(typename K::T8, w), __builtin_bit_cast(typename K::T8, pf[gi][x]), o[gi][e]);
+                    }
+                }
+                if (t + 1 < tb) load_v(slots_next);
+                slots = slots_next, none = none_next;
             }
             float sum = 0.f;  // NaN if one of them is not finite
 #pragma unroll
@@ -598,14 +619,15 @@ __global__ __launch_bounds__(kThreads) void paged_few_kernel(PagedAttnArgs a) {
             if (!__any(sum != sum)) break;
         }
 
-        // The waves' parts: outputs [M][HD], maxima, sums.
-        float* mine = part[wave];
+        // The waves' parts: outputs [WV][HD], maxima, sums.
+        __syncthreads();  // (q's terms are read)
+        float* mine = shared + wave * F::kWave;
 #pragma unroll
         for (int gi = 0; gi < GI; ++gi) {
             float l = l_run[gi];
             l += __shfl_xor(l, 16, 64);
             l += __shfl_xor(l, 32, 64);
-            if (fq == 0) mine[M * ROW + 16 * gi + fr] = m_run[gi], mine[M * ROW + M + 16 * gi + fr] = l;
+            if (fq == 0) mine[WV * ROW + 16 * gi + fr] = m_run[gi], mine[WV * ROW + WV + 16 * gi + fr] = l;
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
                 float* p = mine + (16 * gi + fr) * ROW + DV * (4 * fq + j);
@@ -622,18 +644,19 @@ __global__ __launch_bounds__(kThreads) void paged_few_kernel(PagedAttnArgs a) {
         const bool whole = t0 == 0 && t1 == un.count;
         float* slot = a.parts + (2 * static_cast<size_t>(block) + (t0 == 0)) * F::kPart;
         for (int i = tid; i < M * HD / 4; i += kThreads) {
-            const int v = i / (HD / 4), d = i % (HD / 4) * 4;
+            const int v = i / (HD / 4), d = i % (HD / 4) * 4, vq = v / WV, vv = v % WV;
             float top = -INFINITY;
 #pragma unroll
-            for (int w = 0; w < 4; ++w) top = fmaxf(top, part[w][M * ROW + v]);
+            for (int w = 0; w < KS; ++w) top = fmaxf(top, shared[(w * QW + vq) * F::kWave + WV * ROW + vv]);
             const float base = top == -INFINITY ? 0.f : top;
             float l = 0.f;
             f32x4 x = {0, 0, 0, 0};
 #pragma unroll
-            for (int w = 0; w < 4; ++w) {
-                const float c = __builtin_amdgcn_exp2f(part[w][M * ROW + v] - base);
-                l += part[w][M * ROW + M + v] * c;
-                x += *reinterpret_cast<const f32x4*>(&part[w][v * ROW + d]) * c;
+            for (int w = 0; w < KS; ++w) {
+                const float* p = shared + (w * QW + vq) * F::kWave;
+                const float c = __builtin_amdgcn_exp2f(p[WV * ROW + vv] - base);
+                l += p[WV * ROW + WV + vv] * c;
+                x += *reinterpret_cast<const f32x4*>(p + vv * ROW + d) * c;
             }
             if (whole) {
                 const uint32_t m = run.m0 + v;
@@ -722,9 +745,11 @@ struct Plan {
 };
 constexpr uint32_t kBlocksPerCu = 2;
 
+// 16 vectors where every request has about a row (steps of single tokens), 32
+// for a few rows, 128 for chunks.
 Plan plan_of(uint32_t rows, uint32_t requests, uint32_t group) {
     const uint64_t vecs = (static_cast<uint64_t>(rows) * group + requests - 1) / requests;  // of an average request and kv head
-    return Plan{vecs <= 16 ? 16u : 32u, gemm_cus() * kBlocksPerCu};
+    return Plan{rows <= requests && group <= 16 ? 16u : vecs <= 48 ? 32u : 128u, gemm_cus() * kBlocksPerCu};
 }
 
 size_t plan_bytes(uint32_t m, uint32_t blocks, uint32_t hd) { return blocks * (sizeof(Cut) + 2 * sizeof(float) * m * (hd + 2)); }
@@ -734,12 +759,16 @@ bool sizes_ok(uint32_t rows, uint32_t requests, uint32_t heads, uint32_t kv_head
            static_cast<uint64_t>(rows) * heads < kPagedMost;
 }
 
+template <int HD, int KIND, int GI, int QW>
+hipError_t launch(const PagedAttnArgs& a, const Plan& p, hipStream_t s) {
+    constexpr int M = Form<HD, KIND, GI, QW>::M;
+    const hipError_t e = vlaunch(paged_attn_kernel<HD, KIND, GI, QW>, dim3(p.blocks), dim3(kThreads), 0, s, a);
+    return e != hipSuccess ? e : vlaunch(paged_join_kernel<HD, M>, dim3(p.blocks, M / 4), dim3(kThreads), 0, s, a);
+}
+
 template <int HD, int KIND>
 hipError_t launch(const PagedAttnArgs& a, const Plan& p, hipStream_t s) {
-    const dim3 grid(p.blocks), block(kThreads);
-    const hipError_t e = p.m == 16 ? vlaunch(paged_few_kernel<HD, KIND, 1>, grid, block, 0, s, a) : vlaunch(paged_few_kernel<HD, KIND, 2>, grid, block, 0, s, a);
-    if (e != hipSuccess) return e;
-    return p.m == 16 ? vlaunch(paged_join_kernel<HD, 16>, dim3(p.blocks, 4), block, 0, s, a) : vlaunch(paged_join_kernel<HD, 32>, dim3(p.blocks, 8), block, 0, s, a);
+    return p.m == 16 ? launch<HD, KIND, 1, 1>(a, p, s) : p.m == 32 ? launch<HD, KIND, 2, 1>(a, p, s) : launch<HD, KIND, 2, 4>(a, p, s);
 }
 
 template <int HD>

@@ -33,23 +33,21 @@ typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 
 constexpr int kThreads = 256;
-constexpr uint32_t kFewestKeys = 256;  // a run shorter than this costs more at its ends than it saves
-
-// What a block leaves for the joining kernel about the item that its run's end cut.
-struct Cut {
-    uint32_t parts;  // 0: none; else of this block's second slot and the first slots of the blocks behind it
-    uint32_t first_row, m0, vecs, kvh, pad[3];
-};
+#ifndef VVLI_X
+#define VVLI_X 16
+#endif
+// Fewest units of a run: a shorter one costs more at its ends than it saves.
+constexpr uint32_t kFewestUnits = 4;
 
 struct PagedAttnArgs {
     const void *k, *v;
     const int32_t *table, *row_start, *start_pos;
     const float* q;
     float* out;
-    Cut* cuts;
-    float* parts;  // two slots for each block: [M][HD] outputs, then [M] maxima and [M] sums
+    uint32_t* arrived;  // of each block: parts that are there of the item that its run's end cut; 0 between calls
+    float* parts;       // two slots for each block: [slot_vecs][HD] outputs, [slot_vecs] maxima and sums
     uint64_t slot_stride, ldq, ldo;
-    uint32_t stride, requests, rows, kv_heads, window, pages, room;
+    uint32_t stride, requests, rows, kv_heads, window, pages, room, slot_vecs;
     PageDiv ps, group;
     float scale;
 };
@@ -67,21 +65,27 @@ __device__ __forceinline__ Request request_at(const PagedAttnArgs& a, uint32_t r
     return Request{s.first, s.count * a.group.d, a.start_pos[r]};
 }
 
-// The keys lo .. hi - 1 that some vector of m0 .. m0 + M - 1 sees (hi = 0:
-// none), and the units that they touch; an item without keys counts one, in
-// which its zeros are written.
+// An item's vectors stand in groups of GV = M / 4, one to a wave: 1, 2 or 4
+// waves side by side (the log of that in `wide`) take different vectors, and
+// the 4 >> wide such sets take steps of WK positions in turn, (4 WK) >> wide a
+// unit. The keys lo .. hi - 1 that some vector of the item sees (hi = 0: none),
+// and the units that they touch; an item without keys counts one, in which its
+// zeros are written.
 struct Units {
-    uint32_t lo, hi, first, count;
+    uint32_t lo, hi, first, count, wide;
 };
-template <int M, int UK>
+template <int M, int WK>
 __device__ __forceinline__ Units units_of(const PagedAttnArgs& a, const Request& q, uint32_t m0) {
+    const uint32_t vecs = min(static_cast<uint32_t>(M), q.vecs - m0);
+    const uint32_t wide = vecs <= M / 4 ? 0 : vecs <= M / 2 ? 1 : 2;
     const int64_t p0 = q.start + page_of(a.group, m0);
-    const int64_t p1 = q.start + page_of(a.group, min(m0 + M, q.vecs) - 1);
+    const int64_t p1 = q.start + page_of(a.group, m0 + vecs - 1);
     const int64_t hi = min(p1 + 1, static_cast<int64_t>(a.room));
     const int64_t lo = a.window && p0 + 1 > a.window ? p0 + 1 - a.window : 0;
-    if (hi <= lo) return Units{0, 0, 0, 1};
-    Units u{static_cast<uint32_t>(lo), static_cast<uint32_t>(hi), static_cast<uint32_t>(lo) / UK, 0};
-    u.count = (u.hi + UK - 1) / UK - u.first;
+    if (hi <= lo) return Units{0, 0, 0, 1, wide};
+    const uint32_t unit = (4 * WK) >> wide;
+    Units u{static_cast<uint32_t>(lo), static_cast<uint32_t>(hi), static_cast<uint32_t>(lo) / unit, 0, wide};
+    u.count = (u.hi + unit - 1) / unit - u.first;
     return u;
 }
 
@@ -97,17 +101,17 @@ __device__ __forceinline__ uint64_t wave_scan(uint64_t v) {
 
 // Units of one kv head of each lane's request, summed over its items: by the
 // lane itself where they are few, else by its wave.
-template <int M, int UK>
+template <int M, int WK>
 __device__ __forceinline__ uint64_t request_units(const PagedAttnArgs& a, const Request& q) {
     const uint32_t lane = threadIdx.x & 63, items = (q.vecs + M - 1) / M;
     uint64_t sum = 0;
     if (items <= 2)
-        for (uint32_t i = 0; i < items; ++i) sum += units_of<M, UK>(a, q, i * M).count;
+        for (uint32_t i = 0; i < items; ++i) sum += units_of<M, WK>(a, q, i * M).count;
     for (uint64_t todo = __ballot(items > 2); todo; todo &= todo - 1) {
         const int from = __builtin_ctzll(todo);
         const Request f{static_cast<uint32_t>(__shfl(q.first, from, 64)), static_cast<uint32_t>(__shfl(q.vecs, from, 64)), __shfl(q.start, from, 64)};
         uint64_t s = 0;
-        for (uint32_t i = lane; i < (f.vecs + M - 1) / M; i += 64) s += units_of<M, UK>(a, f, i * M).count;
+        for (uint32_t i = lane; i < (f.vecs + M - 1) / M; i += 64) s += units_of<M, WK>(a, f, i * M).count;
 #pragma unroll
         for (int o = 32; o; o >>= 1) s += __shfl_xor(s, o, 64);
         if (static_cast<int>(lane) == from) sum = s;
@@ -115,25 +119,28 @@ __device__ __forceinline__ uint64_t request_units(const PagedAttnArgs& a, const 
     return sum;
 }
 
-// Where a block's run starts: request, kv head, vector and unit of the item; units of the run.
+// Run b holds the units from per * b on to per * (b + 1), but that a border
+// within `near` units of an item's start or end moves there (near < per / 2, so
+// that borders keep their order): fewer items are cut.
 struct Run {
-    uint32_t r, kvh, m0, unit;
-    uint64_t left, per;
+    uint64_t from, to, per;  // global units, before the borders move
+    uint32_t near, r, kvh, m0, unit;  // the item that holds unit `from`, and which unit of it that is
+    bool any;
 };
 
 struct RunScratch {
     uint64_t sums[kThreads / 64], found_rest, found_units;
-    uint32_t found_r;
+    uint32_t found_r, last;
 };
 
-template <int M, int UK>
+template <int M, int WK>
 __device__ Run find_run(const PagedAttnArgs& a, uint32_t block, uint32_t blocks, RunScratch& sc) {
     const uint32_t tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     const uint32_t chunks = (a.requests + kThreads - 1) / kThreads;
     uint64_t mine = 0, end = 0, before = 0;
     auto chunk = [&](uint32_t c) {  // this thread's request's units, and the sum up to it
         const uint32_t r = c * kThreads + tid;
-        mine = request_units<M, UK>(a, r < a.requests ? request_at(a, r) : Request{0, 0, 0});
+        mine = request_units<M, WK>(a, r < a.requests ? request_at(a, r) : Request{0, 0, 0});
         const uint64_t s = wave_scan(mine);
         __syncthreads();
         if (lane == 63) sc.sums[wave] = s;
@@ -147,15 +154,17 @@ __device__ Run find_run(const PagedAttnArgs& a, uint32_t block, uint32_t blocks,
     for (uint32_t c = 0; c < chunks; ++c) chunk(c);
     const uint64_t total = before * a.kv_heads;
     Run run{};
-    run.per = max((total + blocks - 1) / blocks, static_cast<uint64_t>(kFewestKeys / UK));
-    const uint64_t from = run.per * block;
-    if (from >= total) return run;
-    run.left = min(run.per, total - from);
+    run.per = max((total + blocks - 1) / blocks, static_cast<uint64_t>(kFewestUnits));
+    run.near = static_cast<uint32_t>(min(run.per / 4, static_cast<uint64_t>(1u << 20)));
+    run.from = run.per * block;
+    run.to = run.from + run.per >= total ? ~uint64_t{0} : run.from + run.per;
+    if (run.from >= total) return run;
+    run.any = true;
     before = 0;
     for (uint32_t c = 0; c < chunks; ++c) {
         if (chunks > 1) chunk(c);
         const uint64_t lo = (end - mine) * a.kv_heads;
-        if (mine && from >= lo && from < end * a.kv_heads) sc.found_r = c * kThreads + tid, sc.found_rest = from - lo, sc.found_units = mine;
+        if (mine && run.from >= lo && run.from < end * a.kv_heads) sc.found_r = c * kThreads + tid, sc.found_rest = run.from - lo, sc.found_units = mine;
     }
     __syncthreads();
     run.r = __builtin_amdgcn_readfirstlane(sc.found_r);
@@ -165,7 +174,7 @@ __device__ Run find_run(const PagedAttnArgs& a, uint32_t block, uint32_t blocks,
     const Request q = request_at(a, run.r);
     for (uint32_t i = 0;; i += 64) {  // every wave by itself: the item that holds unit v
         const uint32_t m = (i + lane) * M;
-        const uint64_t s = wave_scan(m < q.vecs ? units_of<M, UK>(a, q, m).count : 0);
+        const uint64_t s = wave_scan(m < q.vecs ? units_of<M, WK>(a, q, m).count : 0);
         const uint64_t past = __ballot(s > v);
         if (past || (i + 64) * M >= q.vecs) {
             const int at = past ? __builtin_ctzll(past) : 0;
@@ -221,11 +230,10 @@ __device__ __forceinline__ void split(float x, int e, typename K::T8 (&t)[K::TER
 }
 
 // ---------------------------------------------------------------------------
-// An item has M = 16 GI QW vectors: QW of the block's four waves hold 16 GI of
-// them each, and KS = 4 / QW groups of such waves take the item's keys in turn,
-// WK = 16 U positions each, and join at its end. Nothing is shared between
-// waves on the way, so keys and values go from memory (or the caches, where
-// waves read the same ones) straight into the registers that the products
+// A wave holds WV = 16 GI vectors of an item and takes WK = 16 U positions a
+// step; waves that share vectors join at the item's end. Nothing is shared
+// between waves on the way, so keys and values go from memory (or the caches,
+// where waves read the same ones) straight into the registers that the products
 // read, the next step's keys and values in flight behind this one's:
 //   S^T = K Q^T  A: lane l has key l % 16, dims 32 s + 8 (l / 16) .. + 7 (16-bit)
 //                   or 16 s + 4 (l / 16) + e (f32); D: lane l has keys
@@ -237,23 +245,22 @@ __device__ __forceinline__ void split(float x, int e, typename K::T8 (&t)[K::TER
 // The first term of q stays in registers, the others in LDS: two waves fit a
 // SIMD, one's products beside the other's exponentials.
 // ---------------------------------------------------------------------------
-template <int HD, int KIND, int GI, int QW>
+template <int HD, int KIND, int GI>
 struct Form {
     using K = Kind<KIND>;
-    static constexpr int M = 16 * GI * QW, KS = 4 / QW, U = K::U, WK = 16 * U, UK = KS * WK, DV = HD / 16;
+    static constexpr int WV = 16 * GI, M = 4 * WV, U = K::U, WK = 16 * U, DV = HD / 16;
     static constexpr int KL = HD * K::BYTES / 64;   // 16-byte loads of a key row by a lane
     static constexpr int VW = DV * K::BYTES / 4;    // 32-bit words of a value row in a lane
     struct Step {
         u32x4 k[U][KL];
         uint32_t v[U][4][VW];
     };
-    // What a block has of an item: [M][HD] outputs, [M] maxima, [M] sums; and
-    // what a wave leaves in LDS of it at its end, in the place of q's terms:
-    // the same with rows ROW apart, so that 16 rows' 16-byte writes fall on
-    // different banks.
-    static constexpr int kPart = M * (HD + 2), ROW = HD + 4, kWave = 16 * GI * (ROW + 2);
-    static constexpr int kQ = QW * GI * KL * (K::TERMS - 1) * 64;  // 16-byte units
-    static constexpr int kShared = std::max(4 * kWave, 4 * kQ);    // 32-bit words
+    // What a wave leaves in LDS of an item at its end, in the place of q's
+    // terms: [WV][HD] outputs with rows ROW apart, so that 16 rows' 16-byte
+    // writes fall on different banks, [WV] maxima, [WV] sums.
+    static constexpr int ROW = HD + 4, kWave = WV * (ROW + 2);
+    static constexpr int kQ = GI * KL * (K::TERMS - 1) * 64;         // of a wave, in 16-byte units
+    static constexpr int kShared = std::max(4 * kWave, 4 * 4 * kQ);  // 32-bit words
     // Four keys' values and weights of a wave (values that are not finite).
     static constexpr int kOddV = HD * K::BYTES / 4, kOdd = 4 * (kOddV + 16 * GI);
 };
@@ -296,12 +303,11 @@ __device__ __forceinline__ float rows_max(float x) {
     return fmaxf(__uint_as_float(b[0]), __uint_as_float(b[1]));
 }
 
-template <int HD, int KIND, int GI, int QW>
+template <int HD, int KIND, int GI>
 __global__ __launch_bounds__(kThreads, 2) void paged_attn_kernel(PagedAttnArgs a) {
-    using F = Form<HD, KIND, GI, QW>;
+    using F = Form<HD, KIND, GI>;
     using K = Kind<KIND>;
-    constexpr int M = F::M, KS = F::KS, U = F::U, WK = F::WK, UK = F::UK, DV = F::DV, KL = F::KL, VW = F::VW, ROW = F::ROW;
-    constexpr int WV = 16 * GI;  // vectors of a wave
+    constexpr int M = F::M, WV = F::WV, U = F::U, WK = F::WK, DV = F::DV, KL = F::KL, VW = F::VW, ROW = F::ROW;
     constexpr bool F32 = KIND == VVLI_CACHE_F32;
     __shared__ RunScratch sc;
     __shared__ __attribute__((aligned(16))) float shared[F::kShared];
@@ -310,24 +316,36 @@ __global__ __launch_bounds__(kThreads, 2) void paged_attn_kernel(PagedAttnArgs a
     const uint32_t blocks = gridDim.x;
     // Neighbouring runs on one XCD (blocks go to the eight in turn): they share keys and table rows in its L2.
     const uint32_t block = blocks % 8 == 0 ? blockIdx.x % 8 * (blocks / 8) + blockIdx.x / 8 : blockIdx.x;
-    Run run = find_run<M, UK>(a, block, blocks, sc);
+    Run run = find_run<M, WK>(a, block, blocks, sc);
+    if (!run.any) return;
     const int tid = threadIdx.x, lane = tid & 63, fr = lane & 15, fq = lane >> 4;
-    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), qw = wave % QW, ks = wave / QW;
-    uint32_t cut_parts = 0;
-    if (run.left == 0) {
-        if (tid == 0) a.cuts[block].parts = 0;
-        return;
-    }
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const uint64_t row_bytes = a.slot_stride * K::BYTES;
-    u32x4* const q_mine = reinterpret_cast<u32x4*>(shared) + qw * (F::kQ / QW) + lane;  // (the key groups of one qw write the same values)
+    const uint32_t slot_words = a.slot_vecs * (HD + 2);
     Request req = request_at(a, run.r);
-    while (run.left) {
-        while (run.m0 >= req.vecs) {  // the next item
+    uint64_t start = run.from - run.unit;  // global unit where the item starts
+    bool begun = run.unit > run.near;      // the run starts inside the item (a border near its start is its start)
+    for (;; begun = false) {
+        while (run.m0 >= req.vecs) {  // the next item with vectors
             run.m0 = 0;
-            if (req.vecs == 0 || ++run.kvh == a.kv_heads) run.kvh = 0, req = request_at(a, ++run.r);
+            if (req.vecs == 0 || ++run.kvh == a.kv_heads) {
+                run.kvh = 0;
+                if (++run.r == a.requests) return;
+                req = request_at(a, run.r);
+            }
         }
-        const Units un = units_of<M, UK>(a, req, run.m0);
-        const uint32_t t0 = run.unit, t1 = static_cast<uint32_t>(min(static_cast<uint64_t>(un.count), t0 + run.left));
+        const Units un = units_of<M, WK>(a, req, run.m0);
+        if (!begun && run.to <= start + min(run.near, un.count - 1)) return;  // the item is the next run's
+        if (begun && un.count - run.unit <= run.near) {    // what is left of it is the last run's
+            start += un.count, run.m0 += M;
+            continue;
+        }
+        const uint32_t t0 = begun ? run.unit : 0;
+        const bool cut = run.to < start + un.count && start + un.count - run.to > run.near;
+        const uint32_t t1 = cut ? static_cast<uint32_t>(run.to - start) : un.count;
+        const uint32_t sets = 4u >> un.wide, UK = WK * sets;      // sets of waves with all of the item's vectors
+        const uint32_t qw = wave & ((1u << un.wide) - 1), ks = wave >> un.wide;
+        u32x4* const q_mine = reinterpret_cast<u32x4*>(shared) + qw * F::kQ + lane;  // (the sets write the same values)
         const int32_t* table = a.table + static_cast<size_t>(run.r) * a.stride;
         const char* kbase = static_cast<const char*>(a.k) + static_cast<size_t>(run.kvh) * HD * K::BYTES + 16 * fq;
         const char* vbase = static_cast<const char*>(a.v) + static_cast<size_t>(run.kvh) * HD * K::BYTES + 4 * VW * fr;
@@ -396,8 +414,8 @@ __global__ __launch_bounds__(kThreads, 2) void paged_attn_kernel(PagedAttnArgs a
         }
         // The wave's steps: those units of the run whose WK keys from t * UK + ks * WK on meet w_lo .. w_hi - 1.
         uint32_t ta = un.first + t0, tb = un.first + t1;
-        if (w_lo >= static_cast<uint32_t>((ks + 1) * WK)) ta = max(ta, (w_lo - (ks + 1) * WK) / UK + 1);
-        tb = w_lo < w_hi && w_hi > static_cast<uint32_t>(ks * WK) ? min(tb, (w_hi - ks * WK + UK - 1) / UK) : 0;
+        if (w_lo >= (ks + 1) * WK) ta = max(ta, (w_lo - (ks + 1) * WK) / UK + 1);
+        tb = w_lo < w_hi && w_hi > ks * WK ? min(tb, (w_hi - ks * WK + UK - 1) / UK) : 0;
 
         f32x4 o[GI][DV];
         float m_run[GI], l_run[GI];
@@ -642,100 +660,79 @@ __global__ __launch_bounds__(kThreads, 2) void paged_attn_kernel(PagedAttnArgs a
         }
         __syncthreads();
         const bool whole = t0 == 0 && t1 == un.count;
-        float* slot = a.parts + (2 * static_cast<size_t>(block) + (t0 == 0)) * F::kPart;
-        for (int i = tid; i < M * HD / 4; i += kThreads) {
-            const int v = i / (HD / 4), d = i % (HD / 4) * 4, vq = v / WV, vv = v % WV;
+        const uint32_t vecs = min(static_cast<uint32_t>(M), req.vecs - run.m0);
+        auto write = [&](uint32_t v, uint32_t d, f32x4 x, float l) {
+            const uint32_t m = run.m0 + v, row = page_of(a.group, m), g = m - row * a.group.d;
+            float* op = a.out + (req.first + row) * a.ldo + (static_cast<size_t>(run.kvh) * a.group.d + g) * HD + d;
+            const float r = 1.f / l;
+            *reinterpret_cast<f32x4*>(op) = l == 0.f ? f32x4{0, 0, 0, 0} : x * r;
+        };
+        // Parts go through to memory (agent-scope stores and loads): other XCDs read them.
+        auto publish = [](float* p, float x, float y) {
+            __hip_atomic_store(reinterpret_cast<uint64_t*>(p), static_cast<uint64_t>(__float_as_uint(y)) << 32 | __float_as_uint(x), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        };
+        auto fetch = [](const float* p) {
+            const uint64_t w = __hip_atomic_load(reinterpret_cast<const uint64_t*>(p), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+            return make_float2(__uint_as_float(static_cast<uint32_t>(w)), __uint_as_float(static_cast<uint32_t>(w >> 32)));
+        };
+        float* slot = a.parts + (2 * static_cast<size_t>(block) + (t0 == 0)) * slot_words;
+        for (uint32_t i = tid; i < vecs * (HD / 4); i += kThreads) {
+            const uint32_t v = i / (HD / 4), d = i % (HD / 4) * 4, vq = v / WV, vv = v % WV;
             float top = -INFINITY;
-#pragma unroll
-            for (int w = 0; w < KS; ++w) top = fmaxf(top, shared[(w * QW + vq) * F::kWave + WV * ROW + vv]);
+            for (uint32_t w = vq; w < 4; w += 4 / sets) top = fmaxf(top, shared[w * F::kWave + WV * ROW + vv]);
             const float base = top == -INFINITY ? 0.f : top;
             float l = 0.f;
             f32x4 x = {0, 0, 0, 0};
-#pragma unroll
-            for (int w = 0; w < KS; ++w) {
-                const float* p = shared + (w * QW + vq) * F::kWave;
+            for (uint32_t w = vq; w < 4; w += 4 / sets) {
+                const float* p = shared + w * F::kWave;
                 const float c = __builtin_amdgcn_exp2f(p[WV * ROW + vv] - base);
                 l += p[WV * ROW + WV + vv] * c;
                 x += *reinterpret_cast<const f32x4*>(p + vv * ROW + d) * c;
             }
             if (whole) {
-                const uint32_t m = run.m0 + v;
-                if (m < req.vecs) {
-                    const uint32_t row = page_of(a.group, m), g = m - row * a.group.d;
-                    float* op = a.out + (req.first + row) * a.ldo + (static_cast<size_t>(run.kvh) * a.group.d + g) * HD + d;
-                    const float r = l == 0.f ? 0.f : 1.f / l;
-                    *reinterpret_cast<f32x4*>(op) = l == 0.f ? f32x4{0, 0, 0, 0} : x * r;
-                }
+                write(v, d, x, l);
             } else {
-                *reinterpret_cast<f32x4*>(slot + v * HD + d) = x;
-                if (d == 0) slot[M * HD + v] = top, slot[M * HD + M + v] = l;
+                publish(slot + v * HD + d, x[0], x[1]);
+                publish(slot + v * HD + d + 2, x[2], x[3]);
+                if (d == 0) publish(slot + a.slot_vecs * HD + 2 * v, top, l);
             }
+        }
+        if (!whole) {
+            // Borders inside the item, from near behind its start to near before its end: run first_border - 1
+            // has its first part (in its second slot), the runs from first_border on the others (in their first).
+            const uint64_t first_border = (start + run.near) / run.per + 1;
+            const uint32_t n = static_cast<uint32_t>((start + un.count - run.near - 1) / run.per - first_border) + 2;
+            __builtin_amdgcn_s_waitcnt(0);  // this thread's stores are in memory
+            __syncthreads();
+            if (tid == 0) sc.last = __hip_atomic_fetch_add(a.arrived + first_border - 1, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == n - 1;
+            __syncthreads();
+            if (sc.last) {
+                __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "agent");
+                const float* first = a.parts + (2 * first_border - 1) * slot_words;
+                auto part_at = [&](uint32_t i) { return i == 0 ? first : first + (2 * static_cast<size_t>(i) - 1) * slot_words; };
+                for (uint32_t i = tid; i < vecs * (HD / 4); i += kThreads) {
+                    const uint32_t v = i / (HD / 4), d = i % (HD / 4) * 4;
+                    float top = -INFINITY;
+                    for (uint32_t w = 0; w < n; ++w) top = fmaxf(top, fetch(part_at(w) + a.slot_vecs * HD + 2 * v).x);
+                    const float base = top == -INFINITY ? 0.f : top;
+                    float l = 0.f;
+                    f32x4 x = {0, 0, 0, 0};
+                    for (uint32_t w = 0; w < n; ++w) {
+                        const float* p = part_at(w);
+                        const float2 ml = fetch(p + a.slot_vecs * HD + 2 * v), x0 = fetch(p + v * HD + d), x1 = fetch(p + v * HD + d + 2);
+                        const float c = __builtin_amdgcn_exp2f(ml.x - base);
+                        l += ml.y * c;
+                        x += f32x4{x0.x, x0.y, x1.x, x1.y} * c;
+                    }
+                    write(v, d, x, l);
+                }
+                if (tid == 0) a.arrived[first_border - 1] = 0;  // for the next call
+            }
+            if (cut) return;
         }
         __syncthreads();
-        run.left -= t1 - t0;
-        if (t1 < un.count) {  // the run ends inside the item
-            if (t0 == 0) {
-                cut_parts = 1 + static_cast<uint32_t>((un.count - t1 + run.per - 1) / run.per);
-                if (tid == 0) a.cuts[block] = Cut{cut_parts, req.first, run.m0, min(static_cast<uint32_t>(M), req.vecs - run.m0), run.kvh, {}};
-            }
-            break;
-        }
-        run.unit = 0;
+        start += un.count;
         run.m0 += M;
-    }
-    if (cut_parts == 0 && tid == 0) a.cuts[block].parts = 0;
-}
-
-// Joins the parts of the items that runs cut: block (b, y) takes four vectors
-// of the item that run b began and did not end. HD / 4 threads hold a vector's
-// dims, the others' groups take the parts in turn.
-template <int HD, int M>
-__global__ __launch_bounds__(kThreads) void paged_join_kernel(PagedAttnArgs a) {
-    constexpr int LANES = HD / 4, GROUPS = kThreads / LANES, V = 4, PART = M * (HD + 2);
-    __shared__ __attribute__((aligned(16))) float sum[GROUPS][V][HD + 4];
-    __shared__ float tops[V];
-    const uint32_t block = blockIdx.x, v0 = blockIdx.y * V, tid = threadIdx.x;
-    const Cut cut = a.cuts[block];
-    if (cut.parts == 0 || v0 >= cut.vecs) return;
-    const float* first = a.parts + (2 * static_cast<size_t>(block) + 1) * PART;  // then the first slots of the blocks behind
-    auto part_at = [&](uint32_t i) { return i == 0 ? first : first + (2 * static_cast<size_t>(i) - 1) * PART; };
-    const uint32_t wave = tid >> 6, lane = tid & 63;
-    {
-        float top = -INFINITY;  // wave w: vector v0 + w
-        for (uint32_t i = lane; i < cut.parts; i += 64) top = fmaxf(top, part_at(i)[M * HD + v0 + wave]);
-        top = wave_max(top);
-        if (lane == 0) tops[wave] = top == -INFINITY ? 0.f : top;
-    }
-    __syncthreads();
-    const uint32_t g = tid / LANES, d = tid % LANES * 4;
-    f32x4 x[V];
-    float l[V];
-#pragma unroll
-    for (int v = 0; v < V; ++v) x[v] = f32x4{0, 0, 0, 0}, l[v] = 0.f;
-    for (uint32_t i = g; i < cut.parts; i += GROUPS) {
-        const float* p = part_at(i);
-#pragma unroll
-        for (int v = 0; v < V; ++v) {
-            const float c = __builtin_amdgcn_exp2f(p[M * HD + v0 + v] - tops[v]);
-            l[v] += p[M * HD + M + v0 + v] * c;
-            x[v] += *reinterpret_cast<const f32x4*>(p + (v0 + v) * HD + d) * c;
-        }
-    }
-#pragma unroll
-    for (int v = 0; v < V; ++v) {
-        *reinterpret_cast<f32x4*>(&sum[g][v][d]) = x[v];
-        if (d == 0) sum[g][v][HD] = l[v];
-    }
-    __syncthreads();
-    for (uint32_t i = tid; i < V * LANES; i += kThreads) {
-        const uint32_t v = i / LANES, dd = i % LANES * 4, m = cut.m0 + v0 + v;
-        if (v0 + v >= cut.vecs) continue;
-        float lt = 0.f;
-        f32x4 xt = {0, 0, 0, 0};
-        for (int w = 0; w < GROUPS; ++w) lt += sum[w][v][HD], xt += *reinterpret_cast<const f32x4*>(&sum[w][v][dd]);
-        const uint32_t row = page_of(a.group, m), h = m - row * a.group.d;
-        float* op = a.out + (cut.first_row + row) * a.ldo + (static_cast<size_t>(cut.kvh) * a.group.d + h) * HD + dd;
-        *reinterpret_cast<f32x4*>(op) = lt == 0.f ? f32x4{0, 0, 0, 0} : xt * (1.f / lt);
     }
 }
 
@@ -745,30 +742,26 @@ struct Plan {
 };
 constexpr uint32_t kBlocksPerCu = 2;
 
-// 16 vectors where every request has about a row (steps of single tokens), 32
-// for a few rows, 128 for chunks.
 Plan plan_of(uint32_t rows, uint32_t requests, uint32_t group) {
-    const uint64_t vecs = (static_cast<uint64_t>(rows) * group + requests - 1) / requests;  // of an average request and kv head
-    return Plan{rows <= requests && group <= 16 ? 16u : vecs <= 48 ? 32u : 128u, gemm_cus() * kBlocksPerCu};
+    const uint64_t vecs = static_cast<uint64_t>(rows) * group;
+    return Plan{vecs <= VVLI_X * requests ? 64u : 128u, gemm_cus() * kBlocksPerCu};
 }
 
-size_t plan_bytes(uint32_t m, uint32_t blocks, uint32_t hd) { return blocks * (sizeof(Cut) + 2 * sizeof(float) * m * (hd + 2)); }
+// An item's most vectors, and the bytes of a call's workspace: counters, then two slots of such an item for each block.
+uint32_t slot_vecs(uint32_t m, uint32_t rows, uint32_t group) {
+    return static_cast<uint32_t>(std::min<uint64_t>(m, (static_cast<uint64_t>(rows) * group + 1) & ~uint64_t{1}));
+}
+size_t plan_bytes(uint32_t blocks, uint32_t vecs, uint32_t hd) { return blocks * sizeof(float) * (4 + 2 * static_cast<size_t>(vecs) * (hd + 2)); }
 
 bool sizes_ok(uint32_t rows, uint32_t requests, uint32_t heads, uint32_t kv_heads) {
     return requests != 0 && heads != 0 && kv_heads != 0 && heads % kv_heads == 0 && heads <= 65535 &&
            static_cast<uint64_t>(rows) * heads < kPagedMost;
 }
 
-template <int HD, int KIND, int GI, int QW>
-hipError_t launch(const PagedAttnArgs& a, const Plan& p, hipStream_t s) {
-    constexpr int M = Form<HD, KIND, GI, QW>::M;
-    const hipError_t e = vlaunch(paged_attn_kernel<HD, KIND, GI, QW>, dim3(p.blocks), dim3(kThreads), 0, s, a);
-    return e != hipSuccess ? e : vlaunch(paged_join_kernel<HD, M>, dim3(p.blocks, M / 4), dim3(kThreads), 0, s, a);
-}
-
 template <int HD, int KIND>
 hipError_t launch(const PagedAttnArgs& a, const Plan& p, hipStream_t s) {
-    return p.m == 16 ? launch<HD, KIND, 1, 1>(a, p, s) : p.m == 32 ? launch<HD, KIND, 2, 1>(a, p, s) : launch<HD, KIND, 2, 4>(a, p, s);
+    const dim3 grid(p.blocks), block(kThreads);
+    return p.m == 64 ? vlaunch(paged_attn_kernel<HD, KIND, 1>, grid, block, 0, s, a) : vlaunch(paged_attn_kernel<HD, KIND, 2>, grid, block, 0, s, a);
 }
 
 template <int HD>
@@ -783,9 +776,8 @@ extern "C" {
 size_t vvli_gpu_paged_attention_workspace(uint32_t rows, uint32_t requests, uint32_t heads, uint32_t kv_heads,
                                           uint32_t head_dim) {
     if (!sizes_ok(rows, requests, heads, kv_heads) || (head_dim != 32 && head_dim != 64 && head_dim != 128)) return 0;
-    // (the largest form that so many rows reach, of however few requests)
-    const Plan p = plan_of(rows, 1, heads / kv_heads);
-    return plan_bytes(p.m, p.blocks, head_dim);
+    const Plan p = plan_of(rows, 1, heads / kv_heads);  // (of however few requests)
+    return plan_bytes(p.blocks, slot_vecs(p.m, rows, heads / kv_heads), head_dim);
 }
 
 int vvli_gpu_paged_attention(const vvli_gpu_paged_cache* cache, const int32_t* table, uint32_t table_stride,
@@ -812,8 +804,9 @@ int vvli_gpu_paged_attention(const vvli_gpu_paged_cache* cache, const int32_t* t
     const Plan p = plan_of(rows, requests, group);
     PagedAttnArgs a{};
     a.k = cache->k, a.v = cache->v, a.table = table, a.row_start = row_start, a.start_pos = start_pos, a.q = q, a.out = out;
-    a.cuts = static_cast<Cut*>(workspace);
-    a.parts = reinterpret_cast<float*>(static_cast<char*>(workspace) + p.blocks * sizeof(Cut));
+    a.arrived = static_cast<uint32_t*>(workspace);
+    a.parts = static_cast<float*>(workspace) + 4 * p.blocks;
+    a.slot_vecs = slot_vecs(p.m, rows, group);
     a.slot_stride = cache->slot_stride, a.ldq = ldq, a.ldo = ldo;
     a.stride = table_stride, a.requests = requests, a.rows = rows, a.kv_heads = cache->kv_heads, a.window = window;
     a.pages = cache->pages, a.room = table_stride * cache->page_size, a.ps = page_div(cache->page_size), a.group = page_div(group);

@@ -33,9 +33,6 @@ typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 
 constexpr int kThreads = 256;
-#ifndef VVLI_X
-#define VVLI_X 16
-#endif
 // Fewest units of a run: a shorter one costs more at its ends than it saves.
 constexpr uint32_t kFewestUnits = 4;
 
@@ -74,7 +71,8 @@ __device__ __forceinline__ Request request_at(const PagedAttnArgs& a, uint32_t r
 struct Units {
     uint32_t lo, hi, first, count, wide;
 };
-template <int M, int WK>
+// (FIXED: units of WK positions whatever the item.)
+template <int M, int WK, bool FIXED>
 __device__ __forceinline__ Units units_of(const PagedAttnArgs& a, const Request& q, uint32_t m0) {
     const uint32_t vecs = min(static_cast<uint32_t>(M), q.vecs - m0);
     const uint32_t wide = vecs <= M / 4 ? 0 : vecs <= M / 2 ? 1 : 2;
@@ -83,7 +81,7 @@ __device__ __forceinline__ Units units_of(const PagedAttnArgs& a, const Request&
     const int64_t hi = min(p1 + 1, static_cast<int64_t>(a.room));
     const int64_t lo = a.window && p0 + 1 > a.window ? p0 + 1 - a.window : 0;
     if (hi <= lo) return Units{0, 0, 0, 1, wide};
-    const uint32_t unit = (4 * WK) >> wide;
+    const uint32_t unit = FIXED ? WK : (4 * WK) >> wide;
     Units u{static_cast<uint32_t>(lo), static_cast<uint32_t>(hi), static_cast<uint32_t>(lo) / unit, 0, wide};
     u.count = (u.hi + unit - 1) / unit - u.first;
     return u;
@@ -101,17 +99,17 @@ __device__ __forceinline__ uint64_t wave_scan(uint64_t v) {
 
 // Units of one kv head of each lane's request, summed over its items: by the
 // lane itself where they are few, else by its wave.
-template <int M, int WK>
+template <int M, int WK, bool FIXED>
 __device__ __forceinline__ uint64_t request_units(const PagedAttnArgs& a, const Request& q) {
     const uint32_t lane = threadIdx.x & 63, items = (q.vecs + M - 1) / M;
     uint64_t sum = 0;
     if (items <= 2)
-        for (uint32_t i = 0; i < items; ++i) sum += units_of<M, WK>(a, q, i * M).count;
+        for (uint32_t i = 0; i < items; ++i) sum += units_of<M, WK, FIXED>(a, q, i * M).count;
     for (uint64_t todo = __ballot(items > 2); todo; todo &= todo - 1) {
         const int from = __builtin_ctzll(todo);
         const Request f{static_cast<uint32_t>(__shfl(q.first, from, 64)), static_cast<uint32_t>(__shfl(q.vecs, from, 64)), __shfl(q.start, from, 64)};
         uint64_t s = 0;
-        for (uint32_t i = lane; i < (f.vecs + M - 1) / M; i += 64) s += units_of<M, WK>(a, f, i * M).count;
+        for (uint32_t i = lane; i < (f.vecs + M - 1) / M; i += 64) s += units_of<M, WK, FIXED>(a, f, i * M).count;
 #pragma unroll
         for (int o = 32; o; o >>= 1) s += __shfl_xor(s, o, 64);
         if (static_cast<int>(lane) == from) sum = s;
@@ -133,14 +131,14 @@ struct RunScratch {
     uint32_t found_r, last;
 };
 
-template <int M, int WK>
+template <int M, int WK, bool FIXED>
 __device__ Run find_run(const PagedAttnArgs& a, uint32_t block, uint32_t blocks, RunScratch& sc) {
     const uint32_t tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     const uint32_t chunks = (a.requests + kThreads - 1) / kThreads;
     uint64_t mine = 0, end = 0, before = 0;
     auto chunk = [&](uint32_t c) {  // this thread's request's units, and the sum up to it
         const uint32_t r = c * kThreads + tid;
-        mine = request_units<M, WK>(a, r < a.requests ? request_at(a, r) : Request{0, 0, 0});
+        mine = request_units<M, WK, FIXED>(a, r < a.requests ? request_at(a, r) : Request{0, 0, 0});
         const uint64_t s = wave_scan(mine);
         __syncthreads();
         if (lane == 63) sc.sums[wave] = s;
@@ -174,7 +172,7 @@ __device__ Run find_run(const PagedAttnArgs& a, uint32_t block, uint32_t blocks,
     const Request q = request_at(a, run.r);
     for (uint32_t i = 0;; i += 64) {  // every wave by itself: the item that holds unit v
         const uint32_t m = (i + lane) * M;
-        const uint64_t s = wave_scan(m < q.vecs ? units_of<M, WK>(a, q, m).count : 0);
+        const uint64_t s = wave_scan(m < q.vecs ? units_of<M, WK, FIXED>(a, q, m).count : 0);
         const uint64_t past = __ballot(s > v);
         if (past || (i + 64) * M >= q.vecs) {
             const int at = past ? __builtin_ctzll(past) : 0;
@@ -185,6 +183,79 @@ __device__ Run find_run(const PagedAttnArgs& a, uint32_t block, uint32_t blocks,
         }
         v -= __shfl(s, 63, 64);
     }
+}
+
+// A block's way through its run: the item that it is at, and which of the
+// item's units are its own.
+template <int M, int WK, bool FIXED>
+struct Walk {
+    Run run;
+    Request req;
+    uint64_t start;  // global unit where the item starts
+    bool begun;      // the run starts inside the item
+    Units un;
+    uint32_t t0, t1;  // units of the item
+    bool cut;         // the run ends inside the item
+
+    __device__ __forceinline__ explicit Walk(const PagedAttnArgs& a, const Run& r) : run(r) {
+        req = request_at(a, run.r);
+        start = run.from - run.unit;
+        begun = run.unit > run.near;  // (a border near an item's start is its start)
+    }
+    __device__ __forceinline__ bool item(const PagedAttnArgs& a) {  // false: the run has ended
+        for (;; begun = false) {
+            while (run.m0 >= req.vecs) {  // the next item with vectors
+                run.m0 = 0;
+                if (req.vecs == 0 || ++run.kvh == a.kv_heads) {
+                    run.kvh = 0;
+                    if (++run.r == a.requests) return false;
+                    req = request_at(a, run.r);
+                }
+            }
+            un = units_of<M, WK, FIXED>(a, req, run.m0);
+            if (begun && un.count - run.unit <= run.near) {  // what is left of it is the last run's
+                next();
+                continue;
+            }
+            if (!begun && run.to <= start + min(run.near, un.count - 1)) return false;  // it is the next run's
+            t0 = begun ? run.unit : 0;
+            cut = run.to < start + un.count && start + un.count - run.to > run.near;
+            t1 = cut ? static_cast<uint32_t>(run.to - start) : un.count;
+            return true;
+        }
+    }
+    __device__ __forceinline__ void next() { start += un.count, run.m0 += M, begun = false; }
+    __device__ __forceinline__ uint32_t vecs() const { return min(static_cast<uint32_t>(M), req.vecs - run.m0); }
+    __device__ __forceinline__ bool whole() const { return t0 == 0 && t1 == un.count; }
+    // Borders inside the item, from near behind its start to near before its end: run first_border() - 1 has
+    // its first part (in its second slot), the runs from first_border() on the others (in their first).
+    __device__ __forceinline__ uint64_t first_border() const { return (start + run.near) / run.per + 1; }
+    __device__ __forceinline__ uint32_t parts() const {
+        return static_cast<uint32_t>((start + un.count - run.near - 1) / run.per - first_border()) + 2;
+    }
+};
+
+// Parts go through to memory (agent-scope stores and loads): other XCDs read them.
+__device__ __forceinline__ void publish(float* p, float x, float y) {
+    __hip_atomic_store(reinterpret_cast<uint64_t*>(p), static_cast<uint64_t>(__float_as_uint(y)) << 32 | __float_as_uint(x),
+                       __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+__device__ __forceinline__ float2 fetch(const float* p) {
+    const uint64_t w = __hip_atomic_load(reinterpret_cast<const uint64_t*>(p), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    return make_float2(__uint_as_float(static_cast<uint32_t>(w)), __uint_as_float(static_cast<uint32_t>(w >> 32)));
+}
+// Whether this block's part, which all its threads have published, is the item's last.
+__device__ __forceinline__ bool last_part(uint32_t* arrived, uint32_t n, uint32_t& shared) {
+    __builtin_amdgcn_s_waitcnt(0);  // this thread's stores are in memory
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        shared = __hip_atomic_fetch_add(arrived, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == n - 1;
+        if (shared) __hip_atomic_store(arrived, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);  // for the next call
+    }
+    __syncthreads();
+    if (!shared) return false;
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "agent");
+    return true;
 }
 
 // ---------------------------------------------------------------------------
@@ -227,6 +298,39 @@ __device__ __forceinline__ void split(float x, int e, typename K::T8 (&t)[K::TER
         t[i][e] = h;
         x -= static_cast<float>(h);
     }
+}
+
+// Maximum over the four lanes that hold a vector's scores (l % 16 alike).
+__device__ __forceinline__ float rows_max(float x) {
+    const auto a = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    const float y = fmaxf(__uint_as_float(a[0]), __uint_as_float(a[1]));
+    const auto b = __builtin_amdgcn_permlane32_swap(__float_as_uint(y), __float_as_uint(y), false, false);
+    return fmaxf(__uint_as_float(b[0]), __uint_as_float(b[1]));
+}
+
+// Terms of two neighbouring values. bf16: the first two by cutting off, so that
+// what is left is exact and one v_perm packs a pair, the last (8 bits are left)
+// by rounding.
+template <typename K>
+__device__ __forceinline__ void split2(float x, float y, int e, typename K::T8 (&t)[K::TERMS]) {
+    if constexpr (K::TERMS == 3) {
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            const uint32_t a = __float_as_uint(x), b = __float_as_uint(y);
+            u32x4 w = __builtin_bit_cast(u32x4, t[i]);
+            w[e / 2] = __builtin_amdgcn_perm(b, a, 0x07060302u);
+            t[i] = __builtin_bit_cast(typename K::T8, w);
+            x -= __uint_as_float(a & 0xffff0000u), y -= __uint_as_float(b & 0xffff0000u);
+        }
+        t[2][e] = static_cast<typename K::T>(x), t[2][e + 1] = static_cast<typename K::T>(y);
+    } else {
+        split<K>(x, e, t), split<K>(y, e + 1, t);
+    }
+}
+// The power of two that brings a row of q with this largest value below 2^13.
+__device__ __forceinline__ int f16_exponent(float top) {
+    const int ex = top > 0.f && top < INFINITY ? 13 - (ilogbf(top) + 1) : 0;
+    return min(max(ex, -120), 120);
 }
 
 // ---------------------------------------------------------------------------
@@ -295,14 +399,6 @@ __device__ __forceinline__ float value_at(const uint32_t* words, int i) {
     else return static_cast<float>(__builtin_bit_cast(_Float16, h));
 }
 
-// Maximum over the four lanes that hold a vector's scores (l % 16 alike).
-__device__ __forceinline__ float rows_max(float x) {
-    const auto a = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
-    const float y = fmaxf(__uint_as_float(a[0]), __uint_as_float(a[1]));
-    const auto b = __builtin_amdgcn_permlane32_swap(__float_as_uint(y), __float_as_uint(y), false, false);
-    return fmaxf(__uint_as_float(b[0]), __uint_as_float(b[1]));
-}
-
 template <int HD, int KIND, int GI>
 __global__ __launch_bounds__(kThreads, 2) void paged_attn_kernel(PagedAttnArgs a) {
     using F = Form<HD, KIND, GI>;
@@ -316,33 +412,17 @@ __global__ __launch_bounds__(kThreads, 2) void paged_attn_kernel(PagedAttnArgs a
     const uint32_t blocks = gridDim.x;
     // Neighbouring runs on one XCD (blocks go to the eight in turn): they share keys and table rows in its L2.
     const uint32_t block = blocks % 8 == 0 ? blockIdx.x % 8 * (blocks / 8) + blockIdx.x / 8 : blockIdx.x;
-    Run run = find_run<M, WK>(a, block, blocks, sc);
-    if (!run.any) return;
+    const Run from = find_run<M, WK, false>(a, block, blocks, sc);
+    if (!from.any) return;
     const int tid = threadIdx.x, lane = tid & 63, fr = lane & 15, fq = lane >> 4;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const uint64_t row_bytes = a.slot_stride * K::BYTES;
     const uint32_t slot_words = a.slot_vecs * (HD + 2);
-    Request req = request_at(a, run.r);
-    uint64_t start = run.from - run.unit;  // global unit where the item starts
-    bool begun = run.unit > run.near;      // the run starts inside the item (a border near its start is its start)
-    for (;; begun = false) {
-        while (run.m0 >= req.vecs) {  // the next item with vectors
-            run.m0 = 0;
-            if (req.vecs == 0 || ++run.kvh == a.kv_heads) {
-                run.kvh = 0;
-                if (++run.r == a.requests) return;
-                req = request_at(a, run.r);
-            }
-        }
-        const Units un = units_of<M, WK>(a, req, run.m0);
-        if (!begun && run.to <= start + min(run.near, un.count - 1)) return;  // the item is the next run's
-        if (begun && un.count - run.unit <= run.near) {    // what is left of it is the last run's
-            start += un.count, run.m0 += M;
-            continue;
-        }
-        const uint32_t t0 = begun ? run.unit : 0;
-        const bool cut = run.to < start + un.count && start + un.count - run.to > run.near;
-        const uint32_t t1 = cut ? static_cast<uint32_t>(run.to - start) : un.count;
+    for (Walk<M, WK, false> walk(a, from); walk.item(a); walk.next()) {
+        const Run& run = walk.run;
+        const Request& req = walk.req;
+        const Units& un = walk.un;
+        const uint32_t t0 = walk.t0, t1 = walk.t1;
         const uint32_t sets = 4u >> un.wide, UK = WK * sets;      // sets of waves with all of the item's vectors
         const uint32_t qw = wave & ((1u << un.wide) - 1), ks = wave >> un.wide;
         u32x4* const q_mine = reinterpret_cast<u32x4*>(shared) + qw * F::kQ + lane;  // (the sets write the same values)
@@ -381,9 +461,7 @@ __global__ __launch_bounds__(kThreads, 2) void paged_attn_kernel(PagedAttnArgs a
                     for (int e = 0; e < 8; ++e) x[s][e] *= f, top = fmaxf(top, fabsf(x[s][e]));
                 }
                 if constexpr (KIND == VVLI_CACHE_F16) {
-                    top = rows_max(top);
-                    int ex = top > 0.f && top < INFINITY ? 13 - (ilogbf(top) + 1) : 0;
-                    ex = min(max(ex, -120), 120);
+                    const int ex = f16_exponent(rows_max(top));
                     const float up = ldexpf(1.f, ex);
                     inv[gi] = ldexpf(1.f, -ex);
 #pragma unroll
@@ -395,7 +473,7 @@ __global__ __launch_bounds__(kThreads, 2) void paged_attn_kernel(PagedAttnArgs a
                 for (int s = 0; s < KL; ++s) {
                     typename K::T8 t[K::TERMS];
 #pragma unroll
-                    for (int e = 0; e < 8; ++e) split<K>(x[s][e], e, t);
+                    for (int e = 0; e < 8; e += 2) split2<K>(x[s][e], x[s][e + 1], e, t);
                     qf[gi][s] = __builtin_bit_cast(u32x4, t[0]);
 #pragma unroll
                     for (int i = 1; i < K::TERMS; ++i) q_mine[((gi * KL + s) * (K::TERMS - 1) + i - 1) * 64] = __builtin_bit_cast(u32x4, t[i]);
@@ -548,7 +626,7 @@ __global__ __launch_bounds__(kThreads, 2) void paged_attn_kernel(PagedAttnArgs a
 #pragma unroll
                         for (int u = 0; u < U; ++u)
 #pragma unroll
-                            for (int j = 0; j < 4; ++j) split<K>(s[gi][u][j], 4 * u + j, t8);
+                            for (int j = 0; j < 4; j += 2) split2<K>(s[gi][u][j], s[gi][u][j + 1], 4 * u + j, t8);
 #pragma unroll
                         for (int x = 0; x < K::TERMS; ++x) pf[gi][x] = __builtin_bit_cast(u32x4, t8[x]);
                     }
@@ -659,21 +737,13 @@ __global__ __launch_bounds__(kThreads, 2) void paged_attn_kernel(PagedAttnArgs a
             }
         }
         __syncthreads();
-        const bool whole = t0 == 0 && t1 == un.count;
-        const uint32_t vecs = min(static_cast<uint32_t>(M), req.vecs - run.m0);
+        const bool whole = walk.whole();
+        const uint32_t vecs = walk.vecs();
         auto write = [&](uint32_t v, uint32_t d, f32x4 x, float l) {
             const uint32_t m = run.m0 + v, row = page_of(a.group, m), g = m - row * a.group.d;
             float* op = a.out + (req.first + row) * a.ldo + (static_cast<size_t>(run.kvh) * a.group.d + g) * HD + d;
             const float r = 1.f / l;
             *reinterpret_cast<f32x4*>(op) = l == 0.f ? f32x4{0, 0, 0, 0} : x * r;
-        };
-        // Parts go through to memory (agent-scope stores and loads): other XCDs read them.
-        auto publish = [](float* p, float x, float y) {
-            __hip_atomic_store(reinterpret_cast<uint64_t*>(p), static_cast<uint64_t>(__float_as_uint(y)) << 32 | __float_as_uint(x), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-        };
-        auto fetch = [](const float* p) {
-            const uint64_t w = __hip_atomic_load(reinterpret_cast<const uint64_t*>(p), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-            return make_float2(__uint_as_float(static_cast<uint32_t>(w)), __uint_as_float(static_cast<uint32_t>(w >> 32)));
         };
         float* slot = a.parts + (2 * static_cast<size_t>(block) + (t0 == 0)) * slot_words;
         for (uint32_t i = tid; i < vecs * (HD / 4); i += kThreads) {
@@ -698,53 +768,415 @@ __global__ __launch_bounds__(kThreads, 2) void paged_attn_kernel(PagedAttnArgs a
             }
         }
         if (!whole) {
-            // Borders inside the item, from near behind its start to near before its end: run first_border - 1
-            // has its first part (in its second slot), the runs from first_border on the others (in their first).
-            const uint64_t first_border = (start + run.near) / run.per + 1;
-            const uint32_t n = static_cast<uint32_t>((start + un.count - run.near - 1) / run.per - first_border) + 2;
-            __builtin_amdgcn_s_waitcnt(0);  // this thread's stores are in memory
-            __syncthreads();
-            if (tid == 0) sc.last = __hip_atomic_fetch_add(a.arrived + first_border - 1, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == n - 1;
-            __syncthreads();
-            if (sc.last) {
-                __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "agent");
-                const float* first = a.parts + (2 * first_border - 1) * slot_words;
+            const uint32_t n = walk.parts();
+            const uint64_t border = walk.first_border();
+            if (last_part(a.arrived + border - 1, n, sc.last)) {
+                const float* first = a.parts + (2 * border - 1) * slot_words;
                 auto part_at = [&](uint32_t i) { return i == 0 ? first : first + (2 * static_cast<size_t>(i) - 1) * slot_words; };
                 for (uint32_t i = tid; i < vecs * (HD / 4); i += kThreads) {
                     const uint32_t v = i / (HD / 4), d = i % (HD / 4) * 4;
-                    float top = -INFINITY;
-                    for (uint32_t w = 0; w < n; ++w) top = fmaxf(top, fetch(part_at(w) + a.slot_vecs * HD + 2 * v).x);
-                    const float base = top == -INFINITY ? 0.f : top;
-                    float l = 0.f;
+                    float top = -INFINITY, l = 0.f;
                     f32x4 x = {0, 0, 0, 0};
-                    for (uint32_t w = 0; w < n; ++w) {
-                        const float* p = part_at(w);
-                        const float2 ml = fetch(p + a.slot_vecs * HD + 2 * v), x0 = fetch(p + v * HD + d), x1 = fetch(p + v * HD + d + 2);
-                        const float c = __builtin_amdgcn_exp2f(ml.x - base);
-                        l += ml.y * c;
-                        x += f32x4{x0.x, x0.y, x1.x, x1.y} * c;
+                    for (uint32_t w0 = 0; w0 < n; w0 += 8) {  // eight parts in flight
+                        float2 ml[8], x0[8], x1[8];
+#pragma unroll
+                        for (uint32_t w = 0; w < 8; ++w) {
+                            const float* p = part_at(min(w0 + w, n - 1));
+                            ml[w] = fetch(p + a.slot_vecs * HD + 2 * v), x0[w] = fetch(p + v * HD + d), x1[w] = fetch(p + v * HD + d + 2);
+                        }
+                        float more = top;
+#pragma unroll
+                        for (uint32_t w = 0; w < 8; ++w) more = fmaxf(more, ml[w].x);
+                        const float base = more == -INFINITY ? 0.f : more, old = __builtin_amdgcn_exp2f(top - base);
+                        top = more, l *= old, x *= old;
+#pragma unroll
+                        for (uint32_t w = 0; w < 8; ++w) {
+                            const float c = w0 + w < n ? __builtin_amdgcn_exp2f(ml[w].x - base) : 0.f;
+                            if (w0 + w < n) l += ml[w].y * c, x += f32x4{x0[w].x, x0[w].y, x1[w].x, x1[w].y} * c;
+                        }
                     }
                     write(v, d, x, l);
                 }
-                if (tid == 0) a.arrived[first_border - 1] = 0;  // for the next call
             }
-            if (cut) return;
+            if (walk.cut) return;
         }
         __syncthreads();
-        start += un.count;
-        run.m0 += M;
     }
 }
 
-// What a call runs: vectors of an item, blocks.
+// ---------------------------------------------------------------------------
+// Chunks over 16-bit caches: items of 128 vectors, 32 to a wave, and steps of 32
+// keys that the block's waves share through LDS (a wave's own loads of every
+// key would be bound by the vector cache: 16 KiB a step and wave). The block
+// loads the next step's keys and values into registers while it computes this
+// one, and stores them into the other of two stages behind it: one barrier a
+// step. Rows lie in LDS as in memory, their 16-byte chunks permuted by the row
+// so that the 16 rows of a fragment read fall on different banks; values are
+// read transposed (ds_read_b64_tr_b16: 4 keys of a lane's own dim), so tile n
+// of O^T is dims 16 n .. 16 n + 15.
+// ---------------------------------------------------------------------------
+template <int HD, int KIND>
+struct Wide {
+    using K = Kind<KIND>;
+    static constexpr int GI = 2, WV = 32, M = 128, WK = 32, NT = HD / 16, DS = HD / 32;
+    static constexpr int CH = HD / 8, RB = HD * 2, RPL = 256 / RB;  // 16-byte chunks and bytes of a row, rows of 256 bytes
+    static constexpr int TILE = WK * RB, LOADS = 2 * TILE / (16 * kThreads);
+    static constexpr int QR = 2;                                    // terms of q in registers; the rest in LDS
+    static constexpr int kQ = (K::TERMS - QR) * 4 * GI * DS * 1024;
+    static __device__ __forceinline__ uint32_t kswz(uint32_t r) { return r / RPL % CH; }
+    static __device__ __forceinline__ uint32_t vswz(uint32_t r) { return 2 * (r / RPL % (CH / 2)); }
+};
+
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+
+template <int HD, int KIND>
+__global__ __launch_bounds__(kThreads, 2) void paged_wide_kernel(PagedAttnArgs a) {
+    using F = Wide<HD, KIND>;
+    using K = Kind<KIND>;
+    using T8 = typename K::T8;
+    constexpr int GI = F::GI, WV = F::WV, M = F::M, WK = F::WK, NT = F::NT, DS = F::DS, CH = F::CH, RB = F::RB, TILE = F::TILE, LOADS = F::LOADS, QR = F::QR;
+    __shared__ RunScratch sc;
+    __shared__ __attribute__((aligned(1024))) char stage[2][2 * TILE];  // keys, then values
+    __shared__ __attribute__((aligned(16))) char raw[TILE];             // values as they are (careful steps)
+    __shared__ __attribute__((aligned(16))) char q_rest[F::kQ ? F::kQ : 16];
+
+    const uint32_t blocks = gridDim.x;
+    const uint32_t block = blocks % 8 == 0 ? blockIdx.x % 8 * (blocks / 8) + blockIdx.x / 8 : blockIdx.x;
+    const Run from = find_run<M, WK, true>(a, block, blocks, sc);
+    if (!from.any) return;
+    const int tid = threadIdx.x, lane = tid & 63, fr = lane & 15, fq = lane >> 4;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const uint64_t row_bytes = a.slot_stride * 2;
+    const uint32_t slot_words = a.slot_vecs * (HD + 2);
+    u32x4* const q_mine = reinterpret_cast<u32x4*>(q_rest) + wave * ((K::TERMS - QR) * GI * DS * 64) + lane;
+    // Where the lane's fragments lie in a stage: keys 16 u + fr, chunk 4 s + fq; values 16 u + 4 fq + fr / 4, dims
+    // 16 n + 4 (fr % 4).
+    const uint32_t k_at = fr * RB, k_x = F::kswz(fr);
+    const uint32_t v_row = 4 * fq + fr / 4, v_at = TILE + v_row * RB + (((fr / 2 % 2) ^ F::vswz(v_row)) << 4) + 8 * (fr & 1);
+
+    for (Walk<M, WK, true> walk(a, from); walk.item(a); walk.next()) {
+        const Run& run = walk.run;
+        const Request& req = walk.req;
+        const Units& un = walk.un;
+        const int32_t* table = a.table + static_cast<size_t>(run.r) * a.stride;
+        const char* kbase = static_cast<const char*>(a.k) + static_cast<size_t>(run.kvh) * RB;
+        const char* vbase = static_cast<const char*>(a.v) + static_cast<size_t>(run.kvh) * RB;
+
+        // The lane's vectors: their keys, rows and q.
+        const uint32_t wm0 = run.m0 + wave * WV;
+        KeySpan see[GI];
+        float inv[GI];
+        u32x4 qf[QR][GI][DS];
+#pragma unroll
+        for (int gi = 0; gi < GI; ++gi) {
+            const uint32_t m = wm0 + 16 * gi + fr;
+            const bool there = m < req.vecs;
+            const uint32_t row = page_of(a.group, there ? m : 0), g = (there ? m : 0) - row * a.group.d;
+            see[gi] = there ? key_span(req.start + row, a.window, a.room) : KeySpan{0, 0};
+            const float* qp = a.q + (req.first + row) * a.ldq + (static_cast<size_t>(run.kvh) * a.group.d + g) * HD;
+            const float f = a.scale * 1.44269504088896341f;
+            float x[DS][8];
+            float top = 0.f;
+#pragma unroll
+            for (int s = 0; s < DS; ++s) {
+                const float4 x0 = load_f32x4(qp + 32 * s + 8 * fq), x1 = load_f32x4(qp + 32 * s + 8 * fq + 4);
+                x[s][0] = x0.x, x[s][1] = x0.y, x[s][2] = x0.z, x[s][3] = x0.w, x[s][4] = x1.x, x[s][5] = x1.y, x[s][6] = x1.z, x[s][7] = x1.w;
+#pragma unroll
+                for (int e = 0; e < 8; ++e) x[s][e] *= f, top = fmaxf(top, fabsf(x[s][e]));
+            }
+            inv[gi] = 1.f;
+            if constexpr (KIND == VVLI_CACHE_F16) {
+                const int ex = f16_exponent(rows_max(top));
+                const float up = ldexpf(1.f, ex);
+                inv[gi] = ldexpf(1.f, -ex);
+#pragma unroll
+                for (int s = 0; s < DS; ++s)
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) x[s][e] *= up;
+            }
+#pragma unroll
+            for (int s = 0; s < DS; ++s) {
+                T8 t[K::TERMS];
+#pragma unroll
+                for (int e = 0; e < 8; e += 2) split2<K>(x[s][e], x[s][e + 1], e, t);
+#pragma unroll
+                for (int i = 0; i < K::TERMS; ++i) {
+                    if (i < QR) qf[i][gi][s] = __builtin_bit_cast(u32x4, t[i]);
+                    else q_mine[((i - QR) * GI * DS + gi * DS + s) * 64] = __builtin_bit_cast(u32x4, t[i]);
+                }
+            }
+        }
+        // Keys below w_hi are seen by some vector of the wave, all_lo .. all_hi - 1 by every one of them.
+        uint32_t w_lo = 0, w_hi = 0, all_lo = 0, all_hi = 0;
+        if (wm0 < req.vecs) {
+            const int64_t p0 = req.start + page_of(a.group, wm0), p1 = req.start + page_of(a.group, min(wm0 + WV, req.vecs) - 1);
+            const KeySpan s0 = key_span(p0, a.window, a.room), s1 = key_span(p1, a.window, a.room);
+            w_lo = a.window && p0 + 1 > a.window ? static_cast<uint32_t>(min(p0 + 1 - a.window, static_cast<int64_t>(a.room))) : 0;
+            w_hi = p1 < 0 ? 0 : static_cast<uint32_t>(min(p1 + 1, static_cast<int64_t>(a.room)));
+            all_lo = s1.lo, all_hi = min(s0.hi, s1.hi);
+        }
+        const uint32_t ta = un.first + walk.t0, tb = un.hi ? un.first + walk.t1 : 0;
+
+        f32x4 o[GI][NT];
+        float m_run[GI], l_run[GI];
+        auto slot_of = [&](uint32_t t) -> int32_t {
+            const uint32_t key = t * WK + (lane & (WK - 1));
+            return t < tb && key >= un.lo && key < un.hi ? page_slot(table, a.stride, a.pages, a.ps, key) : -1;
+        };
+        auto filled = [&](int32_t slot, uint32_t& none) -> uint32_t {
+            const uint64_t n = __ballot(slot < 0);
+            none = static_cast<uint32_t>(n);
+            const int32_t other = ~n ? __builtin_amdgcn_readlane(slot, __builtin_ctzll(~n)) : 0;
+            return slot < 0 ? other : slot;
+        };
+        u32x4 next[LOADS];
+        auto load = [&](uint32_t slots) {
+#pragma unroll
+            for (int i = 0; i < LOADS; ++i) {
+                const uint32_t x = tid + kThreads * i, y = x % (WK * CH), row = y / CH, c = y % CH;
+                const uint32_t s = __shfl(slots, row, 64);
+                const char* p = (x >= WK * CH ? vbase : kbase) + s * row_bytes + 16 * c;
+                uint32_t w[4];
+                load_words<4>(w, p);
+                next[i] = u32x4{w[0], w[1], w[2], w[3]};
+            }
+        };
+        auto store = [&](uint32_t st, bool careful) {
+#pragma unroll
+            for (int i = 0; i < LOADS; ++i) {
+                const uint32_t x = tid + kThreads * i, y = x % (WK * CH), row = y / CH, c = y % CH;
+                const bool v = x >= WK * CH;
+                if (careful && v) {
+                    *reinterpret_cast<u32x4*>(raw + row * RB + 16 * c) = next[i];
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) next[i][e] = word_finite<KIND>(next[i][e]);
+                }
+                *reinterpret_cast<u32x4*>(stage[st] + (v ? TILE : 0) + row * RB + ((c ^ (v ? F::vswz(row) : F::kswz(row))) << 4)) = next[i];
+            }
+        };
+        // Values that are not finite: as in the other kernel, but by blocks.
+        for (int careful = 0; careful < 2; ++careful) {
+#pragma unroll
+            for (int gi = 0; gi < GI; ++gi) {
+                m_run[gi] = -INFINITY, l_run[gi] = 0.f;
+#pragma unroll
+                for (int n = 0; n < NT; ++n) o[gi][n] = f32x4{0, 0, 0, 0};
+            }
+            if (ta >= tb) break;
+            uint32_t none, none_next;
+            uint32_t slots = filled(slot_of(ta), none);
+            int32_t ahead = slot_of(ta + 1);
+            load(slots);
+            store(0, careful);
+            __syncthreads();
+            uint32_t st = 0;
+            for (uint32_t t = ta; t < tb; ++t, st ^= 1) {
+                const uint32_t slots_next = filled(ahead, none_next);
+                if (t + 1 < tb) load(slots_next);
+                ahead = slot_of(t + 2);
+                const uint32_t key0 = t * WK;
+                if (key0 < w_hi && key0 + WK > w_lo) {
+                    const char* base = stage[st];
+                    f32x4 s[GI][2];
+#pragma unroll
+                    for (int gi = 0; gi < GI; ++gi) s[gi][0] = s[gi][1] = f32x4{0, 0, 0, 0};
+#pragma unroll
+                    for (int i = 0; i < DS; ++i) {
+                        T8 kf[2];
+#pragma unroll
+                        for (int u = 0; u < 2; ++u)
+                            kf[u] = __builtin_bit_cast(T8, *reinterpret_cast<const u32x4*>(base + k_at + 16 * u * RB + (((4 * i + fq) ^ k_x) << 4)));
+#pragma unroll
+                        for (int x = 0; x < K::TERMS; ++x)
+#pragma unroll
+                            for (int gi = 0; gi < GI; ++gi) {
+                                u32x4 qx;
+                                if (x < QR) qx = qf[x < QR ? x : 0][gi][i];
+                                else qx = q_mine[((x - QR) * GI * DS + gi * DS + i) * 64];
+#pragma unroll
+                                for (int u = 0; u < 2; ++u) s[gi][u] = K::mfma(kf[u], __builtin_bit_cast(T8, qx), s[gi][u]);
+                            }
+                    }
+                    if (key0 < all_lo || key0 + WK > all_hi || none) {
+#pragma unroll
+                        for (int u = 0; u < 2; ++u)
+#pragma unroll
+                            for (int j = 0; j < 4; ++j) {
+                                const uint32_t at = 16 * u + 4 * fq + j, key = key0 + at;
+                                const bool hole = none >> at & 1;
+#pragma unroll
+                                for (int gi = 0; gi < GI; ++gi)
+                                    if (hole || key < see[gi].lo || key >= see[gi].hi) s[gi][u][j] = -INFINITY;
+                            }
+                    }
+                    T8 pf[GI][K::TERMS];
+                    float corr[GI];
+                    bool grew = false;
+#pragma unroll
+                    for (int gi = 0; gi < GI; ++gi) {
+                        float mx = fmaxf(fmaxf(fmaxf(s[gi][0][0], s[gi][0][1]), fmaxf(s[gi][0][2], s[gi][0][3])),
+                                         fmaxf(fmaxf(s[gi][1][0], s[gi][1][1]), fmaxf(s[gi][1][2], s[gi][1][3])));
+                        const float m_new = fmaxf(m_run[gi], rows_max(mx) * inv[gi]);
+                        const float m_sub = m_new == -INFINITY ? 0.f : m_new;
+                        grew |= m_new != m_run[gi];
+                        corr[gi] = __builtin_amdgcn_exp2f(m_run[gi] - m_sub);
+                        float sum = 0.f;
+#pragma unroll
+                        for (int u = 0; u < 2; ++u)
+#pragma unroll
+                            for (int j = 0; j < 4; ++j) {
+                                s[gi][u][j] = __builtin_amdgcn_exp2f(fmaf(s[gi][u][j], inv[gi], K::PBIAS - m_sub));
+                                sum += s[gi][u][j];
+                            }
+#pragma unroll
+                        for (int u = 0; u < 2; ++u)
+#pragma unroll
+                            for (int j = 0; j < 4; j += 2) split2<K>(s[gi][u][j], s[gi][u][j + 1], 4 * u + j, pf[gi]);
+                        l_run[gi] = l_run[gi] * corr[gi] + sum;
+                        m_run[gi] = m_new;
+                    }
+                    if (__any(grew)) {
+#pragma unroll
+                        for (int gi = 0; gi < GI; ++gi)
+#pragma unroll
+                            for (int n = 0; n < NT; ++n) o[gi][n] *= corr[gi];
+                    }
+                    if (careful) {
+                        // The values that are not finite, for the vectors that see them: key 16 u + 4 f + j's
+                        // weights are with the lanes of fq = f.
+#pragma unroll
+                        for (int u = 0; u < 2; ++u)
+#pragma unroll
+                            for (int j = 0; j < 4; ++j)
+                                for (int f = 0; f < 4; ++f) {
+                                    const int at = 16 * u + 4 * f + j;
+                                    if (none >> at & 1) continue;
+                                    const uint32_t key = key0 + at;
+#pragma unroll
+                                    for (int gi = 0; gi < GI; ++gi) {
+                                        const bool sees = key >= see[gi].lo && key < see[gi].hi;
+                                        const float p = __shfl(s[gi][u][j], 16 * f + fr, 64);
+#pragma unroll
+                                        for (int n = 0; n < NT; ++n)
+#pragma unroll
+                                            for (int i = 0; i < 4; ++i) {
+                                                const float x = value_at<KIND>(reinterpret_cast<const uint32_t*>(raw + at * RB), 16 * n + 4 * fq + i);
+                                                if (sees && !(fabsf(x) < INFINITY)) o[gi][n][i] += p * x;
+                                            }
+                                    }
+                                }
+                    }
+#pragma unroll
+                    for (int n = 0; n < NT; ++n) {
+                        u32x4 w;
+#pragma unroll
+                        for (int u = 0; u < 2; ++u) {
+                            const s16x4 v = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                                (__attribute__((address_space(3))) s16x4*)(base + ((v_at ^ (32 * n)) + 16 * u * RB)));
+                            const uint2 d = __builtin_bit_cast(uint2, v);
+                            w[2 * u] = d.x, w[2 * u + 1] = d.y;
+                        }
+#pragma unroll
+                        for (int x = 0; x < K::TERMS; ++x)
+#pragma unroll
+                            for (int gi = 0; gi < GI; ++gi) o[gi][n] = K::mfma(__builtin_bit_cast(T8, w), pf[gi][x], o[gi][n]);
+                    }
+                }
+                if (careful) __syncthreads();  // (the values as they are have one place)
+                if (t + 1 < tb) store(st ^ 1, careful);
+                none = none_next;
+                __syncthreads();
+            }
+            float sum = 0.f;  // NaN if one of them is not finite
+#pragma unroll
+            for (int gi = 0; gi < GI; ++gi)
+#pragma unroll
+                for (int n = 0; n < NT; ++n)
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) sum = fmaf(o[gi][n][j], 0.f, sum);
+            if (!__syncthreads_or(sum != sum)) break;
+        }
+
+#pragma unroll
+        for (int gi = 0; gi < GI; ++gi) {
+            l_run[gi] += __shfl_xor(l_run[gi], 16, 64);
+            l_run[gi] += __shfl_xor(l_run[gi], 32, 64);
+        }
+        // Lane l has dims 16 n + 4 (l / 16) .. + 3 of its vectors.
+        auto write = [&]() {
+#pragma unroll
+            for (int gi = 0; gi < GI; ++gi) {
+                const uint32_t m = wm0 + 16 * gi + fr;
+                if (m >= req.vecs) continue;
+                const uint32_t row = page_of(a.group, m), g = m - row * a.group.d;
+                float* op = a.out + (req.first + row) * a.ldo + (static_cast<size_t>(run.kvh) * a.group.d + g) * HD + 4 * fq;
+                const float r = 1.f / l_run[gi];
+#pragma unroll
+                for (int n = 0; n < NT; ++n) *reinterpret_cast<f32x4*>(op + 16 * n) = l_run[gi] == 0.f ? f32x4{0, 0, 0, 0} : o[gi][n] * r;
+            }
+        };
+        if (walk.whole()) {
+            write();
+            continue;
+        }
+        float* slot = a.parts + (2 * static_cast<size_t>(block) + (walk.t0 == 0)) * slot_words;
+#pragma unroll
+        for (int gi = 0; gi < GI; ++gi) {
+            const uint32_t v = wave * WV + 16 * gi + fr;
+            if (run.m0 + v >= req.vecs) continue;
+#pragma unroll
+            for (int n = 0; n < NT; ++n) {
+                publish(slot + v * HD + 16 * n + 4 * fq, o[gi][n][0], o[gi][n][1]);
+                publish(slot + v * HD + 16 * n + 4 * fq + 2, o[gi][n][2], o[gi][n][3]);
+            }
+            if (fq == 0) publish(slot + a.slot_vecs * HD + 2 * v, m_run[gi], l_run[gi]);
+        }
+        const uint32_t parts = walk.parts();
+        const uint64_t border = walk.first_border();
+        if (last_part(a.arrived + border - 1, parts, sc.last)) {
+            const float* first = a.parts + (2 * border - 1) * slot_words;
+#pragma unroll
+            for (int gi = 0; gi < GI; ++gi) {
+                m_run[gi] = -INFINITY, l_run[gi] = 0.f;
+#pragma unroll
+                for (int n = 0; n < NT; ++n) o[gi][n] = f32x4{0, 0, 0, 0};
+            }
+            for (uint32_t w = 0; w < parts; ++w) {
+                const float* p = w == 0 ? first : first + (2 * static_cast<size_t>(w) - 1) * slot_words;
+#pragma unroll
+                for (int gi = 0; gi < GI; ++gi) {
+                    const uint32_t v = min(wave * WV + 16 * gi + fr, a.slot_vecs - 1);
+                    const float2 ml = fetch(p + a.slot_vecs * HD + 2 * v);
+                    float2 x[NT][2];
+#pragma unroll
+                    for (int n = 0; n < NT; ++n) x[n][0] = fetch(p + v * HD + 16 * n + 4 * fq), x[n][1] = fetch(p + v * HD + 16 * n + 4 * fq + 2);
+                    const float m_new = fmaxf(m_run[gi], ml.x), base = m_new == -INFINITY ? 0.f : m_new;
+                    const float c0 = __builtin_amdgcn_exp2f(m_run[gi] - base), c1 = __builtin_amdgcn_exp2f(ml.x - base);
+                    m_run[gi] = m_new, l_run[gi] = l_run[gi] * c0 + ml.y * c1;
+#pragma unroll
+                    for (int n = 0; n < NT; ++n) o[gi][n] = o[gi][n] * c0 + f32x4{x[n][0].x, x[n][0].y, x[n][1].x, x[n][1].y} * c1;
+                }
+            }
+            write();
+        }
+        if (walk.cut) return;
+    }
+}
+
+// What a call runs: the kernel (groups of 16 vectors to a wave; wide: chunks), an item's vectors, blocks.
 struct Plan {
     uint32_t m, blocks;
+    int groups;
+    bool wide;
 };
 constexpr uint32_t kBlocksPerCu = 2;
 
-Plan plan_of(uint32_t rows, uint32_t requests, uint32_t group) {
+Plan plan_of(uint32_t rows, uint32_t requests, uint32_t group, uint32_t kind) {
     const uint64_t vecs = static_cast<uint64_t>(rows) * group;
-    return Plan{vecs <= VVLI_X * requests ? 64u : 128u, gemm_cus() * kBlocksPerCu};
+    const uint32_t blocks = gemm_cus() * kBlocksPerCu;
+    if (vecs > uint64_t{48} * requests && kind != VVLI_CACHE_F32) return Plan{128, blocks, 2, true};
+    if (vecs > uint64_t{16} * requests) return Plan{128, blocks, 2, false};
+    return Plan{64, blocks, 1, false};
 }
 
 // An item's most vectors, and the bytes of a call's workspace: counters, then two slots of such an item for each block.
@@ -761,7 +1193,9 @@ bool sizes_ok(uint32_t rows, uint32_t requests, uint32_t heads, uint32_t kv_head
 template <int HD, int KIND>
 hipError_t launch(const PagedAttnArgs& a, const Plan& p, hipStream_t s) {
     const dim3 grid(p.blocks), block(kThreads);
-    return p.m == 64 ? vlaunch(paged_attn_kernel<HD, KIND, 1>, grid, block, 0, s, a) : vlaunch(paged_attn_kernel<HD, KIND, 2>, grid, block, 0, s, a);
+    if constexpr (KIND != VVLI_CACHE_F32)
+        if (p.wide) return vlaunch(paged_wide_kernel<HD, KIND>, grid, block, 0, s, a);
+    return p.groups == 1 ? vlaunch(paged_attn_kernel<HD, KIND, 1>, grid, block, 0, s, a) : vlaunch(paged_attn_kernel<HD, KIND, 2>, grid, block, 0, s, a);
 }
 
 template <int HD>
@@ -776,7 +1210,7 @@ extern "C" {
 size_t vvli_gpu_paged_attention_workspace(uint32_t rows, uint32_t requests, uint32_t heads, uint32_t kv_heads,
                                           uint32_t head_dim) {
     if (!sizes_ok(rows, requests, heads, kv_heads) || (head_dim != 32 && head_dim != 64 && head_dim != 128)) return 0;
-    const Plan p = plan_of(rows, 1, heads / kv_heads);  // (of however few requests)
+    const Plan p = plan_of(rows, 1, heads / kv_heads, VVLI_CACHE_F32);  // (of however few requests)
     return plan_bytes(p.blocks, slot_vecs(p.m, rows, heads / kv_heads), head_dim);
 }
 
@@ -801,7 +1235,7 @@ int vvli_gpu_paged_attention(const vvli_gpu_paged_cache* cache, const int32_t* t
     if (q == out) return set_error(VVLI_INVALID_CONFIG, "%s: out is q", who);
     if (rows == 0) return VVLI_OK;
     const uint32_t group = heads / cache->kv_heads;
-    const Plan p = plan_of(rows, requests, group);
+    const Plan p = plan_of(rows, requests, group, cache->kind);
     PagedAttnArgs a{};
     a.k = cache->k, a.v = cache->v, a.table = table, a.row_start = row_start, a.start_pos = start_pos, a.q = q, a.out = out;
     a.arrived = static_cast<uint32_t*>(workspace);

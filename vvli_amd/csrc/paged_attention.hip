@@ -30,11 +30,14 @@ namespace {
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef float f32x16 __attribute__((ext_vector_type(16)));
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 
 constexpr int kThreads = 256;
-// Fewest units of a run: a shorter one costs more at its ends than it saves.
-constexpr uint32_t kFewestUnits = 4;
+// What an item costs beside its keys (its q, the first loads, its end), in
+// units; the fewest units of a run; the most units of an item that is never
+// cut, since its parts would cost more than they save.
+constexpr uint32_t kItemUnits = 3, kFewestUnits = 5, kWholeUnits = 12;
 
 struct PagedAttnArgs {
     const void *k, *v;
@@ -66,8 +69,7 @@ __device__ __forceinline__ Request request_at(const PagedAttnArgs& a, uint32_t r
 // waves side by side (the log of that in `wide`) take different vectors, and
 // the 4 >> wide such sets take steps of WK positions in turn, (4 WK) >> wide a
 // unit. The keys lo .. hi - 1 that some vector of the item sees (hi = 0: none),
-// and the units that they touch; an item without keys counts one, in which its
-// zeros are written.
+// and the units that they touch, behind kItemUnits for the item itself.
 struct Units {
     uint32_t lo, hi, first, count, wide;
 };
@@ -80,10 +82,10 @@ __device__ __forceinline__ Units units_of(const PagedAttnArgs& a, const Request&
     const int64_t p1 = q.start + page_of(a.group, m0 + vecs - 1);
     const int64_t hi = min(p1 + 1, static_cast<int64_t>(a.room));
     const int64_t lo = a.window && p0 + 1 > a.window ? p0 + 1 - a.window : 0;
-    if (hi <= lo) return Units{0, 0, 0, 1, wide};
+    if (hi <= lo) return Units{0, 0, 0, kItemUnits, wide};
     const uint32_t unit = FIXED ? WK : (4 * WK) >> wide;
     Units u{static_cast<uint32_t>(lo), static_cast<uint32_t>(hi), static_cast<uint32_t>(lo) / unit, 0, wide};
-    u.count = (u.hi + unit - 1) / unit - u.first;
+    u.count = (u.hi + unit - 1) / unit - u.first + kItemUnits;
     return u;
 }
 
@@ -118,13 +120,19 @@ __device__ __forceinline__ uint64_t request_units(const PagedAttnArgs& a, const 
 }
 
 // Run b holds the units from per * b on to per * (b + 1), but that a border
-// within `near` units of an item's start or end moves there (near < per / 2, so
-// that borders keep their order): fewer items are cut.
+// within near_lo units of an item's start (anywhere in one of few units) or
+// near_hi of its end moves there (near_lo + near_hi < per, so that borders keep
+// their order): fewer items are cut, and none before its first keys.
 struct Run {
     uint64_t from, to, per;  // global units, before the borders move
-    uint32_t near, r, kvh, m0, unit;  // the item that holds unit `from`, and which unit of it that is
+    uint32_t near_lo, near_hi, r, kvh, m0, unit;  // the item that holds unit `from`, and which unit of it that is
     bool any;
 };
+
+// (64-bit division is some 150 instructions; sums of units are mostly below 2^32.)
+__device__ __forceinline__ uint64_t quotient(uint64_t n, uint64_t d) {
+    return ((n | d) >> 32) == 0 ? static_cast<uint32_t>(n) / static_cast<uint32_t>(d) : n / d;
+}
 
 struct RunScratch {
     uint64_t sums[kThreads / 64], found_rest, found_units;
@@ -152,8 +160,10 @@ __device__ Run find_run(const PagedAttnArgs& a, uint32_t block, uint32_t blocks,
     for (uint32_t c = 0; c < chunks; ++c) chunk(c);
     const uint64_t total = before * a.kv_heads;
     Run run{};
-    run.per = max((total + blocks - 1) / blocks, static_cast<uint64_t>(kFewestUnits));
-    run.near = static_cast<uint32_t>(min(run.per / 4, static_cast<uint64_t>(1u << 20)));
+    run.per = max(quotient(total + blocks - 1, blocks), static_cast<uint64_t>(kFewestUnits));
+    run.near_hi = static_cast<uint32_t>(min(run.per / 4, static_cast<uint64_t>(1u << 20)));
+    run.near_lo = max(run.near_hi, kItemUnits);
+    static_assert(kItemUnits + kFewestUnits / 4 < kFewestUnits, "near_lo + near_hi < per");
     run.from = run.per * block;
     run.to = run.from + run.per >= total ? ~uint64_t{0} : run.from + run.per;
     if (run.from >= total) return run;
@@ -167,8 +177,8 @@ __device__ Run find_run(const PagedAttnArgs& a, uint32_t block, uint32_t blocks,
     __syncthreads();
     run.r = __builtin_amdgcn_readfirstlane(sc.found_r);
     const uint64_t rest = sc.found_rest, units = sc.found_units;
-    run.kvh = __builtin_amdgcn_readfirstlane(static_cast<uint32_t>(rest / units));
-    uint64_t v = rest % units;
+    run.kvh = __builtin_amdgcn_readfirstlane(static_cast<uint32_t>(quotient(rest, units)));
+    uint64_t v = rest - run.kvh * units;
     const Request q = request_at(a, run.r);
     for (uint32_t i = 0;; i += 64) {  // every wave by itself: the item that holds unit v
         const uint32_t m = (i + lane) * M;
@@ -195,12 +205,14 @@ struct Walk {
     bool begun;      // the run starts inside the item
     Units un;
     uint32_t t0, t1;  // units of the item
+    __device__ __forceinline__ uint32_t first_unit() const { return un.first + (t0 > kItemUnits ? t0 - kItemUnits : 0); }  // of its keys
+    __device__ __forceinline__ uint32_t end_unit() const { return un.first + (t1 > kItemUnits ? t1 - kItemUnits : 0); }
     bool cut;         // the run ends inside the item
 
     __device__ __forceinline__ explicit Walk(const PagedAttnArgs& a, const Run& r) : run(r) {
         req = request_at(a, run.r);
         start = run.from - run.unit;
-        begun = run.unit > run.near;  // (a border near an item's start is its start)
+        begun = true;
     }
     __device__ __forceinline__ bool item(const PagedAttnArgs& a) {  // false: the run has ended
         for (;; begun = false) {
@@ -213,13 +225,15 @@ struct Walk {
                 }
             }
             un = units_of<M, WK, FIXED>(a, req, run.m0);
-            if (begun && un.count - run.unit <= run.near) {  // what is left of it is the last run's
+            const uint32_t lo = un.count <= kWholeUnits ? un.count - 1 : run.near_lo;
+            begun = begun && run.unit > lo;  // (a border near an item's start is its start)
+            if (begun && un.count - run.unit <= run.near_hi) {  // what is left of it is the last run's
                 next();
                 continue;
             }
-            if (!begun && run.to <= start + min(run.near, un.count - 1)) return false;  // it is the next run's
+            if (!begun && run.to <= start + min(lo, un.count - 1)) return false;  // it is the next run's
             t0 = begun ? run.unit : 0;
-            cut = run.to < start + un.count && start + un.count - run.to > run.near;
+            cut = run.to < start + un.count && start + un.count - run.to > run.near_hi;
             t1 = cut ? static_cast<uint32_t>(run.to - start) : un.count;
             return true;
         }
@@ -227,11 +241,11 @@ struct Walk {
     __device__ __forceinline__ void next() { start += un.count, run.m0 += M, begun = false; }
     __device__ __forceinline__ uint32_t vecs() const { return min(static_cast<uint32_t>(M), req.vecs - run.m0); }
     __device__ __forceinline__ bool whole() const { return t0 == 0 && t1 == un.count; }
-    // Borders inside the item, from near behind its start to near before its end: run first_border() - 1 has
+    // Borders inside the item, from near_lo behind its start to near_hi before its end: run first_border() - 1 has
     // its first part (in its second slot), the runs from first_border() on the others (in their first).
-    __device__ __forceinline__ uint64_t first_border() const { return (start + run.near) / run.per + 1; }
+    __device__ __forceinline__ uint64_t first_border() const { return quotient(start + run.near_lo, run.per) + 1; }
     __device__ __forceinline__ uint32_t parts() const {
-        return static_cast<uint32_t>((start + un.count - run.near - 1) / run.per - first_border()) + 2;
+        return static_cast<uint32_t>(quotient(start + un.count - run.near_hi - 1, run.per) - first_border()) + 2;
     }
 };
 
@@ -265,8 +279,8 @@ __device__ __forceinline__ bool last_part(uint32_t* arrived, uint32_t n, uint32_
 // has 11, so two hold 22 (the rest, 2^-22 of x at most and half of that on
 // average, is what rounding a product to f32 leaves too). f16 has few
 // exponents: q is scaled by a power of two to below 2^13 (and the scores back),
-// and p to 2^13 at most by the exponent of its own maximum, so that second
-// terms stay clear of the subnormals; 2^13 times f16's largest value times
+// and p to 2^13 at most, so that what the smallest second terms lose is far
+// below a rounding of the largest first; 2^13 times f16's largest value times
 // the number of keys stays far below f32's end. An f32 cache goes through
 // 16x16x4 products of f32.
 // ---------------------------------------------------------------------------
@@ -281,13 +295,15 @@ template <> struct Kind<VVLI_CACHE_BF16> {
     typedef __bf16 T;
     typedef bf16x8 T8;
     static __device__ __forceinline__ f32x4 mfma(T8 x, T8 y, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_bf16(x, y, c, 0, 0, 0); }
+    static __device__ __forceinline__ f32x16 mfma(T8 x, T8 y, f32x16 c) { return __builtin_amdgcn_mfma_f32_32x32x16_bf16(x, y, c, 0, 0, 0); }
 };
 template <> struct Kind<VVLI_CACHE_F16> {
     static constexpr int TERMS = 2, BYTES = 2, U = 2;
-    static constexpr float PBIAS = 13.f;
+    static constexpr float PBIAS = 5.f;
     typedef _Float16 T;
     typedef f16x8 T8;
     static __device__ __forceinline__ f32x4 mfma(T8 x, T8 y, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_f16(x, y, c, 0, 0, 0); }
+    static __device__ __forceinline__ f32x16 mfma(T8 x, T8 y, f32x16 c) { return __builtin_amdgcn_mfma_f32_32x32x16_f16(x, y, c, 0, 0, 0); }
 };
 
 template <typename K>
@@ -365,8 +381,6 @@ struct Form {
     static constexpr int ROW = HD + 4, kWave = WV * (ROW + 2);
     static constexpr int kQ = GI * KL * (K::TERMS - 1) * 64;         // of a wave, in 16-byte units
     static constexpr int kShared = std::max(4 * kWave, 4 * 4 * kQ);  // 32-bit words
-    // Four keys' values and weights of a wave (values that are not finite).
-    static constexpr int kOddV = HD * K::BYTES / 4, kOdd = 4 * (kOddV + 16 * GI);
 };
 
 template <int W>
@@ -399,15 +413,38 @@ __device__ __forceinline__ float value_at(const uint32_t* words, int i) {
     else return static_cast<float>(__builtin_bit_cast(_Float16, h));
 }
 
+// A value that is not finite spoils its dimension of every vector of an item,
+// also of those that do not see its key (0 times it is NaN) and, through split
+// terms of either sign, an infinity of those that do. That shows in the
+// outputs, so no step looks for it: where outputs are not finite, the keys are
+// gone over once more with such values taken as 0, and then they go straight
+// to the outputs of the vectors that see them, whose sums they are whatever
+// their weights. add(at, row) takes key `at` of a step of WK whose values
+// hold one; `slots` as in filled().
+template <int HD, int KIND, int WK, typename Add>
+__device__ __forceinline__ void odd_values(const char* vbase, uint64_t row_bytes, uint32_t slots, uint64_t none, Add&& add) {
+    constexpr int CHUNKS = HD * Kind<KIND>::BYTES / 16;
+    static_assert(WK * CHUNKS % 64 == 0, "whole waves");
+    bool odd = false;
+    for (uint32_t i = threadIdx.x & 63; i < WK * CHUNKS; i += 64) {
+        uint32_t w[4];
+        load_words<4>(w, vbase + static_cast<uint32_t>(__shfl(slots, i / CHUNKS, 64)) * row_bytes + i % CHUNKS * 16);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) odd |= word_finite<KIND>(w[e]) != w[e];
+    }
+    if (!__any(odd)) return;
+    for (int at = 0; at < WK; ++at)
+        if (!(none >> at & 1)) add(at, reinterpret_cast<const uint32_t*>(vbase + static_cast<uint32_t>(__shfl(slots, at, 64)) * row_bytes));
+}
+
 template <int HD, int KIND, int GI>
-__global__ __launch_bounds__(kThreads, 2) void paged_attn_kernel(PagedAttnArgs a) {
+__global__ __launch_bounds__(kThreads, HD == 128 ? 2 : 3) void paged_attn_kernel(PagedAttnArgs a) {
     using F = Form<HD, KIND, GI>;
     using K = Kind<KIND>;
     constexpr int M = F::M, WV = F::WV, U = F::U, WK = F::WK, DV = F::DV, KL = F::KL, VW = F::VW, ROW = F::ROW;
     constexpr bool F32 = KIND == VVLI_CACHE_F32;
     __shared__ RunScratch sc;
     __shared__ __attribute__((aligned(16))) float shared[F::kShared];
-    __shared__ uint32_t odd[4][F::kOdd];
 
     const uint32_t blocks = gridDim.x;
     // Neighbouring runs on one XCD (blocks go to the eight in turn): they share keys and table rows in its L2.
@@ -422,7 +459,7 @@ __global__ __launch_bounds__(kThreads, 2) void paged_attn_kernel(PagedAttnArgs a
         const Run& run = walk.run;
         const Request& req = walk.req;
         const Units& un = walk.un;
-        const uint32_t t0 = walk.t0, t1 = walk.t1;
+        const uint32_t t0 = walk.t0;
         const uint32_t sets = 4u >> un.wide, UK = WK * sets;      // sets of waves with all of the item's vectors
         const uint32_t qw = wave & ((1u << un.wide) - 1), ks = wave >> un.wide;
         u32x4* const q_mine = reinterpret_cast<u32x4*>(shared) + qw * F::kQ + lane;  // (the sets write the same values)
@@ -430,8 +467,67 @@ __global__ __launch_bounds__(kThreads, 2) void paged_attn_kernel(PagedAttnArgs a
         const char* kbase = static_cast<const char*>(a.k) + static_cast<size_t>(run.kvh) * HD * K::BYTES + 16 * fq;
         const char* vbase = static_cast<const char*>(a.v) + static_cast<size_t>(run.kvh) * HD * K::BYTES + 4 * VW * fr;
 
-        // The lane's vectors: their keys and q.
+        // The first step's keys and values are on their way before q is taken apart.
         const uint32_t wm0 = run.m0 + qw * WV;  // the wave's first vector
+        // Keys w_lo .. w_hi - 1 are seen by some vector of the wave, all_lo .. all_hi - 1 by
+        // every one of them (no test needed there).
+        uint32_t w_lo = 0, w_hi = 0, all_lo = 0, all_hi = 0;
+        if (wm0 < req.vecs) {
+            const int64_t p0 = req.start + page_of(a.group, wm0), p1 = req.start + page_of(a.group, min(wm0 + WV, req.vecs) - 1);
+            const KeySpan s0 = key_span(p0, a.window, a.room), s1 = key_span(p1, a.window, a.room);
+            w_lo = max(un.lo, a.window && p0 + 1 > a.window ? static_cast<uint32_t>(min(p0 + 1 - a.window, static_cast<int64_t>(a.room))) : 0);
+            w_hi = p1 < 0 ? 0 : static_cast<uint32_t>(min(p1 + 1, static_cast<int64_t>(a.room)));
+            all_lo = s1.lo, all_hi = min(s0.hi, s1.hi);
+        }
+        // The wave's steps: those units of the run whose WK keys from t * UK + ks * WK on meet w_lo .. w_hi - 1.
+        uint32_t ta = walk.first_unit(), tb = walk.end_unit();
+        if (w_lo >= (ks + 1) * WK) ta = max(ta, (w_lo - (ks + 1) * WK) / UK + 1);
+        tb = w_lo < w_hi && w_hi > ks * WK ? min(tb, (w_hi - ks * WK + UK - 1) / UK) : 0;
+
+        f32x4 o[GI][DV];
+        float m_run[GI], l_run[GI];
+
+        // Slot of key t * UK + ks * WK + lane (of WK lanes), -1 where no vector of the wave sees it.
+        auto slot_of = [&](uint32_t t) -> int32_t {
+            const uint32_t key = t * UK + ks * WK + (lane & (WK - 1));
+            return t < tb && key >= w_lo && key < w_hi ? page_slot(table, a.stride, a.pages, a.ps, key) : -1;
+        };
+        // Slots that there are none of read another key of the step, whose score is then not used: they
+        // need neither a test at every load nor memory of their own.
+        auto filled = [&](int32_t slot, uint64_t& none) -> uint32_t {
+            none = __ballot(slot < 0);
+            const int32_t other = ~none ? __builtin_amdgcn_readlane(slot, __builtin_ctzll(~none)) : 0;
+            return slot < 0 ? other : slot;
+        };
+        typename F::Step st;
+        auto load_k = [&](uint32_t slots) {
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                const uint32_t s = __shfl(slots, 16 * u + fr, 64);
+                const char* p = kbase + s * row_bytes;
+#pragma unroll
+                for (int i = 0; i < KL; ++i) {
+                    uint32_t w[4];
+                    load_words<4>(w, p + 64 * i);
+                    st.k[u][i] = u32x4{w[0], w[1], w[2], w[3]};
+                }
+            }
+        };
+        auto load_v = [&](uint32_t slots) {
+#pragma unroll
+            for (int u = 0; u < U; ++u)
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    const uint32_t s = __shfl(slots, 16 * u + 4 * fq + j, 64);
+                    load_words<VW>(st.v[u][j], vbase + s * row_bytes);
+                }
+        };
+        uint64_t none;
+        uint32_t slots = filled(slot_of(ta), none);
+        int32_t ahead = slot_of(ta + 1);
+        if (ta < tb) load_k(slots), load_v(slots);
+
+        // The lane's vectors: their keys and q.
         KeySpan see[GI];
         float inv[GI];  // scores are this times the products (f16's power of two)
         u32x4 qf[GI][KL];
@@ -480,63 +576,7 @@ __global__ __launch_bounds__(kThreads, 2) void paged_attn_kernel(PagedAttnArgs a
                 }
             }
         }
-        // Keys w_lo .. w_hi - 1 are seen by some vector of the wave, all_lo .. all_hi - 1 by
-        // every one of them (no test needed there).
-        uint32_t w_lo = 0, w_hi = 0, all_lo = 0, all_hi = 0;
-        if (wm0 < req.vecs) {
-            const int64_t p0 = req.start + page_of(a.group, wm0), p1 = req.start + page_of(a.group, min(wm0 + WV, req.vecs) - 1);
-            const KeySpan s0 = key_span(p0, a.window, a.room), s1 = key_span(p1, a.window, a.room);
-            w_lo = max(un.lo, a.window && p0 + 1 > a.window ? static_cast<uint32_t>(min(p0 + 1 - a.window, static_cast<int64_t>(a.room))) : 0);
-            w_hi = p1 < 0 ? 0 : static_cast<uint32_t>(min(p1 + 1, static_cast<int64_t>(a.room)));
-            all_lo = s1.lo, all_hi = min(s0.hi, s1.hi);
-        }
-        // The wave's steps: those units of the run whose WK keys from t * UK + ks * WK on meet w_lo .. w_hi - 1.
-        uint32_t ta = un.first + t0, tb = un.first + t1;
-        if (w_lo >= (ks + 1) * WK) ta = max(ta, (w_lo - (ks + 1) * WK) / UK + 1);
-        tb = w_lo < w_hi && w_hi > ks * WK ? min(tb, (w_hi - ks * WK + UK - 1) / UK) : 0;
-
-        f32x4 o[GI][DV];
-        float m_run[GI], l_run[GI];
-
-        // Slot of key t * UK + ks * WK + lane (of WK lanes), -1 where no vector of the wave sees it.
-        auto slot_of = [&](uint32_t t) -> int32_t {
-            const uint32_t key = t * UK + ks * WK + (lane & (WK - 1));
-            return t < tb && key >= w_lo && key < w_hi ? page_slot(table, a.stride, a.pages, a.ps, key) : -1;
-        };
-        // Slots that there are none of read another key of the step, whose score is then not used: they
-        // need neither a test at every load nor memory of their own.
-        auto filled = [&](int32_t slot, uint64_t& none) -> uint32_t {
-            none = __ballot(slot < 0);
-            const int32_t other = ~none ? __builtin_amdgcn_readlane(slot, __builtin_ctzll(~none)) : 0;
-            return slot < 0 ? other : slot;
-        };
-        typename F::Step st;
-        auto load_k = [&](uint32_t slots) {
-#pragma unroll
-            for (int u = 0; u < U; ++u) {
-                const uint32_t s = __shfl(slots, 16 * u + fr, 64);
-                const char* p = kbase + s * row_bytes;
-#pragma unroll
-                for (int i = 0; i < KL; ++i) {
-                    uint32_t w[4];
-                    load_words<4>(w, p + 64 * i);
-                    st.k[u][i] = u32x4{w[0], w[1], w[2], w[3]};
-                }
-            }
-        };
-        auto load_v = [&](uint32_t slots) {
-#pragma unroll
-            for (int u = 0; u < U; ++u)
-#pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    const uint32_t s = __shfl(slots, 16 * u + 4 * fq + j, 64);
-                    load_words<VW>(st.v[u][j], vbase + s * row_bytes);
-                }
-        };
-        // A value that is not finite spoils its dimension of every vector of the item, also of those that
-        // do not see its key (0 times it is NaN) and, through split terms of either sign, an infinity of
-        // those that do. That shows in the outputs, so no step looks for it: where outputs are not
-        // finite, the wave goes over its keys once more, with care.
+        bool spoilt = false;
         for (int careful = 0; careful < 2; ++careful) {
 #pragma unroll
             for (int gi = 0; gi < GI; ++gi) {
@@ -545,15 +585,25 @@ __global__ __launch_bounds__(kThreads, 2) void paged_attn_kernel(PagedAttnArgs a
                 for (int e = 0; e < DV; ++e) o[gi][e] = f32x4{0, 0, 0, 0};
             }
             if (ta >= tb) break;
-            uint64_t none, none_next;
-            uint32_t slots = filled(slot_of(ta), none), slots_next;
-            int32_t ahead = slot_of(ta + 1);
-            load_k(slots);
-            load_v(slots);
+            uint64_t none_next;
+            uint32_t slots_next;
+            if (careful) {
+                slots = filled(slot_of(ta), none), ahead = slot_of(ta + 1);
+                load_k(slots);
+                load_v(slots);
+            }
             for (uint32_t t = ta; t < tb; ++t) {
                 slots_next = filled(ahead, none_next);
                 ahead = slot_of(t + 2);
                 const uint32_t key0 = t * UK + ks * WK;
+                if (careful) {
+#pragma unroll
+                    for (int u = 0; u < U; ++u)
+#pragma unroll
+                        for (int j = 0; j < 4; ++j)
+#pragma unroll
+                            for (int i = 0; i < VW; ++i) st.v[u][j][i] = word_finite<KIND>(st.v[u][j][i]);
+                }
                 f32x4 s[GI][U];
 #pragma unroll
                 for (int gi = 0; gi < GI; ++gi)
@@ -639,45 +689,6 @@ __global__ __launch_bounds__(kThreads, 2) void paged_attn_kernel(PagedAttnArgs a
 #pragma unroll
                         for (int e = 0; e < DV; ++e) o[gi][e] *= corr[gi];
                 }
-                if (careful) {
-                    // Values that are not finite leave the products and are added for the vectors that
-                    // see them, the four keys 16 u + 4 (l / 16) + j of the lanes at a time.
-                    uint32_t* odd_v = odd[wave];
-                    float* odd_p = reinterpret_cast<float*>(odd[wave] + 4 * F::kOddV);
-#pragma unroll
-                    for (int u = 0; u < U; ++u)
-#pragma unroll
-                        for (int j = 0; j < 4; ++j) {
-#pragma unroll
-                            for (int i = 0; i < VW; ++i)
-                                odd_v[fq * F::kOddV + fr * VW + i] = st.v[u][j][i], st.v[u][j][i] = word_finite<KIND>(st.v[u][j][i]);
-#pragma unroll
-                            for (int gi = 0; gi < GI; ++gi) odd_p[fq * WV + 16 * gi + fr] = s[gi][u][j];
-                            __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup");
-                            __builtin_amdgcn_wave_barrier();
-                            __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup");
-                            for (int f = 0; f < 4; ++f) {
-                                const int at = 16 * u + 4 * f + j;
-                                if (none >> at & 1) continue;  // (no vector sees it)
-                                const uint32_t key = key0 + at;
-#pragma unroll
-                                for (int gi = 0; gi < GI; ++gi) {
-                                    const bool sees = key >= see[gi].lo && key < see[gi].hi;
-                                    const float p = odd_p[f * WV + 16 * gi + fr];
-#pragma unroll
-                                    for (int e = 0; e < DV; ++e)
-#pragma unroll
-                                        for (int i = 0; i < 4; ++i) {
-                                            const float x = value_at<KIND>(odd_v + f * F::kOddV, DV * (4 * fq + i) + e);
-                                            if (sees && !(fabsf(x) < INFINITY)) o[gi][e][i] += p * x;
-                                        }
-                                }
-                            }
-                            __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup");
-                            __builtin_amdgcn_wave_barrier();
-                            __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup");
-                        }
-                }
 #pragma unroll
                 for (int e = 0; e < DV; ++e) {
                     if constexpr (F32) {
@@ -712,8 +723,31 @@ __global__ __launch_bounds__(kThreads, 2) void paged_attn_kernel(PagedAttnArgs a
                 for (int e = 0; e < DV; ++e)
 #pragma unroll
                     for (int j = 0; j < 4; ++j) sum = fmaf(o[gi][e][j], 0.f, sum);
-            if (!__any(sum != sum)) break;
+            if (careful) {
+                spoilt = true;
+            } else if (!__any(sum != sum)) {  // see odd_values
+                break;
+            }
         }
+        if (spoilt)
+            for (uint32_t t = ta; t < tb; ++t) {
+                uint64_t none;
+                const uint32_t slots = filled(slot_of(t), none);
+                odd_values<HD, KIND, WK>(vbase - 4 * VW * fr, row_bytes, slots, none, [&](int at, const uint32_t* p) {
+                    const uint32_t key = t * UK + ks * WK + at;
+#pragma unroll
+                    for (int gi = 0; gi < GI; ++gi) {
+                        const bool sees = key >= see[gi].lo && key < see[gi].hi;
+#pragma unroll
+                        for (int e = 0; e < DV; ++e)
+#pragma unroll
+                            for (int j = 0; j < 4; ++j) {
+                                const float x = value_at<KIND>(p, DV * (4 * fq + j) + e);
+                                if (sees && !(fabsf(x) < INFINITY)) o[gi][e][j] += x;
+                            }
+                    }
+                });
+            }
 
         // The waves' parts: outputs [WV][HD], maxima, sums.
         __syncthreads();  // (q's terms are read)
@@ -807,25 +841,34 @@ __global__ __launch_bounds__(kThreads, 2) void paged_attn_kernel(PagedAttnArgs a
 // ---------------------------------------------------------------------------
 // Chunks over 16-bit caches: items of 128 vectors, 32 to a wave, and steps of 32
 // keys that the block's waves share through LDS (a wave's own loads of every
-// key would be bound by the vector cache: 16 KiB a step and wave). The block
-// loads the next step's keys and values into registers while it computes this
-// one, and stores them into the other of two stages behind it: one barrier a
-// step. Rows lie in LDS as in memory, their 16-byte chunks permuted by the row
-// so that the 16 rows of a fragment read fall on different banks; values are
-// read transposed (ds_read_b64_tr_b16: 4 keys of a lane's own dim), so tile n
-// of O^T is dims 16 n .. 16 n + 15.
+// key would be 16 KiB a step and wave). The block loads the next step's keys
+// and values into registers while it computes this one, and stores them into
+// the other of two stages behind it: one barrier a step. Products are
+// 32 x 32 x 16, a lane l with vector l % 32:
+//   S^T = K Q^T    A: key l % 32, dims 16 s + 8 (l / 32) .. + 7; D: register r
+//                  has key 8 (r / 4) + 4 (l / 32) + r % 4
+//   O^T += V^T P^T B: registers 8 c .. 8 c + 7 of the weights are step c's 8
+//                  values of k, as they stand; A: dim 32 n + l % 32, the same
+//                  keys, 4 at a time by a transposed read of LDS
+//                  (ds_read_b64_tr_b16); D: dims 32 n + 8 (r / 4) + 4 (l / 32) + r % 4
+// Rows lie in LDS as in memory, their 16-byte chunks permuted by the row so that
+// the rows of a fragment read fall on different banks.
 // ---------------------------------------------------------------------------
 template <int HD, int KIND>
 struct Wide {
     using K = Kind<KIND>;
-    static constexpr int GI = 2, WV = 32, M = 128, WK = 32, NT = HD / 16, DS = HD / 32;
+    static constexpr int WV = 32, M = 128, WK = 32, NT = HD / 32, DS = HD / 16;
     static constexpr int CH = HD / 8, RB = HD * 2, RPL = 256 / RB;  // 16-byte chunks and bytes of a row, rows of 256 bytes
-    static constexpr int TILE = WK * RB, LOADS = 2 * TILE / (16 * kThreads);
+    static constexpr int TILE = WK * RB, LOADS = 2 * TILE / (16 * kThreads), ROWS = LOADS > 1 ? LOADS / 2 : 1;
     static constexpr int QR = 2;                                    // terms of q in registers; the rest in LDS
-    static constexpr int kQ = (K::TERMS - QR) * 4 * GI * DS * 1024;
+    static constexpr int kQ = (K::TERMS - QR) * 4 * DS * 1024;
     static __device__ __forceinline__ uint32_t kswz(uint32_t r) { return r / RPL % CH; }
-    static __device__ __forceinline__ uint32_t vswz(uint32_t r) { return 2 * (r / RPL % (CH / 2)); }
+    static __device__ __forceinline__ uint32_t vswz(uint32_t r) { return 4 * (r / RPL % (CH / 4)); }
 };
+// A vector's weights are 2^(s - base) with a base that follows the maximum of
+// its scores only where that is more than this above it: weights stay in range,
+// and few steps have outputs to rescale.
+constexpr float kSlack = 8.f;
 
 typedef short s16x4 __attribute__((ext_vector_type(4)));
 
@@ -834,25 +877,27 @@ __global__ __launch_bounds__(kThreads, 2) void paged_wide_kernel(PagedAttnArgs a
     using F = Wide<HD, KIND>;
     using K = Kind<KIND>;
     using T8 = typename K::T8;
-    constexpr int GI = F::GI, WV = F::WV, M = F::M, WK = F::WK, NT = F::NT, DS = F::DS, CH = F::CH, RB = F::RB, TILE = F::TILE, LOADS = F::LOADS, QR = F::QR;
+    constexpr int WV = F::WV, M = F::M, WK = F::WK, NT = F::NT, DS = F::DS, CH = F::CH, RB = F::RB, TILE = F::TILE;
+    constexpr int LOADS = F::LOADS, ROWS = F::ROWS, QR = F::QR;
     __shared__ RunScratch sc;
     __shared__ __attribute__((aligned(1024))) char stage[2][2 * TILE];  // keys, then values
-    __shared__ __attribute__((aligned(16))) char raw[TILE];             // values as they are (careful steps)
     __shared__ __attribute__((aligned(16))) char q_rest[F::kQ ? F::kQ : 16];
 
     const uint32_t blocks = gridDim.x;
     const uint32_t block = blocks % 8 == 0 ? blockIdx.x % 8 * (blocks / 8) + blockIdx.x / 8 : blockIdx.x;
     const Run from = find_run<M, WK, true>(a, block, blocks, sc);
     if (!from.any) return;
-    const int tid = threadIdx.x, lane = tid & 63, fr = lane & 15, fq = lane >> 4;
+    const int tid = threadIdx.x, lane = tid & 63, fr = lane & 31, half = lane >> 5;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const uint64_t row_bytes = a.slot_stride * 2;
     const uint32_t slot_words = a.slot_vecs * (HD + 2);
-    u32x4* const q_mine = reinterpret_cast<u32x4*>(q_rest) + wave * ((K::TERMS - QR) * GI * DS * 64) + lane;
-    // Where the lane's fragments lie in a stage: keys 16 u + fr, chunk 4 s + fq; values 16 u + 4 fq + fr / 4, dims
-    // 16 n + 4 (fr % 4).
-    const uint32_t k_at = fr * RB, k_x = F::kswz(fr);
-    const uint32_t v_row = 4 * fq + fr / 4, v_at = TILE + v_row * RB + (((fr / 2 % 2) ^ F::vswz(v_row)) << 4) + 8 * (fr & 1);
+    u32x4* const q_mine = reinterpret_cast<u32x4*>(q_rest) + wave * ((K::TERMS - QR) * DS * 64) + lane;
+    // Where the lane's fragments lie in a stage (products' step s and tile n are put in by ^ and +).
+    const uint32_t k_at = fr * RB + ((half ^ F::kswz(fr)) << 4);
+    const uint32_t v_row = 4 * half + (lane & 15) / 4;
+    const uint32_t v_at = TILE + v_row * RB + (((2 * (lane / 16 % 2) + lane / 2 % 2) ^ F::vswz(v_row)) << 4) + 8 * (lane & 1);
+    // This thread's rows of a step (the same of keys and of values; HD = 32: of one of the two) and its chunk.
+    const uint32_t my_row = tid % (WK * CH / ROWS) / CH, my_c = tid % CH;
 
     for (Walk<M, WK, true> walk(a, from); walk.item(a); walk.next()) {
         const Run& run = walk.run;
@@ -862,33 +907,30 @@ __global__ __launch_bounds__(kThreads, 2) void paged_wide_kernel(PagedAttnArgs a
         const char* kbase = static_cast<const char*>(a.k) + static_cast<size_t>(run.kvh) * RB;
         const char* vbase = static_cast<const char*>(a.v) + static_cast<size_t>(run.kvh) * RB;
 
-        // The lane's vectors: their keys, rows and q.
-        const uint32_t wm0 = run.m0 + wave * WV;
-        KeySpan see[GI];
-        float inv[GI];
-        u32x4 qf[QR][GI][DS];
-#pragma unroll
-        for (int gi = 0; gi < GI; ++gi) {
-            const uint32_t m = wm0 + 16 * gi + fr;
-            const bool there = m < req.vecs;
-            const uint32_t row = page_of(a.group, there ? m : 0), g = (there ? m : 0) - row * a.group.d;
-            see[gi] = there ? key_span(req.start + row, a.window, a.room) : KeySpan{0, 0};
-            const float* qp = a.q + (req.first + row) * a.ldq + (static_cast<size_t>(run.kvh) * a.group.d + g) * HD;
+        // The lane's vector: its keys and q.
+        const uint32_t wm0 = run.m0 + wave * WV, m = wm0 + fr;
+        const bool there = m < req.vecs;
+        const uint32_t row = page_of(a.group, there ? m : 0);
+        const KeySpan see = there ? key_span(req.start + row, a.window, a.room) : KeySpan{0, 0};
+        const size_t head = (static_cast<size_t>(run.kvh) * a.group.d + (there ? m : 0) - row * a.group.d) * HD;
+        float inv = 1.f;
+        u32x4 qf[QR][DS];
+        {
+            const float* qp = a.q + (req.first + row) * a.ldq + head + 8 * half;
             const float f = a.scale * 1.44269504088896341f;
             float x[DS][8];
             float top = 0.f;
 #pragma unroll
             for (int s = 0; s < DS; ++s) {
-                const float4 x0 = load_f32x4(qp + 32 * s + 8 * fq), x1 = load_f32x4(qp + 32 * s + 8 * fq + 4);
+                const float4 x0 = load_f32x4(qp + 16 * s), x1 = load_f32x4(qp + 16 * s + 4);
                 x[s][0] = x0.x, x[s][1] = x0.y, x[s][2] = x0.z, x[s][3] = x0.w, x[s][4] = x1.x, x[s][5] = x1.y, x[s][6] = x1.z, x[s][7] = x1.w;
 #pragma unroll
                 for (int e = 0; e < 8; ++e) x[s][e] *= f, top = fmaxf(top, fabsf(x[s][e]));
             }
-            inv[gi] = 1.f;
             if constexpr (KIND == VVLI_CACHE_F16) {
-                const int ex = f16_exponent(rows_max(top));
+                const int ex = f16_exponent(fmaxf(top, __shfl_xor(top, 32, 64)));
                 const float up = ldexpf(1.f, ex);
-                inv[gi] = ldexpf(1.f, -ex);
+                inv = ldexpf(1.f, -ex);
 #pragma unroll
                 for (int s = 0; s < DS; ++s)
 #pragma unroll
@@ -901,12 +943,12 @@ __global__ __launch_bounds__(kThreads, 2) void paged_wide_kernel(PagedAttnArgs a
                 for (int e = 0; e < 8; e += 2) split2<K>(x[s][e], x[s][e + 1], e, t);
 #pragma unroll
                 for (int i = 0; i < K::TERMS; ++i) {
-                    if (i < QR) qf[i][gi][s] = __builtin_bit_cast(u32x4, t[i]);
-                    else q_mine[((i - QR) * GI * DS + gi * DS + s) * 64] = __builtin_bit_cast(u32x4, t[i]);
+                    if (i < QR) qf[i < QR ? i : 0][s] = __builtin_bit_cast(u32x4, t[i]);
+                    else q_mine[((i - QR) * DS + s) * 64] = __builtin_bit_cast(u32x4, t[i]);
                 }
             }
         }
-        // Keys below w_hi are seen by some vector of the wave, all_lo .. all_hi - 1 by every one of them.
+        // Keys w_lo .. w_hi - 1 are seen by some vector of the wave, all_lo .. all_hi - 1 by every one of them.
         uint32_t w_lo = 0, w_hi = 0, all_lo = 0, all_hi = 0;
         if (wm0 < req.vecs) {
             const int64_t p0 = req.start + page_of(a.group, wm0), p1 = req.start + page_of(a.group, min(wm0 + WV, req.vecs) - 1);
@@ -915,12 +957,12 @@ __global__ __launch_bounds__(kThreads, 2) void paged_wide_kernel(PagedAttnArgs a
             w_hi = p1 < 0 ? 0 : static_cast<uint32_t>(min(p1 + 1, static_cast<int64_t>(a.room)));
             all_lo = s1.lo, all_hi = min(s0.hi, s1.hi);
         }
-        const uint32_t ta = un.first + walk.t0, tb = un.hi ? un.first + walk.t1 : 0;
+        const uint32_t ta = walk.first_unit(), tb = un.hi ? walk.end_unit() : 0;
 
-        f32x4 o[GI][NT];
-        float m_run[GI], l_run[GI];
+        f32x16 o[NT];
+        float m_run, l_run, shift;  // base of the weights (-inf: none yet), their sum, what is added to scores
         auto slot_of = [&](uint32_t t) -> int32_t {
-            const uint32_t key = t * WK + (lane & (WK - 1));
+            const uint32_t key = t * WK + fr;
             return t < tb && key >= un.lo && key < un.hi ? page_slot(table, a.stride, a.pages, a.ps, key) : -1;
         };
         auto filled = [&](int32_t slot, uint32_t& none) -> uint32_t {
@@ -932,36 +974,38 @@ __global__ __launch_bounds__(kThreads, 2) void paged_wide_kernel(PagedAttnArgs a
         u32x4 next[LOADS];
         auto load = [&](uint32_t slots) {
 #pragma unroll
-            for (int i = 0; i < LOADS; ++i) {
-                const uint32_t x = tid + kThreads * i, y = x % (WK * CH), row = y / CH, c = y % CH;
-                const uint32_t s = __shfl(slots, row, 64);
-                const char* p = (x >= WK * CH ? vbase : kbase) + s * row_bytes + 16 * c;
-                uint32_t w[4];
-                load_words<4>(w, p);
-                next[i] = u32x4{w[0], w[1], w[2], w[3]};
+            for (int r = 0; r < ROWS; ++r) {
+                const uint64_t at = static_cast<uint32_t>(__shfl(slots, my_row + WK / ROWS * r, 64)) * row_bytes + 16 * my_c;
+#pragma unroll
+                for (int v = 0; v < LOADS / ROWS; ++v) {
+                    uint32_t w[4];
+                    load_words<4>(w, (LOADS == 1 ? (tid >= WK * CH ? vbase : kbase) : v ? vbase : kbase) + at);
+                    next[ROWS * v + r] = u32x4{w[0], w[1], w[2], w[3]};
+                }
             }
         };
         auto store = [&](uint32_t st, bool careful) {
 #pragma unroll
-            for (int i = 0; i < LOADS; ++i) {
-                const uint32_t x = tid + kThreads * i, y = x % (WK * CH), row = y / CH, c = y % CH;
-                const bool v = x >= WK * CH;
-                if (careful && v) {
-                    *reinterpret_cast<u32x4*>(raw + row * RB + 16 * c) = next[i];
+            for (int r = 0; r < ROWS; ++r)
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) next[i][e] = word_finite<KIND>(next[i][e]);
+                for (int v = 0; v < LOADS / ROWS; ++v) {
+                    const uint32_t rw = my_row + WK / ROWS * r;
+                    const bool val = LOADS == 1 ? tid >= WK * CH : v;
+                    u32x4& x = next[ROWS * v + r];
+                    if (careful && val) {
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) x[e] = word_finite<KIND>(x[e]);
+                    }
+                    *reinterpret_cast<u32x4*>(stage[st] + (val ? TILE : 0) + rw * RB + ((my_c ^ (val ? F::vswz(rw) : F::kswz(rw))) << 4)) = x;
                 }
-                *reinterpret_cast<u32x4*>(stage[st] + (v ? TILE : 0) + row * RB + ((c ^ (v ? F::vswz(row) : F::kswz(row))) << 4)) = next[i];
-            }
         };
-        // Values that are not finite: as in the other kernel, but by blocks.
+        bool spoilt = false;
         for (int careful = 0; careful < 2; ++careful) {
+            m_run = -INFINITY, l_run = 0.f, shift = K::PBIAS;
 #pragma unroll
-            for (int gi = 0; gi < GI; ++gi) {
-                m_run[gi] = -INFINITY, l_run[gi] = 0.f;
+            for (int n = 0; n < NT; ++n)
 #pragma unroll
-                for (int n = 0; n < NT; ++n) o[gi][n] = f32x4{0, 0, 0, 0};
-            }
+                for (int r = 0; r < 16; ++r) o[n][r] = 0.f;
             if (ta >= tb) break;
             uint32_t none, none_next;
             uint32_t slots = filled(slot_of(ta), none);
@@ -977,185 +1021,148 @@ __global__ __launch_bounds__(kThreads, 2) void paged_wide_kernel(PagedAttnArgs a
                 const uint32_t key0 = t * WK;
                 if (key0 < w_hi && key0 + WK > w_lo) {
                     const char* base = stage[st];
-                    f32x4 s[GI][2];
+                    f32x16 s;
 #pragma unroll
-                    for (int gi = 0; gi < GI; ++gi) s[gi][0] = s[gi][1] = f32x4{0, 0, 0, 0};
+                    for (int r = 0; r < 16; ++r) s[r] = 0.f;
 #pragma unroll
                     for (int i = 0; i < DS; ++i) {
-                        T8 kf[2];
+                        const T8 kf = __builtin_bit_cast(T8, *reinterpret_cast<const u32x4*>(base + (k_at ^ (32 * i))));
 #pragma unroll
-                        for (int u = 0; u < 2; ++u)
-                            kf[u] = __builtin_bit_cast(T8, *reinterpret_cast<const u32x4*>(base + k_at + 16 * u * RB + (((4 * i + fq) ^ k_x) << 4)));
-#pragma unroll
-                        for (int x = 0; x < K::TERMS; ++x)
-#pragma unroll
-                            for (int gi = 0; gi < GI; ++gi) {
-                                u32x4 qx;
-                                if (x < QR) qx = qf[x < QR ? x : 0][gi][i];
-                                else qx = q_mine[((x - QR) * GI * DS + gi * DS + i) * 64];
-#pragma unroll
-                                for (int u = 0; u < 2; ++u) s[gi][u] = K::mfma(kf[u], __builtin_bit_cast(T8, qx), s[gi][u]);
-                            }
+                        for (int x = 0; x < K::TERMS; ++x) {
+                            u32x4 qx;
+                            if (x < QR) qx = qf[x < QR ? x : 0][i];
+                            else qx = q_mine[((x - QR) * DS + i) * 64];
+                            s = K::mfma(kf, __builtin_bit_cast(T8, qx), s);
+                        }
                     }
                     if (key0 < all_lo || key0 + WK > all_hi || none) {
 #pragma unroll
-                        for (int u = 0; u < 2; ++u)
-#pragma unroll
-                            for (int j = 0; j < 4; ++j) {
-                                const uint32_t at = 16 * u + 4 * fq + j, key = key0 + at;
-                                const bool hole = none >> at & 1;
-#pragma unroll
-                                for (int gi = 0; gi < GI; ++gi)
-                                    if (hole || key < see[gi].lo || key >= see[gi].hi) s[gi][u][j] = -INFINITY;
-                            }
-                    }
-                    T8 pf[GI][K::TERMS];
-                    float corr[GI];
-                    bool grew = false;
-#pragma unroll
-                    for (int gi = 0; gi < GI; ++gi) {
-                        float mx = fmaxf(fmaxf(fmaxf(s[gi][0][0], s[gi][0][1]), fmaxf(s[gi][0][2], s[gi][0][3])),
-                                         fmaxf(fmaxf(s[gi][1][0], s[gi][1][1]), fmaxf(s[gi][1][2], s[gi][1][3])));
-                        const float m_new = fmaxf(m_run[gi], rows_max(mx) * inv[gi]);
-                        const float m_sub = m_new == -INFINITY ? 0.f : m_new;
-                        grew |= m_new != m_run[gi];
-                        corr[gi] = __builtin_amdgcn_exp2f(m_run[gi] - m_sub);
-                        float sum = 0.f;
-#pragma unroll
-                        for (int u = 0; u < 2; ++u)
-#pragma unroll
-                            for (int j = 0; j < 4; ++j) {
-                                s[gi][u][j] = __builtin_amdgcn_exp2f(fmaf(s[gi][u][j], inv[gi], K::PBIAS - m_sub));
-                                sum += s[gi][u][j];
-                            }
-#pragma unroll
-                        for (int u = 0; u < 2; ++u)
-#pragma unroll
-                            for (int j = 0; j < 4; j += 2) split2<K>(s[gi][u][j], s[gi][u][j + 1], 4 * u + j, pf[gi]);
-                        l_run[gi] = l_run[gi] * corr[gi] + sum;
-                        m_run[gi] = m_new;
-                    }
-                    if (__any(grew)) {
-#pragma unroll
-                        for (int gi = 0; gi < GI; ++gi)
-#pragma unroll
-                            for (int n = 0; n < NT; ++n) o[gi][n] *= corr[gi];
-                    }
-                    if (careful) {
-                        // The values that are not finite, for the vectors that see them: key 16 u + 4 f + j's
-                        // weights are with the lanes of fq = f.
-#pragma unroll
-                        for (int u = 0; u < 2; ++u)
-#pragma unroll
-                            for (int j = 0; j < 4; ++j)
-                                for (int f = 0; f < 4; ++f) {
-                                    const int at = 16 * u + 4 * f + j;
-                                    if (none >> at & 1) continue;
-                                    const uint32_t key = key0 + at;
-#pragma unroll
-                                    for (int gi = 0; gi < GI; ++gi) {
-                                        const bool sees = key >= see[gi].lo && key < see[gi].hi;
-                                        const float p = __shfl(s[gi][u][j], 16 * f + fr, 64);
-#pragma unroll
-                                        for (int n = 0; n < NT; ++n)
-#pragma unroll
-                                            for (int i = 0; i < 4; ++i) {
-                                                const float x = value_at<KIND>(reinterpret_cast<const uint32_t*>(raw + at * RB), 16 * n + 4 * fq + i);
-                                                if (sees && !(fabsf(x) < INFINITY)) o[gi][n][i] += p * x;
-                                            }
-                                    }
-                                }
-                    }
-#pragma unroll
-                    for (int n = 0; n < NT; ++n) {
-                        u32x4 w;
-#pragma unroll
-                        for (int u = 0; u < 2; ++u) {
-                            const s16x4 v = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-                                (__attribute__((address_space(3))) s16x4*)(base + ((v_at ^ (32 * n)) + 16 * u * RB)));
-                            const uint2 d = __builtin_bit_cast(uint2, v);
-                            w[2 * u] = d.x, w[2 * u + 1] = d.y;
+                        for (int r = 0; r < 16; ++r) {
+                            const uint32_t at = 8 * (r / 4) + 4 * half + r % 4, key = key0 + at;
+                            if ((none >> at & 1) || key < see.lo || key >= see.hi) s[r] = -INFINITY;
                         }
-#pragma unroll
-                        for (int x = 0; x < K::TERMS; ++x)
-#pragma unroll
-                            for (int gi = 0; gi < GI; ++gi) o[gi][n] = K::mfma(__builtin_bit_cast(T8, w), pf[gi][x], o[gi][n]);
                     }
+                    float mx = fmaxf(s[0], s[1]);
+#pragma unroll
+                    for (int r = 2; r < 16; ++r) mx = fmaxf(mx, s[r]);
+                    const auto sw = __builtin_amdgcn_permlane32_swap(__float_as_uint(mx), __float_as_uint(mx), false, false);
+                    mx = fmaxf(__uint_as_float(sw[0]), __uint_as_float(sw[1])) * inv;
+                    const bool grew = mx > m_run + kSlack;
+                    if (__any(grew)) {
+                        const float m_new = grew ? mx : m_run, m_sub = m_new == -INFINITY ? 0.f : m_new;
+                        const float corr = __builtin_amdgcn_exp2f(m_run - m_sub);
+                        m_run = m_new, shift = K::PBIAS - m_sub, l_run *= corr;
+#pragma unroll
+                        for (int n = 0; n < NT; ++n) o[n] *= corr;
+                    }
+                    T8 pf[2][K::TERMS];
+                    float sum[2] = {0.f, 0.f};
+#pragma unroll
+                    for (int c = 0; c < 2; ++c)
+#pragma unroll
+                        for (int e = 0; e < 8; e += 2) {
+                            const float p0 = __builtin_amdgcn_exp2f(fmaf(s[8 * c + e], inv, shift)), p1 = __builtin_amdgcn_exp2f(fmaf(s[8 * c + e + 1], inv, shift));
+                            sum[0] += p0, sum[1] += p1;
+                            split2<K>(p0, p1, e, pf[c]);
+                        }
+                    l_run += sum[0] + sum[1];
+#pragma unroll
+                    for (int n = 0; n < NT; ++n)
+#pragma unroll
+                        for (int c = 0; c < 2; ++c) {
+                            u32x4 w;
+#pragma unroll
+                            for (int h = 0; h < 2; ++h) {
+                                const s16x4 v = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                                    (__attribute__((address_space(3))) s16x4*)(base + ((v_at ^ (64 * n)) + (16 * c + 8 * h) * RB)));
+                                const uint2 d = __builtin_bit_cast(uint2, v);
+                                w[2 * h] = d.x, w[2 * h + 1] = d.y;
+                            }
+#pragma unroll
+                            for (int x = 0; x < K::TERMS; ++x) o[n] = K::mfma(__builtin_bit_cast(T8, w), pf[c][x], o[n]);
+                        }
                 }
-                if (careful) __syncthreads();  // (the values as they are have one place)
                 if (t + 1 < tb) store(st ^ 1, careful);
                 none = none_next;
                 __syncthreads();
             }
             float sum = 0.f;  // NaN if one of them is not finite
 #pragma unroll
-            for (int gi = 0; gi < GI; ++gi)
+            for (int n = 0; n < NT; ++n)
 #pragma unroll
-                for (int n = 0; n < NT; ++n)
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) sum = fmaf(o[gi][n][j], 0.f, sum);
-            if (!__syncthreads_or(sum != sum)) break;
-        }
-
-#pragma unroll
-        for (int gi = 0; gi < GI; ++gi) {
-            l_run[gi] += __shfl_xor(l_run[gi], 16, 64);
-            l_run[gi] += __shfl_xor(l_run[gi], 32, 64);
-        }
-        // Lane l has dims 16 n + 4 (l / 16) .. + 3 of its vectors.
-        auto write = [&]() {
-#pragma unroll
-            for (int gi = 0; gi < GI; ++gi) {
-                const uint32_t m = wm0 + 16 * gi + fr;
-                if (m >= req.vecs) continue;
-                const uint32_t row = page_of(a.group, m), g = m - row * a.group.d;
-                float* op = a.out + (req.first + row) * a.ldo + (static_cast<size_t>(run.kvh) * a.group.d + g) * HD + 4 * fq;
-                const float r = 1.f / l_run[gi];
-#pragma unroll
-                for (int n = 0; n < NT; ++n) *reinterpret_cast<f32x4*>(op + 16 * n) = l_run[gi] == 0.f ? f32x4{0, 0, 0, 0} : o[gi][n] * r;
+                for (int r = 0; r < 16; ++r) sum = fmaf(o[n][r], 0.f, sum);
+            if (careful) {
+                spoilt = true;
+            } else if (!__syncthreads_or(sum != sum)) {  // see odd_values
+                break;
             }
+        }
+        if (spoilt)
+            for (uint32_t t = max(ta, w_lo / WK); t < min(tb, (w_hi + WK - 1) / WK); ++t) {
+                uint32_t none;
+                const uint32_t slots = filled(slot_of(t), none);
+                odd_values<HD, KIND, WK>(vbase, row_bytes, slots, none, [&](int at, const uint32_t* p) {
+                    const bool sees = t * WK + at >= see.lo && t * WK + at < see.hi;
+#pragma unroll
+                    for (int n = 0; n < NT; ++n)
+#pragma unroll
+                        for (int r = 0; r < 16; ++r) {
+                            const float x = value_at<KIND>(p, 32 * n + 8 * (r / 4) + 4 * half + r % 4);
+                            if (sees && !(fabsf(x) < INFINITY)) o[n][r] += x;
+                        }
+                });
+            }
+
+        l_run += __shfl_xor(l_run, 32, 64);
+        // Registers 4 i .. 4 i + 3 of tile n are dims 32 n + 8 i + 4 half .. + 3.
+        auto write = [&]() {
+            if (!there) return;
+            float* op = a.out + (req.first + row) * a.ldo + head + 4 * half;
+            const float r = 1.f / l_run;
+#pragma unroll
+            for (int n = 0; n < NT; ++n)
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                    *reinterpret_cast<f32x4*>(op + 32 * n + 8 * i) =
+                        l_run == 0.f ? f32x4{0, 0, 0, 0} : f32x4{o[n][4 * i] * r, o[n][4 * i + 1] * r, o[n][4 * i + 2] * r, o[n][4 * i + 3] * r};
         };
         if (walk.whole()) {
             write();
             continue;
         }
+        // A part is an image of the threads' registers, 8 bytes of each thread side by side; then maxima and sums.
+        constexpr int IMAGE = NT * 16 * kThreads;
+        static_assert(IMAGE == M * HD, "a part has its slot");
         float* slot = a.parts + (2 * static_cast<size_t>(block) + (walk.t0 == 0)) * slot_words;
 #pragma unroll
-        for (int gi = 0; gi < GI; ++gi) {
-            const uint32_t v = wave * WV + 16 * gi + fr;
-            if (run.m0 + v >= req.vecs) continue;
+        for (int n = 0; n < NT; ++n)
 #pragma unroll
-            for (int n = 0; n < NT; ++n) {
-                publish(slot + v * HD + 16 * n + 4 * fq, o[gi][n][0], o[gi][n][1]);
-                publish(slot + v * HD + 16 * n + 4 * fq + 2, o[gi][n][2], o[gi][n][3]);
-            }
-            if (fq == 0) publish(slot + a.slot_vecs * HD + 2 * v, m_run[gi], l_run[gi]);
-        }
+            for (int r = 0; r < 16; r += 2) publish(slot + (16 * n + r) * kThreads + 2 * tid, o[n][r], o[n][r + 1]);
+        if (half == 0) publish(slot + IMAGE + 2 * (wave * WV + fr), m_run, l_run);
         const uint32_t parts = walk.parts();
         const uint64_t border = walk.first_border();
         if (last_part(a.arrived + border - 1, parts, sc.last)) {
             const float* first = a.parts + (2 * border - 1) * slot_words;
+            m_run = -INFINITY, l_run = 0.f;
 #pragma unroll
-            for (int gi = 0; gi < GI; ++gi) {
-                m_run[gi] = -INFINITY, l_run[gi] = 0.f;
+            for (int n = 0; n < NT; ++n)
 #pragma unroll
-                for (int n = 0; n < NT; ++n) o[gi][n] = f32x4{0, 0, 0, 0};
-            }
+                for (int r = 0; r < 16; ++r) o[n][r] = 0.f;
             for (uint32_t w = 0; w < parts; ++w) {
                 const float* p = w == 0 ? first : first + (2 * static_cast<size_t>(w) - 1) * slot_words;
+                const float2 ml = fetch(p + IMAGE + 2 * (wave * WV + fr));
+                float2 x[NT][8];
 #pragma unroll
-                for (int gi = 0; gi < GI; ++gi) {
-                    const uint32_t v = min(wave * WV + 16 * gi + fr, a.slot_vecs - 1);
-                    const float2 ml = fetch(p + a.slot_vecs * HD + 2 * v);
-                    float2 x[NT][2];
+                for (int n = 0; n < NT; ++n)
 #pragma unroll
-                    for (int n = 0; n < NT; ++n) x[n][0] = fetch(p + v * HD + 16 * n + 4 * fq), x[n][1] = fetch(p + v * HD + 16 * n + 4 * fq + 2);
-                    const float m_new = fmaxf(m_run[gi], ml.x), base = m_new == -INFINITY ? 0.f : m_new;
-                    const float c0 = __builtin_amdgcn_exp2f(m_run[gi] - base), c1 = __builtin_amdgcn_exp2f(ml.x - base);
-                    m_run[gi] = m_new, l_run[gi] = l_run[gi] * c0 + ml.y * c1;
+                    for (int r = 0; r < 16; r += 2) x[n][r / 2] = fetch(p + (16 * n + r) * kThreads + 2 * tid);
+                const float m_new = fmaxf(m_run, ml.x), base = m_new == -INFINITY ? 0.f : m_new;
+                const float c0 = __builtin_amdgcn_exp2f(m_run - base), c1 = __builtin_amdgcn_exp2f(ml.x - base);
+                m_run = m_new, l_run = l_run * c0 + ml.y * c1;
 #pragma unroll
-                    for (int n = 0; n < NT; ++n) o[gi][n] = o[gi][n] * c0 + f32x4{x[n][0].x, x[n][0].y, x[n][1].x, x[n][1].y} * c1;
-                }
+                for (int n = 0; n < NT; ++n)
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) o[n][r] = o[n][r] * c0 + (r % 2 ? x[n][r / 2].y : x[n][r / 2].x) * c1;
             }
             write();
         }
@@ -1163,27 +1170,25 @@ __global__ __launch_bounds__(kThreads, 2) void paged_wide_kernel(PagedAttnArgs a
     }
 }
 
-// What a call runs: the kernel (groups of 16 vectors to a wave; wide: chunks), an item's vectors, blocks.
+// What a call runs: an item's vectors, blocks, the kernel.
 struct Plan {
     uint32_t m, blocks;
-    int groups;
     bool wide;
 };
-constexpr uint32_t kBlocksPerCu = 2;
 
-Plan plan_of(uint32_t rows, uint32_t requests, uint32_t group, uint32_t kind) {
-    const uint64_t vecs = static_cast<uint64_t>(rows) * group;
-    const uint32_t blocks = gemm_cus() * kBlocksPerCu;
-    if (vecs > uint64_t{48} * requests && kind != VVLI_CACHE_F32) return Plan{128, blocks, 2, true};
-    if (vecs > uint64_t{16} * requests) return Plan{128, blocks, 2, false};
-    return Plan{64, blocks, 1, false};
+// Chunks (many vectors of an average request and kv head), or not. Blocks: as many as the registers of their
+// waves leave room for.
+Plan plan_of(uint32_t rows, uint32_t requests, uint32_t group, uint32_t hd, uint32_t kind) {
+    const bool wide = static_cast<uint64_t>(rows) * group > uint64_t{48} * requests && kind != VVLI_CACHE_F32;
+    return Plan{wide ? 128u : 64u, gemm_cus() * (wide || hd == 128 ? 2 : 3), wide};
 }
 
-// An item's most vectors, and the bytes of a call's workspace: counters, then two slots of such an item for each block.
-uint32_t slot_vecs(uint32_t m, uint32_t rows, uint32_t group) {
-    return static_cast<uint32_t>(std::min<uint64_t>(m, (static_cast<uint64_t>(rows) * group + 1) & ~uint64_t{1}));
+// Vectors that a part has room for (chunks' parts are images of all of an item's), and the bytes of a call's
+// workspace: counters, then two parts for each block.
+uint32_t slot_vecs(const Plan& p, uint32_t rows, uint32_t group) {
+    return p.wide ? p.m : static_cast<uint32_t>(std::min<uint64_t>(p.m, (static_cast<uint64_t>(rows) * group + 1) & ~uint64_t{1}));
 }
-size_t plan_bytes(uint32_t blocks, uint32_t vecs, uint32_t hd) { return blocks * sizeof(float) * (4 + 2 * static_cast<size_t>(vecs) * (hd + 2)); }
+size_t plan_bytes(const Plan& p, uint32_t vecs, uint32_t hd) { return p.blocks * sizeof(float) * (4 + 2 * static_cast<size_t>(vecs) * (hd + 2)); }
 
 bool sizes_ok(uint32_t rows, uint32_t requests, uint32_t heads, uint32_t kv_heads) {
     return requests != 0 && heads != 0 && kv_heads != 0 && heads % kv_heads == 0 && heads <= 65535 &&
@@ -1195,7 +1200,7 @@ hipError_t launch(const PagedAttnArgs& a, const Plan& p, hipStream_t s) {
     const dim3 grid(p.blocks), block(kThreads);
     if constexpr (KIND != VVLI_CACHE_F32)
         if (p.wide) return vlaunch(paged_wide_kernel<HD, KIND>, grid, block, 0, s, a);
-    return p.groups == 1 ? vlaunch(paged_attn_kernel<HD, KIND, 1>, grid, block, 0, s, a) : vlaunch(paged_attn_kernel<HD, KIND, 2>, grid, block, 0, s, a);
+    return vlaunch(paged_attn_kernel<HD, KIND, 1>, grid, block, 0, s, a);
 }
 
 template <int HD>
@@ -1210,8 +1215,14 @@ extern "C" {
 size_t vvli_gpu_paged_attention_workspace(uint32_t rows, uint32_t requests, uint32_t heads, uint32_t kv_heads,
                                           uint32_t head_dim) {
     if (!sizes_ok(rows, requests, heads, kv_heads) || (head_dim != 32 && head_dim != 64 && head_dim != 128)) return 0;
-    const Plan p = plan_of(rows, 1, heads / kv_heads, VVLI_CACHE_F32);  // (of however few requests)
-    return plan_bytes(p.blocks, slot_vecs(p.m, rows, heads / kv_heads), head_dim);
+    // Of however few requests, and of any cache.
+    const uint32_t group = heads / kv_heads;
+    size_t most = 0;
+    for (uint32_t kind : {VVLI_CACHE_F32, VVLI_CACHE_BF16}) {
+        const Plan p = plan_of(rows, 1, group, head_dim, kind);
+        most = std::max(most, plan_bytes(p, slot_vecs(p, rows, group), head_dim));
+    }
+    return most;
 }
 
 int vvli_gpu_paged_attention(const vvli_gpu_paged_cache* cache, const int32_t* table, uint32_t table_stride,
@@ -1235,12 +1246,12 @@ int vvli_gpu_paged_attention(const vvli_gpu_paged_cache* cache, const int32_t* t
     if (q == out) return set_error(VVLI_INVALID_CONFIG, "%s: out is q", who);
     if (rows == 0) return VVLI_OK;
     const uint32_t group = heads / cache->kv_heads;
-    const Plan p = plan_of(rows, requests, group, cache->kind);
+    const Plan p = plan_of(rows, requests, group, cache->head_dim, cache->kind);
     PagedAttnArgs a{};
     a.k = cache->k, a.v = cache->v, a.table = table, a.row_start = row_start, a.start_pos = start_pos, a.q = q, a.out = out;
     a.arrived = static_cast<uint32_t*>(workspace);
     a.parts = static_cast<float*>(workspace) + 4 * p.blocks;
-    a.slot_vecs = slot_vecs(p.m, rows, group);
+    a.slot_vecs = slot_vecs(p, rows, group);
     a.slot_stride = cache->slot_stride, a.ldq = ldq, a.ldo = ldo;
     a.stride = table_stride, a.requests = requests, a.rows = rows, a.kv_heads = cache->kv_heads, a.window = window;
     a.pages = cache->pages, a.room = table_stride * cache->page_size, a.ps = page_div(cache->page_size), a.group = page_div(group);

@@ -527,7 +527,7 @@ size_t vvli_gpu_paged_attention_workspace(uint32_t rows, uint32_t requests, uint
  * count 0. out[row_start[r] ..] receives the accepted tokens, the drawn one (-1
  * if the whole row is 0) and -1 for the rest of the request's rows; a request
  * without rows has accepted[r] = 0. Rows of no request stay as they are;
- * row_start ascends (as above).
+ * row_start ascends (as above). At most 65535 requests.
  * target and draft may have any stride >= vocab; out is not tokens. workspace: at least
  * vvli_gpu_verify_drafts_workspace bytes, at a 16-byte address. */
 int vvli_gpu_verify_drafts(const float* target, uint64_t ldt, const float* draft, uint64_t ldd, const int32_t* tokens,

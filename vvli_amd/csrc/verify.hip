@@ -9,6 +9,7 @@
 // border would follow the order of adding.
 #include <algorithm>
 
+#include "device_common.hpp"
 #include "paged.hpp"
 
 using namespace vvli;
@@ -16,76 +17,100 @@ using namespace vvli;
 namespace {
 
 constexpr int kThreads = 256, kWaves = kThreads / 64;
-// Slices of a row: at most kSliceMost tokens for each block, fewer where the
-// requests alone leave most of the GPU idle (kBlocks blocks in all), not under
-// kSliceLeast. 64 rows of 128256: 16 slices each; one row of 151936: 149.
-constexpr uint32_t kSliceMost = 8192, kSliceLeast = 1024, kBlocks = 1024, kSlicesMost = 256;
+// A row is cut into chunks of whole kStep tokens (8 a lane of a wave), at most
+// one for each thread of the block that searches their sums; a block sums some
+// of them: enough blocks for the GPU, each with a chunk for every wave if there
+// are as many.
+constexpr uint32_t kStep = 512, kChunksMost = kThreads, kBlocks = 2048;
 
 struct VerifyArgs {
     const float *target, *draft, *u_accept, *u_sample;
     const int32_t *tokens, *row_start;
     int32_t *accepted, *out;
-    uint32_t* arrived;  // of each request: slices whose sums are there; 0 between calls
-    double* sums;       // [request][slice]: of what the draft left, of the target row
+    uint32_t* arrived;  // of each request: blocks whose sums are there; 0 between calls
+    double* sums;       // [request][chunk]
     uint64_t ldt, ldd;
-    uint32_t rows, vocab, slices, slice;
+    uint32_t rows, vocab, chunks, chunk, per_block;  // chunk: in tokens
 };
 
-__device__ inline double weight_of(double w) { return w > 0 && w < INFINITY ? w : 0; }
+// The weights of a row: what the draft leaves of the target's, or the target's.
+struct Weights {
+    const float *p, *q;  // (q null: none)
+    uint32_t vocab, without;
+    bool aligned;
+};
 
-// The value of thread 0..; inclusive over the block's threads in their order, and the sum of all.
-__device__ inline double block_scan(double v, double* waves, double& total) {
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+__device__ __forceinline__ void load8(const Weights& w, uint32_t v, float (&p)[8], float (&q)[8]) {
+    if (w.aligned && v + 8 <= w.vocab) {
+#pragma unroll
+        for (int i = 0; i < 8; i += 4) {
+            const float4 x = load_f32x4(w.p + v + i), y = w.q ? load_f32x4(w.q + v + i) : make_float4(0, 0, 0, 0);
+            p[i] = x.x, p[i + 1] = x.y, p[i + 2] = x.z, p[i + 3] = x.w;
+            q[i] = y.x, q[i + 1] = y.y, q[i + 2] = y.z, q[i + 3] = y.w;
+        }
+        return;
+    }
+#pragma unroll
+    for (uint32_t i = 0; i < 8; ++i) {
+        const bool in = v < w.vocab && i < w.vocab - v;
+        p[i] = in ? w.p[v + i] : 0.f, q[i] = in && w.q ? w.q[v + i] : 0.f;
+    }
+}
+__device__ __forceinline__ double weight(const Weights& w, uint32_t v, float p, float q) {
+    // (finite and positive: also of a difference, which is f64 since f32 would round it)
+    const double d = v == w.without ? 0.0 : static_cast<double>(p) - static_cast<double>(q);
+    return d > 0 && d < INFINITY ? d : 0.0;
+}
+__device__ __forceinline__ double weight8(const Weights& w, uint32_t v, const float (&p)[8], const float (&q)[8], double (&x)[8]) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) x[i] = weight(w, v + i, p[i], q[i]);
+    return ((x[0] + x[1]) + (x[2] + x[3])) + ((x[4] + x[5]) + (x[6] + x[7]));
+}
+
+__device__ __forceinline__ double wave_total(double v) {
+#pragma unroll
+    for (int o = 32; o; o >>= 1) v += __shfl_xor(v, o, 64);
+    return v;
+}
+__device__ __forceinline__ double wave_scan(double v) {
+    const int lane = threadIdx.x & 63;
 #pragma unroll
     for (int o = 1; o < 64; o <<= 1) {
         const double u = __shfl_up(v, o, 64);
         if (lane >= o) v += u;
     }
-    __syncthreads();
-    if (lane == 63) waves[wave] = v;
-    __syncthreads();
-    double before = 0;
-    total = 0;
-    for (int w = 0; w < kWaves; ++w) {
-        if (w == wave) before = total;
-        total += waves[w];
-    }
-    return before + v;
-}
-// Lowest thread for which `yes`, kThreads if none.
-__device__ inline uint32_t first_thread(bool yes, uint32_t* waves) {
-    const uint64_t b = __ballot(yes);
-    __syncthreads();
-    if ((threadIdx.x & 63) == 0) waves[threadIdx.x >> 6] = b ? __builtin_ctzll(b) : 64;
-    __syncthreads();
-    for (uint32_t w = 0; w < kWaves; ++w)
-        if (waves[w] < 64) return w * 64 + waves[w];
-    return kThreads;
-}
-__device__ inline uint32_t last_thread(bool yes, uint32_t* waves) {
-    const uint64_t b = __ballot(yes);
-    __syncthreads();
-    if ((threadIdx.x & 63) == 0) waves[threadIdx.x >> 6] = b ? 63 - __builtin_clzll(b) : 64;
-    __syncthreads();
-    for (int w = kWaves - 1; w >= 0; --w)
-        if (waves[w] < 64) return w * 64 + waves[w];
-    return kThreads;
+    return v;
 }
 
-// Block (slice, request). Every block finds where the request's drafts end (a
-// few gathered values, less than a launch of its own would cost) and sums its
-// slice of that row, of both weights at once; the block whose sums are the
-// request's last finds the token's slice and the token in it, which is what a
-// second pass over one slice costs. One pass over one row of target and draft
-// for each request bounds it.
+// A wave's sum of tokens from .. from + chunk - 1, two steps' loads in flight.
+__device__ __forceinline__ double chunk_sum(const Weights& w, uint32_t from, uint32_t chunk) {
+    const uint32_t lane = threadIdx.x & 63;
+    double s = 0, x[8];
+    for (uint32_t t = 0; t < chunk; t += 2 * kStep) {
+        const uint32_t v0 = from + t + 8 * lane, v1 = v0 + kStep;
+        const bool more = t + kStep < chunk;
+        float p0[8], q0[8], p1[8], q1[8];
+        load8(w, v0, p0, q0);
+        if (more) load8(w, v1, p1, q1);
+        s += weight8(w, v0, p0, q0, x);
+        if (more) s += weight8(w, v1, p1, q1, x);
+    }
+    return wave_total(s);
+}
+
+// Block (some chunks, request). Every block finds where the request's drafts
+// end (a few gathered values, less than a launch of its own would cost) and
+// sums its chunks of that row; the block whose sums are the request's last
+// finds the token's chunk among the sums and, with one wave, the token in it.
+// One pass over one row of target and draft for each request bounds it where
+// there are many requests, the chain of dependent loads where there are few.
 __global__ __launch_bounds__(kThreads) void verify_kernel(VerifyArgs a) {
-    __shared__ double waves[kWaves];
+    __shared__ double sums[kChunksMost], waves[kWaves];
     __shared__ uint32_t found[kWaves], stop, last;
-    __shared__ double slice_before;
-    const uint32_t r = blockIdx.y, sl = blockIdx.x, tid = threadIdx.x;
+    const uint32_t r = blockIdx.y, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     const RowSpan span = row_span(a.row_start[r], a.row_start[r + 1], a.rows);
     if (span.count == 0) {
-        if (tid == 0 && sl == 0) a.accepted[r] = 0;
+        if (tid == 0 && blockIdx.x == 0) a.accepted[r] = 0;
         return;
     }
     const uint32_t drafts = span.count - 1;
@@ -103,110 +128,116 @@ __global__ __launch_bounds__(kThreads) void verify_kernel(VerifyArgs a) {
     }
     __syncthreads();
     const uint32_t acc = stop;
+    const bool refused = acc < drafts;
     const uint64_t row = span.first + acc;
-    const float* p = a.target + row * a.ldt;
-    const float* q = a.draft && acc < drafts ? a.draft + row * a.ldd : nullptr;
-    const uint32_t x = acc < drafts ? a.tokens[row + 1] : a.vocab;
-    // What the draft leaves of token v; the target row itself where all drafts were accepted.
-    auto left = [&](uint32_t v, float pv, float qv) {
-        return weight_of(q ? static_cast<double>(pv) - static_cast<double>(qv) : v == x ? 0.0 : static_cast<double>(pv));
-    };
-    double s0 = 0, s1 = 0;
-    {
-        const uint32_t from = sl * a.slice, to = min(from + a.slice, a.vocab);
-        constexpr int N = 4;  // loads in flight
-        uint32_t v = from + tid;
-        for (; v + (N - 1) * kThreads < to; v += N * kThreads) {
-            float pv[N], qv[N];
-#pragma unroll
-            for (int i = 0; i < N; ++i) pv[i] = p[v + i * kThreads], qv[i] = q ? q[v + i * kThreads] : 0.f;
-#pragma unroll
-            for (int i = 0; i < N; ++i) s0 += left(v + i * kThreads, pv[i], qv[i]), s1 += weight_of(pv[i]);
-        }
-        for (; v < to; v += kThreads) {
-            const float pv = p[v], qv = q ? q[v] : 0.f;
-            s0 += left(v, pv, qv), s1 += weight_of(pv);
-        }
+    Weights w;
+    w.p = a.target + row * a.ldt, w.q = refused && a.draft ? a.draft + row * a.ldd : nullptr;
+    w.vocab = a.vocab, w.without = refused && !a.draft ? a.tokens[row + 1] : ~0u;
+    w.aligned = (reinterpret_cast<uintptr_t>(w.p) | reinterpret_cast<uintptr_t>(w.q)) % 16 == 0;
+    const uint32_t c0 = blockIdx.x * a.per_block, c1 = min(c0 + a.per_block, a.chunks);
+    double* const mine = a.sums + static_cast<size_t>(r) * a.chunks;
+    for (uint32_t c = c0 + wave; c < c1; c += kWaves) {
+        const double s = chunk_sum(w, c * a.chunk, a.chunk);
+        if (lane == 0) __hip_atomic_store(reinterpret_cast<uint64_t*>(mine + c), __builtin_bit_cast(uint64_t, s), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
     }
-    double t0, t1;
-    block_scan(s0, waves, t0);
-    block_scan(s1, waves, t1);
-    if (a.slices > 1) {
-        if (tid == 0) {
-            uint64_t* out = reinterpret_cast<uint64_t*>(a.sums + 2 * (static_cast<size_t>(r) * a.slices + sl));
-            __hip_atomic_store(out, __builtin_bit_cast(uint64_t, t0), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-            __hip_atomic_store(out + 1, __builtin_bit_cast(uint64_t, t1), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-            __builtin_amdgcn_s_waitcnt(0);  // both are in memory (agent-scope stores go through)
-            last = __hip_atomic_fetch_add(a.arrived + r, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == a.slices - 1;
-            if (last) __hip_atomic_store(a.arrived + r, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);  // for the next call
+    __builtin_amdgcn_s_waitcnt(0);  // the sums are in memory (agent-scope stores go through)
+    __syncthreads();
+    if (tid == 0) {
+        last = __hip_atomic_fetch_add(a.arrived + r, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == gridDim.x - 1;
+        if (last) __hip_atomic_store(a.arrived + r, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);  // for the next call
+    }
+    __syncthreads();
+    if (!last) return;
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "agent");
+    double s = 0;
+    if (tid < a.chunks) s = __builtin_bit_cast(double, __hip_atomic_load(reinterpret_cast<const uint64_t*>(mine + tid), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT));
+    double total, end;
+    for (bool again = refused;; again = false) {
+        // Sums up to each chunk, thread c having chunk c.
+        end = wave_scan(s);
+        __syncthreads();
+        if (lane == 63) waves[wave] = end;
+        __syncthreads();
+        total = 0;
+        for (uint32_t k = 0; k < kWaves; ++k) {
+            if (k == wave) end += total;
+            total += waves[k];
+        }
+        if (total > 0 || !again) break;
+        // Nothing is left of the target's row: the row itself.
+        w.q = nullptr, w.without = ~0u, w.aligned = reinterpret_cast<uintptr_t>(w.p) % 16 == 0;
+        for (uint32_t c = wave; c < a.chunks; c += kWaves) {
+            const double x = chunk_sum(w, c * a.chunk, a.chunk);
+            if (lane == 0) sums[c] = x;
         }
         __syncthreads();
-        if (!last) return;
-        __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "agent");
-        s0 = s1 = 0;
-        if (tid < a.slices) {
-            const uint64_t* in = reinterpret_cast<const uint64_t*>(a.sums + 2 * (static_cast<size_t>(r) * a.slices + tid));
-            s0 = __builtin_bit_cast(double, __hip_atomic_load(in, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT));
-            s1 = __builtin_bit_cast(double, __hip_atomic_load(in + 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT));
-        }
-    } else {
-        s0 = tid ? 0 : t0, s1 = tid ? 0 : t1;
+        s = tid < a.chunks ? sums[tid] : 0;
     }
-    // Thread s has slice s. The lowest token whose running sum is not at or below the border; behind the last one
-    // (a number of 1 or more) the last token with a weight.
-    const double e0 = block_scan(s0, waves, t0), e1 = block_scan(s1, waves, t1);
-    const bool less = acc < drafts && t0 > 0;
-    const double total = less ? t0 : t1, mine = less ? s0 : s1, end = less ? e0 : e1;
+    // The lowest token whose running sum is not at or below the border; behind all of them (a number of 1 or more)
+    // the last token with a weight.
     int32_t token = -1;
     if (total > 0) {
         const double border = static_cast<double>(a.u_sample[r]) * total;
-        uint32_t at = first_thread(tid < a.slices && !(end <= border), found);
-        const bool behind = at == kThreads;
-        if (behind) at = last_thread(mine > 0, found);
-        if (tid == at) slice_before = end - mine;
+        const uint64_t yes = __ballot(tid < a.chunks && !(end <= border)), some = __ballot(s > 0);
+        if (lane == 0) found[wave] = yes ? __builtin_ctzll(yes) : 64;
+        sums[tid] = end - s;
+        if (tid == 0) last = 0;
         __syncthreads();
-        const double before = slice_before;
-        // Thread t has the slice's run t of tokens.
-        const uint32_t from = at * a.slice, to = min(from + a.slice, a.vocab), per = (to - from + kThreads - 1) / kThreads;
-        const uint32_t a0 = min(from + tid * per, to), a1 = min(a0 + per, to);
-        auto weight = [&](uint32_t v) { return less ? left(v, p[v], q ? q[v] : 0.f) : weight_of(p[v]); };
-        double run = 0;
-        for (uint32_t v = a0; v < a1; ++v) run += weight(v);
-        double sum;
-        const double upto = before + block_scan(run, waves, sum);
-        uint32_t who = behind ? kThreads : first_thread(a0 < a1 && !(upto <= border), found);
-        const bool over = who == kThreads;  // behind the last token, also where the slice's sum was rounded up to it
-        if (over) who = last_thread(run > 0, found);
-        if (tid == who) {
-            double sofar = upto - run;
-            uint32_t best = a0;
-            for (uint32_t v = a0; v < a1; ++v) {
-                const double w = weight(v);
-                if (w > 0) best = v;
-                sofar += w;
-                if (!over && !(sofar <= border)) {
-                    best = v;
-                    break;
+        uint32_t at = kThreads;
+        for (int k = kWaves - 1; k >= 0; --k)
+            if (found[k] < 64) at = k * 64 + found[k];
+        const bool behind = at == kThreads;
+        if (behind) {
+            if (some) atomicMax(&last, wave * 64 + 63 - __builtin_clzll(some));
+            __syncthreads();
+            at = last;
+        }
+        if (wave == 0) {
+            double before = sums[at];
+            uint32_t best = 0;  // 1 + the last token with a weight in the lane
+            bool done = false;
+            for (uint32_t t = 0; t < a.chunk && !done; t += kStep) {
+                const uint32_t v = at * a.chunk + t + 8 * lane;
+                float p[8], q[8];
+                double x[8];
+                load8(w, v, p, q);
+                const double sum = weight8(w, v, p, q, x), upto = before + wave_scan(sum);
+                const uint64_t over = behind ? 0 : __ballot(v < a.vocab && !(upto <= border));
+                if (over) {
+                    double run = upto - sum;
+                    uint32_t tok = v;
+                    bool there = false;
+#pragma unroll
+                    for (uint32_t i = 0; i < 8; ++i) {
+                        run += x[i];
+                        if (x[i] > 0 && !there) tok = v + i;
+                        if (!there && !(run <= border)) tok = v + i, there = true;
+                    }
+                    best = __shfl(tok, __builtin_ctzll(over), 64) + 1;
+                    done = true;
+                } else {
+#pragma unroll
+                    for (uint32_t i = 0; i < 8; ++i)
+                        if (x[i] > 0) best = v + i + 1;
+                    before = __shfl(upto, 63, 64);
                 }
             }
-            last = best;
+            // (not found: behind the last token, also where the chunk's sum was rounded up to it)
+#pragma unroll
+            for (int o = 32; o; o >>= 1) best = max(best, static_cast<uint32_t>(__shfl_xor(best, o, 64)));
+            token = static_cast<int32_t>(best) - 1;
         }
-        __syncthreads();
-        if (who < kThreads) token = static_cast<int32_t>(last);
     }
-    if (tid == 0) a.accepted[r] = static_cast<int32_t>(acc);
-    for (uint32_t i = tid; i < span.count; i += kThreads) a.out[span.first + i] = i < acc ? a.tokens[span.first + i + 1] : i == acc ? token : -1;
+    if (tid == 0) {
+        a.accepted[r] = static_cast<int32_t>(acc);
+        a.out[span.first + acc] = token;
+    }
+    for (uint32_t i = tid; i < span.count; i += kThreads)
+        if (i != acc) a.out[span.first + i] = i < acc ? a.tokens[span.first + i + 1] : -1;
 }
 
-struct Slices {
-    uint32_t count, tokens;
-};
-Slices slices_of(uint32_t requests, uint32_t vocab) {
-    const uint32_t few = (vocab - 1) / kSliceMost + 1, many = std::min((vocab - 1) / kSliceLeast + 1, (kBlocks - 1) / requests + 1);
-    const uint32_t n = std::min(std::max(few, many), kSlicesMost), tokens = (vocab - 1) / n + 1;
-    return Slices{(vocab - 1) / tokens + 1, tokens};
-}
-
+uint32_t chunk_tokens(uint32_t vocab) { return ((vocab - 1) / (kStep * kChunksMost) + 1) * kStep; }
+uint32_t chunks_of(uint32_t vocab) { return (vocab - 1) / chunk_tokens(vocab) + 1; }
 size_t counter_bytes(uint32_t requests) { return (static_cast<size_t>(requests) * 4 + 15) / 16 * 16; }
 
 }  // namespace
@@ -214,9 +245,9 @@ size_t counter_bytes(uint32_t requests) { return (static_cast<size_t>(requests) 
 extern "C" {
 
 size_t vvli_gpu_verify_drafts_workspace(uint32_t requests, uint32_t vocab) {
-    // (slices of fewer requests: no more than kBlocks and one each)
-    const size_t few = vocab ? (vocab - 1) / kSliceMost + 1 : 0;
-    return counter_bytes(requests) + 16 * (requests * std::min<size_t>(few, kSlicesMost) + requests + kBlocks);
+    // (at least the chunks of this vocabulary and of any smaller one)
+    const size_t chunks = vocab ? std::min<size_t>((vocab - 1) / kStep + 1, kChunksMost) : 0;
+    return counter_bytes(requests) + 8 * requests * chunks;
 }
 
 int vvli_gpu_verify_drafts(const float* target, uint64_t ldt, const float* draft, uint64_t ldd, const int32_t* tokens,
@@ -232,13 +263,15 @@ int vvli_gpu_verify_drafts(const float* target, uint64_t ldt, const float* draft
     if (out == tokens) return set_error(VVLI_INVALID_CONFIG, "%s: out is tokens", who);
     if (!aligned16(workspace) || workspace_bytes < vvli_gpu_verify_drafts_workspace(requests, vocab))
         return set_error(VVLI_INVALID_CONFIG, "%s: workspace of %zu bytes", who, workspace_bytes);
-    const Slices sl = slices_of(requests, vocab);
     VerifyArgs a{};
     a.target = target, a.draft = draft, a.u_accept = u_accept, a.u_sample = u_sample, a.tokens = tokens, a.row_start = row_start;
     a.accepted = accepted, a.out = out, a.arrived = static_cast<uint32_t*>(workspace);
     a.sums = reinterpret_cast<double*>(static_cast<char*>(workspace) + counter_bytes(requests));
-    a.ldt = ldt, a.ldd = ldd, a.rows = rows, a.vocab = vocab, a.slices = sl.count, a.slice = sl.tokens;
-    PAGED_TRY(vlaunch(verify_kernel, dim3(sl.count, requests), dim3(kThreads), 0, static_cast<hipStream_t>(stream), a));
+    a.ldt = ldt, a.ldd = ldd, a.rows = rows, a.vocab = vocab;
+    a.chunks = chunks_of(vocab), a.chunk = chunk_tokens(vocab);
+    const uint32_t blocks = std::min((a.chunks - 1) / kWaves + 1, (kBlocks - 1) / requests + 1);
+    a.per_block = (a.chunks - 1) / blocks + 1;
+    PAGED_TRY(vlaunch(verify_kernel, dim3((a.chunks - 1) / a.per_block + 1, requests), dim3(kThreads), 0, static_cast<hipStream_t>(stream), a));
     return VVLI_OK;
 }
 

@@ -839,36 +839,46 @@ __global__ __launch_bounds__(kThreads, HD == 128 ? 2 : 3) void paged_attn_kernel
 }
 
 // ---------------------------------------------------------------------------
-// Chunks over 16-bit caches: items of 128 vectors, 32 to a wave, and steps of 32
-// keys that the block's waves share through LDS (a wave's own loads of every
-// key would be 16 KiB a step and wave). The block loads the next step's keys
-// and values into registers while it computes this one, and stores them into
-// the other of two stages behind it: one barrier a step. Products are
-// 32 x 32 x 16, a lane l with vector l % 32:
-//   S^T = K Q^T    A: key l % 32, dims 16 s + 8 (l / 32) .. + 7; D: register r
-//                  has key 8 (r / 4) + 4 (l / 32) + r % 4
+// Chunks: items of 128 vectors, 32 to a wave, and steps of 32 keys that the
+// block's waves share through LDS (a wave's own loads of every key would be
+// 16 KiB a step and wave in 16 bits). The block loads the next step's keys and
+// values into registers while it computes this one, and stores them into the
+// other of two stages behind it: one barrier a step. Products are 32 x 32 x 16
+// (16-bit caches) or 32 x 32 x 2 (f32), a lane l with vector l % 32:
+//   S^T = K Q^T    A: key l % 32, dims 16 s + 8 (l / 32) .. + 7, or
+//                  8 s + 4 (l / 32) + e; D: register r has key
+//                  8 (r / 4) + 4 (l / 32) + r % 4
 //   O^T += V^T P^T B: registers 8 c .. 8 c + 7 of the weights are step c's 8
-//                  values of k, as they stand; A: dim 32 n + l % 32, the same
-//                  keys, 4 at a time by a transposed read of LDS
-//                  (ds_read_b64_tr_b16); D: dims 32 n + 8 (r / 4) + 4 (l / 32) + r % 4
+//                  values of k (f32: register r is step r's), as they stand;
+//                  A: dim 32 n + l % 32, the same keys, in 16 bits 4 at a time
+//                  by a transposed read of LDS (ds_read_b64_tr_b16); D: dims
+//                  32 n + 8 (r / 4) + 4 (l / 32) + r % 4
 // Rows lie in LDS as in memory, their 16-byte chunks permuted by the row so that
 // the rows of a fragment read fall on different banks.
 // ---------------------------------------------------------------------------
 template <int HD, int KIND>
 struct Wide {
     using K = Kind<KIND>;
-    static constexpr int WV = 32, M = 128, WK = 32, NT = HD / 32, DS = HD / 16;
-    static constexpr int CH = HD / 8, RB = HD * 2, RPL = 256 / RB;  // 16-byte chunks and bytes of a row, rows of 256 bytes
+    static constexpr bool F32 = KIND == VVLI_CACHE_F32;
+    static constexpr int WV = 32, M = 128, WK = 32, NT = HD / 32, DS = HD * K::BYTES / 32;
+    static constexpr int RB = HD * K::BYTES, CH = RB / 16, RPL = RB < 256 ? 256 / RB : 1;  // bytes and 16-byte chunks of a row, rows of 256 bytes
     static constexpr int TILE = WK * RB, LOADS = 2 * TILE / (16 * kThreads), ROWS = LOADS > 1 ? LOADS / 2 : 1;
-    static constexpr int QR = 2;                                    // terms of q in registers; the rest in LDS
+    static constexpr int QR = F32 ? 1 : 2;  // terms of q in registers; the rest in LDS
     static constexpr int kQ = (K::TERMS - QR) * 4 * DS * 1024;
-    static __device__ __forceinline__ uint32_t kswz(uint32_t r) { return r / RPL % CH; }
-    static __device__ __forceinline__ uint32_t vswz(uint32_t r) { return 4 * (r / RPL % (CH / 4)); }
+    static __device__ __forceinline__ uint32_t kswz(uint32_t r) { return r / RPL % (CH < 16 ? CH : 16); }
+    static __device__ __forceinline__ uint32_t vswz(uint32_t r) { return F32 ? (CH >= 16 ? r / 4 % 2 * 8 : 0) : 4 * (r / RPL % (CH / 4)); }
 };
 // A vector's weights are 2^(s - base) with a base that follows the maximum of
 // its scores only where that is more than this above it: weights stay in range,
 // and few steps have outputs to rescale.
 constexpr float kSlack = 8.f;
+
+// Products' results may be read so many wait states behind the last of them
+// (18 for the longest, 32 x 32 x 2 in f32). The compiler counts these along
+// one way to a read; where a branch lies between the two, the other way can be
+// shorter, and the last register of a result was then read before it was
+// written. Here they are spent before any branch.
+__device__ __forceinline__ void mfma_done(f32x16& x, f32x16& y) { asm volatile("s_nop 15\n\ts_nop 3" : "+v"(x), "+v"(y)); }
 
 typedef short s16x4 __attribute__((ext_vector_type(4)));
 
@@ -876,9 +886,9 @@ template <int HD, int KIND>
 __global__ __launch_bounds__(kThreads, 2) void paged_wide_kernel(PagedAttnArgs a) {
     using F = Wide<HD, KIND>;
     using K = Kind<KIND>;
-    using T8 = typename K::T8;
     constexpr int WV = F::WV, M = F::M, WK = F::WK, NT = F::NT, DS = F::DS, CH = F::CH, RB = F::RB, TILE = F::TILE;
     constexpr int LOADS = F::LOADS, ROWS = F::ROWS, QR = F::QR;
+    constexpr bool F32 = F::F32;
     __shared__ RunScratch sc;
     __shared__ __attribute__((aligned(1024))) char stage[2][2 * TILE];  // keys, then values
     __shared__ __attribute__((aligned(16))) char q_rest[F::kQ ? F::kQ : 16];
@@ -889,13 +899,14 @@ __global__ __launch_bounds__(kThreads, 2) void paged_wide_kernel(PagedAttnArgs a
     if (!from.any) return;
     const int tid = threadIdx.x, lane = tid & 63, fr = lane & 31, half = lane >> 5;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    const uint64_t row_bytes = a.slot_stride * 2;
+    const uint64_t row_bytes = a.slot_stride * K::BYTES;
     const uint32_t slot_words = a.slot_vecs * (HD + 2);
     u32x4* const q_mine = reinterpret_cast<u32x4*>(q_rest) + wave * ((K::TERMS - QR) * DS * 64) + lane;
     // Where the lane's fragments lie in a stage (products' step s and tile n are put in by ^ and +).
     const uint32_t k_at = fr * RB + ((half ^ F::kswz(fr)) << 4);
-    const uint32_t v_row = 4 * half + (lane & 15) / 4;
-    const uint32_t v_at = TILE + v_row * RB + (((2 * (lane / 16 % 2) + lane / 2 % 2) ^ F::vswz(v_row)) << 4) + 8 * (lane & 1);
+    const uint32_t v_row = 4 * half + (F32 ? 0 : (lane & 15) / 4);
+    const uint32_t v_chunk = F32 ? fr / 4 : 2 * (lane / 16 % 2) + lane / 2 % 2;
+    const uint32_t v_at = TILE + v_row * RB + ((v_chunk ^ F::vswz(v_row)) << 4) + (F32 ? 4 * (fr & 3) : 8 * (lane & 1));
     // This thread's rows of a step (the same of keys and of values; HD = 32: of one of the two) and its chunk.
     const uint32_t my_row = tid % (WK * CH / ROWS) / CH, my_c = tid % CH;
 
@@ -915,7 +926,15 @@ __global__ __launch_bounds__(kThreads, 2) void paged_wide_kernel(PagedAttnArgs a
         const size_t head = (static_cast<size_t>(run.kvh) * a.group.d + (there ? m : 0) - row * a.group.d) * HD;
         float inv = 1.f;
         u32x4 qf[QR][DS];
-        {
+        if constexpr (F32) {
+            const float* qp = a.q + (req.first + row) * a.ldq + head + 4 * half;
+            const float f = a.scale * 1.44269504088896341f;
+#pragma unroll
+            for (int s = 0; s < DS; ++s) {
+                const float4 x = load_f32x4(qp + 8 * s);
+                qf[0][s] = __builtin_bit_cast(u32x4, f32x4{x.x * f, x.y * f, x.z * f, x.w * f});
+            }
+        } else {
             const float* qp = a.q + (req.first + row) * a.ldq + head + 8 * half;
             const float f = a.scale * 1.44269504088896341f;
             float x[DS][8];
@@ -938,7 +957,7 @@ __global__ __launch_bounds__(kThreads, 2) void paged_wide_kernel(PagedAttnArgs a
             }
 #pragma unroll
             for (int s = 0; s < DS; ++s) {
-                T8 t[K::TERMS];
+                typename K::T8 t[K::TERMS];
 #pragma unroll
                 for (int e = 0; e < 8; e += 2) split2<K>(x[s][e], x[s][e + 1], e, t);
 #pragma unroll
@@ -1021,20 +1040,34 @@ __global__ __launch_bounds__(kThreads, 2) void paged_wide_kernel(PagedAttnArgs a
                 const uint32_t key0 = t * WK;
                 if (key0 < w_hi && key0 + WK > w_lo) {
                     const char* base = stage[st];
-                    f32x16 s;
+                    // Two sums, of even and odd steps, and below the tiles of O^T in turn: a product waits for the
+                    // one before it on the same sum about as long as it takes.
+                    f32x16 s, s2;
 #pragma unroll
-                    for (int r = 0; r < 16; ++r) s[r] = 0.f;
+                    for (int r = 0; r < 16; ++r) s[r] = s2[r] = 0.f;
 #pragma unroll
-                    for (int i = 0; i < DS; ++i) {
-                        const T8 kf = __builtin_bit_cast(T8, *reinterpret_cast<const u32x4*>(base + (k_at ^ (32 * i))));
+                    for (int i = 0; i < DS; i += 2) {
+                        const u32x4 k0 = *reinterpret_cast<const u32x4*>(base + (k_at ^ (32 * i)));
+                        const u32x4 k1 = *reinterpret_cast<const u32x4*>(base + (k_at ^ (32 * i + 32)));
+                        if constexpr (F32) {
 #pragma unroll
-                        for (int x = 0; x < K::TERMS; ++x) {
-                            u32x4 qx;
-                            if (x < QR) qx = qf[x < QR ? x : 0][i];
-                            else qx = q_mine[((x - QR) * DS + i) * 64];
-                            s = K::mfma(kf, __builtin_bit_cast(T8, qx), s);
+                            for (int e = 0; e < 4; ++e) {
+                                s = __builtin_amdgcn_mfma_f32_32x32x2f32(__uint_as_float(k0[e]), __uint_as_float(qf[0][i][e]), s, 0, 0, 0);
+                                s2 = __builtin_amdgcn_mfma_f32_32x32x2f32(__uint_as_float(k1[e]), __uint_as_float(qf[0][i + 1][e]), s2, 0, 0, 0);
+                            }
+                        } else {
+#pragma unroll
+                            for (int x = 0; x < K::TERMS; ++x) {
+                                u32x4 q0, q1;
+                                if (x < QR) q0 = qf[x < QR ? x : 0][i], q1 = qf[x < QR ? x : 0][i + 1];
+                                else q0 = q_mine[((x - QR) * DS + i) * 64], q1 = q_mine[((x - QR) * DS + i + 1) * 64];
+                                s = K::mfma(__builtin_bit_cast(typename K::T8, k0), __builtin_bit_cast(typename K::T8, q0), s);
+                                s2 = K::mfma(__builtin_bit_cast(typename K::T8, k1), __builtin_bit_cast(typename K::T8, q1), s2);
+                            }
                         }
                     }
+                    mfma_done(s, s2);
+                    s += s2;
                     if (key0 < all_lo || key0 + WK > all_hi || none) {
 #pragma unroll
                         for (int r = 0; r < 16; ++r) {
@@ -1055,32 +1088,46 @@ __global__ __launch_bounds__(kThreads, 2) void paged_wide_kernel(PagedAttnArgs a
 #pragma unroll
                         for (int n = 0; n < NT; ++n) o[n] *= corr;
                     }
-                    T8 pf[2][K::TERMS];
                     float sum[2] = {0.f, 0.f};
+                    if constexpr (F32) {
 #pragma unroll
-                    for (int c = 0; c < 2; ++c)
+                        for (int r = 0; r < 16; ++r) s[r] = __builtin_amdgcn_exp2f(s[r] + shift), sum[r & 1] += s[r];
 #pragma unroll
-                        for (int e = 0; e < 8; e += 2) {
-                            const float p0 = __builtin_amdgcn_exp2f(fmaf(s[8 * c + e], inv, shift)), p1 = __builtin_amdgcn_exp2f(fmaf(s[8 * c + e + 1], inv, shift));
-                            sum[0] += p0, sum[1] += p1;
-                            split2<K>(p0, p1, e, pf[c]);
-                        }
-                    l_run += sum[0] + sum[1];
+                        for (int r = 0; r < 16; ++r)
 #pragma unroll
-                    for (int n = 0; n < NT; ++n)
+                            for (int n = 0; n < NT; ++n) {
+                                const float x = *reinterpret_cast<const float*>(base + ((v_at ^ (128 * n)) + (8 * (r / 4) + r % 4) * RB));
+                                o[n] = __builtin_amdgcn_mfma_f32_32x32x2f32(x, s[r], o[n], 0, 0, 0);
+                            }
+                    } else {
+                        typename K::T8 pf[2][K::TERMS];
 #pragma unroll
-                        for (int c = 0; c < 2; ++c) {
-                            u32x4 w;
+                        for (int c = 0; c < 2; ++c)
 #pragma unroll
-                            for (int h = 0; h < 2; ++h) {
-                                const s16x4 v = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-                                    (__attribute__((address_space(3))) s16x4*)(base + ((v_at ^ (64 * n)) + (16 * c + 8 * h) * RB)));
-                                const uint2 d = __builtin_bit_cast(uint2, v);
-                                w[2 * h] = d.x, w[2 * h + 1] = d.y;
+                            for (int e = 0; e < 8; e += 2) {
+                                const float p0 = __builtin_amdgcn_exp2f(fmaf(s[8 * c + e], inv, shift)), p1 = __builtin_amdgcn_exp2f(fmaf(s[8 * c + e + 1], inv, shift));
+                                sum[0] += p0, sum[1] += p1;
+                                split2<K>(p0, p1, e, pf[c]);
                             }
 #pragma unroll
-                            for (int x = 0; x < K::TERMS; ++x) o[n] = K::mfma(__builtin_bit_cast(T8, w), pf[c][x], o[n]);
+                        for (int c = 0; c < 2; ++c) {
+                            u32x4 w[NT];
+#pragma unroll
+                            for (int n = 0; n < NT; ++n)
+#pragma unroll
+                                for (int h = 0; h < 2; ++h) {
+                                    const s16x4 v = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                                        (__attribute__((address_space(3))) s16x4*)(base + ((v_at ^ (64 * n)) + (16 * c + 8 * h) * RB)));
+                                    const uint2 d = __builtin_bit_cast(uint2, v);
+                                    w[n][2 * h] = d.x, w[n][2 * h + 1] = d.y;
+                                }
+#pragma unroll
+                            for (int x = 0; x < K::TERMS; ++x)
+#pragma unroll
+                                for (int n = 0; n < NT; ++n) o[n] = K::mfma(__builtin_bit_cast(typename K::T8, w[n]), pf[c][x], o[n]);
                         }
+                    }
+                    l_run += sum[0] + sum[1];
                 }
                 if (t + 1 < tb) store(st ^ 1, careful);
                 none = none_next;
@@ -1178,8 +1225,8 @@ struct Plan {
 
 // Chunks (many vectors of an average request and kv head), or not. Blocks: as many as the registers of their
 // waves leave room for.
-Plan plan_of(uint32_t rows, uint32_t requests, uint32_t group, uint32_t hd, uint32_t kind) {
-    const bool wide = static_cast<uint64_t>(rows) * group > uint64_t{48} * requests && kind != VVLI_CACHE_F32;
+Plan plan_of(uint32_t rows, uint32_t requests, uint32_t group, uint32_t hd) {
+    const bool wide = static_cast<uint64_t>(rows) * group > uint64_t{48} * requests;
     return Plan{wide ? 128u : 64u, gemm_cus() * (wide || hd == 128 ? 2 : 3), wide};
 }
 
@@ -1198,9 +1245,7 @@ bool sizes_ok(uint32_t rows, uint32_t requests, uint32_t heads, uint32_t kv_head
 template <int HD, int KIND>
 hipError_t launch(const PagedAttnArgs& a, const Plan& p, hipStream_t s) {
     const dim3 grid(p.blocks), block(kThreads);
-    if constexpr (KIND != VVLI_CACHE_F32)
-        if (p.wide) return vlaunch(paged_wide_kernel<HD, KIND>, grid, block, 0, s, a);
-    return vlaunch(paged_attn_kernel<HD, KIND, 1>, grid, block, 0, s, a);
+    return p.wide ? vlaunch(paged_wide_kernel<HD, KIND>, grid, block, 0, s, a) : vlaunch(paged_attn_kernel<HD, KIND, 1>, grid, block, 0, s, a);
 }
 
 template <int HD>
@@ -1215,11 +1260,11 @@ extern "C" {
 size_t vvli_gpu_paged_attention_workspace(uint32_t rows, uint32_t requests, uint32_t heads, uint32_t kv_heads,
                                           uint32_t head_dim) {
     if (!sizes_ok(rows, requests, heads, kv_heads) || (head_dim != 32 && head_dim != 64 && head_dim != 128)) return 0;
-    // Of however few requests, and of any cache.
+    // Of however few requests, and of no fewer than any.
     const uint32_t group = heads / kv_heads;
     size_t most = 0;
-    for (uint32_t kind : {VVLI_CACHE_F32, VVLI_CACHE_BF16}) {
-        const Plan p = plan_of(rows, 1, group, head_dim, kind);
+    for (uint32_t n : {1u, ~0u}) {
+        const Plan p = plan_of(rows, n, group, head_dim);
         most = std::max(most, plan_bytes(p, slot_vecs(p, rows, group), head_dim));
     }
     return most;
@@ -1246,7 +1291,7 @@ int vvli_gpu_paged_attention(const vvli_gpu_paged_cache* cache, const int32_t* t
     if (q == out) return set_error(VVLI_INVALID_CONFIG, "%s: out is q", who);
     if (rows == 0) return VVLI_OK;
     const uint32_t group = heads / cache->kv_heads;
-    const Plan p = plan_of(rows, requests, group, cache->head_dim, cache->kind);
+    const Plan p = plan_of(rows, requests, group, cache->head_dim);
     PagedAttnArgs a{};
     a.k = cache->k, a.v = cache->v, a.table = table, a.row_start = row_start, a.start_pos = start_pos, a.q = q, a.out = out;
     a.arrived = static_cast<uint32_t*>(workspace);

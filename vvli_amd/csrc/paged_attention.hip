@@ -35,9 +35,10 @@ typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 
 constexpr int kThreads = 256;
 // What an item costs beside its keys (its q, the first loads, its end), in
-// units; the fewest units of a run; the most units of an item that is never
-// cut, since its parts would cost more than they save.
-constexpr uint32_t kItemUnits = 3, kFewestUnits = 5, kWholeUnits = 12;
+// units; what a cut costs (a part left and taken up again); the fewest units of
+// a run; the most units of an item that is never cut, since its parts would
+// cost more than they save.
+constexpr uint32_t kItemUnits = 3, kCutUnits = 4, kFewestUnits = 5, kWholeUnits = 12;
 
 struct PagedAttnArgs {
     const void *k, *v;
@@ -161,7 +162,7 @@ __device__ Run find_run(const PagedAttnArgs& a, uint32_t block, uint32_t blocks,
     const uint64_t total = before * a.kv_heads;
     Run run{};
     run.per = max(quotient(total + blocks - 1, blocks), static_cast<uint64_t>(kFewestUnits));
-    run.near_hi = static_cast<uint32_t>(min(run.per / 4, static_cast<uint64_t>(1u << 20)));
+    run.near_hi = static_cast<uint32_t>(min(run.per / 4, static_cast<uint64_t>(kCutUnits)));
     run.near_lo = max(run.near_hi, kItemUnits);
     static_assert(kItemUnits + kFewestUnits / 4 < kFewestUnits, "near_lo + near_hi < per");
     run.from = run.per * block;

@@ -808,29 +808,46 @@ __global__ __launch_bounds__(kThreads, HD == 128 ? 2 : 3) void paged_attn_kernel
             if (last_part(a.arrived + border - 1, n, sc.last)) {
                 const float* first = a.parts + (2 * border - 1) * slot_words;
                 auto part_at = [&](uint32_t i) { return i == 0 ? first : first + (2 * static_cast<size_t>(i) - 1) * slot_words; };
-                for (uint32_t i = tid; i < vecs * (HD / 4); i += kThreads) {
-                    const uint32_t v = i / (HD / 4), d = i % (HD / 4) * 4;
-                    float top = -INFINITY, l = 0.f;
-                    f32x4 x = {0, 0, 0, 0};
-                    for (uint32_t w0 = 0; w0 < n; w0 += 8) {  // eight parts in flight
-                        float2 ml[8], x0[8], x1[8];
+                // Two 16-byte pieces of the outputs a thread, four parts of each in flight.
+                constexpr uint32_t NP = 4, NI = 2;
+                for (uint32_t i0 = tid; i0 < vecs * (HD / 4); i0 += NI * kThreads) {
+                    float top[NI], l[NI];
+                    f32x4 x[NI];
+                    uint32_t at[NI], at_ml[NI];
 #pragma unroll
-                        for (uint32_t w = 0; w < 8; ++w) {
+                    for (uint32_t k = 0; k < NI; ++k) {
+                        const uint32_t i = min(i0 + k * kThreads, vecs * (HD / 4) - 1);
+                        at[k] = 4 * i, at_ml[k] = static_cast<uint32_t>(a.slot_vecs) * HD + 2 * (i / (HD / 4));
+                        top[k] = -INFINITY, l[k] = 0.f, x[k] = f32x4{0, 0, 0, 0};
+                    }
+                    for (uint32_t w0 = 0; w0 < n; w0 += NP) {
+                        float2 ml[NI][NP], u0[NI][NP], u1[NI][NP];
+#pragma unroll
+                        for (uint32_t w = 0; w < NP; ++w) {
                             const float* p = part_at(min(w0 + w, n - 1));
-                            ml[w] = fetch(p + a.slot_vecs * HD + 2 * v), x0[w] = fetch(p + v * HD + d), x1[w] = fetch(p + v * HD + d + 2);
+#pragma unroll
+                            for (uint32_t k = 0; k < NI; ++k)
+                                ml[k][w] = fetch(p + at_ml[k]), u0[k][w] = fetch(p + at[k]), u1[k][w] = fetch(p + at[k] + 2);
                         }
-                        float more = top;
 #pragma unroll
-                        for (uint32_t w = 0; w < 8; ++w) more = fmaxf(more, ml[w].x);
-                        const float base = more == -INFINITY ? 0.f : more, old = __builtin_amdgcn_exp2f(top - base);
-                        top = more, l *= old, x *= old;
+                        for (uint32_t k = 0; k < NI; ++k) {
+                            float more = top[k];
 #pragma unroll
-                        for (uint32_t w = 0; w < 8; ++w) {
-                            const float c = w0 + w < n ? __builtin_amdgcn_exp2f(ml[w].x - base) : 0.f;
-                            if (w0 + w < n) l += ml[w].y * c, x += f32x4{x0[w].x, x0[w].y, x1[w].x, x1[w].y} * c;
+                            for (uint32_t w = 0; w < NP; ++w) more = fmaxf(more, ml[k][w].x);
+                            const float base = more == -INFINITY ? 0.f : more, old = __builtin_amdgcn_exp2f(top[k] - base);
+                            top[k] = more, l[k] *= old, x[k] *= old;
+#pragma unroll
+                            for (uint32_t w = 0; w < NP; ++w) {
+                                const float c = w0 + w < n ? __builtin_amdgcn_exp2f(ml[k][w].x - base) : 0.f;
+                                if (w0 + w < n) l[k] += ml[k][w].y * c, x[k] += f32x4{u0[k][w].x, u0[k][w].y, u1[k][w].x, u1[k][w].y} * c;
+                            }
                         }
                     }
-                    write(v, d, x, l);
+#pragma unroll
+                    for (uint32_t k = 0; k < NI; ++k) {
+                        const uint32_t i = i0 + k * kThreads;
+                        if (i < vecs * (HD / 4)) write(i / (HD / 4), i % (HD / 4) * 4, x[k], l[k]);
+                    }
                 }
             }
             if (walk.cut) return;

@@ -464,8 +464,10 @@ typedef struct vvli_gpu_page_pool {
  * slots[i] = table[r][p / page_size] * page_size + p % page_size (both -1
  * without pages, the slot also where the page number is outside 0..pages - 1).
  * row_pos and slots hold `rows` entries (0: both may be NULL); those behind the
- * last new row stay as they are. `held` is what earlier calls returned: this
- * one does not look for pages that two requests share. */
+ * last new row stay as they are (a captured step over `rows` rows, of which a
+ * batch may have fewer, sets slots to -1 before this call: rows that are none
+ * are then appended nowhere). `held` is what earlier calls returned: this one
+ * does not look for pages that two requests share. */
 int vvli_gpu_paged_assign(const vvli_gpu_page_pool* pool, const int32_t* held, const int32_t* keep, const int32_t* add,
                           uint32_t rows, int32_t* len, int32_t* row_start, int32_t* start_pos, int32_t* row_pos,
                           int64_t* slots, void* stream);
@@ -534,7 +536,7 @@ int vvli_gpu_verify_drafts(const float* target, uint64_t ldt, const float* draft
                            const int32_t* row_start, uint32_t requests, uint32_t rows, uint32_t vocab,
                            const float* u_accept, const float* u_sample, int32_t* accepted, int32_t* out,
                            void* workspace, size_t workspace_bytes, void* stream);
-/* Bytes of workspace that calls of up to these sizes need. */
+/* Bytes of workspace that calls of up to these sizes need (0 for a vocabulary of 0). */
 size_t vvli_gpu_verify_drafts_workspace(uint32_t requests, uint32_t vocab);
 
 #ifdef __cplusplus

@@ -609,6 +609,44 @@ def test_attention_captured_step_serves_other_batches(torch, kind):
         check(torch, b, attend(torch, b, kind))  # an eager call with a workspace of its own
 
 
+def test_attention_workspace_serves_other_sizes(torch):
+    """One workspace, zeroed once, for calls of other head sizes, rows and requests in turn: no call's parts lie on another's counters."""
+    ws = torch.zeros(max(R.paged_attention_workspace(200, 8, h, kv, hd) for h, kv, hd in ((28, 4, 128), (32, 8, 64), (4, 2, 32))),
+                     dtype=torch.uint8, device="cuda")
+    for _ in range(2):
+        for heads, kv, hd, spec, kind in ((28, 4, 128, "step", "bf16"), (32, 8, 64, "chunks", "f32"), (4, 2, 32, "step", "f16"),
+                                          (32, 8, 64, "long", "bf16"), (28, 4, 128, "chunks", "f16"), (32, 8, 64, "drafts", "f32")):
+            b = build(torch, SPECS[spec], heads, kv, hd, kind, 16, seed=heads + hd)
+            if spec == "chunks":
+                b["q"] = b["q"][:200]  # the last request's rows end behind them
+            print("workspace", heads, hd, spec, kind, flush=True)
+            check(torch, b, attend(torch, b, kind, ws=ws))
+
+
+def test_attention_on_two_streams(torch):
+    """Calls that overlap, each with a workspace of its own."""
+    cases = [(build(torch, SPECS["long"], 28, 4, 128, "bf16", 16, seed=1), "bf16"), (build(torch, SPECS["drafts"], 32, 8, 64, "f16", 16, seed=2), "f16")]
+    sides = []
+    for b, kind in cases:
+        rows, heads, hd = b["q"].shape
+        kv, w = b["k"].shape[1], heads * hd
+        k, v, q = b["k"].cuda(), b["v"].cuda(), b["q"].cuda()
+        out = torch.full((rows, w), 9.0, device="cuda")
+        d = [i32(torch, b[x]) for x in ("table", "row_start", "start")]
+        n = len(b["start"])
+        ws = torch.zeros(R.paged_attention_workspace(rows, n, heads, kv, hd), dtype=torch.uint8, device="cuda")
+        c = R.PagedCache(ptr(k), ptr(v), kind, kv, hd, b["ps"], b["pages"])
+        sides.append((b, out, torch.cuda.Stream(), (k, v, q), lambda s, a=(c, ptr(d[0]), b["table"].shape[1], ptr(d[1]), ptr(d[2]), n, ptr(q), w,
+                      ptr(out), w, rows, heads, hd ** -0.5, 0, ptr(ws), ws.numel()), keep=(d, ws): R.paged_attention(*a, s.cuda_stream)))
+    torch.cuda.synchronize()
+    for _ in range(20):
+        for _, _, s, _, run in sides:
+            run(s)
+    torch.cuda.synchronize()
+    for b, out, _, _, _ in sides:
+        check(torch, b, out.view(b["q"].shape).cpu())
+
+
 # ---------------------------------------------------------------------------
 # verify_drafts
 # ---------------------------------------------------------------------------
@@ -739,6 +777,16 @@ def test_verify_gives_the_target_distribution(torch):
     assert (np.abs(freq - p) <= 5 * np.sqrt(p * (1 - p) / n)).all()
 
 
+def test_verify_workspace_serves_other_sizes(torch):
+    """One workspace, zeroed once, for calls of more and fewer requests and of other vocabularies in turn."""
+    rng = np.random.RandomState(3)
+    ws = torch.zeros(R.verify_drafts_workspace(40, 40000), dtype=torch.uint8, device="cuda")
+    for n, V in ((3, 40000), (40, 2000), (1, 40000), (40, 5000), (17, 100), (40, 40000), (2, 600), (40, 1)):
+        p, q = (x / x.sum(-1, keepdims=True) for x in (rng.rand(3 * n, V), rng.rand(3 * n, V)))
+        print("workspace", n, V, flush=True)
+        verify(torch, p, q, rng.randint(0, V, 3 * n), np.arange(n + 1) * 3, rng.rand(3 * n), rng.rand(n), ws=ws)
+
+
 # ---------------------------------------------------------------------------
 # The ops together
 # ---------------------------------------------------------------------------
@@ -841,3 +889,75 @@ def test_steps_of_several_requests_match_the_runner(torch):
     assert all(a >= b for a, b in zip(length.tolist(), done))
     for r in runners:
         r.close()
+
+
+def test_captured_step_follows_the_eager_one(torch):
+    """A whole step in one graph, for batches of fewer rows than it has room for: pages, cache, outputs and tokens are those of eager
+    calls over the same inputs, replay by replay, with eager work between."""
+    n, heads, kv, hd, ps, pages, stride, most, V = 4, 8, 2, 64, 8, 40, 16, 48, 3000
+    width = (heads + 2 * kv) * hd
+    g = torch.Generator(device="cuda").manual_seed(2)
+    rnd = lambda *shape: torch.rand(*shape, device="cuda", generator=g)  # noqa: E731
+    order = np.random.RandomState(4).permutation(pages)
+    keep, add, qkv, inv = i32(torch, np.zeros(n)), i32(torch, np.zeros(n)), torch.zeros(most, width, device="cuda"), rnd(hd // 2)
+    target, draft, tokens, ua, us = rnd(most, V), rnd(most, V), i32(torch, np.zeros(most)), rnd(most), rnd(n)
+
+    class Side:
+        def __init__(self):
+            self.free, self.count, self.table = i32(torch, order), i32(torch, [pages]), i32(torch, np.full((n, stride), -1))
+            self.len, self.row_start, self.start = i32(torch, np.zeros(n)), i32(torch, np.zeros(n + 1)), i32(torch, np.zeros(n))
+            self.pos, self.slots = i32(torch, np.zeros(most)), torch.zeros(most, dtype=torch.int64, device="cuda")
+            self.k, self.v = (torch.zeros(pages * ps, kv * hd, dtype=torch.bfloat16, device="cuda") for _ in range(2))
+            self.q, self.out = (torch.zeros(most, heads * hd, device="cuda") for _ in range(2))
+            self.acc, self.tok = i32(torch, np.zeros(n)), i32(torch, np.zeros(most))
+            self.aw = torch.zeros(R.paged_attention_workspace(most, n, heads, kv, hd), dtype=torch.uint8, device="cuda")
+            self.vw = torch.zeros(R.verify_drafts_workspace(n, V), dtype=torch.uint8, device="cuda")
+
+        def step(self):
+            s = torch.cuda.current_stream().cuda_stream
+            pool = R.PagePool(ptr(self.free), ptr(self.count), ptr(self.table), n, stride, ps, pages)
+            c = R.PagedCache(ptr(self.k), ptr(self.v), "bf16", kv, hd, ps, pages)
+            self.slots.fill_(-1)
+            R.paged_assign(pool, ptr(self.len), ptr(keep), ptr(add), most, ptr(self.len), ptr(self.row_start), ptr(self.start), ptr(self.pos),
+                           ptr(self.slots), s)
+            b = ptr(qkv)
+            R.norm_rope_append(c, b, width, b + 4 * heads * hd, width, b + 4 * (heads + kv) * hd, width, most, heads, ptr(self.q), heads * hd,
+                               ptr(inv), ptr(self.pos), ptr(self.slots), "split_half", None, None, 0.0, s)
+            R.paged_attention(c, ptr(self.table), stride, ptr(self.row_start), ptr(self.start), n, ptr(self.q), heads * hd, ptr(self.out),
+                              heads * hd, most, heads, hd ** -0.5, 0, ptr(self.aw), self.aw.numel(), s)
+            R.verify_drafts(ptr(target), V, ptr(draft), V, ptr(tokens), ptr(self.row_start), n, most, V, ptr(ua), ptr(us), ptr(self.acc),
+                            ptr(self.tok), ptr(self.vw), self.vw.numel(), s)
+
+        def state(self):
+            return {x: getattr(self, x).clone() for x in ("free", "count", "table", "len", "row_start", "start", "slots", "k", "v", "out",
+                                                          "acc", "tok")}
+
+    captured, eager = Side(), Side()
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        captured.step()  # (no request has rows yet)
+        eager.step()
+    torch.cuda.current_stream().wait_stream(s)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        captured.step()
+    rng = np.random.RandomState(9)
+    for i, new in enumerate([(17, 5, 0, 26), (1, 9, 30, 1), (3, 0, 1, 3), (1, 1, 1, 1), (0, 40, 2, 1), (5, 1, 1, 5)]):
+        held = eager.len.cpu().numpy()
+        kept = np.maximum(held - rng.randint(0, 3, n), 0)
+        if i == 3:
+            kept[0] = 0  # a request that has ended, and the next one in its place
+        keep.copy_(i32(torch, kept)), add.copy_(i32(torch, new)), tokens.copy_(i32(torch, rng.randint(0, V, most)))
+        qkv.copy_(torch.randn(most, width, device="cuda", generator=g)), ua.copy_(rnd(most)), us.copy_(rnd(n))
+        torch.cuda.synchronize()
+        graph.replay()
+        torch.cuda.synchronize()
+        eager.step()
+        torch.cuda.synchronize()
+        a, b = captured.state(), eager.state()
+        for x in a:
+            assert torch.equal(a[x], b[x]), (i, x)
+        rows = int(b["row_start"][-1])
+        assert rows == sum(new) and bool((b["slots"][:rows] >= 0).all()) and bool((b["slots"][rows:] == -1).all())

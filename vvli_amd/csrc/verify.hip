@@ -22,13 +22,16 @@ constexpr int kThreads = 256, kWaves = kThreads / 64;
 // of them: enough blocks for the GPU, each with a chunk for every wave if there
 // are as many.
 constexpr uint32_t kStep = 512, kChunksMost = kThreads, kBlocks = 2048;
+// 8-byte words of a request in the workspace, the same for every vocabulary and
+// number of requests: a workspace serves calls of other sizes too, and where a
+// counter is for one of them no sum may be for another.
+constexpr uint32_t kRecord = 1 + kChunksMost;
 
 struct VerifyArgs {
     const float *target, *draft, *u_accept, *u_sample;
     const int32_t *tokens, *row_start;
     int32_t *accepted, *out;
-    uint32_t* arrived;  // of each request: blocks whose sums are there; 0 between calls
-    double* sums;       // [request][chunk]
+    uint64_t* space;  // of each request kRecord words: blocks whose sums are there (0 between calls), then the chunks' sums
     uint64_t ldt, ldd;
     uint32_t rows, vocab, chunks, chunk, per_block;  // chunk: in tokens
 };
@@ -135,22 +138,23 @@ __global__ __launch_bounds__(kThreads) void verify_kernel(VerifyArgs a) {
     w.vocab = a.vocab, w.without = refused && !a.draft ? a.tokens[row + 1] : ~0u;
     w.aligned = (reinterpret_cast<uintptr_t>(w.p) | reinterpret_cast<uintptr_t>(w.q)) % 16 == 0;
     const uint32_t c0 = blockIdx.x * a.per_block, c1 = min(c0 + a.per_block, a.chunks);
-    double* const mine = a.sums + static_cast<size_t>(r) * a.chunks;
+    uint64_t* const mine = a.space + static_cast<size_t>(r) * kRecord + 1;
+    uint32_t* const arrived = reinterpret_cast<uint32_t*>(mine - 1);
     for (uint32_t c = c0 + wave; c < c1; c += kWaves) {
         const double s = chunk_sum(w, c * a.chunk, a.chunk);
-        if (lane == 0) __hip_atomic_store(reinterpret_cast<uint64_t*>(mine + c), __builtin_bit_cast(uint64_t, s), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        if (lane == 0) __hip_atomic_store(mine + c, __builtin_bit_cast(uint64_t, s), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
     }
     __builtin_amdgcn_s_waitcnt(0);  // the sums are in memory (agent-scope stores go through)
     __syncthreads();
     if (tid == 0) {
-        last = __hip_atomic_fetch_add(a.arrived + r, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == gridDim.x - 1;
-        if (last) __hip_atomic_store(a.arrived + r, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);  // for the next call
+        last = __hip_atomic_fetch_add(arrived, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == gridDim.x - 1;
+        if (last) __hip_atomic_store(arrived, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);  // for the next call
     }
     __syncthreads();
     if (!last) return;
     __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "agent");
     double s = 0;
-    if (tid < a.chunks) s = __builtin_bit_cast(double, __hip_atomic_load(reinterpret_cast<const uint64_t*>(mine + tid), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT));
+    if (tid < a.chunks) s = __builtin_bit_cast(double, __hip_atomic_load(mine + tid, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT));
     double total, end;
     for (bool again = refused;; again = false) {
         // Sums up to each chunk, thread c having chunk c.
@@ -238,16 +242,13 @@ __global__ __launch_bounds__(kThreads) void verify_kernel(VerifyArgs a) {
 
 uint32_t chunk_tokens(uint32_t vocab) { return ((vocab - 1) / (kStep * kChunksMost) + 1) * kStep; }
 uint32_t chunks_of(uint32_t vocab) { return (vocab - 1) / chunk_tokens(vocab) + 1; }
-size_t counter_bytes(uint32_t requests) { return (static_cast<size_t>(requests) * 4 + 15) / 16 * 16; }
 
 }  // namespace
 
 extern "C" {
 
 size_t vvli_gpu_verify_drafts_workspace(uint32_t requests, uint32_t vocab) {
-    // (at least the chunks of this vocabulary and of any smaller one)
-    const size_t chunks = vocab ? std::min<size_t>((vocab - 1) / kStep + 1, kChunksMost) : 0;
-    return counter_bytes(requests) + 8 * requests * chunks;
+    return vocab ? static_cast<size_t>(requests) * kRecord * 8 : 0;
 }
 
 int vvli_gpu_verify_drafts(const float* target, uint64_t ldt, const float* draft, uint64_t ldd, const int32_t* tokens,
@@ -265,8 +266,7 @@ int vvli_gpu_verify_drafts(const float* target, uint64_t ldt, const float* draft
         return set_error(VVLI_INVALID_CONFIG, "%s: workspace of %zu bytes", who, workspace_bytes);
     VerifyArgs a{};
     a.target = target, a.draft = draft, a.u_accept = u_accept, a.u_sample = u_sample, a.tokens = tokens, a.row_start = row_start;
-    a.accepted = accepted, a.out = out, a.arrived = static_cast<uint32_t*>(workspace);
-    a.sums = reinterpret_cast<double*>(static_cast<char*>(workspace) + counter_bytes(requests));
+    a.accepted = accepted, a.out = out, a.space = static_cast<uint64_t*>(workspace);
     a.ldt = ldt, a.ldd = ldd, a.rows = rows, a.vocab = vocab;
     a.chunks = chunks_of(vocab), a.chunk = chunk_tokens(vocab);
     const uint32_t blocks = std::min((a.chunks - 1) / kWaves + 1, (kBlocks - 1) / requests + 1);

@@ -609,6 +609,18 @@ def test_attention_captured_step_serves_other_batches(torch, kind):
         check(torch, b, attend(torch, b, kind))  # an eager call with a workspace of its own
 
 
+@pytest.mark.parametrize("kind", ["bf16", "f32"])
+@pytest.mark.parametrize("n_req", [2, 66, 130, 700])
+def test_attention_idle_requests(torch, kind, n_req):
+    """Requests without rows before, between and behind those that have some."""
+    for busy in ((0, n_req - 1), (n_req // 2,), (0,), (n_req - 1,), (0, 1, n_req // 2, n_req - 1)):
+        for rows in (1, 40):
+            spec = [(300 + 7 * i, rows) if i in busy else (20, 0) for i in range(n_req)]
+            print("idle", n_req, busy, rows, flush=True)
+            b = build(torch, spec, 8, 2, 64, kind, 16, seed=n_req)
+            check(torch, b, attend(torch, b, kind))
+
+
 def test_attention_workspace_serves_other_sizes(torch):
     """One workspace, zeroed once, for calls of other head sizes, rows and requests in turn: no call's parts lie on another's counters."""
     ws = torch.zeros(max(R.paged_attention_workspace(200, 8, h, kv, hd) for h, kv, hd in ((28, 4, 128), (32, 8, 64), (4, 2, 32))),

@@ -166,7 +166,7 @@ __device__ Run find_run(const PagedAttnArgs& a, uint32_t block, uint32_t blocks,
     run.near_lo = max(run.near_hi, kItemUnits);
     static_assert(kItemUnits + kFewestUnits / 4 < kFewestUnits, "near_lo + near_hi < per");
     run.from = run.per * block;
-    run.to = run.from + run.per >= total ? ~uint64_t{0} : run.from + run.per;
+    run.to = min(run.from + run.per, total);
     if (run.from >= total) return run;
     run.any = true;
     before = 0;
@@ -215,14 +215,30 @@ struct Walk {
         start = run.from - run.unit;
         begun = true;
     }
+    // The first request from r on that has rows. (Idle ones are looked at 64 at a time: one after the other, 254
+    // between two that have rows made 22 us 56 us.)
+    __device__ __forceinline__ static uint32_t with_rows(const PagedAttnArgs& a, uint32_t r) {
+        for (; r < a.requests; r += 64) {
+            const uint32_t i = r + (threadIdx.x & 63);
+            const uint64_t some = __ballot(i < a.requests && row_span(a.row_start[i], a.row_start[i + 1], a.rows).count != 0);
+            if (some) return r + __builtin_ctzll(some);
+        }
+        return a.requests;
+    }
     __device__ __forceinline__ bool item(const PagedAttnArgs& a) {  // false: the run has ended
         for (;; begun = false) {
+            if (start >= run.to) return false;
             while (run.m0 >= req.vecs) {  // the next item with vectors
                 run.m0 = 0;
                 if (req.vecs == 0 || ++run.kvh == a.kv_heads) {
                     run.kvh = 0;
                     if (++run.r == a.requests) return false;
                     req = request_at(a, run.r);
+                    if (req.vecs == 0) {
+                        run.r = __builtin_amdgcn_readfirstlane(with_rows(a, run.r));
+                        if (run.r == a.requests) return false;
+                        req = request_at(a, run.r);
+                    }
                 }
             }
             un = units_of<M, WK, FIXED>(a, req, run.m0);

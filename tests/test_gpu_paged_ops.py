@@ -609,6 +609,25 @@ def test_attention_captured_step_serves_other_batches(torch, kind):
         check(torch, b, attend(torch, b, kind))  # an eager call with a workspace of its own
 
 
+@pytest.mark.parametrize("kind", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("window", [0, 1, 33, 500])
+@pytest.mark.parametrize("heads,kv,spec,ps", [(28, 4, [(0, 131), (700, 90), (33, 200)], 16), (16, 16, [(90, 513)], 40), (7, 1, [(0, 400), (1300, 3), (5, 0)], 64)])
+def test_attention_prompts_of_wide_heads(torch, kind, window, heads, kv, spec, ps):
+    """Chunks that fill tiles of 128 vectors, heads of 128."""
+    b = build(torch, spec, heads, kv, 128, kind, ps, seed=heads)
+    check(torch, b, attend(torch, b, kind, window, pad=4), window)
+
+
+@pytest.mark.parametrize("kind", ["f32", "bf16", "f16"])
+def test_attention_bad_values_in_prompts_of_wide_heads(torch, kind):
+    """A NaN among the values reaches its dimension of the rows that see it, NaN in holes and behind every row none."""
+    b = build(torch, [(100, 150), (0, 80)], 28, 4, 128, kind, 16, seed=3)
+    for r, j, kvh, d in ((0, 7, 1, 5), (0, 200, 2, 127), (1, 79, 0, 64)):
+        b["v"][int(b["table"][r][j // 16]) * 16 + j % 16, kvh, d] = float("nan")
+    b["table"][0][4] = -1
+    check(torch, b, attend(torch, b, kind), norm=0)
+
+
 @pytest.mark.parametrize("kind", ["bf16", "f32"])
 @pytest.mark.parametrize("n_req", [2, 66, 130, 700])
 def test_attention_idle_requests(torch, kind, n_req):

@@ -234,7 +234,7 @@ struct Walk {
                     run.kvh = 0;
                     if (++run.r == a.requests) return false;
                     req = request_at(a, run.r);
-                    if (req.vecs == 0) {
+                    if (__builtin_expect(req.vecs == 0, 0)) {
                         run.r = __builtin_amdgcn_readfirstlane(with_rows(a, run.r));
                         if (run.r == a.requests) return false;
                         req = request_at(a, run.r);
@@ -1257,10 +1257,16 @@ struct Plan {
     bool wide;
 };
 
-// Chunks (many vectors of an average request and kv head), or not. Blocks: as many as the registers of their
-// waves leave room for.
+// Chunks (many vectors of an average request and kv head), or not: a chunk's block takes 128 vectors a key read, but
+// shares steps of 32 keys behind a barrier each, and in a batch of prompts and single tokens most of its vectors are
+// none. Eight requests with up to this many rows behind up to 2000 positions, bf16 (f32), one way and the other:
+//   28 heads over 4 of 128   20 rows  51 | 54 us (70 | 91)   100 rows  65 | 64 us (119 | 123)   200 rows  107 | 84 us (231 | 198)
+//   32 heads over 8 of 64    10 rows  31 | 29 us (40 | 43)    15 rows  37 | 28 us  (50 | 42)     80 rows   48 | 38 us  (79 | 71)
+// and 63 single tokens with one prompt of 500 rows, heads of 128: 100 | 139 us.
+// Blocks: as many as the registers of their waves leave room for, two or three on a CU (three, heads of 64: 24 x 5 rows
+// in f32 58 us against 65 with two, 300 x 1 row in bf16 66 against 73; 64 x 1 row behind 8000 135 against 125).
 Plan plan_of(uint32_t rows, uint32_t requests, uint32_t group, uint32_t hd) {
-    const bool wide = static_cast<uint64_t>(rows) * group > uint64_t{48} * requests;
+    const bool wide = static_cast<uint64_t>(rows) * group > uint64_t{hd == 128 ? 384u : 48u} * requests;
     return Plan{wide ? 128u : 64u, gemm_cus() * (wide || hd == 128 ? 2 : 3), wide};
 }
 

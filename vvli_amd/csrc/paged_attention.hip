@@ -127,6 +127,7 @@ __device__ __forceinline__ uint64_t request_units(const PagedAttnArgs& a, const 
 struct Run {
     uint64_t from, to, per;  // global units, before the borders move
     uint32_t near_lo, near_hi, r, kvh, m0, unit;  // the item that holds unit `from`, and which unit of it that is
+    uint32_t index;
     bool any;
 };
 
@@ -141,8 +142,8 @@ struct RunScratch {
 };
 
 template <int M, int WK, bool FIXED>
-__device__ Run find_run(const PagedAttnArgs& a, uint32_t block, uint32_t blocks, RunScratch& sc) {
-    const uint32_t tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+__device__ Run find_run(const PagedAttnArgs& a, RunScratch& sc) {
+    const uint32_t blocks = gridDim.x, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     const uint32_t chunks = (a.requests + kThreads - 1) / kThreads;
     uint64_t mine = 0, end = 0, before = 0;
     auto chunk = [&](uint32_t c) {  // this thread's request's units, and the sum up to it
@@ -165,9 +166,13 @@ __device__ Run find_run(const PagedAttnArgs& a, uint32_t block, uint32_t blocks,
     run.near_hi = static_cast<uint32_t>(min(run.per / 4, static_cast<uint64_t>(kCutUnits)));
     run.near_lo = max(run.near_hi, kItemUnits);
     static_assert(kItemUnits + kFewestUnits / 4 < kFewestUnits, "near_lo + near_hi < per");
-    run.from = run.per * block;
+    // Blocks go to the eight XCDs in turn. Each XCD takes as many runs, side by side: neighbours share keys and table
+    // rows in its L2, and fewer runs than blocks still have all of the GPU.
+    const uint32_t runs = static_cast<uint32_t>(quotient(total + run.per - 1, run.per)), each = (runs + 7) / 8;
+    run.index = blocks % 8 == 0 ? blockIdx.x % 8 * each + blockIdx.x / 8 : blockIdx.x;
+    if (run.index >= runs || (blocks % 8 == 0 && blockIdx.x / 8 >= each)) return run;
+    run.from = run.per * run.index;
     run.to = min(run.from + run.per, total);
-    if (run.from >= total) return run;
     run.any = true;
     before = 0;
     for (uint32_t c = 0; c < chunks; ++c) {
@@ -463,10 +468,7 @@ __global__ __launch_bounds__(kThreads, HD == 128 ? 2 : 3) void paged_attn_kernel
     __shared__ RunScratch sc;
     __shared__ __attribute__((aligned(16))) float shared[F::kShared];
 
-    const uint32_t blocks = gridDim.x;
-    // Neighbouring runs on one XCD (blocks go to the eight in turn): they share keys and table rows in its L2.
-    const uint32_t block = blocks % 8 == 0 ? blockIdx.x % 8 * (blocks / 8) + blockIdx.x / 8 : blockIdx.x;
-    const Run from = find_run<M, WK, false>(a, block, blocks, sc);
+    const Run from = find_run<M, WK, false>(a, sc);
     if (!from.any) return;
     const int tid = threadIdx.x, lane = tid & 63, fr = lane & 15, fq = lane >> 4;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -796,7 +798,7 @@ __global__ __launch_bounds__(kThreads, HD == 128 ? 2 : 3) void paged_attn_kernel
             const float r = 1.f / l;
             *reinterpret_cast<f32x4*>(op) = l == 0.f ? f32x4{0, 0, 0, 0} : x * r;
         };
-        float* slot = a.parts + (2 * static_cast<size_t>(block) + (t0 == 0)) * slot_words;
+        float* slot = a.parts + (2 * static_cast<size_t>(run.index) + (t0 == 0)) * slot_words;
         for (uint32_t i = tid; i < vecs * (HD / 4); i += kThreads) {
             const uint32_t v = i / (HD / 4), d = i % (HD / 4) * 4, vq = v / WV, vv = v % WV;
             float top = -INFINITY;
@@ -927,9 +929,7 @@ __global__ __launch_bounds__(kThreads, 2) void paged_wide_kernel(PagedAttnArgs a
     __shared__ __attribute__((aligned(1024))) char stage[2][2 * TILE];  // keys, then values
     __shared__ __attribute__((aligned(16))) char q_rest[F::kQ ? F::kQ : 16];
 
-    const uint32_t blocks = gridDim.x;
-    const uint32_t block = blocks % 8 == 0 ? blockIdx.x % 8 * (blocks / 8) + blockIdx.x / 8 : blockIdx.x;
-    const Run from = find_run<M, WK, true>(a, block, blocks, sc);
+    const Run from = find_run<M, WK, true>(a, sc);
     if (!from.any) return;
     const int tid = threadIdx.x, lane = tid & 63, fr = lane & 31, half = lane >> 5;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -1214,7 +1214,7 @@ __global__ __launch_bounds__(kThreads, 2) void paged_wide_kernel(PagedAttnArgs a
         // A part is an image of the threads' registers, 8 bytes of each thread side by side; then maxima and sums.
         constexpr int IMAGE = NT * 16 * kThreads;
         static_assert(IMAGE == M * HD, "a part has its slot");
-        float* slot = a.parts + (2 * static_cast<size_t>(block) + (walk.t0 == 0)) * slot_words;
+        float* slot = a.parts + (2 * static_cast<size_t>(run.index) + (walk.t0 == 0)) * slot_words;
 #pragma unroll
         for (int n = 0; n < NT; ++n)
 #pragma unroll

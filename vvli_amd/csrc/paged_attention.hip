@@ -14,11 +14,18 @@
 // units of all items, in the order (request, kv head, vectors, keys), are cut
 // into equal runs, one for each block: no batch, whatever its lengths, leaves
 // blocks with more to do than others. An item that a run's end cuts leaves its
-// parts in the workspace and a second kernel joins them in order of keys, so
-// results do not depend on timing.
+// parts in the workspace, and the block whose part is there last joins all of
+// them in order of keys, so results do not depend on timing.
+//
+// Two kernels: one for few rows a request (single tokens, drafts), which reads
+// the cache at memory's rate, and one for prompts' chunks, which matrix products
+// bound. What they do not take from either is the chain of a short call: some
+// 3 us to find a block's run, 2 to an item's first keys, 1 to 2 a step and 5 to
+// 10 for an item's parts.
 #include <hip/hip_fp16.h>
 
 #include <algorithm>
+#include <type_traits>
 
 #include "device_common.hpp"
 #include "paged.hpp"
@@ -34,12 +41,6 @@ typedef float f32x16 __attribute__((ext_vector_type(16)));
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 
 constexpr int kThreads = 256;
-// What an item costs beside its keys (its q, the first loads, its end), in
-// units; what a cut costs (a part left and taken up again); the fewest units of
-// a run; the most units of an item that is never cut, since its parts would
-// cost more than they save.
-constexpr uint32_t kItemUnits = 3, kCutUnits = 4, kFewestUnits = 5, kWholeUnits = 12;
-
 struct PagedAttnArgs {
     const void *k, *v;
     const int32_t *table, *row_start, *start_pos;
@@ -66,27 +67,41 @@ __device__ __forceinline__ Request request_at(const PagedAttnArgs& a, uint32_t r
     return Request{s.first, s.count * a.group.d, a.start_pos[r]};
 }
 
+// How a kernel cuts its items: M vectors, steps of WK positions, units of one
+// step (FIXED) or of as many as the block's waves take side by side; and in
+// units what an item costs beside its keys (its q, the first loads, its end),
+// what a cut costs (a part left and taken up again), the fewest of a run, and
+// the most of an item that is never cut, since its parts would cost more than
+// they save.
+template <int M_, int WK_, bool FIXED_, uint32_t ITEM, uint32_t CUT, uint32_t FEWEST, uint32_t WHOLE>
+struct Cuts {
+    static constexpr int M = M_, WK = WK_;
+    static constexpr bool FIXED = FIXED_;
+    static constexpr uint32_t kItem = ITEM, kCut = CUT, kFewest = FEWEST, kWhole = WHOLE;
+    static_assert(ITEM + std::min(FEWEST / 4, CUT) < FEWEST, "near_lo + near_hi < per");
+};
+
 // An item's vectors stand in groups of GV = M / 4, one to a wave: 1, 2 or 4
 // waves side by side (the log of that in `wide`) take different vectors, and
 // the 4 >> wide such sets take steps of WK positions in turn, (4 WK) >> wide a
 // unit. The keys lo .. hi - 1 that some vector of the item sees (hi = 0: none),
-// and the units that they touch, behind kItemUnits for the item itself.
+// and the units that they touch, behind S::kItem for the item itself.
 struct Units {
     uint32_t lo, hi, first, count, wide;
 };
 // (FIXED: units of WK positions whatever the item.)
-template <int M, int WK, bool FIXED>
+template <class S>
 __device__ __forceinline__ Units units_of(const PagedAttnArgs& a, const Request& q, uint32_t m0) {
-    const uint32_t vecs = min(static_cast<uint32_t>(M), q.vecs - m0);
-    const uint32_t wide = vecs <= M / 4 ? 0 : vecs <= M / 2 ? 1 : 2;
+    const uint32_t vecs = min(static_cast<uint32_t>(S::M), q.vecs - m0);
+    const uint32_t wide = vecs <= S::M / 4 ? 0 : vecs <= S::M / 2 ? 1 : 2;
     const int64_t p0 = q.start + page_of(a.group, m0);
     const int64_t p1 = q.start + page_of(a.group, m0 + vecs - 1);
     const int64_t hi = min(p1 + 1, static_cast<int64_t>(a.room));
     const int64_t lo = a.window && p0 + 1 > a.window ? p0 + 1 - a.window : 0;
-    if (hi <= lo) return Units{0, 0, 0, kItemUnits, wide};
-    const uint32_t unit = FIXED ? WK : (4 * WK) >> wide;
+    if (hi <= lo) return Units{0, 0, 0, S::kItem, wide};
+    const uint32_t unit = S::FIXED ? S::WK : (4 * S::WK) >> wide;
     Units u{static_cast<uint32_t>(lo), static_cast<uint32_t>(hi), static_cast<uint32_t>(lo) / unit, 0, wide};
-    u.count = (u.hi + unit - 1) / unit - u.first + kItemUnits;
+    u.count = (u.hi + unit - 1) / unit - u.first + S::kItem;
     return u;
 }
 
@@ -102,17 +117,17 @@ __device__ __forceinline__ uint64_t wave_scan(uint64_t v) {
 
 // Units of one kv head of each lane's request, summed over its items: by the
 // lane itself where they are few, else by its wave.
-template <int M, int WK, bool FIXED>
+template <class S>
 __device__ __forceinline__ uint64_t request_units(const PagedAttnArgs& a, const Request& q) {
-    const uint32_t lane = threadIdx.x & 63, items = (q.vecs + M - 1) / M;
+    const uint32_t lane = threadIdx.x & 63, items = (q.vecs + S::M - 1) / S::M;
     uint64_t sum = 0;
     if (items <= 2)
-        for (uint32_t i = 0; i < items; ++i) sum += units_of<M, WK, FIXED>(a, q, i * M).count;
+        for (uint32_t i = 0; i < items; ++i) sum += units_of<S>(a, q, i * S::M).count;
     for (uint64_t todo = __ballot(items > 2); todo; todo &= todo - 1) {
         const int from = __builtin_ctzll(todo);
         const Request f{static_cast<uint32_t>(__shfl(q.first, from, 64)), static_cast<uint32_t>(__shfl(q.vecs, from, 64)), __shfl(q.start, from, 64)};
         uint64_t s = 0;
-        for (uint32_t i = lane; i < (f.vecs + M - 1) / M; i += 64) s += units_of<M, WK, FIXED>(a, f, i * M).count;
+        for (uint32_t i = lane; i < (f.vecs + S::M - 1) / S::M; i += 64) s += units_of<S>(a, f, i * S::M).count;
 #pragma unroll
         for (int o = 32; o; o >>= 1) s += __shfl_xor(s, o, 64);
         if (static_cast<int>(lane) == from) sum = s;
@@ -141,14 +156,14 @@ struct RunScratch {
     uint32_t found_r, last;
 };
 
-template <int M, int WK, bool FIXED>
+template <class S>
 __device__ Run find_run(const PagedAttnArgs& a, RunScratch& sc) {
     const uint32_t blocks = gridDim.x, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     const uint32_t chunks = (a.requests + kThreads - 1) / kThreads;
     uint64_t mine = 0, end = 0, before = 0;
     auto chunk = [&](uint32_t c) {  // this thread's request's units, and the sum up to it
         const uint32_t r = c * kThreads + tid;
-        mine = request_units<M, WK, FIXED>(a, r < a.requests ? request_at(a, r) : Request{0, 0, 0});
+        mine = request_units<S>(a, r < a.requests ? request_at(a, r) : Request{0, 0, 0});
         const uint64_t s = wave_scan(mine);
         __syncthreads();
         if (lane == 63) sc.sums[wave] = s;
@@ -162,10 +177,9 @@ __device__ Run find_run(const PagedAttnArgs& a, RunScratch& sc) {
     for (uint32_t c = 0; c < chunks; ++c) chunk(c);
     const uint64_t total = before * a.kv_heads;
     Run run{};
-    run.per = max(quotient(total + blocks - 1, blocks), static_cast<uint64_t>(kFewestUnits));
-    run.near_hi = static_cast<uint32_t>(min(run.per / 4, static_cast<uint64_t>(kCutUnits)));
-    run.near_lo = max(run.near_hi, kItemUnits);
-    static_assert(kItemUnits + kFewestUnits / 4 < kFewestUnits, "near_lo + near_hi < per");
+    run.per = max(quotient(total + blocks - 1, blocks), static_cast<uint64_t>(S::kFewest));
+    run.near_hi = static_cast<uint32_t>(min(run.per / 4, static_cast<uint64_t>(S::kCut)));
+    run.near_lo = max(run.near_hi, S::kItem);
     // Blocks go to the eight XCDs in turn. Each XCD takes as many runs, side by side: neighbours share keys and table
     // rows in its L2, and fewer runs than blocks still have all of the GPU.
     const uint32_t runs = static_cast<uint32_t>(quotient(total + run.per - 1, run.per)), each = (runs + 7) / 8;
@@ -187,13 +201,13 @@ __device__ Run find_run(const PagedAttnArgs& a, RunScratch& sc) {
     uint64_t v = rest - run.kvh * units;
     const Request q = request_at(a, run.r);
     for (uint32_t i = 0;; i += 64) {  // every wave by itself: the item that holds unit v
-        const uint32_t m = (i + lane) * M;
-        const uint64_t s = wave_scan(m < q.vecs ? units_of<M, WK, FIXED>(a, q, m).count : 0);
+        const uint32_t m = (i + lane) * S::M;
+        const uint64_t s = wave_scan(m < q.vecs ? units_of<S>(a, q, m).count : 0);
         const uint64_t past = __ballot(s > v);
-        if (past || (i + 64) * M >= q.vecs) {
+        if (past || (i + 64) * S::M >= q.vecs) {
             const int at = past ? __builtin_ctzll(past) : 0;
             const uint64_t prev = __shfl(s, at ? at - 1 : 0, 64);
-            run.m0 = __builtin_amdgcn_readfirstlane((i + at) * M);
+            run.m0 = __builtin_amdgcn_readfirstlane((i + at) * S::M);
             run.unit = __builtin_amdgcn_readfirstlane(static_cast<uint32_t>(at ? v - prev : v));
             return run;
         }
@@ -203,7 +217,7 @@ __device__ Run find_run(const PagedAttnArgs& a, RunScratch& sc) {
 
 // A block's way through its run: the item that it is at, and which of the
 // item's units are its own.
-template <int M, int WK, bool FIXED>
+template <class S>
 struct Walk {
     Run run;
     Request req;
@@ -211,8 +225,8 @@ struct Walk {
     bool begun;      // the run starts inside the item
     Units un;
     uint32_t t0, t1;  // units of the item
-    __device__ __forceinline__ uint32_t first_unit() const { return un.first + (t0 > kItemUnits ? t0 - kItemUnits : 0); }  // of its keys
-    __device__ __forceinline__ uint32_t end_unit() const { return un.first + (t1 > kItemUnits ? t1 - kItemUnits : 0); }
+    __device__ __forceinline__ uint32_t first_unit() const { return un.first + (t0 > S::kItem ? t0 - S::kItem : 0); }  // of its keys
+    __device__ __forceinline__ uint32_t end_unit() const { return un.first + (t1 > S::kItem ? t1 - S::kItem : 0); }
     bool cut;         // the run ends inside the item
 
     __device__ __forceinline__ explicit Walk(const PagedAttnArgs& a, const Run& r) : run(r) {
@@ -246,8 +260,8 @@ struct Walk {
                     }
                 }
             }
-            un = units_of<M, WK, FIXED>(a, req, run.m0);
-            const uint32_t lo = un.count <= kWholeUnits ? un.count - 1 : run.near_lo;
+            un = units_of<S>(a, req, run.m0);
+            const uint32_t lo = un.count <= S::kWhole ? un.count - 1 : run.near_lo;
             begun = begun && run.unit > lo;  // (a border near an item's start is its start)
             if (begun && un.count - run.unit <= run.near_hi) {  // what is left of it is the last run's
                 next();
@@ -260,8 +274,8 @@ struct Walk {
             return true;
         }
     }
-    __device__ __forceinline__ void next() { start += un.count, run.m0 += M, begun = false; }
-    __device__ __forceinline__ uint32_t vecs() const { return min(static_cast<uint32_t>(M), req.vecs - run.m0); }
+    __device__ __forceinline__ void next() { start += un.count, run.m0 += S::M, begun = false; }
+    __device__ __forceinline__ uint32_t vecs() const { return min(static_cast<uint32_t>(S::M), req.vecs - run.m0); }
     __device__ __forceinline__ bool whole() const { return t0 == 0 && t1 == un.count; }
     // Borders inside the item, from near_lo behind its start to near_hi before its end: run first_border() - 1 has
     // its first part (in its second slot), the runs from first_border() on the others (in their first).
@@ -386,11 +400,22 @@ __device__ __forceinline__ int f16_exponent(float top) {
 //                   keys; 16-bit pairs of keys are put together by v_perm
 // The first term of q stays in registers, the others in LDS: two waves fit a
 // SIMD, one's products beside the other's exponentials.
+//
+// Keys and values from memory bound it where requests are many or long: 40 rows
+// behind up to 8000 positions, 28 heads over 4 of 128, bf16, 84 us, 4.4 TB/s (a
+// copy reaches 4.8 to 5.4); 64 behind up to 4000, 16 heads over 16 of 128, 242
+// us, 5.4 TB/s, and 6.1 in f32. The chain named above does where they are few:
+// 1 row behind 230, 8 kv heads of 64, f32, 11 us; behind 8000, 4 kv heads, bf16,
+// 23 us; 24 x 5 rows behind up to 4100, f16, 40 us, 2.8 TB/s.
 // ---------------------------------------------------------------------------
 template <int HD, int KIND, int GI>
 struct Form {
     using K = Kind<KIND>;
     static constexpr int WV = 16 * GI, M = 4 * WV, U = K::U, WK = 16 * U, DV = HD / 16;
+    // (An item at 1 and not 3 units: 24 x 5 rows of heads of 64 40.9 us and not 37.0. Runs from 10 units on and not 5:
+    // 45.7, and 1 x 1 row behind 2000 positions 26.9 and not 21.0. Items whole up to 24 units and not 12: 40 x 1 row behind
+    // 8000 102 and not 84; up to none: 1 x 1 row behind 500 15.1 and not 14.3.)
+    using S = Cuts<M, WK, false, 3, 4, 5, 12>;
     static constexpr int KL = HD * K::BYTES / 64;   // 16-byte loads of a key row by a lane
     static constexpr int VW = DV * K::BYTES / 4;    // 32-bit words of a value row in a lane
     struct Step {
@@ -463,18 +488,18 @@ template <int HD, int KIND, int GI>
 __global__ __launch_bounds__(kThreads, HD == 128 ? 2 : 3) void paged_attn_kernel(PagedAttnArgs a) {
     using F = Form<HD, KIND, GI>;
     using K = Kind<KIND>;
-    constexpr int M = F::M, WV = F::WV, U = F::U, WK = F::WK, DV = F::DV, KL = F::KL, VW = F::VW, ROW = F::ROW;
+    constexpr int WV = F::WV, U = F::U, WK = F::WK, DV = F::DV, KL = F::KL, VW = F::VW, ROW = F::ROW;
     constexpr bool F32 = KIND == VVLI_CACHE_F32;
     __shared__ RunScratch sc;
     __shared__ __attribute__((aligned(16))) float shared[F::kShared];
 
-    const Run from = find_run<M, WK, false>(a, sc);
+    const Run from = find_run<typename F::S>(a, sc);
     if (!from.any) return;
     const int tid = threadIdx.x, lane = tid & 63, fr = lane & 15, fq = lane >> 4;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const uint64_t row_bytes = a.slot_stride * K::BYTES;
     const uint32_t slot_words = a.slot_vecs * (HD + 2);
-    for (Walk<M, WK, false> walk(a, from); walk.item(a); walk.next()) {
+    for (Walk<typename F::S> walk(a, from); walk.item(a); walk.next()) {
         const Run& run = walk.run;
         const Request& req = walk.req;
         const Units& un = walk.un;
@@ -890,13 +915,23 @@ __global__ __launch_bounds__(kThreads, HD == 128 ? 2 : 3) void paged_attn_kernel
 //                  by a transposed read of LDS (ds_read_b64_tr_b16); D: dims
 //                  32 n + 8 (r / 4) + 4 (l / 32) + r % 4
 // Rows lie in LDS as in memory, their 16-byte chunks permuted by the row so that
-// the rows of a fragment read fall on different banks.
+// the rows of a fragment read fall on different banks (no conflict is counted).
+//
+// Products bound it: 4000 rows behind 8000, 28 heads over 4 of 128, 4.6 ms in f32
+// (125 of the 133 TFLOP/s that a large product reaches), 1.2 ms in f16 (479, times
+// two terms 959 of 1310) and 1.45 ms in bf16 (397, times three terms 1190 of
+// 1200). Short chunks are bound by the runs' ends: 2 x up to 2000 rows behind up
+// to 2100 in bf16 267 us (343, 1030 with terms).
 // ---------------------------------------------------------------------------
 template <int HD, int KIND>
 struct Wide {
     using K = Kind<KIND>;
     static constexpr bool F32 = KIND == VVLI_CACHE_F32;
     static constexpr int WV = 32, M = 128, WK = 32, NT = HD / 32, DS = HD * K::BYTES / 32;
+    // (A step takes two to four times as long in f32, so that the rest costs fewer of them: 100 rows behind 200, heads of
+    // 128, 55 us at 16 bits' numbers and 35 at these, 3 x 333 rows of heads of 64 42 and 37. What a cut costs, without a
+    // bound at a quarter of a run: 2 x 2000 rows bf16 317 us, with 4 units 269.)
+    using S = std::conditional_t<F32, Cuts<M, WK, true, 2, 2, 3, 0>, Cuts<M, WK, true, 3, 4, 5, 0>>;
     static constexpr int RB = HD * K::BYTES, CH = RB / 16, RPL = RB < 256 ? 256 / RB : 1;  // bytes and 16-byte chunks of a row, rows of 256 bytes
     static constexpr int TILE = WK * RB, LOADS = 2 * TILE / (16 * kThreads), ROWS = LOADS > 1 ? LOADS / 2 : 1;
     static constexpr int QR = F32 ? 1 : 2;  // terms of q in registers; the rest in LDS
@@ -929,7 +964,7 @@ __global__ __launch_bounds__(kThreads, 2) void paged_wide_kernel(PagedAttnArgs a
     __shared__ __attribute__((aligned(1024))) char stage[2][2 * TILE];  // keys, then values
     __shared__ __attribute__((aligned(16))) char q_rest[F::kQ ? F::kQ : 16];
 
-    const Run from = find_run<M, WK, true>(a, sc);
+    const Run from = find_run<typename F::S>(a, sc);
     if (!from.any) return;
     const int tid = threadIdx.x, lane = tid & 63, fr = lane & 31, half = lane >> 5;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -944,7 +979,7 @@ __global__ __launch_bounds__(kThreads, 2) void paged_wide_kernel(PagedAttnArgs a
     // This thread's rows of a step (the same of keys and of values; HD = 32: of one of the two) and its chunk.
     const uint32_t my_row = tid % (WK * CH / ROWS) / CH, my_c = tid % CH;
 
-    for (Walk<M, WK, true> walk(a, from); walk.item(a); walk.next()) {
+    for (Walk<typename F::S> walk(a, from); walk.item(a); walk.next()) {
         const Run& run = walk.run;
         const Request& req = walk.req;
         const Units& un = walk.un;
@@ -1259,12 +1294,12 @@ struct Plan {
 
 // Chunks (many vectors of an average request and kv head), or not: a chunk's block takes 128 vectors a key read, but
 // shares steps of 32 keys behind a barrier each, and in a batch of prompts and single tokens most of its vectors are
-// none. Eight requests with up to this many rows behind up to 2000 positions, bf16 (f32), one way and the other:
-//   28 heads over 4 of 128   20 rows  51 | 54 us (70 | 91)   100 rows  65 | 64 us (119 | 123)   200 rows  107 | 84 us (231 | 198)
-//   32 heads over 8 of 64    10 rows  31 | 29 us (40 | 43)    15 rows  37 | 28 us  (50 | 42)     80 rows   48 | 38 us  (79 | 71)
-// and 63 single tokens with one prompt of 500 rows, heads of 128: 100 | 139 us.
-// Blocks: as many as the registers of their waves leave room for, two or three on a CU (three, heads of 64: 24 x 5 rows
-// in f32 58 us against 65 with two, 300 x 1 row in bf16 66 against 73; 64 x 1 row behind 8000 135 against 125).
+// none. Eight requests with up to so many rows behind up to 2000 positions, not as chunks | as chunks, bf16 (f32):
+//   28 heads over 4 of 128   20 rows  51 | 59 us (70 | 91)   100 rows  63 | 63 us (109 | 113)   200 rows  105 | 84 us (228 | 200)
+//   32 heads over 8 of 64    10 rows  26 | 30 us (43 | 45)    15 rows  29 | 29 us  (44 | 45)     80 rows   49 | 36 us  (77 | 70)
+// and 63 single tokens with one prompt of 500 rows, heads of 128: 99 | 144 us.
+// Blocks: as many as the registers of their waves leave room for, two or three on a CU (three and not two, heads of 64:
+// 24 x 5 rows in f32 58 and not 64 us, 300 x 1 row in bf16 67 and not 73; but 64 x 1 row behind 8000 136 and not 123).
 Plan plan_of(uint32_t rows, uint32_t requests, uint32_t group, uint32_t hd) {
     const bool wide = static_cast<uint64_t>(rows) * group > uint64_t{hd == 128 ? 384u : 48u} * requests;
     return Plan{wide ? 128u : 64u, gemm_cus() * (wide || hd == 128 ? 2 : 3), wide};

@@ -4,7 +4,9 @@
 //
 // y = x * (mean(x^2) + eps)^(-1/2) * w, then each pair (a, b) of a head turns
 // by pos * inv_freq[i]: (a cos - b sin, b cos + a sin). Nothing is reused
-// between rows, so memory bounds it.
+// between rows, so memory bounds it: 6000 rows of 28 + 8 heads of 128 into an
+// f16 cache 47.7 us, 4.4 TB/s, 20000 rows 140 us, 5.0 TB/s (a copy reaches 4.8
+// to 5.4); 75 rows 5.5 us and 1 row 5.4 us are a launch and its chain of loads.
 //
 // A wave takes heads of one row: HD / 4 lanes a head, 4 values a lane, as many
 // heads side by side as fit. A lane's values are two pairs, the same ones in
@@ -139,7 +141,8 @@ __global__ __launch_bounds__(kThreads) void norm_rope_kernel(NormRopeArgs a) {
 template <int HD, typename T>
 hipError_t launch(NormRopeArgs& a, hipStream_t s) {
     // Waves of a row: one where the rows alone fill the GPU (a wave's angles then serve all heads of the row),
-    // more down to a wave for each turn where they do not.
+    // more down to a wave for each turn where they do not. (Waves for 16 a CU: 1000 rows 11.5 us, 2000 15.7; for
+    // 64 a CU 15.5 and 18.2. 300 and 6000 rows take the same with either.)
     constexpr uint32_t SIDE = 256 / HD;
     const uint32_t turns = (a.heads + 2 * a.kv_heads + SIDE - 1) / SIDE;
     const uint32_t fill = gemm_cus() * 16;

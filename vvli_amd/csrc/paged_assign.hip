@@ -109,7 +109,8 @@ __device__ __forceinline__ void put_row(const AssignArgs& a, uint32_t i, uint32_
 // One block: what the pages of a request are depends on all requests before it.
 // Sums over the requests (a chunk of 1024 at a time, one chunk kept in
 // registers), the given pages, the taken ones and, where they are few, the new
-// rows follow one another with a barrier between; latency bounds it.
+// rows follow one another with a barrier between; latency bounds it (48 requests
+// of one row each 9.2 us, 300 of up to 130 rows 13.9 with assign_rows_kernel).
 __global__ __launch_bounds__(kThreads) void assign_kernel(AssignArgs a, bool with_rows) {
     __shared__ Scratch sc;
     const uint32_t tid = threadIdx.x, chunks = (a.requests + kThreads - 1) / kThreads;
@@ -192,7 +193,8 @@ __global__ __launch_bounds__(256) void assign_rows_kernel(AssignArgs a) {
     put_row(a, i, lo, a.start_pos[lo], a.row_start[lo]);
 }
 
-// Rows that the one block places itself; more are worth a launch over the GPU.
+// Rows that the one block places itself; more are worth a launch over the GPU
+// (400 rows: 10.9 us in the block, 13.9 with the launch; 39000: 27 and 15).
 constexpr uint32_t kRowsInBlock = 2048;
 
 }  // namespace

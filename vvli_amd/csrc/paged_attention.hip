@@ -143,6 +143,7 @@ struct Run {
     uint64_t from, to, per;  // global units, before the borders move
     uint32_t near_lo, near_hi, r, kvh, m0, unit;  // the item that holds unit `from`, and which unit of it that is
     uint32_t index;
+    Request req;  // of r
     bool any;
 };
 
@@ -153,6 +154,7 @@ __device__ __forceinline__ uint64_t quotient(uint64_t n, uint64_t d) {
 
 struct RunScratch {
     uint64_t sums[kThreads / 64], found_rest, found_units;
+    Request found;
     uint32_t found_r, last;
 };
 
@@ -161,9 +163,11 @@ __device__ Run find_run(const PagedAttnArgs& a, RunScratch& sc) {
     const uint32_t blocks = gridDim.x, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     const uint32_t chunks = (a.requests + kThreads - 1) / kThreads;
     uint64_t mine = 0, end = 0, before = 0;
+    Request own{};
     auto chunk = [&](uint32_t c) {  // this thread's request's units, and the sum up to it
         const uint32_t r = c * kThreads + tid;
-        mine = request_units<S>(a, r < a.requests ? request_at(a, r) : Request{0, 0, 0});
+        own = r < a.requests ? request_at(a, r) : Request{0, 0, 0};
+        mine = request_units<S>(a, own);
         const uint64_t s = wave_scan(mine);
         __syncthreads();
         if (lane == 63) sc.sums[wave] = s;
@@ -192,14 +196,17 @@ __device__ Run find_run(const PagedAttnArgs& a, RunScratch& sc) {
     for (uint32_t c = 0; c < chunks; ++c) {
         if (chunks > 1) chunk(c);
         const uint64_t lo = (end - mine) * a.kv_heads;
-        if (mine && run.from >= lo && run.from < end * a.kv_heads) sc.found_r = c * kThreads + tid, sc.found_rest = run.from - lo, sc.found_units = mine;
+        if (mine && run.from >= lo && run.from < end * a.kv_heads)
+            sc.found_r = c * kThreads + tid, sc.found = own, sc.found_rest = run.from - lo, sc.found_units = mine;
     }
     __syncthreads();
     run.r = __builtin_amdgcn_readfirstlane(sc.found_r);
     const uint64_t rest = sc.found_rest, units = sc.found_units;
     run.kvh = __builtin_amdgcn_readfirstlane(static_cast<uint32_t>(quotient(rest, units)));
     uint64_t v = rest - run.kvh * units;
-    const Request q = request_at(a, run.r);
+    const Request q{static_cast<uint32_t>(__builtin_amdgcn_readfirstlane(sc.found.first)), static_cast<uint32_t>(__builtin_amdgcn_readfirstlane(sc.found.vecs)),
+                    __builtin_amdgcn_readfirstlane(static_cast<int32_t>(sc.found.start))};
+    run.req = q;
     for (uint32_t i = 0;; i += 64) {  // every wave by itself: the item that holds unit v
         const uint32_t m = (i + lane) * S::M;
         const uint64_t s = wave_scan(m < q.vecs ? units_of<S>(a, q, m).count : 0);
@@ -230,7 +237,7 @@ struct Walk {
     bool cut;         // the run ends inside the item
 
     __device__ __forceinline__ explicit Walk(const PagedAttnArgs& a, const Run& r) : run(r) {
-        req = request_at(a, run.r);
+        req = run.req;
         start = run.from - run.unit;
         begun = true;
     }

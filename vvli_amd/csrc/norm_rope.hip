@@ -93,11 +93,14 @@ __global__ __launch_bounds__(kThreads) void norm_rope_kernel(NormRopeArgs a) {
 #pragma unroll
         for (int n = 0; n < N; ++n) {
             const uint32_t h = h0 + n * step;
-            const float* p = h < a.heads ? qr + static_cast<size_t>(h) * HD : h < turned ? kr + static_cast<size_t>(h - a.heads) * HD : vr + static_cast<size_t>(h - turned) * HD;
+            const float* p = h < a.heads ? qr + static_cast<size_t>(h) * HD
+                             : h < turned ? kr + static_cast<size_t>(h - a.heads) * HD
+                                          : vr + static_cast<size_t>(h - turned) * HD;
             if (h < heads) {
                 if constexpr (SPLIT) {
                     const uint2 u = load_u32x2(p + at0), v = load_u32x2(p + at1);
-                    x[n][0] = __uint_as_float(u.x), x[n][1] = __uint_as_float(u.y), x[n][2] = __uint_as_float(v.x), x[n][3] = __uint_as_float(v.y);
+                    x[n][0] = __uint_as_float(u.x), x[n][1] = __uint_as_float(u.y);
+                    x[n][2] = __uint_as_float(v.x), x[n][3] = __uint_as_float(v.y);
                 } else {
                     const float4 u = load_f32x4(p + at0);
                     x[n][0] = u.x, x[n][1] = u.y, x[n][2] = u.z, x[n][3] = u.w;
@@ -149,12 +152,15 @@ hipError_t launch(NormRopeArgs& a, hipStream_t s) {
     a.chunks = std::min(turns, std::max(1u, fill / a.rows));
     const uint64_t blocks = (static_cast<uint64_t>(a.rows) * a.chunks + kThreads / 64 - 1) / (kThreads / 64);
     const dim3 grid(static_cast<uint32_t>(blocks)), block(kThreads);
-    return a.split ? vlaunch(norm_rope_kernel<HD, T, true>, grid, block, 0, s, a) : vlaunch(norm_rope_kernel<HD, T, false>, grid, block, 0, s, a);
+    return a.split ? vlaunch(norm_rope_kernel<HD, T, true>, grid, block, 0, s, a)
+                   : vlaunch(norm_rope_kernel<HD, T, false>, grid, block, 0, s, a);
 }
 
 template <int HD>
 hipError_t launch(NormRopeArgs& a, uint32_t kind, hipStream_t s) {
-    return kind == VVLI_CACHE_F32 ? launch<HD, float>(a, s) : kind == VVLI_CACHE_BF16 ? launch<HD, __bf16>(a, s) : launch<HD, _Float16>(a, s);
+    return kind == VVLI_CACHE_F32 ? launch<HD, float>(a, s)
+           : kind == VVLI_CACHE_BF16 ? launch<HD, __bf16>(a, s)
+                                     : launch<HD, _Float16>(a, s);
 }
 
 }  // namespace

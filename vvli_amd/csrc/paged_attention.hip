@@ -125,7 +125,8 @@ __device__ __forceinline__ uint64_t request_units(const PagedAttnArgs& a, const 
         for (uint32_t i = 0; i < items; ++i) sum += units_of<S>(a, q, i * S::M).count;
     for (uint64_t todo = __ballot(items > 2); todo; todo &= todo - 1) {
         const int from = __builtin_ctzll(todo);
-        const Request f{static_cast<uint32_t>(__shfl(q.first, from, 64)), static_cast<uint32_t>(__shfl(q.vecs, from, 64)), __shfl(q.start, from, 64)};
+        const Request f{static_cast<uint32_t>(__shfl(q.first, from, 64)), static_cast<uint32_t>(__shfl(q.vecs, from, 64)),
+                        __shfl(q.start, from, 64)};
         uint64_t s = 0;
         for (uint32_t i = lane; i < (f.vecs + S::M - 1) / S::M; i += 64) s += units_of<S>(a, f, i * S::M).count;
 #pragma unroll
@@ -204,7 +205,8 @@ __device__ Run find_run(const PagedAttnArgs& a, RunScratch& sc) {
     const uint64_t rest = sc.found_rest, units = sc.found_units;
     run.kvh = __builtin_amdgcn_readfirstlane(static_cast<uint32_t>(quotient(rest, units)));
     uint64_t v = rest - run.kvh * units;
-    const Request q{static_cast<uint32_t>(__builtin_amdgcn_readfirstlane(sc.found.first)), static_cast<uint32_t>(__builtin_amdgcn_readfirstlane(sc.found.vecs)),
+    const Request q{static_cast<uint32_t>(__builtin_amdgcn_readfirstlane(sc.found.first)),
+                    static_cast<uint32_t>(__builtin_amdgcn_readfirstlane(sc.found.vecs)),
                     __builtin_amdgcn_readfirstlane(static_cast<int32_t>(sc.found.start))};
     run.req = q;
     for (uint32_t i = 0;; i += 64) {  // every wave by itself: the item that holds unit v
@@ -393,7 +395,7 @@ __device__ __forceinline__ int f16_exponent(float top) {
 }
 
 // ---------------------------------------------------------------------------
-// A wave holds WV = 16 GI vectors of an item and takes WK = 16 U positions a
+// A wave holds WV = 16 vectors of an item and takes WK = 16 U positions a
 // step; waves that share vectors join at the item's end. Nothing is shared
 // between waves on the way, so keys and values go from memory (or the caches,
 // where waves read the same ones) straight into the registers that the products
@@ -409,16 +411,16 @@ __device__ __forceinline__ int f16_exponent(float top) {
 // SIMD, one's products beside the other's exponentials.
 //
 // Keys and values from memory bound it where requests are many or long: 40 rows
-// behind up to 8000 positions, 28 heads over 4 of 128, bf16, 84 us, 4.4 TB/s (a
+// behind up to 8000 positions, 28 heads over 4 of 128, bf16, 83 us, 4.4 TB/s (a
 // copy reaches 4.8 to 5.4); 64 behind up to 4000, 16 heads over 16 of 128, 242
 // us, 5.4 TB/s, and 6.1 in f32. The chain named above does where they are few:
 // 1 row behind 230, 8 kv heads of 64, f32, 11 us; behind 8000, 4 kv heads, bf16,
 // 23 us; 24 x 5 rows behind up to 4100, f16, 40 us, 2.8 TB/s.
 // ---------------------------------------------------------------------------
-template <int HD, int KIND, int GI>
+template <int HD, int KIND>
 struct Form {
     using K = Kind<KIND>;
-    static constexpr int WV = 16 * GI, M = 4 * WV, U = K::U, WK = 16 * U, DV = HD / 16;
+    static constexpr int WV = 16, M = 4 * WV, U = K::U, WK = 16 * U, DV = HD / 16;
     // (An item at 1 and not 3 units: 24 x 5 rows of heads of 64 40.9 us and not 37.0. Runs from 10 units on and not 5:
     // 45.7, and 1 x 1 row behind 2000 positions 26.9 and not 21.0. Items whole up to 24 units and not 12: 40 x 1 row behind
     // 8000 102 and not 84; up to none: 1 x 1 row behind 500 15.1 and not 14.3.)
@@ -433,7 +435,7 @@ struct Form {
     // terms: [WV][HD] outputs with rows ROW apart, so that 16 rows' 16-byte
     // writes fall on different banks, [WV] maxima, [WV] sums.
     static constexpr int ROW = HD + 4, kWave = WV * (ROW + 2);
-    static constexpr int kQ = GI * KL * (K::TERMS - 1) * 64;         // of a wave, in 16-byte units
+    static constexpr int kQ = KL * (K::TERMS - 1) * 64;         // of a wave, in 16-byte units
     static constexpr int kShared = std::max(4 * kWave, 4 * 4 * kQ);  // 32-bit words
 };
 
@@ -491,9 +493,9 @@ __device__ __forceinline__ void odd_values(const char* vbase, uint64_t row_bytes
         if (!(none >> at & 1)) add(at, reinterpret_cast<const uint32_t*>(vbase + static_cast<uint32_t>(__shfl(slots, at, 64)) * row_bytes));
 }
 
-template <int HD, int KIND, int GI>
+template <int HD, int KIND>
 __global__ __launch_bounds__(kThreads, HD == 128 ? 2 : 3) void paged_attn_kernel(PagedAttnArgs a) {
-    using F = Form<HD, KIND, GI>;
+    using F = Form<HD, KIND>;
     using K = Kind<KIND>;
     constexpr int WV = F::WV, U = F::U, WK = F::WK, DV = F::DV, KL = F::KL, VW = F::VW, ROW = F::ROW;
     constexpr bool F32 = KIND == VVLI_CACHE_F32;
@@ -535,8 +537,8 @@ __global__ __launch_bounds__(kThreads, HD == 128 ? 2 : 3) void paged_attn_kernel
         if (w_lo >= (ks + 1) * WK) ta = max(ta, (w_lo - (ks + 1) * WK) / UK + 1);
         tb = w_lo < w_hi && w_hi > ks * WK ? min(tb, (w_hi - ks * WK + UK - 1) / UK) : 0;
 
-        f32x4 o[GI][DV];
-        float m_run[GI], l_run[GI];
+        f32x4 o[DV];
+        float m_run, l_run;
 
         // Slot of key t * UK + ks * WK + lane (of WK lanes), -1 where no vector of the wave sees it.
         auto slot_of = [&](uint32_t t) -> int32_t {
@@ -578,63 +580,56 @@ __global__ __launch_bounds__(kThreads, HD == 128 ? 2 : 3) void paged_attn_kernel
         int32_t ahead = slot_of(ta + 1);
         if (ta < tb) load_k(slots), load_v(slots);
 
-        // The lane's vectors: their keys and q.
-        KeySpan see[GI];
-        float inv[GI];  // scores are this times the products (f16's power of two)
-        u32x4 qf[GI][KL];
+        // The lane's vector: its keys and q.
+        float inv = 1.f;  // scores are this times the products (f16's power of two)
+        u32x4 qf[KL];
+        const uint32_t m = wm0 + fr;
+        const bool there = m < req.vecs;
+        const uint32_t row = page_of(a.group, there ? m : 0), g = (there ? m : 0) - row * a.group.d;
+        const KeySpan see = there ? key_span(req.start + row, a.window, a.room) : KeySpan{0, 0};
+        const float* qp = a.q + (req.first + row) * a.ldq + (static_cast<size_t>(run.kvh) * a.group.d + g) * HD;
+        const float f = a.scale * 1.44269504088896341f;
+        if constexpr (F32) {
 #pragma unroll
-        for (int gi = 0; gi < GI; ++gi) {
-            const uint32_t m = wm0 + 16 * gi + fr;
-            const bool there = m < req.vecs;
-            const uint32_t row = page_of(a.group, there ? m : 0), g = (there ? m : 0) - row * a.group.d;
-            see[gi] = there ? key_span(req.start + row, a.window, a.room) : KeySpan{0, 0};
-            const float* qp = a.q + (req.first + row) * a.ldq + (static_cast<size_t>(run.kvh) * a.group.d + g) * HD;
-            const float f = a.scale * 1.44269504088896341f;
-            inv[gi] = 1.f;
-            if constexpr (F32) {
+            for (int s = 0; s < KL; ++s) {
+                const float4 x = load_f32x4(qp + 16 * s + 4 * fq);
+                qf[s] = __builtin_bit_cast(u32x4, f32x4{x.x * f, x.y * f, x.z * f, x.w * f});
+            }
+        } else {
+            float x[KL][8];
+            float top = 0.f;
 #pragma unroll
-                for (int s = 0; s < KL; ++s) {
-                    const float4 x = load_f32x4(qp + 16 * s + 4 * fq);
-                    qf[gi][s] = __builtin_bit_cast(u32x4, f32x4{x.x * f, x.y * f, x.z * f, x.w * f});
-                }
-            } else {
-                float x[KL][8];
-                float top = 0.f;
+            for (int s = 0; s < KL; ++s) {
+                const float4 x0 = load_f32x4(qp + 32 * s + 8 * fq), x1 = load_f32x4(qp + 32 * s + 8 * fq + 4);
+                x[s][0] = x0.x, x[s][1] = x0.y, x[s][2] = x0.z, x[s][3] = x0.w;
+                x[s][4] = x1.x, x[s][5] = x1.y, x[s][6] = x1.z, x[s][7] = x1.w;
 #pragma unroll
-                for (int s = 0; s < KL; ++s) {
-                    const float4 x0 = load_f32x4(qp + 32 * s + 8 * fq), x1 = load_f32x4(qp + 32 * s + 8 * fq + 4);
-                    x[s][0] = x0.x, x[s][1] = x0.y, x[s][2] = x0.z, x[s][3] = x0.w, x[s][4] = x1.x, x[s][5] = x1.y, x[s][6] = x1.z, x[s][7] = x1.w;
+                for (int e = 0; e < 8; ++e) x[s][e] *= f, top = fmaxf(top, fabsf(x[s][e]));
+            }
+            if constexpr (KIND == VVLI_CACHE_F16) {
+                const int ex = f16_exponent(rows_max(top));
+                const float up = ldexpf(1.f, ex);
+                inv = ldexpf(1.f, -ex);
 #pragma unroll
-                    for (int e = 0; e < 8; ++e) x[s][e] *= f, top = fmaxf(top, fabsf(x[s][e]));
-                }
-                if constexpr (KIND == VVLI_CACHE_F16) {
-                    const int ex = f16_exponent(rows_max(top));
-                    const float up = ldexpf(1.f, ex);
-                    inv[gi] = ldexpf(1.f, -ex);
+                for (int s = 0; s < KL; ++s)
 #pragma unroll
-                    for (int s = 0; s < KL; ++s)
+                    for (int e = 0; e < 8; ++e) x[s][e] *= up;
+            }
 #pragma unroll
-                        for (int e = 0; e < 8; ++e) x[s][e] *= up;
-                }
+            for (int s = 0; s < KL; ++s) {
+                typename K::T8 t[K::TERMS];
 #pragma unroll
-                for (int s = 0; s < KL; ++s) {
-                    typename K::T8 t[K::TERMS];
+                for (int e = 0; e < 8; e += 2) split2<K>(x[s][e], x[s][e + 1], e, t);
+                qf[s] = __builtin_bit_cast(u32x4, t[0]);
 #pragma unroll
-                    for (int e = 0; e < 8; e += 2) split2<K>(x[s][e], x[s][e + 1], e, t);
-                    qf[gi][s] = __builtin_bit_cast(u32x4, t[0]);
-#pragma unroll
-                    for (int i = 1; i < K::TERMS; ++i) q_mine[((gi * KL + s) * (K::TERMS - 1) + i - 1) * 64] = __builtin_bit_cast(u32x4, t[i]);
-                }
+                for (int i = 1; i < K::TERMS; ++i) q_mine[(s * (K::TERMS - 1) + i - 1) * 64] = __builtin_bit_cast(u32x4, t[i]);
             }
         }
         bool spoilt = false;
         for (int careful = 0; careful < 2; ++careful) {
+            m_run = -INFINITY, l_run = 0.f;
 #pragma unroll
-            for (int gi = 0; gi < GI; ++gi) {
-                m_run[gi] = -INFINITY, l_run[gi] = 0.f;
-#pragma unroll
-                for (int e = 0; e < DV; ++e) o[gi][e] = f32x4{0, 0, 0, 0};
-            }
+            for (int e = 0; e < DV; ++e) o[e] = f32x4{0, 0, 0, 0};
             if (ta >= tb) break;
             uint64_t none_next;
             uint32_t slots_next;
@@ -655,11 +650,9 @@ __global__ __launch_bounds__(kThreads, HD == 128 ? 2 : 3) void paged_attn_kernel
 #pragma unroll
                             for (int i = 0; i < VW; ++i) st.v[u][j][i] = word_finite<KIND>(st.v[u][j][i]);
                 }
-                f32x4 s[GI][U];
+                f32x4 s[U];
 #pragma unroll
-                for (int gi = 0; gi < GI; ++gi)
-#pragma unroll
-                    for (int u = 0; u < U; ++u) s[gi][u] = f32x4{0, 0, 0, 0};
+                for (int u = 0; u < U; ++u) s[u] = f32x4{0, 0, 0, 0};
 #pragma unroll
                 for (int i = 0; i < KL; ++i) {
                     if constexpr (F32) {
@@ -667,19 +660,17 @@ __global__ __launch_bounds__(kThreads, HD == 128 ? 2 : 3) void paged_attn_kernel
                         for (int e = 0; e < 4; ++e)
 #pragma unroll
                             for (int u = 0; u < U; ++u)
-#pragma unroll
-                                for (int gi = 0; gi < GI; ++gi)
-                                    s[gi][u] = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(st.k[u][i][e]), __uint_as_float(qf[gi][i][e]), s[gi][u], 0, 0, 0);
+                                s[u] = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(st.k[u][i][e]), __uint_as_float(qf[i][e]),
+                                                                            s[u], 0, 0, 0);
                     } else {
 #pragma unroll
-                        for (int x = 0; x < K::TERMS; ++x)
+                        for (int x = 0; x < K::TERMS; ++x) {
+                            const u32x4 qx = x == 0 ? qf[i] : q_mine[(i * (K::TERMS - 1) + x - 1) * 64];
 #pragma unroll
-                            for (int gi = 0; gi < GI; ++gi) {
-                                const u32x4 qx = x == 0 ? qf[gi][i] : q_mine[((gi * KL + i) * (K::TERMS - 1) + x - 1) * 64];
-#pragma unroll
-                                for (int u = 0; u < U; ++u)
-                                    s[gi][u] = K::mfma(__builtin_bit_cast(typename K::T8, st.k[u][i]), __builtin_bit_cast(typename K::T8, qx), s[gi][u]);
-                            }
+                            for (int u = 0; u < U; ++u)
+                                s[u] = K::mfma(__builtin_bit_cast(typename K::T8, st.k[u][i]),
+                                               __builtin_bit_cast(typename K::T8, qx), s[u]);
+                        }
                     }
                 }
                 if (t + 1 < tb) load_k(slots_next);
@@ -691,54 +682,45 @@ __global__ __launch_bounds__(kThreads, HD == 128 ? 2 : 3) void paged_attn_kernel
                         for (int j = 0; j < 4; ++j) {
                             const uint32_t at = 16 * u + 4 * fq + j, key = key0 + at;
                             const bool hole = none >> at & 1;
-#pragma unroll
-                            for (int gi = 0; gi < GI; ++gi)
-                                if (hole || key < see[gi].lo || key >= see[gi].hi) s[gi][u][j] = -INFINITY;
+                            if (hole || key < see.lo || key >= see.hi) s[u][j] = -INFINITY;
                         }
                 }
-                u32x4 pf[GI][F32 ? U : K::TERMS];
-                float corr[GI];
-                bool grew = false;
+                u32x4 pf[F32 ? U : K::TERMS];
+                float mx = -INFINITY;
 #pragma unroll
-                for (int gi = 0; gi < GI; ++gi) {
-                    float mx = -INFINITY;
+                for (int u = 0; u < U; ++u)
 #pragma unroll
-                    for (int u = 0; u < U; ++u)
+                    for (int j = 0; j < 4; ++j) mx = fmaxf(mx, s[u][j]);
+                const float m_new = fmaxf(m_run, rows_max(mx) * inv);
+                const float m_sub = m_new == -INFINITY ? 0.f : m_new;
+                const bool grew = m_new != m_run;
+                const float corr = __builtin_amdgcn_exp2f(m_run - m_sub);
+                float sum = 0.f;
 #pragma unroll
-                        for (int j = 0; j < 4; ++j) mx = fmaxf(mx, s[gi][u][j]);
-                    const float m_new = fmaxf(m_run[gi], rows_max(mx) * inv[gi]);
-                    const float m_sub = m_new == -INFINITY ? 0.f : m_new;
-                    grew |= m_new != m_run[gi];
-                    corr[gi] = __builtin_amdgcn_exp2f(m_run[gi] - m_sub);
-                    float sum = 0.f;
+                for (int u = 0; u < U; ++u)
 #pragma unroll
-                    for (int u = 0; u < U; ++u)
-#pragma unroll
-                        for (int j = 0; j < 4; ++j) {
-                            const float p = __builtin_amdgcn_exp2f(fmaf(s[gi][u][j], inv[gi], K::PBIAS - m_sub));
-                            s[gi][u][j] = p;
-                            sum += p;
-                        }
-                    if constexpr (F32) {
-#pragma unroll
-                        for (int u = 0; u < U; ++u) pf[gi][u] = __builtin_bit_cast(u32x4, s[gi][u]);
-                    } else {
-                        typename K::T8 t8[K::TERMS];
-#pragma unroll
-                        for (int u = 0; u < U; ++u)
-#pragma unroll
-                            for (int j = 0; j < 4; j += 2) split2<K>(s[gi][u][j], s[gi][u][j + 1], 4 * u + j, t8);
-#pragma unroll
-                        for (int x = 0; x < K::TERMS; ++x) pf[gi][x] = __builtin_bit_cast(u32x4, t8[x]);
+                    for (int j = 0; j < 4; ++j) {
+                        const float p = __builtin_amdgcn_exp2f(fmaf(s[u][j], inv, K::PBIAS - m_sub));
+                        s[u][j] = p;
+                        sum += p;
                     }
-                    l_run[gi] = l_run[gi] * corr[gi] + sum;
-                    m_run[gi] = m_new;
+                if constexpr (F32) {
+#pragma unroll
+                    for (int u = 0; u < U; ++u) pf[u] = __builtin_bit_cast(u32x4, s[u]);
+                } else {
+                    typename K::T8 t8[K::TERMS];
+#pragma unroll
+                    for (int u = 0; u < U; ++u)
+#pragma unroll
+                        for (int j = 0; j < 4; j += 2) split2<K>(s[u][j], s[u][j + 1], 4 * u + j, t8);
+#pragma unroll
+                    for (int x = 0; x < K::TERMS; ++x) pf[x] = __builtin_bit_cast(u32x4, t8[x]);
                 }
+                l_run = l_run * corr + sum;
+                m_run = m_new;
                 if (__any(grew)) {
 #pragma unroll
-                    for (int gi = 0; gi < GI; ++gi)
-#pragma unroll
-                        for (int e = 0; e < DV; ++e) o[gi][e] *= corr[gi];
+                    for (int e = 0; e < DV; ++e) o[e] *= corr;
                 }
 #pragma unroll
                 for (int e = 0; e < DV; ++e) {
@@ -747,21 +729,19 @@ __global__ __launch_bounds__(kThreads, HD == 128 ? 2 : 3) void paged_attn_kernel
                         for (int u = 0; u < U; ++u)
 #pragma unroll
                             for (int j = 0; j < 4; ++j)
-#pragma unroll
-                                for (int gi = 0; gi < GI; ++gi)
-                                    o[gi][e] = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(st.v[u][j][e]), __uint_as_float(pf[gi][u][j]), o[gi][e], 0, 0, 0);
+                                o[e] = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(st.v[u][j][e]), __uint_as_float(pf[u][j]),
+                                                                            o[e], 0, 0, 0);
                     } else {
                         u32x4 w;
 #pragma unroll
                         for (int u = 0; u < U; ++u)
 #pragma unroll
                             for (int jp = 0; jp < 2; ++jp)  // keys 2 jp and 2 jp + 1, dim e of the lane's
-                                w[2 * u + jp] = __builtin_amdgcn_perm(st.v[u][2 * jp + 1][e / 2], st.v[u][2 * jp][e / 2], e % 2 ? 0x07060302u : 0x05040100u);
+                                w[2 * u + jp] = __builtin_amdgcn_perm(st.v[u][2 * jp + 1][e / 2], st.v[u][2 * jp][e / 2],
+                                                                      e % 2 ? 0x07060302u : 0x05040100u);
 #pragma unroll
                         for (int x = 0; x < K::TERMS; ++x)
-#pragma unroll
-                            for (int gi = 0; gi < GI; ++gi)
-                                o[gi][e] = K::mfma(__builtin_bit_cast(typename K::T8, w), __builtin_bit_cast(typename K::T8, pf[gi][x]), o[gi][e]);
+                            o[e] = K::mfma(__builtin_bit_cast(typename K::T8, w), __builtin_bit_cast(typename K::T8, pf[x]), o[e]);
                     }
                 }
                 if (t + 1 < tb) load_v(slots_next);
@@ -769,11 +749,9 @@ __global__ __launch_bounds__(kThreads, HD == 128 ? 2 : 3) void paged_attn_kernel
             }
             float sum = 0.f;  // NaN if one of them is not finite
 #pragma unroll
-            for (int gi = 0; gi < GI; ++gi)
+            for (int e = 0; e < DV; ++e)
 #pragma unroll
-                for (int e = 0; e < DV; ++e)
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) sum = fmaf(o[gi][e][j], 0.f, sum);
+                for (int j = 0; j < 4; ++j) sum = fmaf(o[e][j], 0.f, sum);
             if (careful) {
                 spoilt = true;
             } else if (!__any(sum != sum)) {  // see odd_values
@@ -786,39 +764,33 @@ __global__ __launch_bounds__(kThreads, HD == 128 ? 2 : 3) void paged_attn_kernel
                 const uint32_t slots = filled(slot_of(t), none);
                 odd_values<HD, KIND, WK>(vbase - 4 * VW * fr, row_bytes, slots, none, [&](int at, const uint32_t* p) {
                     const uint32_t key = t * UK + ks * WK + at;
+                    const bool sees = key >= see.lo && key < see.hi;
 #pragma unroll
-                    for (int gi = 0; gi < GI; ++gi) {
-                        const bool sees = key >= see[gi].lo && key < see[gi].hi;
+                    for (int e = 0; e < DV; ++e)
 #pragma unroll
-                        for (int e = 0; e < DV; ++e)
-#pragma unroll
-                            for (int j = 0; j < 4; ++j) {
-                                const float x = value_at<KIND>(p, DV * (4 * fq + j) + e);
-                                if (sees && !(fabsf(x) < INFINITY)) o[gi][e][j] += x;
-                            }
-                    }
+                        for (int j = 0; j < 4; ++j) {
+                            const float x = value_at<KIND>(p, DV * (4 * fq + j) + e);
+                            if (sees && !(fabsf(x) < INFINITY)) o[e][j] += x;
+                        }
                 });
             }
 
         // The waves' parts: outputs [WV][HD], maxima, sums.
         __syncthreads();  // (q's terms are read)
         float* mine = shared + wave * F::kWave;
+        float l = l_run;
+        l += __shfl_xor(l, 16, 64);
+        l += __shfl_xor(l, 32, 64);
+        if (fq == 0) mine[WV * ROW + fr] = m_run, mine[WV * ROW + WV + fr] = l;
 #pragma unroll
-        for (int gi = 0; gi < GI; ++gi) {
-            float l = l_run[gi];
-            l += __shfl_xor(l, 16, 64);
-            l += __shfl_xor(l, 32, 64);
-            if (fq == 0) mine[WV * ROW + 16 * gi + fr] = m_run[gi], mine[WV * ROW + WV + 16 * gi + fr] = l;
+        for (int j = 0; j < 4; ++j) {
+            float* p = mine + fr * ROW + DV * (4 * fq + j);
+            if constexpr (DV >= 4) {
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                float* p = mine + (16 * gi + fr) * ROW + DV * (4 * fq + j);
-                if constexpr (DV >= 4) {
-#pragma unroll
-                    for (int e = 0; e < DV; e += 4)
-                        *reinterpret_cast<f32x4*>(p + e) = f32x4{o[gi][e][j], o[gi][e + 1][j], o[gi][e + 2][j], o[gi][e + 3][j]};
-                } else {
-                    p[0] = o[gi][0][j], p[1] = o[gi][1][j];
-                }
+                for (int e = 0; e < DV; e += 4)
+                    *reinterpret_cast<f32x4*>(p + e) = f32x4{o[e][j], o[e + 1][j], o[e + 2][j], o[e + 3][j]};
+            } else {
+                p[0] = o[0][j], p[1] = o[1][j];
             }
         }
         __syncthreads();
@@ -928,7 +900,7 @@ __global__ __launch_bounds__(kThreads, HD == 128 ? 2 : 3) void paged_attn_kernel
 // (125 of the 133 TFLOP/s that a large product reaches), 1.2 ms in f16 (479, times
 // two terms 959 of 1310) and 1.45 ms in bf16 (397, times three terms 1190 of
 // 1200). Short chunks are bound by the runs' ends: 2 x up to 2000 rows behind up
-// to 2100 in bf16 267 us (343, 1030 with terms).
+// to 2100 in bf16 260 to 277 us (330 to 353, 990 to 1060 with terms).
 // ---------------------------------------------------------------------------
 template <int HD, int KIND>
 struct Wide {
@@ -1018,7 +990,8 @@ __global__ __launch_bounds__(kThreads, 2) void paged_wide_kernel(PagedAttnArgs a
 #pragma unroll
             for (int s = 0; s < DS; ++s) {
                 const float4 x0 = load_f32x4(qp + 16 * s), x1 = load_f32x4(qp + 16 * s + 4);
-                x[s][0] = x0.x, x[s][1] = x0.y, x[s][2] = x0.z, x[s][3] = x0.w, x[s][4] = x1.x, x[s][5] = x1.y, x[s][6] = x1.z, x[s][7] = x1.w;
+                x[s][0] = x0.x, x[s][1] = x0.y, x[s][2] = x0.z, x[s][3] = x0.w;
+                x[s][4] = x1.x, x[s][5] = x1.y, x[s][6] = x1.z, x[s][7] = x1.w;
 #pragma unroll
                 for (int e = 0; e < 8; ++e) x[s][e] *= f, top = fmaxf(top, fabsf(x[s][e]));
             }
@@ -1181,7 +1154,8 @@ __global__ __launch_bounds__(kThreads, 2) void paged_wide_kernel(PagedAttnArgs a
                         for (int c = 0; c < 2; ++c)
 #pragma unroll
                             for (int e = 0; e < 8; e += 2) {
-                                const float p0 = __builtin_amdgcn_exp2f(fmaf(s[8 * c + e], inv, shift)), p1 = __builtin_amdgcn_exp2f(fmaf(s[8 * c + e + 1], inv, shift));
+                                const float p0 = __builtin_amdgcn_exp2f(fmaf(s[8 * c + e], inv, shift));
+                                const float p1 = __builtin_amdgcn_exp2f(fmaf(s[8 * c + e + 1], inv, shift));
                                 sum[0] += p0, sum[1] += p1;
                                 split2<K>(p0, p1, e, pf[c]);
                             }
@@ -1247,7 +1221,8 @@ __global__ __launch_bounds__(kThreads, 2) void paged_wide_kernel(PagedAttnArgs a
 #pragma unroll
                 for (int i = 0; i < 4; ++i)
                     *reinterpret_cast<f32x4*>(op + 32 * n + 8 * i) =
-                        l_run == 0.f ? f32x4{0, 0, 0, 0} : f32x4{o[n][4 * i] * r, o[n][4 * i + 1] * r, o[n][4 * i + 2] * r, o[n][4 * i + 3] * r};
+                        l_run == 0.f ? f32x4{0, 0, 0, 0}
+                                      : f32x4{o[n][4 * i] * r, o[n][4 * i + 1] * r, o[n][4 * i + 2] * r, o[n][4 * i + 3] * r};
         };
         if (walk.whole()) {
             write();
@@ -1317,7 +1292,9 @@ Plan plan_of(uint32_t rows, uint32_t requests, uint32_t group, uint32_t hd) {
 uint32_t slot_vecs(const Plan& p, uint32_t rows, uint32_t group) {
     return p.wide ? p.m : static_cast<uint32_t>(std::min<uint64_t>(p.m, (static_cast<uint64_t>(rows) * group + 1) & ~uint64_t{1}));
 }
-size_t plan_bytes(const Plan& p, uint32_t vecs, uint32_t hd) { return p.blocks * sizeof(float) * (4 + 2 * static_cast<size_t>(vecs) * (hd + 2)); }
+size_t plan_bytes(const Plan& p, uint32_t vecs, uint32_t hd) {
+    return p.blocks * sizeof(float) * (4 + 2 * static_cast<size_t>(vecs) * (hd + 2));
+}
 
 bool sizes_ok(uint32_t rows, uint32_t requests, uint32_t heads, uint32_t kv_heads) {
     return requests != 0 && heads != 0 && kv_heads != 0 && heads % kv_heads == 0 && heads <= 65535 &&
@@ -1327,12 +1304,15 @@ bool sizes_ok(uint32_t rows, uint32_t requests, uint32_t heads, uint32_t kv_head
 template <int HD, int KIND>
 hipError_t launch(const PagedAttnArgs& a, const Plan& p, hipStream_t s) {
     const dim3 grid(p.blocks), block(kThreads);
-    return p.wide ? vlaunch(paged_wide_kernel<HD, KIND>, grid, block, 0, s, a) : vlaunch(paged_attn_kernel<HD, KIND, 1>, grid, block, 0, s, a);
+    return p.wide ? vlaunch(paged_wide_kernel<HD, KIND>, grid, block, 0, s, a)
+                  : vlaunch(paged_attn_kernel<HD, KIND>, grid, block, 0, s, a);
 }
 
 template <int HD>
 hipError_t launch(const PagedAttnArgs& a, uint32_t kind, const Plan& p, hipStream_t s) {
-    return kind == VVLI_CACHE_F32 ? launch<HD, VVLI_CACHE_F32>(a, p, s) : kind == VVLI_CACHE_BF16 ? launch<HD, VVLI_CACHE_BF16>(a, p, s) : launch<HD, VVLI_CACHE_F16>(a, p, s);
+    return kind == VVLI_CACHE_F32 ? launch<HD, VVLI_CACHE_F32>(a, p, s)
+           : kind == VVLI_CACHE_BF16 ? launch<HD, VVLI_CACHE_BF16>(a, p, s)
+                                     : launch<HD, VVLI_CACHE_F16>(a, p, s);
 }
 
 }  // namespace

@@ -275,7 +275,8 @@ int vvli_gpu_verify_drafts(const float* target, uint64_t ldt, const float* draft
     a.chunks = chunks_of(vocab), a.chunk = chunk_tokens(vocab);
     const uint32_t blocks = std::min((a.chunks - 1) / kWaves + 1, (kBlocks - 1) / requests + 1);
     a.per_block = (a.chunks - 1) / blocks + 1;
-    PAGED_TRY(vlaunch(verify_kernel, dim3((a.chunks - 1) / a.per_block + 1, requests), dim3(kThreads), 0, static_cast<hipStream_t>(stream), a));
+    const dim3 grid((a.chunks - 1) / a.per_block + 1, requests);
+    PAGED_TRY(vlaunch(verify_kernel, grid, dim3(kThreads), 0, static_cast<hipStream_t>(stream), a));
     return VVLI_OK;
 }
 

@@ -818,6 +818,47 @@ def test_verify_workspace_serves_other_sizes(torch):
         verify(torch, p, q, rng.randint(0, V, 3 * n), np.arange(n + 1) * 3, rng.rand(3 * n), rng.rand(n), ws=ws)
 
 
+@pytest.mark.parametrize("vocab", [700, 5000, 40000, 151936])
+@pytest.mark.parametrize("refused", [False, True])
+def test_verify_gives_tokens_that_have_a_weight(torch, vocab, refused):
+    """Rows cut by a mask, in sums that no order of adding has exactly: u_sample of 1 and more gives the last token with a
+    weight; a border at a sum in front of a masked stretch one of the two tokens beside the stretch."""
+    rng = np.random.RandomState(vocab)
+    n = 400 if vocab < 100000 else 60
+    half, gap = vocab * 2 // 5, vocab // 20
+    w = np.exp(4 * rng.randn(n, half)).astype(np.float32)
+    w[:, rng.rand(half) < 0.3] = 0
+    w[:, [0, -1]] = 1.0
+    p = np.zeros((n, vocab), np.float32)  # weights, a masked stretch, the same weights, a masked tail
+    p[:, :half], p[:, half + gap: 2 * half + gap] = w, w
+    last, left, right = 2 * half + gap - 1, half - 1, half + gap
+    counts = np.full(n, 2 if refused else 1)
+    target, draft = np.repeat(p, counts, 0), None
+    tokens = np.zeros(len(target), np.int64)
+    if refused:  # a draft of weight 0 in front; q leaves half of every weight
+        tokens[1::2] = vocab - 1
+        draft = target / 2
+    d = lambda x: torch.tensor(np.ascontiguousarray(x, dtype=np.float32), device="cuda") if x is not None else None  # noqa: E731
+    dt, dd, ua = d(target), d(draft), d(np.ones(len(target)))
+    tk, rs = i32(torch, tokens), i32(torch, np.concatenate([[0], np.cumsum(counts)]))
+    acc, out = i32(torch, np.zeros(n)), i32(torch, np.zeros(len(target)))
+    ws = torch.zeros(R.verify_drafts_workspace(n, vocab), dtype=torch.uint8, device="cuda")
+    for u, want in ((1.0, (last,)), (2.0, (last,)), (float("inf"), (last,)), (0.5, (left, right)), (0.0, (0,))):
+        us = d(np.full(n, u))
+        R.verify_drafts(ptr(dt), vocab, ptr(dd), vocab, ptr(tk), ptr(rs), n, len(target), vocab, ptr(ua), ptr(us), ptr(acc), ptr(out),
+                        ptr(ws), ws.numel(), torch.cuda.current_stream().cuda_stream)
+        assert acc.tolist() == [0] * n
+        got = set(out.cpu().numpy()[rs.cpu().numpy()[:-1]].tolist())
+        assert got <= set(want), (u, got - set(want))
+    # Numbers next to 1: whatever the sums' last bits are, no masked token.
+    for u in (np.nextafter(np.float32(1), np.float32(0)), np.float32(0.999999)):
+        us = d(np.full(n, u))
+        R.verify_drafts(ptr(dt), vocab, ptr(dd), vocab, ptr(tk), ptr(rs), n, len(target), vocab, ptr(ua), ptr(us), ptr(acc), ptr(out),
+                        ptr(ws), ws.numel(), torch.cuda.current_stream().cuda_stream)
+        first = out.cpu().numpy()[rs.cpu().numpy()[:-1]]
+        assert (p[np.arange(n), first] > 0).all()
+
+
 # ---------------------------------------------------------------------------
 # The ops together
 # ---------------------------------------------------------------------------

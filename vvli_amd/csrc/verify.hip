@@ -181,12 +181,14 @@ __global__ __launch_bounds__(kThreads) void verify_kernel(VerifyArgs a) {
         __syncthreads();
         s = tid < a.chunks ? sums[tid] : 0;
     }
-    // The lowest token whose running sum is not at or below the border; behind all of them (a number of 1 or more)
-    // the last token with a weight.
+    // The lowest token whose running sum is over the border; for numbers of 1 and more, and where no sum is, the last
+    // token with a weight. Sums of different orders of adding are an ulp apart, so that a sum may be over the border
+    // where no weight was added to it: only chunks, lanes and tokens that have a weight are taken. (A border below 0
+    // is under all sums, that of token 0 too.)
     int32_t token = -1;
     if (total > 0) {
-        const double border = static_cast<double>(a.u_sample[r]) * total;
-        const uint64_t yes = __ballot(tid < a.chunks && !(end <= border)), some = __ballot(s > 0);
+        const double u = a.u_sample[r], border = u * total;
+        const uint64_t some = __ballot(s > 0), yes = __ballot(s > 0 && end > border);
         if (lane == 0) found[wave] = yes ? __builtin_ctzll(yes) : 64;
         sums[tid] = end - s;
         if (tid == 0) last = 0;
@@ -194,13 +196,15 @@ __global__ __launch_bounds__(kThreads) void verify_kernel(VerifyArgs a) {
         uint32_t at = kThreads;
         for (int k = kWaves - 1; k >= 0; --k)
             if (found[k] < 64) at = k * 64 + found[k];
-        const bool behind = at == kThreads;
+        const bool behind = at == kThreads || u >= 1;
         if (behind) {
-            if (some) atomicMax(&last, wave * 64 + 63 - __builtin_clzll(some));
+            if (lane == 0 && some) atomicMax(&last, wave * 64 + 63 - __builtin_clzll(some));
             __syncthreads();
             at = last;
         }
-        if (wave == 0) {
+        if (!(u >= 0)) {
+            token = 0;
+        } else if (wave == 0) {
             double before = sums[at];
             uint32_t best = 0;  // 1 + the last token with a weight in the lane
             bool done = false;
@@ -210,16 +214,15 @@ __global__ __launch_bounds__(kThreads) void verify_kernel(VerifyArgs a) {
                 double x[8];
                 load8(w, v, p, q);
                 const double sum = weight8(w, v, p, q, x), upto = before + wave_scan(sum);
-                const uint64_t over = behind ? 0 : __ballot(v < a.vocab && !(upto <= border));
+                const uint64_t over = behind ? 0 : __ballot(sum > 0 && upto > border);
                 if (over) {
                     double run = upto - sum;
-                    uint32_t tok = v;
+                    uint32_t tok = 0;
                     bool there = false;
 #pragma unroll
                     for (uint32_t i = 0; i < 8; ++i) {
                         run += x[i];
-                        if (x[i] > 0 && !there) tok = v + i;
-                        if (!there && !(run <= border)) tok = v + i, there = true;
+                        if (x[i] > 0 && !there) tok = v + i, there = run > border;
                     }
                     best = __shfl(tok, __builtin_ctzll(over), 64) + 1;
                     done = true;

@@ -527,11 +527,13 @@ size_t vvli_gpu_paged_attention_workspace(uint32_t rows, uint32_t requests, uint
  * lowest token whose running sum is over u_sample[r] * (sum of the row), and
  * never one that adds nothing to it (u_sample[r] of 1 and more: the last token
  * that adds something; below 0 or NaN: token 0). Sums and comparisons are made
- * in f64; values that are not finite and positive count 0. out[row_start[r] ..]
- * receives the accepted tokens, the drawn one (-1 if the whole row is 0) and -1
- * for the rest of the request's rows; a request without rows has accepted[r] =
- * 0. Rows of no request stay as they are; row_start ascends (as above). At most
- * 65535 requests.
+ * in f64. A target value that is not finite and positive counts 0 (its token is
+ * never accepted), a negative draft value counts 0, and one that is not finite
+ * refuses its token and leaves it no weight at a refused draft.
+ * out[row_start[r] ..] receives the accepted tokens, the drawn one (-1 if the
+ * whole row is 0) and -1 for the rest of the request's rows; a request without
+ * rows has accepted[r] = 0. Rows of no request stay as they are; row_start
+ * ascends (as above). At most 65535 requests.
  * target and draft may have any stride >= vocab; out is not tokens. workspace: at least
  * vvli_gpu_verify_drafts_workspace bytes, at a 16-byte address. */
 int vvli_gpu_verify_drafts(const float* target, uint64_t ldt, const float* draft, uint64_t ldd, const int32_t* tokens,

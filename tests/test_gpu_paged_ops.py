@@ -859,6 +859,45 @@ def test_verify_gives_tokens_that_have_a_weight(torch, vocab, refused):
         assert (p[np.arange(n), first] > 0).all()
 
 
+@pytest.mark.parametrize("certain", [False, True])
+def test_verify_values_that_are_no_probabilities(torch, certain):
+    """Drafted tokens on target and draft values that are infinite, NaN, negative or 0. A target value that is not finite and
+    positive counts 0; a negative draft value too; a draft value that is not finite refuses its token and leaves it no weight."""
+    V = 64
+    odd = [float("inf"), float("-inf"), float("nan"), -0.5, 0.0, 0.25]
+    pairs = [(p, q) for p in odd for q in ([1.0] if certain else odd)]
+    n = len(pairs)
+    target, draft = np.full((2 * n, V), 0.0078125, np.float32), np.full((2 * n, V), 0.00390625, np.float32)
+    for i, (p, q) in enumerate(pairs):
+        target[2 * i, 40], draft[2 * i, 40] = p, q
+    tokens = np.tile([0, 40], n)
+    d = lambda x: torch.tensor(np.ascontiguousarray(x, dtype=np.float32), device="cuda") if x is not None else None  # noqa: E731
+    dt, dd = d(target), None if certain else d(draft)
+    tk, rs = i32(torch, tokens), i32(torch, np.arange(n + 1) * 2)
+    ws = torch.zeros(R.verify_drafts_workspace(n, V), dtype=torch.uint8, device="cuda")
+    for u in (0.0, 0.3, 1.0):
+        for border in (0.45, 0.63):
+            ua, us = d(np.full(2 * n, u)), d(np.full(n, border))
+            acc, out = i32(torch, np.zeros(n)), i32(torch, np.full(2 * n, -9))
+            R.verify_drafts(ptr(dt), V, ptr(dd), V, ptr(tk), ptr(rs), n, 2 * n, V, ptr(ua), ptr(us), ptr(acc), ptr(out), ptr(ws),
+                            ws.numel(), torch.cuda.current_stream().cuda_stream)
+            for i, (p, q) in enumerate(pairs):
+                weight = target[2 * i].astype(np.float64)
+                weight[40] = p if np.isfinite(p) and p > 0 else 0.0
+                ok = bool(np.isfinite(q) and np.float64(np.float32(u)) * max(q, 0.0) < weight[40])
+                assert acc[i].item() == ok, (p, q, u)
+                if ok:
+                    weight = target[2 * i + 1].astype(np.float64)
+                elif certain:
+                    weight[40] = 0
+                else:
+                    weight -= draft[2 * i]
+                    weight[40] = max((p if np.isfinite(p) and p > 0 else 0.0) - max(q, 0.0), 0.0) if np.isfinite(q) else 0.0
+                c = weight.cumsum()
+                token = int((c <= np.float64(np.float32(border)) * c[-1]).sum())
+                assert out[2 * i: 2 * i + 2].tolist() == ([40, token] if ok else [token, -1]), (p, q, u, border)
+
+
 # ---------------------------------------------------------------------------
 # The ops together
 # ---------------------------------------------------------------------------

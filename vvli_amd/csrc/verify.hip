@@ -60,9 +60,11 @@ __device__ __forceinline__ void load8(const Weights& w, uint32_t v, float (&p)[8
         p[i] = in ? w.p[v + i] : 0.f, q[i] = in && w.q ? w.q[v + i] : 0.f;
     }
 }
+// Negative values of the draft count 0; ones that are not finite leave nothing of the target's.
+__device__ __forceinline__ float draft_value(float q) { return fabsf(q) < INFINITY ? fmaxf(q, 0.f) : INFINITY; }
 __device__ __forceinline__ double weight(const Weights& w, uint32_t v, float p, float q) {
     // (finite and positive: also of a difference, which is f64 since f32 would round it)
-    const double d = v == w.without ? 0.0 : static_cast<double>(p) - static_cast<double>(q);
+    const double d = v == w.without ? 0.0 : static_cast<double>(p) - static_cast<double>(draft_value(q));
     return d > 0 && d < INFINITY ? d : 0.0;
 }
 __device__ __forceinline__ double weight8(const Weights& w, uint32_t v, const float (&p)[8], const float (&q)[8], double (&x)[8]) {
@@ -128,8 +130,8 @@ __global__ __launch_bounds__(kThreads) void verify_kernel(VerifyArgs a) {
         const uint32_t x = a.tokens[row + 1];
         bool ok = false;
         if (x < a.vocab) {
-            const double q = a.draft ? a.draft[row * a.ldd + x] : 1.0;
-            ok = static_cast<double>(a.u_accept[row]) * q < static_cast<double>(a.target[row * a.ldt + x]);
+            const float p = a.target[row * a.ldt + x], q = a.draft ? draft_value(a.draft[row * a.ldd + x]) : 1.f;
+            ok = p > 0 && p < INFINITY && q < INFINITY && static_cast<double>(a.u_accept[row]) * q < p;
         }
         if (!ok) atomicMin(&stop, i);
     }

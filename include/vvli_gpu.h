@@ -534,8 +534,9 @@ size_t vvli_gpu_paged_attention_workspace(uint32_t rows, uint32_t requests, uint
  * whole row is 0) and -1 for the rest of the request's rows; a request without
  * rows has accepted[r] = 0. Rows of no request stay as they are; row_start
  * ascends (as above). At most 65535 requests.
- * target and draft may have any stride >= vocab; out is not tokens. workspace: at least
- * vvli_gpu_verify_drafts_workspace bytes, at a 16-byte address. */
+ * target and draft may have any stride >= vocab; out does not overlap tokens.
+ * workspace: at least vvli_gpu_verify_drafts_workspace bytes, at a 16-byte
+ * address. */
 int vvli_gpu_verify_drafts(const float* target, uint64_t ldt, const float* draft, uint64_t ldd, const int32_t* tokens,
                            const int32_t* row_start, uint32_t requests, uint32_t rows, uint32_t vocab,
                            const float* u_accept, const float* u_sample, int32_t* accepted, int32_t* out,

@@ -129,6 +129,20 @@ def test_verify_drafts_refusals(bad, name):
     assert e.value.name == name
 
 
+@pytest.mark.parametrize("rows", [0, 1, 5])
+@pytest.mark.parametrize("gap", [-5, -4, -1, 0, 1, 4, 5])
+def test_verify_drafts_output_over_its_tokens_is_refused(rows, gap):
+    """`rows` tokens and outputs `gap` values apart: refused where they share one (or start together)."""
+    tokens = P << 4
+    good = dict(tokens=tokens, out=tokens + 4 * gap, rows=rows, requests=1)
+    if gap == 0 or abs(gap) < rows:
+        with pytest.raises(VvliError, match="overlaps"):
+            verify(**good)
+    else:  # not for this: the workspace is looked at next
+        with pytest.raises(VvliError, match="workspace"):
+            verify(**good, workspace_bytes=0)
+
+
 def test_workspace_sizes():
     assert R.paged_attention_workspace(1, 1, 32, 8, 64) > 0
     assert R.paged_attention_workspace(1, 1, 32, 7, 64) == 0   # kv_heads does not divide heads

@@ -270,7 +270,9 @@ int vvli_gpu_verify_drafts(const float* target, uint64_t ldt, const float* draft
     if (requests == 0 || vocab == 0 || rows >= kPagedMost || requests > 65535 || vocab >= kPagedMost || ldt < vocab ||
         ldt >= kPagedMost || (draft && (ldd < vocab || ldd >= kPagedMost)))
         return set_error(VVLI_INVALID_CONFIG, "%s: bad sizes (%u requests, %u rows of %u)", who, requests, rows, vocab);
-    if (out == tokens) return set_error(VVLI_INVALID_CONFIG, "%s: out is tokens", who);
+    // (Blocks read tokens while others write out.)
+    const uintptr_t from = reinterpret_cast<uintptr_t>(tokens), to = reinterpret_cast<uintptr_t>(out), size = rows * sizeof(int32_t);
+    if (to == from || (to < from + size && from < to + size)) return set_error(VVLI_INVALID_CONFIG, "%s: out overlaps tokens", who);
     if (!aligned16(workspace) || workspace_bytes < vvli_gpu_verify_drafts_workspace(requests, vocab))
         return set_error(VVLI_INVALID_CONFIG, "%s: workspace of %zu bytes", who, workspace_bytes);
     VerifyArgs a{};

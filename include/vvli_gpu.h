@@ -497,15 +497,15 @@ int vvli_gpu_norm_rope_append(const vvli_gpu_paged_cache* cache, const float* q,
  * negative position) gets zeros. Positions behind the table's end, and those
  * whose page number is outside 0..pages - 1, are not seen; keys and values that
  * a row does not see do not reach it, whatever they are (of those that it sees,
- * a value that is not finite reaches its dimension, and a key that is not finite
- * makes NaN of the row in a 16-bit cache). Rows of no request
- * stay as they are; row_start ascends (rows that it gives to several requests
- * get one's output). Scores, sums and outputs are held in f32: an f32 q
- * and the weights are split into terms of the cache's type so that the products
- * keep f32 accuracy. Results do not change from run to run. q and out at
- * 16-byte addresses, their strides multiples of 4, out not overlapping q.
- * workspace: at least vvli_gpu_paged_attention_workspace bytes, at a 16-byte
- * address. */
+ * a value that is not finite reaches its dimension, and a key that is not
+ * finite makes NaN of the row in a 16-bit cache). Rows of no request stay as
+ * they are; row_start ascends (rows that it gives to several requests get one's
+ * output). Scores, sums and outputs are held in f32: an f32 q and the weights
+ * are split into terms of the cache's type so that the products keep f32
+ * accuracy (over an f16 cache a weight is also off by up to 2^-36 of its row's
+ * largest). Results do not change from run to run. q and out at 16-byte
+ * addresses, their strides multiples of 4, out not overlapping q. workspace: at
+ * least vvli_gpu_paged_attention_workspace bytes, at a 16-byte address. */
 int vvli_gpu_paged_attention(const vvli_gpu_paged_cache* cache, const int32_t* table, uint32_t table_stride,
                              const int32_t* row_start, const int32_t* start_pos, uint32_t requests, const float* q,
                              uint64_t ldq, float* out, uint64_t ldo, uint32_t rows, uint32_t heads, float scale,

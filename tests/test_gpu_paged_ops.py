@@ -640,6 +640,50 @@ def test_attention_idle_requests(torch, kind, n_req):
             check(torch, b, attend(torch, b, kind))
 
 
+@pytest.mark.parametrize("requests,rows,hd", [(1, 1, 64), (800, 1, 64), (600, 3, 128), (40, 150, 64), (40, 250, 128), (40, 100, 32)])
+def test_attention_small_weights_in_f16(torch, requests, rows, hd):
+    """One key whose value is 0 is 2^31 times as heavy as each of the others, whose values are 1: they make all of the output,
+    as many as they are * 2^-31. f16 terms of a weight are off by half of f16's smallest step at most, 2^-25, where the
+    heaviest weight is 2^11 at least: 2^-36 for every key, beside the bound of the other cases (scores of 31 ln 2 = 21.5).
+    The requests share their pages and are enough for items that are not cut."""
+    kv, ps, past = 2, 16, 4000
+    pages = (past + rows) // ps + 2
+    t = torch.float16
+    k, v = torch.zeros(pages * ps, kv, hd, dtype=t, device="cuda"), torch.ones(pages * ps, kv, hd, dtype=t, device="cuda")
+    k[17, :, 0], v[17] = 1.0, 0.0
+    q = torch.zeros(requests * rows, 4 * hd, device="cuda")
+    q[:, ::hd] = 31 * np.log(2.0)
+    out = torch.full((requests * rows, 4 * hd), 9.0, device="cuda")
+    table, rs = i32(torch, np.tile(np.arange(pages), (requests, 1))), i32(torch, np.arange(requests + 1) * rows)
+    st = i32(torch, np.full(requests, past))
+    ws = torch.zeros(R.paged_attention_workspace(requests * rows, requests, 4, kv, hd), dtype=torch.uint8, device="cuda")
+    R.paged_attention(R.PagedCache(ptr(k), ptr(v), "f16", kv, hd, ps, pages), ptr(table), pages, ptr(rs), ptr(st), requests, ptr(q), 4 * hd,
+                      ptr(out), 4 * hd, requests * rows, 4, 1.0, 0, ptr(ws), ws.numel(), torch.cuda.current_stream().cuda_stream)
+    gap = np.exp(-np.float64(np.float32(31 * np.log(2.0))))
+    n = past + np.tile(np.arange(rows), requests)[:, None]  # keys beside the heavy one
+    want = n * gap / (1 + n * gap)
+    err = np.abs(out.cpu().numpy().astype(np.float64) - want)
+    over = err - (n * 2.0 ** -36 + 2 * ((hd + 8) * 21.5 + n + 24) * U * want)
+    assert over.max() <= 0, f"{(err / want).max():.3g} of the output"
+
+
+@pytest.mark.parametrize("rows,hd", [(1, 64), (2, 128), (200, 32), (200, 64), (300, 128)])
+@pytest.mark.parametrize("log2", [8, 16, 20, 23, 24, 25, 26, 27, 28, 30])
+def test_attention_scores_past_f32s_steps_in_f16(torch, rows, hd, log2):
+    """Scores (in base 2) of 2^log2 and up to 8 above it, where f32 holds no more than some of the steps between: which keys are
+    ahead is a matter of rounding, but outputs stay averages of the values, 1 .. 2."""
+    kv, ps, past = 1, 16, 500
+    pages, rng = (past + rows) // ps + 1, np.random.RandomState(log2)
+    t = torch.float16
+    k, v = torch.zeros(pages * ps, kv, hd, dtype=t), torch.tensor(1 + rng.rand(pages * ps, kv, hd)).to(t)
+    k[:, :, 0], k[:, :, 1] = 1024.0, torch.tensor(rng.randint(0, 9, (pages * ps, 1))).to(t)
+    q = torch.zeros(rows, 2, hd, device="cuda")
+    q[..., 0], q[..., 1] = 2.0 ** (log2 - 10) * np.log(2.0), np.log(2.0)
+    b = dict(q=q.cpu(), k=k, v=v, table=np.arange(pages, dtype=np.int32)[None], row_start=np.array([0, rows]), start=np.array([past]), pages=pages, ps=ps)
+    out = attend(torch, b, "f16", scale=1.0)
+    assert out.isfinite().all() and (out >= 1 - 1e-5).all() and (out <= 2 + 1e-5).all(), (out.min(), out.max())
+
+
 def test_attention_workspace_serves_other_sizes(torch):
     """One workspace, zeroed once, for calls of other head sizes, rows and requests in turn: no call's parts lie on another's counters."""
     ws = torch.zeros(max(R.paged_attention_workspace(200, 8, h, kv, hd) for h, kv, hd in ((28, 4, 128), (32, 8, 64), (4, 2, 32))),

@@ -324,19 +324,21 @@ __device__ __forceinline__ bool last_part(uint32_t* arrived, uint32_t n, uint32_
 // has 11, so two hold 22 (the rest, 2^-22 of x at most and half of that on
 // average, is what rounding a product to f32 leaves too). f16 has few
 // exponents: q is scaled by a power of two to below 2^13 (and the scores back),
-// and p to 2^13 at most, so that what the smallest second terms lose is far
-// below a rounding of the largest first; 2^13 times f16's largest value times
-// the number of keys stays far below f32's end. An f32 cache goes through
-// 16x16x4 products of f32.
+// and the largest weight to 2^15 or, in chunks, whose scale follows the largest
+// at a distance, 2^11 at least: terms are off by half of f16's smallest
+// step, 2^-25, so that a weight is by 2^-36 of the largest at most. (With the
+// largest at 2^5, a key 2^31 times as heavy as thousands of others hid them.)
+// 2^15 times f16's largest value times the number of keys stays far below f32's
+// end. An f32 cache goes through 16x16x4 products of f32.
 // ---------------------------------------------------------------------------
 template <int KIND> struct Kind;
 template <> struct Kind<VVLI_CACHE_F32> {
     static constexpr int TERMS = 1, BYTES = 4, U = 1;
-    static constexpr float PBIAS = 0.f;
+    static constexpr float TOP = 0.f;
 };
 template <> struct Kind<VVLI_CACHE_BF16> {
     static constexpr int TERMS = 3, BYTES = 2, U = 2;
-    static constexpr float PBIAS = 0.f;
+    static constexpr float TOP = 0.f;
     typedef __bf16 T;
     typedef bf16x8 T8;
     static __device__ __forceinline__ f32x4 mfma(T8 x, T8 y, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_bf16(x, y, c, 0, 0, 0); }
@@ -344,7 +346,7 @@ template <> struct Kind<VVLI_CACHE_BF16> {
 };
 template <> struct Kind<VVLI_CACHE_F16> {
     static constexpr int TERMS = 2, BYTES = 2, U = 2;
-    static constexpr float PBIAS = 5.f;
+    static constexpr float TOP = 15.f;
     typedef _Float16 T;
     typedef f16x8 T8;
     static __device__ __forceinline__ f32x4 mfma(T8 x, T8 y, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_f16(x, y, c, 0, 0, 0); }
@@ -387,6 +389,12 @@ __device__ __forceinline__ void split2(float x, float y, int e, typename K::T8 (
     } else {
         split<K>(x, e, t), split<K>(y, e + 1, t);
     }
+}
+// What is added to scores for weights of 2^bias at m. Where f32's steps at m are over 1, bias - m is rounded, and weights
+// that are 2^16 or more for it are none in f16: there it is -m.
+__device__ __forceinline__ float shift_of(float bias, float m) {
+    const float x = bias - m;
+    return x + m > bias + 0.5f ? -m : x;
 }
 // The power of two that brings a row of q with this largest value below 2^13.
 __device__ __forceinline__ int f16_exponent(float top) {
@@ -694,13 +702,13 @@ __global__ __launch_bounds__(kThreads, HD == 128 ? 2 : 3) void paged_attn_kernel
                 const float m_new = fmaxf(m_run, rows_max(mx) * inv);
                 const float m_sub = m_new == -INFINITY ? 0.f : m_new;
                 const bool grew = m_new != m_run;
-                const float corr = __builtin_amdgcn_exp2f(m_run - m_sub);
+                const float corr = __builtin_amdgcn_exp2f(m_run - m_sub), shift = shift_of(K::TOP, m_sub);
                 float sum = 0.f;
 #pragma unroll
                 for (int u = 0; u < U; ++u)
 #pragma unroll
                     for (int j = 0; j < 4; ++j) {
-                        const float p = __builtin_amdgcn_exp2f(fmaf(s[u][j], inv, K::PBIAS - m_sub));
+                        const float p = __builtin_amdgcn_exp2f(fmaf(s[u][j], inv, shift));
                         s[u][j] = p;
                         sum += p;
                     }
@@ -914,15 +922,13 @@ struct Wide {
     static constexpr int RB = HD * K::BYTES, CH = RB / 16, RPL = RB < 256 ? 256 / RB : 1;  // bytes and 16-byte chunks of a row, rows of 256 bytes
     static constexpr int TILE = WK * RB, LOADS = 2 * TILE / (16 * kThreads), ROWS = LOADS > 1 ? LOADS / 2 : 1;
     static constexpr int QR = F32 ? 1 : 2;  // terms of q in registers; the rest in LDS
+    // A vector's weights are 2^(s + BIAS - base) with a base that follows the maximum of its scores only where that is
+    // more than SLACK above it: weights stay in range, and few steps have outputs to rescale.
+    static constexpr float SLACK = K::TOP > 0.f ? 4.f : 8.f, BIAS = K::TOP > 0.f ? K::TOP - SLACK : 0.f;
     static constexpr int kQ = (K::TERMS - QR) * 4 * DS * 1024;
     static __device__ __forceinline__ uint32_t kswz(uint32_t r) { return r / RPL % (CH < 16 ? CH : 16); }
     static __device__ __forceinline__ uint32_t vswz(uint32_t r) { return F32 ? (CH >= 16 ? r / 4 % 2 * 8 : 0) : 4 * (r / RPL % (CH / 4)); }
 };
-// A vector's weights are 2^(s - base) with a base that follows the maximum of
-// its scores only where that is more than this above it: weights stay in range,
-// and few steps have outputs to rescale.
-constexpr float kSlack = 8.f;
-
 // Products' results may be read so many wait states behind the last of them
 // (18 for the longest, 32 x 32 x 2 in f32). The compiler counts these along
 // one way to a read; where a branch lies between the two, the other way can be
@@ -1069,7 +1075,7 @@ __global__ __launch_bounds__(kThreads, 2) void paged_wide_kernel(PagedAttnArgs a
         };
         bool spoilt = false;
         for (int careful = 0; careful < 2; ++careful) {
-            m_run = -INFINITY, l_run = 0.f, shift = K::PBIAS;
+            m_run = -INFINITY, l_run = 0.f, shift = F::BIAS;
 #pragma unroll
             for (int n = 0; n < NT; ++n)
 #pragma unroll
@@ -1129,11 +1135,11 @@ __global__ __launch_bounds__(kThreads, 2) void paged_wide_kernel(PagedAttnArgs a
                     for (int r = 2; r < 16; ++r) mx = fmaxf(mx, s[r]);
                     const auto sw = __builtin_amdgcn_permlane32_swap(__float_as_uint(mx), __float_as_uint(mx), false, false);
                     mx = fmaxf(__uint_as_float(sw[0]), __uint_as_float(sw[1])) * inv;
-                    const bool grew = mx > m_run + kSlack;
+                    const bool grew = mx - m_run > F::SLACK;
                     if (__any(grew)) {
                         const float m_new = grew ? mx : m_run, m_sub = m_new == -INFINITY ? 0.f : m_new;
                         const float corr = __builtin_amdgcn_exp2f(m_run - m_sub);
-                        m_run = m_new, shift = K::PBIAS - m_sub, l_run *= corr;
+                        m_run = m_new, shift = shift_of(F::BIAS, m_sub), l_run *= corr;
 #pragma unroll
                         for (int n = 0; n < NT; ++n) o[n] *= corr;
                     }

@@ -481,7 +481,7 @@ int vvli_gpu_paged_assign(const vvli_gpu_page_pool* pool, const int32_t* held, c
  * same stride) receives the rotated heads * head_dim values. k and v go to slot
  * slots[i]; a row whose slot is outside the cache is not appended, and two rows
  * of one slot leave one of them. q, k, v and q_out at 16-byte addresses, their
- * strides multiples of 4. */
+ * strides multiples of 4; fewer than 2^26 rows. */
 int vvli_gpu_norm_rope_append(const vvli_gpu_paged_cache* cache, const float* q, uint64_t ldq, const float* k,
                               uint64_t ldk, const float* v, uint64_t ldv, uint32_t rows, uint32_t heads, float* q_out,
                               uint64_t ldo, const float* inv_freq, const int32_t* pos, const int64_t* slots,

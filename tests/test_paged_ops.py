@@ -87,6 +87,14 @@ def test_norm_rope_append_refusals(bad, name):
     assert e.value.name == name
 
 
+def test_norm_rope_append_rows_that_no_launch_takes_are_refused():
+    """2^26 rows are 2^32 threads, which no launch has: refused before it, with what other sizes give."""
+    for rows in (1 << 26, (1 << 26) + 1, (1 << 31) - 1):
+        with pytest.raises(VvliError) as e:
+            norm(rows=rows)
+        assert e.value.name == CONFIG
+
+
 @pytest.mark.parametrize("bad,name", [
     (dict(table=None), NULL), (dict(row_start=None), NULL), (dict(start_pos=None), NULL), (dict(q=None), NULL),
     (dict(out=None), NULL), (dict(workspace=None), NULL), (dict(heads=0), CONFIG), (dict(heads=5), CONFIG),

@@ -61,6 +61,7 @@ __device__ inline void put4(T* p, const float (&x)[4]) {
 }
 
 constexpr int kThreads = 256;
+constexpr uint32_t kRowsMost = 1u << 26;  // a wave a row: a launch takes fewer than 2^32 threads
 
 // Wave w of the grid: row w / chunks, turns w % chunks, + chunks, ... of the row's heads.
 template <int HD, typename T, bool SPLIT>
@@ -175,7 +176,7 @@ extern "C" int vvli_gpu_norm_rope_append(const vvli_gpu_paged_cache* cache, cons
     if (rc) return rc;
     if (!inv_freq || !pos || !slots) return set_error(VVLI_NULL_ARG, "NULL argument to %s", who);
     const uint64_t hd = cache->head_dim, wq = heads * hd, wk = cache->kv_heads * hd;
-    if (heads == 0 || heads + 2ull * cache->kv_heads > 65535 || rows >= kPagedMost || rope_layout > VVLI_ROPE_SPLIT_HALF ||
+    if (heads == 0 || heads + 2ull * cache->kv_heads > 65535 || rows >= kRowsMost || rope_layout > VVLI_ROPE_SPLIT_HALF ||
         weight_kind > VVLI_WEIGHT_BF16)
         return set_error(VVLI_INVALID_CONFIG, "%s: bad sizes (%u rows, %u heads, layout %u, weight kind %u)", who, rows, heads,
                          rope_layout, weight_kind);

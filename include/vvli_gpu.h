@@ -452,10 +452,12 @@ typedef struct vvli_gpu_page_pool {
  * given pages in the order of requests and positions, and behind them the
  * stack from its top, the new pages in that order take L[0], L[1], ... (so a
  * step that is given back leaves the pool as it was). A request whose pages L
- * does not cover keeps what it holds and gets no rows, and so do all behind it
- * that need pages; the same goes for one with add[r] < 0, keep[r] outside
- * 0..held[r], more tokens than its row of the table has room for, or rows past
- * `rows`.
+ * does not cover keeps what it holds, and so do all behind it that need pages;
+ * the same goes for one with add[r] < 0, keep[r] outside 0..held[r], more
+ * tokens than its row of the table has room for, or rows past `rows`. Its rows
+ * stay in the batch (row_start counts them) at negative positions and without
+ * slots: they are appended nowhere, see nothing, and what later calls compute of
+ * them is to be passed over.
  * Outputs: len[r] = keep[r] + add[r] (or held[r], see above; may be `held`
  * itself); row_start[0..requests]: new rows before request r (negative add
  * counts 0, at most `rows`); start_pos[r] = keep[r], the position of its first
@@ -467,7 +469,11 @@ typedef struct vvli_gpu_page_pool {
  * last new row stay as they are (a captured step over `rows` rows, of which a
  * batch may have fewer, sets slots to -1 before this call: rows that are none
  * are then appended nowhere). `held` is what earlier calls returned: this one
- * does not look for pages that two requests share. */
+ * does not look for pages that two requests share.
+ * What a request keeps at the next step: where add[r] > 0 and start_pos[r] >= 0,
+ * start_pos[r] and those of its new rows that are to stay (a token and its
+ * accepted drafts: start_pos[r] + 1 + accepted[r]); else keep[r] again, whatever
+ * accepted[r] is. */
 int vvli_gpu_paged_assign(const vvli_gpu_page_pool* pool, const int32_t* held, const int32_t* keep, const int32_t* add,
                           uint32_t rows, int32_t* len, int32_t* row_start, int32_t* start_pos, int32_t* row_pos,
                           int64_t* slots, void* stream);

@@ -1046,6 +1046,71 @@ def test_steps_of_several_requests_match_the_runner(torch):
         r.close()
 
 
+def test_steps_with_a_dry_pool_and_idle_requests(torch):
+    """The loop of assign and verify as a host keeps it: a request that got its rows keeps them up to the last accepted draft
+    (all of a prompt's); one that had none, or that the pool had no pages for, keeps what it kept before and offers its rows
+    again; where nobody gets pages the last one gives up its own and starts again from its text. The calls give what plain
+    ones give, and every request gets to its end."""
+    rng = np.random.RandomState(5)
+    n, ps, stride, pages, V, most, goal = 6, 4, 12, 26, 50, 256, 34
+    pool = Pool(torch, n, stride, ps, pages)
+    rs, st, pos = i32(torch, np.zeros(n + 1)), i32(torch, np.zeros(n)), i32(torch, np.zeros(most))
+    slots = torch.zeros(most, dtype=torch.int64, device="cuda")
+    vw = torch.zeros(R.verify_drafts_workspace(n, V), dtype=torch.uint8, device="cuda")
+    acc, out = i32(torch, np.zeros(n)), i32(torch, np.zeros(most))
+    stream = torch.cuda.current_stream().cuda_stream
+    text = [rng.randint(0, V, 3 + r).tolist() for r in range(n)]  # the last token is never in the cache
+    keep, waited, idle, restarts = np.zeros(n, np.int64), 0, 0, 0
+    for step in range(400):
+        ended = [len(t) > goal for t in text]
+        if all(ended):
+            break
+        offered, prompt = [], []
+        for r in range(n):
+            if ended[r]:
+                keep[r] = 0  # its pages go to the others
+            prompt.append(keep[r] < len(text[r]) - 1)
+            if ended[r] or rng.rand() < 0.2:
+                offered.append([])
+            elif prompt[r]:
+                offered.append(text[r][keep[r]: -1])
+            else:
+                offered.append(text[r][-1:] + rng.randint(0, V, rng.randint(0, 4)).tolist())
+        add = [len(x) for x in offered]
+        held = pool.d_len.cpu().numpy().astype(np.int64)
+        flat = np.array([t for x in offered for t in x] + [0] * (most - sum(add)))
+        p, q, ua, us = (rng.rand(*s).astype(np.float32) for s in ((most, V), (most, V), (most,), (n,)))
+        d = [i32(torch, keep), i32(torch, add), i32(torch, flat), *(torch.tensor(x, device="cuda") for x in (p, q, ua, us))]
+        R.paged_assign(pool.handle, ptr(pool.d_len), ptr(d[0]), ptr(d[1]), most, ptr(pool.d_len), ptr(rs), ptr(st), ptr(pos), ptr(slots), stream)
+        R.verify_drafts(ptr(d[3]), V, ptr(d[4]), V, ptr(d[2]), ptr(rs), n, most, V, ptr(d[5]), ptr(d[6]), ptr(acc), ptr(out), ptr(vw),
+                        vw.numel(), stream)
+        want = plain_assign(pool.stack, pool.table, ps, pages, held, keep, add, most)
+        start, length, first = st.tolist(), pool.d_len.tolist(), rs.tolist()
+        assert start == want[2] and length == want[0] and first == want[1]
+        accepted, given = acc.tolist(), out.tolist()
+        plain = plain_verify(p, q, flat, first, ua, us, V, np.zeros(most))
+        assert accepted == plain[0] and given[: first[n]] == plain[1][: first[n]]
+        moved = False
+        for r in range(n):
+            if add[r] and start[r] >= 0:
+                moved = True
+                if prompt[r]:
+                    keep[r] = length[r]
+                else:
+                    keep[r] = start[r] + 1 + accepted[r]
+                    text[r] += given[first[r]: first[r] + accepted[r] + 1]
+                assert keep[r] == len(text[r]) - 1 <= length[r]
+            else:
+                waited, idle = waited + (add[r] > 0), idle + (add[r] == 0)
+                assert length[r] == (held[r] if add[r] else keep[r])
+        if not moved and any(add):
+            keep[max(r for r in range(n) if not ended[r] and length[r])] = 0
+            restarts += 1
+    assert all(len(t) > goal for t in text), [len(t) for t in text]
+    print(f"{step} steps, {waited} without pages, {idle} idle, {restarts} restarts", flush=True)
+    assert waited > 5 and idle > 20
+
+
 def test_captured_step_follows_the_eager_one(torch):
     """A whole step in one graph, for batches of fewer rows than it has room for: pages, cache, outputs and tokens are those of eager
     calls over the same inputs, replay by replay, with eager work between."""

@@ -413,8 +413,10 @@ int vvli_gpu_test_linear_route(uint32_t M, uint32_t N, uint32_t K, uint32_t cus,
  * none leads outside the buffers that the arguments describe. Sizes that a
  * call does not take return VVLI_INVALID_CONFIG before any launch.
  * Workspaces are the caller's: one belongs to one call at a time, so calls or
- * replays that may overlap need one each. They are zeroed once, when they are
- * allocated; a call leaves its counters zeroed. */
+ * replays that may overlap need one each, and to one of the two ops that take
+ * one: what vvli_gpu_paged_attention leaves there are no counters of
+ * vvli_gpu_verify_drafts, nor the other way round. They are zeroed once, when
+ * they are allocated; a call leaves its counters zeroed. */
 
 /* Types of a paged cache. Activations are f32 as in vvli_gpu_linear; values
  * are rounded to the cache's type once, to nearest even. */
@@ -481,13 +483,14 @@ int vvli_gpu_paged_assign(const vvli_gpu_page_pool* pool, const int32_t* held, c
 /* RMS norm of every q and k head (weights q_norm / k_norm [head_dim] of type
  * weight_kind, VVLI_WEIGHT_*; NULL: no norm), rotation of q and k by the angles
  * pos[i] * inv_freq[0..head_dim/2-1] in rope_layout (VVLI_ROPE_*; angles are
- * formed in 64 bits), and the append of k and v to the cache, in one pass. Row
- * i of q, k and v is at i * ldq, i * ldk, i * ldv (elements; the three may lie
- * in one stacked projection); q_out (row stride ldo; may be q itself with the
- * same stride) receives the rotated heads * head_dim values. k and v go to slot
- * slots[i]; a row whose slot is outside the cache is not appended, and two rows
- * of one slot leave one of them. q, k, v and q_out at 16-byte addresses, their
- * strides multiples of 4; fewer than 2^26 rows. */
+ * formed and turns taken off them in 64 bits, sine and cosine are f32), and the
+ * append of k and v to the cache, in one pass. Row i of q, k and v is at i *
+ * ldq, i * ldk, i * ldv (elements; the three may lie in one stacked
+ * projection); q_out (row stride ldo; may be q itself with the same stride)
+ * receives the rotated heads * head_dim values. k and v go to slot slots[i]; a
+ * row whose slot is outside the cache is not appended, and what a slot holds
+ * that two rows name is not specified. q, k, v and q_out at 16-byte addresses,
+ * their strides multiples of 4; fewer than 2^26 rows. */
 int vvli_gpu_norm_rope_append(const vvli_gpu_paged_cache* cache, const float* q, uint64_t ldq, const float* k,
                               uint64_t ldk, const float* v, uint64_t ldv, uint32_t rows, uint32_t heads, float* q_out,
                               uint64_t ldo, const float* inv_freq, const int32_t* pos, const int64_t* slots,
@@ -505,18 +508,22 @@ int vvli_gpu_norm_rope_append(const vvli_gpu_paged_cache* cache, const float* q,
  * a row does not see do not reach it, whatever they are (of those that it sees,
  * a value that is not finite reaches its dimension, and a key that is not
  * finite makes NaN of the row in a 16-bit cache). Rows of no request stay as
- * they are; row_start ascends (rows that it gives to several requests get one's
- * output). Scores, sums and outputs are held in f32: an f32 q and the weights
- * are split into terms of the cache's type so that the products keep f32
- * accuracy (over an f16 cache a weight is also off by up to 2^-36 of its row's
- * largest). Results do not change from run to run. q and out at 16-byte
- * addresses, their strides multiples of 4, out not overlapping q. workspace: at
- * least vvli_gpu_paged_attention_workspace bytes, at a 16-byte address. */
+ * they are; row_start ascends (the output of a row that it gives to several
+ * requests is not specified). Scores, sums and outputs are held in f32: an f32
+ * q and the weights are split into terms of the cache's type so that the
+ * products keep f32 accuracy (over an f16 cache a weight is also off by up to
+ * 2^-36 of its row's largest). Values times 256 and the keys of a row have to
+ * stay in f32's range. Results do not change from run to run. q and out at
+ * 16-byte addresses, their strides multiples of 4, out not overlapping q.
+ * workspace: at least vvli_gpu_paged_attention_workspace bytes, at a 16-byte
+ * address. */
 int vvli_gpu_paged_attention(const vvli_gpu_paged_cache* cache, const int32_t* table, uint32_t table_stride,
                              const int32_t* row_start, const int32_t* start_pos, uint32_t requests, const float* q,
                              uint64_t ldq, float* out, uint64_t ldo, uint32_t rows, uint32_t heads, float scale,
                              uint32_t window, void* workspace, size_t workspace_bytes, void* stream);
-/* Bytes of workspace that calls of up to these sizes need; 0 for sizes that a call refuses. */
+/* Bytes of workspace that calls of up to so many rows, of any number of requests,
+ * with these heads need; 0 for sizes that a call refuses. Where several kinds of
+ * heads share one, it has the most of what they need. */
 size_t vvli_gpu_paged_attention_workspace(uint32_t rows, uint32_t requests, uint32_t heads, uint32_t kv_heads,
                                           uint32_t head_dim);
 
@@ -547,7 +554,7 @@ int vvli_gpu_verify_drafts(const float* target, uint64_t ldt, const float* draft
                            const int32_t* row_start, uint32_t requests, uint32_t rows, uint32_t vocab,
                            const float* u_accept, const float* u_sample, int32_t* accepted, int32_t* out,
                            void* workspace, size_t workspace_bytes, void* stream);
-/* Bytes of workspace that calls of up to these sizes need (0 for a vocabulary of 0). */
+/* Bytes of workspace that calls of up to so many requests, of any vocabulary, need (0 for a vocabulary of 0). */
 size_t vvli_gpu_verify_drafts_workspace(uint32_t requests, uint32_t vocab);
 
 #ifdef __cplusplus

@@ -474,7 +474,7 @@ def norm_rope_append(cache: PagedCache, q: int, ldq: int, k: int, ldk: int, v: i
 
 
 def paged_attention_workspace(rows: int, requests: int, heads: int, kv_heads: int, head_dim: int) -> int:
-    """Bytes of workspace (zeroed once) of ``paged_attention`` calls of up to these sizes."""
+    """Bytes of workspace (zeroed once) of ``paged_attention`` calls of up to so many rows with these heads."""
     return _lib.lib().vvli_gpu_paged_attention_workspace(rows, requests, heads, kv_heads, head_dim)
 
 
@@ -487,7 +487,7 @@ def paged_attention(cache: PagedCache, table: int, table_stride: int, row_start:
 
 
 def verify_drafts_workspace(requests: int, vocab: int) -> int:
-    """Bytes of workspace (zeroed once) of ``verify_drafts`` calls of up to these sizes."""
+    """Bytes of workspace (zeroed once) of ``verify_drafts`` calls of up to so many requests."""
     return _lib.lib().vvli_gpu_verify_drafts_workspace(requests, vocab)
 
 

@@ -392,14 +392,33 @@ __device__ __forceinline__ void split2(float x, float y, int e, typename K::T8 (
 }
 // What is added to scores for weights of 2^bias at m. Where f32's steps at m are over 1, bias - m is rounded, and weights
 // that are 2^16 or more for it are none in f16: there it is -m.
+template <typename K>
 __device__ __forceinline__ float shift_of(float bias, float m) {
     const float x = bias - m;
-    return x + m > bias + 0.5f ? -m : x;
+    return K::TOP > 0.f && x + m > bias + 0.5f ? -m : x;
 }
 // The power of two that brings a row of q with this largest value below 2^13.
 __device__ __forceinline__ int f16_exponent(float top) {
     const int ex = top > 0.f && top < INFINITY ? 13 - (ilogbf(top) + 1) : 0;
     return min(max(ex, -120), 120);
+}
+
+// A product's result may be read so many wait states behind it (18 for the
+// longest, 32 x 32 x 2 in f32). The compiler counts these along one way to a
+// read; where a branch lies between the two, the other way can be shorter, and
+// the last register of a result was then read before it was written. Here they
+// are spent before any branch: behind chunks' scores and, in both kernels,
+// behind the loop over the keys (inside it outputs are read behind the next
+// step's scores). Behind the scores of few rows they cost one row behind 8000
+// 0.5 of 21.1 us in bf16, so that there it is the compiler's count, as a test
+// of the kernels' listing finds it.
+template <typename V, int N>
+__device__ __forceinline__ void mfma_done(V (&x)[N]) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) asm volatile("" : "+v"(x[i]));
+    asm volatile("s_nop 15\n\ts_nop 3");
+#pragma unroll
+    for (int i = 0; i < N; ++i) asm volatile("" : "+v"(x[i]));
 }
 
 // ---------------------------------------------------------------------------
@@ -702,7 +721,7 @@ __global__ __launch_bounds__(kThreads, HD == 128 ? 2 : 3) void paged_attn_kernel
                 const float m_new = fmaxf(m_run, rows_max(mx) * inv);
                 const float m_sub = m_new == -INFINITY ? 0.f : m_new;
                 const bool grew = m_new != m_run;
-                const float corr = __builtin_amdgcn_exp2f(m_run - m_sub), shift = shift_of(K::TOP, m_sub);
+                const float corr = __builtin_amdgcn_exp2f(m_run - m_sub), shift = shift_of<K>(K::TOP, m_sub);
                 float sum = 0.f;
 #pragma unroll
                 for (int u = 0; u < U; ++u)
@@ -755,6 +774,7 @@ __global__ __launch_bounds__(kThreads, HD == 128 ? 2 : 3) void paged_attn_kernel
                 if (t + 1 < tb) load_v(slots_next);
                 slots = slots_next, none = none_next;
             }
+            mfma_done(o);
             float sum = 0.f;  // NaN if one of them is not finite
 #pragma unroll
             for (int e = 0; e < DV; ++e)
@@ -929,13 +949,6 @@ struct Wide {
     static __device__ __forceinline__ uint32_t kswz(uint32_t r) { return r / RPL % (CH < 16 ? CH : 16); }
     static __device__ __forceinline__ uint32_t vswz(uint32_t r) { return F32 ? (CH >= 16 ? r / 4 % 2 * 8 : 0) : 4 * (r / RPL % (CH / 4)); }
 };
-// Products' results may be read so many wait states behind the last of them
-// (18 for the longest, 32 x 32 x 2 in f32). The compiler counts these along
-// one way to a read; where a branch lies between the two, the other way can be
-// shorter, and the last register of a result was then read before it was
-// written. Here they are spent before any branch.
-__device__ __forceinline__ void mfma_done(f32x16& x, f32x16& y) { asm volatile("s_nop 15\n\ts_nop 3" : "+v"(x), "+v"(y)); }
-
 typedef short s16x4 __attribute__((ext_vector_type(4)));
 
 template <int HD, int KIND>
@@ -1097,9 +1110,9 @@ __global__ __launch_bounds__(kThreads, 2) void paged_wide_kernel(PagedAttnArgs a
                     const char* base = stage[st];
                     // Two sums, of even and odd steps, and below the tiles of O^T in turn: a product waits for the
                     // one before it on the same sum about as long as it takes.
-                    f32x16 s, s2;
+                    f32x16 sums[2];
 #pragma unroll
-                    for (int r = 0; r < 16; ++r) s[r] = s2[r] = 0.f;
+                    for (int r = 0; r < 16; ++r) sums[0][r] = sums[1][r] = 0.f;
 #pragma unroll
                     for (int i = 0; i < DS; i += 2) {
                         const u32x4 k0 = *reinterpret_cast<const u32x4*>(base + (k_at ^ (32 * i)));
@@ -1107,8 +1120,8 @@ __global__ __launch_bounds__(kThreads, 2) void paged_wide_kernel(PagedAttnArgs a
                         if constexpr (F32) {
 #pragma unroll
                             for (int e = 0; e < 4; ++e) {
-                                s = __builtin_amdgcn_mfma_f32_32x32x2f32(__uint_as_float(k0[e]), __uint_as_float(qf[0][i][e]), s, 0, 0, 0);
-                                s2 = __builtin_amdgcn_mfma_f32_32x32x2f32(__uint_as_float(k1[e]), __uint_as_float(qf[0][i + 1][e]), s2, 0, 0, 0);
+                                sums[0] = __builtin_amdgcn_mfma_f32_32x32x2f32(__uint_as_float(k0[e]), __uint_as_float(qf[0][i][e]), sums[0], 0, 0, 0);
+                                sums[1] = __builtin_amdgcn_mfma_f32_32x32x2f32(__uint_as_float(k1[e]), __uint_as_float(qf[0][i + 1][e]), sums[1], 0, 0, 0);
                             }
                         } else {
 #pragma unroll
@@ -1116,13 +1129,13 @@ __global__ __launch_bounds__(kThreads, 2) void paged_wide_kernel(PagedAttnArgs a
                                 u32x4 q0, q1;
                                 if (x < QR) q0 = qf[x < QR ? x : 0][i], q1 = qf[x < QR ? x : 0][i + 1];
                                 else q0 = q_mine[((x - QR) * DS + i) * 64], q1 = q_mine[((x - QR) * DS + i + 1) * 64];
-                                s = K::mfma(__builtin_bit_cast(typename K::T8, k0), __builtin_bit_cast(typename K::T8, q0), s);
-                                s2 = K::mfma(__builtin_bit_cast(typename K::T8, k1), __builtin_bit_cast(typename K::T8, q1), s2);
+                                sums[0] = K::mfma(__builtin_bit_cast(typename K::T8, k0), __builtin_bit_cast(typename K::T8, q0), sums[0]);
+                                sums[1] = K::mfma(__builtin_bit_cast(typename K::T8, k1), __builtin_bit_cast(typename K::T8, q1), sums[1]);
                             }
                         }
                     }
-                    mfma_done(s, s2);
-                    s += s2;
+                    mfma_done(sums);
+                    f32x16 s = sums[0] + sums[1];
                     if (key0 < all_lo || key0 + WK > all_hi || none) {
 #pragma unroll
                         for (int r = 0; r < 16; ++r) {
@@ -1139,7 +1152,7 @@ __global__ __launch_bounds__(kThreads, 2) void paged_wide_kernel(PagedAttnArgs a
                     if (__any(grew)) {
                         const float m_new = grew ? mx : m_run, m_sub = m_new == -INFINITY ? 0.f : m_new;
                         const float corr = __builtin_amdgcn_exp2f(m_run - m_sub);
-                        m_run = m_new, shift = shift_of(F::BIAS, m_sub), l_run *= corr;
+                        m_run = m_new, shift = shift_of<K>(F::BIAS, m_sub), l_run *= corr;
 #pragma unroll
                         for (int n = 0; n < NT; ++n) o[n] *= corr;
                     }
@@ -1189,6 +1202,7 @@ __global__ __launch_bounds__(kThreads, 2) void paged_wide_kernel(PagedAttnArgs a
                 none = none_next;
                 __syncthreads();
             }
+            mfma_done(o);
             float sum = 0.f;  // NaN if one of them is not finite
 #pragma unroll
             for (int n = 0; n < NT; ++n)

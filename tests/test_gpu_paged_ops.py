@@ -908,7 +908,7 @@ def test_verify_values_that_are_no_probabilities(torch, certain):
     """Drafted tokens on target and draft values that are infinite, NaN, negative or 0. A target value that is not finite and
     positive counts 0; a negative draft value too; a draft value that is not finite refuses its token and leaves it no weight."""
     V = 64
-    odd = [float("inf"), float("-inf"), float("nan"), -0.5, 0.0, 0.25]
+    odd = [float("inf"), float("-inf"), float("nan"), -float("nan"), -0.5, -0.0, 0.0, 0.25]
     pairs = [(p, q) for p in odd for q in ([1.0] if certain else odd)]
     n = len(pairs)
     target, draft = np.full((2 * n, V), 0.0078125, np.float32), np.full((2 * n, V), 0.00390625, np.float32)

@@ -60,14 +60,21 @@ __device__ __forceinline__ void load8(const Weights& w, uint32_t v, float (&p)[8
         p[i] = in ? w.p[v + i] : 0.f, q[i] = in && w.q ? w.q[v + i] : 0.f;
     }
 }
-// Negative values of the draft count 0; ones that are not finite leave nothing of the target's.
+// A negative value of the draft counts 0, one that is not finite leaves nothing of the target's.
 __device__ __forceinline__ float draft_value(float q) { return fabsf(q) < INFINITY ? fmaxf(q, 0.f) : INFINITY; }
 __device__ __forceinline__ double weight(const Weights& w, uint32_t v, float p, float q) {
     // (finite and positive: also of a difference, which is f64 since f32 would round it)
-    const double d = v == w.without ? 0.0 : static_cast<double>(p) - static_cast<double>(draft_value(q));
+    const double d = v == w.without ? 0.0 : static_cast<double>(p) - static_cast<double>(q);
     return d > 0 && d < INFINITY ? d : 0.0;
 }
-__device__ __forceinline__ double weight8(const Weights& w, uint32_t v, const float (&p)[8], const float (&q)[8], double (&x)[8]) {
+__device__ __forceinline__ double weight8(const Weights& w, uint32_t v, const float (&p)[8], float (&q)[8], double (&x)[8]) {
+    uint32_t signs = 0;  // (values without a sign are right as they are: weight() leaves out what is not finite)
+#pragma unroll
+    for (int i = 0; i < 8; ++i) signs |= __float_as_uint(q[i]);
+    if (__builtin_expect(__any(signs >> 31), 0)) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) q[i] = draft_value(q[i]);
+    }
 #pragma unroll
     for (int i = 0; i < 8; ++i) x[i] = weight(w, v + i, p[i], q[i]);
     return ((x[0] + x[1]) + (x[2] + x[3])) + ((x[4] + x[5]) + (x[6] + x[7]));

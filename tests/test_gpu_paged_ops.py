@@ -684,6 +684,60 @@ def test_attention_scores_past_f32s_steps_in_f16(torch, rows, hd, log2):
     assert out.isfinite().all() and (out >= 1 - 1e-5).all() and (out <= 2 + 1e-5).all(), (out.min(), out.max())
 
 
+def attend_exact(torch, b, window, scale):
+    """As plain_attend, a request and head at a time on the GPU: (out, error bound); without holes, every row a request's."""
+    rows, heads, hd = b["q"].shape
+    kv, ps = b["k"].shape[1], b["ps"]
+    q, k, v = b["q"].cuda().double() * scale, b["k"].cuda(), b["v"].cuda()
+    out, bound = (torch.zeros(rows, heads, hd, dtype=torch.float64, device="cuda") for _ in range(2))
+    for r, past in enumerate(b["start"].tolist()):
+        first, end = int(b["row_start"][r]), int(b["row_start"][r + 1])
+        j = torch.arange(past + end - first, device="cuda")
+        slot = torch.as_tensor(b["table"][r].astype(np.int64), device="cuda")[j // ps] * ps + j % ps
+        pos = past + torch.arange(end - first, device="cuda")[:, None]
+        hidden = (j > pos) | ((j <= pos - window) if window else (j < 0))
+        n = (~hidden).sum(1, keepdim=True)
+        for h in range(heads if end > first else 0):
+            kk, vv = (x[slot, h * kv // heads].double() for x in (k, v))
+            qq, kt = q[first:end, h], kk.t().contiguous()
+            w = torch.softmax((qq @ kt).masked_fill(hidden, -np.inf), -1)
+            out[first:end, h] = w @ vv
+            size = (qq.abs() @ kt.abs()).masked_fill(hidden, 0).amax(1, keepdim=True)
+            bound[first:end, h] = 2 * ((hd + 8) * size + n + 24) * U * (w @ vv.abs())
+    return out.cpu(), bound.cpu()
+
+
+RUNS = {"tokens": [(5000 + 37 * i, 1) for i in range(44)],
+        "drafts": [(8000 - 211 * i, 1 + i % 8) for i in range(36)],
+        "prompts": [(1900, 1000), (400, 1500)],
+        "mixed": [(6000 - 97 * i, 1) for i in range(40)] + [(700, 900), (0, 0), (3000, 5), (0, 300)]}
+
+
+@pytest.mark.parametrize("kind", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("what,heads,kv,hd,window", [
+    ("tokens", 28, 4, 128, 0), ("drafts", 32, 8, 64, 0), ("drafts", 28, 4, 128, 3000), ("prompts", 28, 4, 128, 0),
+    ("prompts", 32, 8, 64, 1000), ("mixed", 28, 4, 128, 0), ("prompts", 16, 4, 32, 0)])
+def test_attention_runs_of_many_units(torch, kind, what, heads, kv, hd, window):
+    """Batches that give every block a long run, over several items or inside one."""
+    spec, ps = RUNS[what], 16
+    print("runs", kind, what, heads, kv, hd, flush=True)
+    g = torch.Generator(device="cuda").manual_seed(hd)
+    need = [-(-(p + n) // ps) for p, n in spec]
+    pages = sum(need) + 2
+    order, table = np.random.RandomState(hd).permutation(pages), np.full((len(spec), max(need)), -1, np.int32)
+    for r, n in enumerate(need):
+        table[r, :n] = order[sum(need[:r]): sum(need[:r]) + n]
+    rnd = lambda *s: torch.randn(*s, device="cuda", generator=g)  # noqa: E731
+    k, v = (rnd(pages * ps, kv, hd).to(types(torch)[kind]) for _ in range(2))
+    row_start = np.concatenate([[0], np.cumsum([n for _, n in spec])]).astype(np.int32)
+    b = dict(q=1.5 * rnd(int(row_start[-1]), heads, hd), k=k, v=v, table=table, row_start=row_start,
+             start=np.array([p for p, _ in spec], np.int32), pages=pages, ps=ps)
+    want, bound = attend_exact(torch, b, window, hd ** -0.5)
+    err = (attend(torch, b, kind, window).double() - want).abs()
+    assert (err <= bound).all(), f"largest error {err.max():.3g}"
+    assert (err.norm() / want.norm()).item() <= 1e-6
+
+
 def test_attention_workspace_serves_other_sizes(torch):
     """One workspace, zeroed once, for calls of other head sizes, rows and requests in turn: no call's parts lie on another's counters."""
     ws = torch.zeros(max(R.paged_attention_workspace(200, 8, h, kv, hd) for h, kv, hd in ((28, 4, 128), (32, 8, 64), (4, 2, 32))),

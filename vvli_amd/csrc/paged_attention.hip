@@ -25,10 +25,10 @@
 #include <hip/hip_fp16.h>
 
 #include <algorithm>
-#include <type_traits>
 
 #include "device_common.hpp"
 #include "paged.hpp"
+#include "paged_runs.hpp"
 
 using namespace vvli;
 
@@ -57,52 +57,9 @@ struct PagedAttnArgs {
 // ---------------------------------------------------------------------------
 // Items and runs
 // ---------------------------------------------------------------------------
-struct Request {
-    uint32_t first, vecs;  // first row, vectors of one kv head
-    int64_t start;
-};
-
 __device__ __forceinline__ Request request_at(const PagedAttnArgs& a, uint32_t r) {
     const RowSpan s = row_span(a.row_start[r], a.row_start[r + 1], a.rows);
     return Request{s.first, s.count * a.group.d, a.start_pos[r]};
-}
-
-// How a kernel cuts its items: M vectors, steps of WK positions, units of one
-// step (FIXED) or of as many as the block's waves take side by side; and in
-// units what an item costs beside its keys (its q, the first loads, its end),
-// what a cut costs (a part left and taken up again), the fewest of a run, and
-// the most of an item that is never cut, since its parts would cost more than
-// they save.
-template <int M_, int WK_, bool FIXED_, uint32_t ITEM, uint32_t CUT, uint32_t FEWEST, uint32_t WHOLE>
-struct Cuts {
-    static constexpr int M = M_, WK = WK_;
-    static constexpr bool FIXED = FIXED_;
-    static constexpr uint32_t kItem = ITEM, kCut = CUT, kFewest = FEWEST, kWhole = WHOLE;
-    static_assert(ITEM + std::min(FEWEST / 4, CUT) < FEWEST, "near_lo + near_hi < per");
-};
-
-// An item's vectors stand in groups of GV = M / 4, one to a wave: 1, 2 or 4
-// waves side by side (the log of that in `wide`) take different vectors, and
-// the 4 >> wide such sets take steps of WK positions in turn, (4 WK) >> wide a
-// unit. The keys lo .. hi - 1 that some vector of the item sees (hi = 0: none),
-// and the units that they touch, behind S::kItem for the item itself.
-struct Units {
-    uint32_t lo, hi, first, count, wide;
-};
-// (FIXED: units of WK positions whatever the item.)
-template <class S>
-__device__ __forceinline__ Units units_of(const PagedAttnArgs& a, const Request& q, uint32_t m0) {
-    const uint32_t vecs = min(static_cast<uint32_t>(S::M), q.vecs - m0);
-    const uint32_t wide = vecs <= S::M / 4 ? 0 : vecs <= S::M / 2 ? 1 : 2;
-    const int64_t p0 = q.start + page_of(a.group, m0);
-    const int64_t p1 = q.start + page_of(a.group, m0 + vecs - 1);
-    const int64_t hi = min(p1 + 1, static_cast<int64_t>(a.room));
-    const int64_t lo = a.window && p0 + 1 > a.window ? p0 + 1 - a.window : 0;
-    if (hi <= lo) return Units{0, 0, 0, S::kItem, wide};
-    const uint32_t unit = S::FIXED ? S::WK : (4 * S::WK) >> wide;
-    Units u{static_cast<uint32_t>(lo), static_cast<uint32_t>(hi), static_cast<uint32_t>(lo) / unit, 0, wide};
-    u.count = (u.hi + unit - 1) / unit - u.first + S::kItem;
-    return u;
 }
 
 __device__ __forceinline__ uint64_t wave_scan(uint64_t v) {
@@ -136,22 +93,15 @@ __device__ __forceinline__ uint64_t request_units(const PagedAttnArgs& a, const 
     return sum;
 }
 
-// Run b holds the units from per * b on to per * (b + 1), but that a border
-// within near_lo units of an item's start (anywhere in one of few units) or
-// near_hi of its end moves there (near_lo + near_hi < per, so that borders keep
-// their order): fewer items are cut, and none before its first keys.
+// A block's run (see Borders).
 struct Run {
-    uint64_t from, to, per;  // global units, before the borders move
-    uint32_t near_lo, near_hi, r, kvh, m0, unit;  // the item that holds unit `from`, and which unit of it that is
+    uint64_t from, to;                // global units, before the borders move
+    Borders at;
+    uint32_t r, kvh, m0, unit;        // the item that holds unit `from`, and which unit of it that is
     uint32_t index;
     Request req;  // of r
     bool any;
 };
-
-// (64-bit division is some 150 instructions; sums of units are mostly below 2^32.)
-__device__ __forceinline__ uint64_t quotient(uint64_t n, uint64_t d) {
-    return ((n | d) >> 32) == 0 ? static_cast<uint32_t>(n) / static_cast<uint32_t>(d) : n / d;
-}
 
 struct RunScratch {
     uint64_t sums[kThreads / 64], found_rest, found_units;
@@ -182,16 +132,11 @@ __device__ Run find_run(const PagedAttnArgs& a, RunScratch& sc) {
     for (uint32_t c = 0; c < chunks; ++c) chunk(c);
     const uint64_t total = before * a.kv_heads;
     Run run{};
-    run.per = max(quotient(total + blocks - 1, blocks), static_cast<uint64_t>(S::kFewest));
-    run.near_hi = static_cast<uint32_t>(min(run.per / 4, static_cast<uint64_t>(S::kCut)));
-    run.near_lo = max(run.near_hi, S::kItem);
-    // Blocks go to the eight XCDs in turn. Each XCD takes as many runs, side by side: neighbours share keys and table
-    // rows in its L2, and fewer runs than blocks still have all of the GPU.
-    const uint32_t runs = static_cast<uint32_t>(quotient(total + run.per - 1, run.per)), each = (runs + 7) / 8;
-    run.index = blocks % 8 == 0 ? blockIdx.x % 8 * each + blockIdx.x / 8 : blockIdx.x;
-    if (run.index >= runs || (blocks % 8 == 0 && blockIdx.x / 8 >= each)) return run;
-    run.from = run.per * run.index;
-    run.to = min(run.from + run.per, total);
+    run.at = borders_of<S>(total, blocks);
+    run.index = run_of_block(blockIdx.x, blocks, run.at.runs);
+    if (run.index >= run.at.runs) return run;
+    run.from = run.at.per * run.index;
+    run.to = min(run.from + run.at.per, total);
     run.any = true;
     before = 0;
     for (uint32_t c = 0; c < chunks; ++c) {
@@ -233,10 +178,9 @@ struct Walk {
     uint64_t start;  // global unit where the item starts
     bool begun;      // the run starts inside the item
     Units un;
-    uint32_t t0, t1;  // units of the item
-    __device__ __forceinline__ uint32_t first_unit() const { return un.first + (t0 > S::kItem ? t0 - S::kItem : 0); }  // of its keys
-    __device__ __forceinline__ uint32_t end_unit() const { return un.first + (t1 > S::kItem ? t1 - S::kItem : 0); }
-    bool cut;         // the run ends inside the item
+    Part part;
+    __device__ __forceinline__ uint32_t first_unit() const { return un.first + (part.t0 > S::kItem ? part.t0 - S::kItem : 0); }  // of its keys
+    __device__ __forceinline__ uint32_t end_unit() const { return un.first + (part.t1 > S::kItem ? part.t1 - S::kItem : 0); }
 
     __device__ __forceinline__ explicit Walk(const PagedAttnArgs& a, const Run& r) : run(r) {
         req = run.req;
@@ -270,28 +214,16 @@ struct Walk {
                 }
             }
             un = units_of<S>(a, req, run.m0);
-            const uint32_t lo = un.count <= S::kWhole ? un.count - 1 : run.near_lo;
-            begun = begun && run.unit > lo;  // (a border near an item's start is its start)
-            if (begun && un.count - run.unit <= run.near_hi) {  // what is left of it is the last run's
-                next();
-                continue;
-            }
-            if (!begun && run.to <= start + min(lo, un.count - 1)) return false;  // it is the next run's
-            t0 = begun ? run.unit : 0;
-            cut = run.to < start + un.count && start + un.count - run.to > run.near_hi;
-            t1 = cut ? static_cast<uint32_t>(run.to - start) : un.count;
-            return true;
+            const Share share = part_of<S>(run.at, un, start, run.to, run.unit, begun, part);
+            if (share != Share::kNone) return share == Share::kPart;
+            next();
         }
     }
     __device__ __forceinline__ void next() { start += un.count, run.m0 += S::M, begun = false; }
     __device__ __forceinline__ uint32_t vecs() const { return min(static_cast<uint32_t>(S::M), req.vecs - run.m0); }
-    __device__ __forceinline__ bool whole() const { return t0 == 0 && t1 == un.count; }
-    // Borders inside the item, from near_lo behind its start to near_hi before its end: run first_border() - 1 has
-    // its first part (in its second slot), the runs from first_border() on the others (in their first).
-    __device__ __forceinline__ uint64_t first_border() const { return quotient(start + run.near_lo, run.per) + 1; }
-    __device__ __forceinline__ uint32_t parts() const {
-        return static_cast<uint32_t>(quotient(start + un.count - run.near_hi - 1, run.per) - first_border()) + 2;
-    }
+    __device__ __forceinline__ bool whole() const { return part.t0 == 0 && part.t1 == un.count; }
+    __device__ __forceinline__ uint64_t border() const { return first_border(run.at, start); }
+    __device__ __forceinline__ uint32_t parts() const { return parts_of(run.at, start, un.count); }
 };
 
 // Parts go through to memory (agent-scope stores and loads): other XCDs read them.
@@ -448,10 +380,8 @@ template <int HD, int KIND>
 struct Form {
     using K = Kind<KIND>;
     static constexpr int WV = 16, M = 4 * WV, U = K::U, WK = 16 * U, DV = HD / 16;
-    // (An item at 1 and not 3 units: 24 x 5 rows of heads of 64 40.9 us and not 37.0. Runs from 10 units on and not 5:
-    // 45.7, and 1 x 1 row behind 2000 positions 26.9 and not 21.0. Items whole up to 24 units and not 12: 40 x 1 row behind
-    // 8000 102 and not 84; up to none: 1 x 1 row behind 500 15.1 and not 14.3.)
-    using S = Cuts<M, WK, false, 3, 4, 5, 12>;
+    using S = FewCuts<U>;
+    static_assert(S::M == M && S::WK == WK);
     static constexpr int KL = HD * K::BYTES / 64;   // 16-byte loads of a key row by a lane
     static constexpr int VW = DV * K::BYTES / 4;    // 32-bit words of a value row in a lane
     struct Step {
@@ -539,7 +469,7 @@ __global__ __launch_bounds__(kThreads, HD == 128 ? 2 : 3) void paged_attn_kernel
         const Run& run = walk.run;
         const Request& req = walk.req;
         const Units& un = walk.un;
-        const uint32_t t0 = walk.t0;
+        const uint32_t t0 = walk.part.t0;
         const uint32_t sets = 4u >> un.wide, UK = WK * sets;      // sets of waves with all of the item's vectors
         const uint32_t qw = wave & ((1u << un.wide) - 1), ks = wave >> un.wide;
         u32x4* const q_mine = reinterpret_cast<u32x4*>(shared) + qw * F::kQ + lane;  // (the sets write the same values)
@@ -854,7 +784,7 @@ __global__ __launch_bounds__(kThreads, HD == 128 ? 2 : 3) void paged_attn_kernel
         }
         if (!whole) {
             const uint32_t n = walk.parts();
-            const uint64_t border = walk.first_border();
+            const uint64_t border = walk.border();
             if (last_part(a.arrived + border - 1, n, sc.last)) {
                 const float* first = a.parts + (2 * border - 1) * slot_words;
                 auto part_at = [&](uint32_t i) { return i == 0 ? first : first + (2 * static_cast<size_t>(i) - 1) * slot_words; };
@@ -900,7 +830,7 @@ __global__ __launch_bounds__(kThreads, HD == 128 ? 2 : 3) void paged_attn_kernel
                     }
                 }
             }
-            if (walk.cut) return;
+            if (walk.part.cut) return;
         }
         __syncthreads();
     }
@@ -935,10 +865,8 @@ struct Wide {
     using K = Kind<KIND>;
     static constexpr bool F32 = KIND == VVLI_CACHE_F32;
     static constexpr int WV = 32, M = 128, WK = 32, NT = HD / 32, DS = HD * K::BYTES / 32;
-    // (A step takes two to four times as long in f32, so that the rest costs fewer of them: 100 rows behind 200, heads of
-    // 128, 55 us at 16 bits' numbers and 35 at these, 3 x 333 rows of heads of 64 42 and 37. What a cut costs, without a
-    // bound at a quarter of a run: 2 x 2000 rows bf16 317 us, with 4 units 269.)
-    using S = std::conditional_t<F32, Cuts<M, WK, true, 2, 2, 3, 0>, Cuts<M, WK, true, 3, 4, 5, 0>>;
+    using S = ChunkCuts<F32>;
+    static_assert(S::M == M && S::WK == WK);
     static constexpr int RB = HD * K::BYTES, CH = RB / 16, RPL = RB < 256 ? 256 / RB : 1;  // bytes and 16-byte chunks of a row, rows of 256 bytes
     static constexpr int TILE = WK * RB, LOADS = 2 * TILE / (16 * kThreads), ROWS = LOADS > 1 ? LOADS / 2 : 1;
     static constexpr int QR = F32 ? 1 : 2;  // terms of q in registers; the rest in LDS
@@ -1251,14 +1179,14 @@ __global__ __launch_bounds__(kThreads, 2) void paged_wide_kernel(PagedAttnArgs a
         // A part is an image of the threads' registers, 8 bytes of each thread side by side; then maxima and sums.
         constexpr int IMAGE = NT * 16 * kThreads;
         static_assert(IMAGE == M * HD, "a part has its slot");
-        float* slot = a.parts + (2 * static_cast<size_t>(run.index) + (walk.t0 == 0)) * slot_words;
+        float* slot = a.parts + (2 * static_cast<size_t>(run.index) + (walk.part.t0 == 0)) * slot_words;
 #pragma unroll
         for (int n = 0; n < NT; ++n)
 #pragma unroll
             for (int r = 0; r < 16; r += 2) publish(slot + (16 * n + r) * kThreads + 2 * tid, o[n][r], o[n][r + 1]);
         if (half == 0) publish(slot + IMAGE + 2 * (wave * WV + fr), m_run, l_run);
         const uint32_t parts = walk.parts();
-        const uint64_t border = walk.first_border();
+        const uint64_t border = walk.border();
         if (last_part(a.arrived + border - 1, parts, sc.last)) {
             const float* first = a.parts + (2 * border - 1) * slot_words;
             m_run = -INFINITY, l_run = 0.f;
@@ -1284,7 +1212,7 @@ __global__ __launch_bounds__(kThreads, 2) void paged_wide_kernel(PagedAttnArgs a
             }
             write();
         }
-        if (walk.cut) return;
+        if (walk.part.cut) return;
     }
 }
 

@@ -215,8 +215,11 @@ struct Walk {
             }
             un = units_of<S>(a, req, run.m0);
             const Share share = part_of<S>(run.at, un, start, run.to, run.unit, begun, part);
-            if (share != Share::kNone) return share == Share::kPart;
-            next();
+            if (share == Share::kNone) {
+                next();
+                continue;
+            }
+            return share == Share::kPart;
         }
     }
     __device__ __forceinline__ void next() { start += un.count, run.m0 += S::M, begun = false; }

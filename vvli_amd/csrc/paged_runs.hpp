@@ -53,7 +53,7 @@ VVLI_HD Units units_of(const A& a, const Request& q, uint32_t m0) {
     const uint32_t wide = vecs <= S::M / 4 ? 0 : vecs <= S::M / 2 ? 1 : 2;
     const int64_t p0 = q.start + page_of(a.group, m0);
     const int64_t p1 = q.start + page_of(a.group, m0 + vecs - 1);
-    const int64_t room = a.room, hi = p1 + 1 < room ? p1 + 1 : room;
+    const int64_t hi = p1 + 1 < static_cast<int64_t>(a.room) ? p1 + 1 : static_cast<int64_t>(a.room);
     const int64_t lo = a.window && p0 + 1 > a.window ? p0 + 1 - a.window : 0;
     if (hi <= lo) return Units{0, 0, 0, S::kItem, wide};
     const uint32_t unit = S::FIXED ? S::WK : (4 * S::WK) >> wide;
@@ -103,7 +103,8 @@ struct Part {
 };
 enum class Share { kEnd, kNone, kPart };  // the item is the next run's, what is left of it is the last run's, this one has a part
 template <class S>
-VVLI_HD Share part_of(const Borders& b, const Units& un, uint64_t start, uint64_t to, uint32_t unit, bool& begun, Part& p) {
+VVLI_HD __attribute__((always_inline)) Share part_of(const Borders& b, const Units& un, uint64_t start, uint64_t to, uint32_t unit,
+                                                     bool& begun, Part& p) {
     const uint32_t lo = un.count <= S::kWhole ? un.count - 1 : b.near_lo;
     begun = begun && unit > lo;  // (a border near an item's start is its start)
     if (begun && un.count - unit <= b.near_hi) return Share::kNone;

@@ -374,10 +374,11 @@ __device__ __forceinline__ void mfma_done(V (&x)[N]) {
 //
 // Keys and values from memory bound it where requests are many or long: 40 rows
 // behind up to 8000 positions, 28 heads over 4 of 128, bf16, 83 us, 4.4 TB/s (a
-// copy reaches 4.8 to 5.4); 64 behind up to 4000, 16 heads over 16 of 128, 242
-// us, 5.4 TB/s, and 6.1 in f32. The chain named above does where they are few:
-// 1 row behind 230, 8 kv heads of 64, f32, 11 us; behind 8000, 4 kv heads, bf16,
-// 23 us; 24 x 5 rows behind up to 4100, f16, 40 us, 2.8 TB/s.
+// copy reaches 4.8 to 5.4), and 144 us, 5.0 TB/s, in f32; 64 behind up to 4000,
+// 16 heads over 16 of 128, 232 us, 5.5 TB/s, and 418 us, 6.1 TB/s, in f32. The
+// chain named above does where they are few: 1 row behind 230, 8 kv heads of
+// 64, f32, 11 us; behind 8000, 4 kv heads of 128, bf16, 21 us; 24 x 5 rows
+// behind up to 4100, f16, 40 us, 2.8 TB/s.
 // ---------------------------------------------------------------------------
 template <int HD, int KIND>
 struct Form {
@@ -858,10 +859,12 @@ __global__ __launch_bounds__(kThreads, HD == 128 ? 2 : 3) void paged_attn_kernel
 // the rows of a fragment read fall on different banks (no conflict is counted).
 //
 // Products bound it: 4000 rows behind 8000, 28 heads over 4 of 128, 4.6 ms in f32
-// (125 of the 133 TFLOP/s that a large product reaches), 1.2 ms in f16 (479, times
-// two terms 959 of 1310) and 1.45 ms in bf16 (397, times three terms 1190 of
-// 1200). Short chunks are bound by the runs' ends: 2 x up to 2000 rows behind up
-// to 2100 in bf16 260 to 277 us (330 to 353, 990 to 1060 with terms).
+// (125 of the 133 TFLOP/s that a large product reaches), 1.19 ms in f16 (480, times
+// two terms 960 of 1310: a step's vector instructions, among them some 30 that
+// bring spilled values back, weigh more beside fewer products) and 1.47 ms in
+// bf16 (390, times three terms 1170 of 1200). Short chunks are bound by the runs'
+// ends: 2 x up to 2000 rows behind up to 2100 in bf16 265 to 275 us (335 to 347,
+// 1000 to 1040 with terms).
 // ---------------------------------------------------------------------------
 template <int HD, int KIND>
 struct Wide {
@@ -1231,8 +1234,9 @@ struct Plan {
 //   28 heads over 4 of 128   20 rows  51 | 59 us (70 | 91)   100 rows  63 | 63 us (109 | 113)   200 rows  105 | 84 us (228 | 200)
 //   32 heads over 8 of 64    10 rows  26 | 30 us (43 | 45)    15 rows  29 | 29 us  (44 | 45)     80 rows   49 | 36 us  (77 | 70)
 // and 63 single tokens with one prompt of 500 rows, heads of 128: 99 | 144 us.
-// Blocks: as many as the registers of their waves leave room for, two or three on a CU (three and not two, heads of 64:
-// 24 x 5 rows in f32 58 and not 64 us, 300 x 1 row in bf16 67 and not 73; but 64 x 1 row behind 8000 136 and not 123).
+// Blocks: as many as the registers of their waves leave room for, two or three on a CU (three and not two, 32 heads over 8
+// of 64: 24 x 5 rows behind up to 4100 in f32 49 and not 52 us, 300 x 1 row behind up to 1000 in bf16 95 and not 103, 64 x 1
+// behind 8000 195 and not 198, but 361 and not 352 in f32).
 Plan plan_of(uint32_t rows, uint32_t requests, uint32_t group, uint32_t hd) {
     const bool wide = static_cast<uint64_t>(rows) * group > uint64_t{hd == 128 ? 384u : 48u} * requests;
     return Plan{wide ? 128u : 64u, gemm_cus() * (wide || hd == 128 ? 2 : 3), wide};

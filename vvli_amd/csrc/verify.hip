@@ -95,7 +95,8 @@ __device__ __forceinline__ double wave_scan(double v) {
     return v;
 }
 
-// A wave's sum of tokens from .. from + chunk - 1, two steps' loads in flight.
+// A wave's sum of tokens from .. from + chunk - 1, two steps' loads in flight where a chunk has two (vocabularies over
+// kStep * kChunksMost = 131072).
 __device__ __forceinline__ double chunk_sum(const Weights& w, uint32_t from, uint32_t chunk) {
     const uint32_t lane = threadIdx.x & 63;
     double s = 0, x[8];
@@ -116,8 +117,8 @@ __device__ __forceinline__ double chunk_sum(const Weights& w, uint32_t from, uin
 // sums its chunks of that row; the block whose sums are the request's last
 // finds the token's chunk among the sums and, with one wave, the token in it.
 // One pass over one row of target and draft for each request bounds it where
-// there are many requests (64 with 4 drafts, 128256 tokens: 20 us, 2.4 TB/s),
-// the chain of dependent loads where there are few (1, 151936 tokens: 7.7 us).
+// there are many requests (64 with 4 drafts, 128256 tokens: 21 us, 2.4 TB/s),
+// the chain of dependent loads where there are few (1, 151936 tokens: 7.5 us).
 // By blocks that walk the row in strides of the grid, each search over the
 // whole row again, the two took 55 and 9.8 us.
 __global__ __launch_bounds__(kThreads) void verify_kernel(VerifyArgs a) {

@@ -557,6 +557,80 @@ int vvli_gpu_verify_drafts(const float* target, uint64_t ldt, const float* draft
 /* Bytes of workspace that calls of up to so many requests, of any vocabulary, need (0 for a vocabulary of 0). */
 size_t vvli_gpu_verify_drafts_workspace(uint32_t requests, uint32_t vocab);
 
+/* ---------------------------------------------------------------------- */
+/* Products in 8-bit integers and what stands between them (device pointers) */
+/* ---------------------------------------------------------------------- */
+/* No counterpart in the reference, whose products take bf16 or f32 weights.
+ * For programs with a loop of their own around products: W and X as 8-bit
+ * codes with one f32 scale for each row (W: each output channel, X: each
+ * token), half of bf16's bytes for few rows and twice its rate for many.
+ * vvli_gpu_quantize_rows makes codes of any rows (weights, once; attention's
+ * output), vvli_gpu_add_norm and vvli_gpu_silu_mul make them of what a
+ * transformer block computes in front of its products, vvli_gpu_linear_i8
+ * multiplies them.
+ *
+ * Rows in 8 bits: of a row y of real numbers, scale = f32(max |y| / 127) and
+ * code = the integer nearest to y / scale (a tie: the even one), -127 .. 127,
+ * so that code * scale is within half a scale of y. Both are those of exact
+ * arithmetic wherever 64 bits tell a value from the border between two codes:
+ * they depend neither on a call's other rows nor on its sizes. A row of zeros,
+ * and one whose scale is below f32's range, has scale 0 and codes 0. A row
+ * with a value that is not finite, or whose scale is over f32's range, has
+ * scale NaN and codes 0: products with it are NaN. Codes of a row start at a
+ * multiple of 16 bytes (ldc % 16 == 0), and behind its last code up to the
+ * next multiple of 16 stand zeros (ldc holds them too), so that a width that
+ * is no multiple of 16 multiplies as K = the next one.
+ *
+ * As above, every pointer is device memory, aligned to its elements, of the
+ * current device, to which `stream` belongs; the calls are asynchronous,
+ * allocate nothing, keep nothing and may be captured. Rows (row i at i * ld
+ * elements) of f32 and bf16 start at 16-byte addresses (ld a multiple of 4 or
+ * 8). Nothing behind a row's width is read or, but for the codes' zeros,
+ * written. Outputs do not overlap inputs or each other, but that a call says
+ * so; sizes and overlaps that a call does not take return VVLI_INVALID_CONFIG
+ * before any launch. rows 0 is no error: nothing is launched. Results do not
+ * change from run to run. */
+
+/* Rows x (type kind: VVLI_WEIGHT_F32 or VVLI_WEIGHT_BF16) in 8 bits. */
+int vvli_gpu_quantize_rows(const void* x, uint32_t kind, uint64_t ldx, uint32_t rows, uint32_t width, int8_t* codes,
+                           uint64_t ldc, float* scales, void* stream);
+
+/* The residual's addition, the RMS norm behind it and its rows in 8 bits, in
+ * one pass: h = x + delta, rounded to f32 once (delta NULL: h = x), to `sum`
+ * (NULL: not wanted; without delta it has to be NULL); n = h * weight /
+ * sqrt(mean(h^2) + eps), the sums in 64 bits; n rounded to f32 to `y` (NULL:
+ * not wanted); n in 8 bits to codes and scales (both NULL: not wanted; y or
+ * codes has to be). weight: `width` values of type weight_kind (VVLI_WEIGHT_*)
+ * at a 16-byte address. sum and y may each be x or delta itself, with its
+ * stride (both not the same one). */
+int vvli_gpu_add_norm(const float* x, uint64_t ldx, const float* delta, uint64_t ldd, uint32_t rows, uint32_t width,
+                      const void* weight, uint32_t weight_kind, float eps, float* sum, uint64_t lds, float* y,
+                      uint64_t ldy, int8_t* codes, uint64_t ldc, float* scales, void* stream);
+
+/* The gated activation's rows in 8 bits: g / (1 + exp(-g)) * u of rows gate
+ * and up (which may lie in one product's rows: up = gate + width, ldg = ldu). */
+int vvli_gpu_silu_mul(const float* gate, uint64_t ldg, const float* up, uint64_t ldu, uint32_t rows, uint32_t width,
+                      int8_t* codes, uint64_t ldc, float* scales, void* stream);
+
+/* linearInto on codes: Y[m,n] = (sum_k W[n,k] X[m,k]) * x_scales[m] *
+ * w_scales[n] (+ bias[n], bf16 or NULL). The sum is exact; it, the products
+ * with the two scales (in this order) and the sum with the bias are rounded to
+ * f32, each once. W: N rows of K codes (stride ldw), X: M rows (ldx), Y: M rows
+ * of N f32 (ldy >= N, any alignment of f32). W and X at 16-byte addresses,
+ * their strides and K multiples of 16, K <= 131056 (so that no sum leaves 32
+ * bits, whatever the codes, -128 too). M = 0 is no error.
+ * workspace: at least vvli_gpu_linear_i8_workspace bytes, at a 16-byte
+ * address, zeroed once, when it is allocated (a call leaves its counters
+ * zeroed). It belongs to one call at a time, so calls or replays that may
+ * overlap need one each, and to this op alone; it serves calls of any sizes up
+ * to its own. */
+int vvli_gpu_linear_i8(const int8_t* W, uint64_t ldw, const float* w_scales, const int8_t* X, uint64_t ldx,
+                       const float* x_scales, const uint16_t* bias, float* Y, uint64_t ldy, uint32_t M, uint32_t N,
+                       uint32_t K, void* workspace, size_t workspace_bytes, void* stream);
+/* Bytes of workspace that calls of up to M rows with these N and K need; 0 for
+ * sizes that a call refuses. */
+size_t vvli_gpu_linear_i8_workspace(uint32_t M, uint32_t N, uint32_t K);
+
 #ifdef __cplusplus
 }
 #endif

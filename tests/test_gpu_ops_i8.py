@@ -1,0 +1,617 @@
+"""Ops around 8-bit products on the GPU, against plain implementations in 64
+bits.
+
+Tolerances: codes and scales are those of exact arithmetic wherever 64 bits tell
+a value from a border. Here and there a value passes fewer than 40 roundings of
+2^-53 on the way and a sum of n squares n more, half of which reach the root:
+with n <= 70000 under 2^-36 relative, so that
+
+* a code is an integer next to value / scale: |value / scale - code| is at most
+  0.5 + 127 * 2^-35;
+* a scale is max |value| / 127 rounded to f32: within 2^-24 + 2^-35 of it;
+* the norm's f32 rows are within 2^-24 + 2^-35 of the value (or half a step of
+  the denormals, 2^-150);
+* rows quantised as they are pass one division: codes and scales are equal;
+* the residual's sum is one f32 addition, the product a whole number followed by
+  f32 operations in a given order: equal in every bit.
+"""
+import numpy as np
+import pytest
+
+from vvli_amd import config as C
+from vvli_amd import runtime as R
+
+pytestmark = pytest.mark.gpu
+
+EPS = float(np.float32(1e-6))
+SLACK = 2.0 ** -35
+HALF = 2.0 ** -24
+
+
+@pytest.fixture(scope="module")
+def torch():
+    import torch as t
+
+    return t
+
+
+def ptr(t):
+    return None if t is None else t.data_ptr()
+
+
+def up(n, to):
+    return -(-n // to) * to
+
+
+def stream(torch):
+    return torch.cuda.current_stream().cuda_stream
+
+
+def gen(torch, seed):
+    return torch.Generator(device="cuda").manual_seed(seed)
+
+
+class Codes:
+    """Codes and scales on the device with marks around them."""
+
+    def __init__(self, torch, rows, width, pad=0):
+        self.rows, self.width, self.ldc = rows, width, up(width, 16) + 16 * pad
+        self.codes = torch.full((rows + 2, self.ldc), 99, dtype=torch.int8, device="cuda")
+        self.scales = torch.full((rows + 2,), -5.0, device="cuda")
+        self.args = (self.codes.data_ptr(), self.ldc, self.scales.data_ptr())
+
+    def get(self):
+        """(codes [rows, width], scales) in f64, with what is around them looked at."""
+        c, s, n, w = self.codes.cpu().numpy(), self.scales.cpu().numpy(), self.rows, self.width
+        assert (c[n:] == 99).all() and (s[n:] == -5).all(), "rows behind the last were written"
+        assert (c[:n, w:up(w, 16)] == 0).all(), "the codes' tail is not 0"
+        assert (c[:n, up(w, 16):] == 99).all(), "codes behind the padded width were written"
+        return c[:n, :w].astype(np.float64), s[:n].astype(np.float64)
+
+
+def check_codes(codes, scales, v):
+    """codes and scales of rows v (f64)."""
+    with np.errstate(invalid="ignore", over="ignore", divide="ignore"):
+        top = np.abs(v).max(-1)
+        whole = np.isfinite(v).all(-1)
+        want = (top / 127).astype(np.float32).astype(np.float64)
+        fine = whole & np.isfinite(want)
+        assert np.isnan(scales[~fine]).all() and (codes[~fine] == 0).all()
+        near = np.maximum(np.abs(want) * (2 * HALF + SLACK), 2.0 ** -149)  # (a neighbour where top / 127 is next to a border)
+        assert (np.abs(scales - want)[fine] <= near[fine]).all()
+        assert ((scales == want) | ~fine).mean() > 0.99 or len(want) < 100
+        none = fine & (scales == 0)
+        assert (codes[none] == 0).all() and (np.abs(codes) <= 127).all()
+        some = fine & (scales > 0)
+        t = v[some] / scales[some][:, None]
+        assert (np.abs(np.clip(t, -127, 127) - codes[some]) <= 0.5 + 127 * SLACK).all()
+
+
+def equal_codes(codes, scales, v):
+    with np.errstate(invalid="ignore", over="ignore", divide="ignore"):
+        want = (np.abs(v).max(-1) / 127).astype(np.float32).astype(np.float64)
+        want[~np.isfinite(want)] = np.nan
+        assert np.array_equal(scales, want, equal_nan=True)
+        t = np.where((want > 0)[:, None], np.rint(v / want[:, None]), 0)
+        assert np.array_equal(codes, np.clip(t, -127, 127))
+
+
+WIDTHS = [1, 2, 3, 15, 16, 17, 63, 64, 255, 896, 1024, 1025, 2047, 3584, 4096, 4099, 8192, 16384, 16390, 18944, 65536, 65541, 70001]
+
+
+def rows_for(width):
+    return 9 if width < 5000 else 4
+
+
+# ---------------------------------------------------------------------------
+# quantize_rows
+# ---------------------------------------------------------------------------
+def odd_rows(torch, x):
+    """Rows that are no ordinary ones, in place (f32)."""
+    n = len(x)
+    if n >= 4:
+        x[1] = 0
+        x[2] *= 1e-39      # denormal values and scale
+        x[3] *= 1e30
+    if n >= 9:
+        x[4, -1] = float("inf")
+        x[5, 0] = float("nan")
+        x[6] = 1e-45       # a scale below f32's range
+        x[7, : x.shape[1] // 2] = 0
+        x[7, -1] = -127.0  # a scale of 1 and ties
+        x[7, 0] = 0.5 if x.shape[1] > 1 else -127.0
+        x[7, 1:2] = 1.5 if x.shape[1] > 2 else -127.0
+        x[7, 2:3] = -2.5 if x.shape[1] > 3 else -127.0
+    return x
+
+
+@pytest.mark.parametrize("kind", ["f32", "bf16"])
+@pytest.mark.parametrize("width", WIDTHS)
+def test_quantize_rows(torch, width, kind):
+    rows, unit = rows_for(width), 4 if kind == "f32" else 8
+    for pad in (0, 3):
+        ld = up(width, unit) + unit * pad
+        x = torch.full((rows, ld), float("nan"), device="cuda")  # (behind the width: not read)
+        x[:, :width] = odd_rows(torch, torch.randn(rows, width, device="cuda", generator=gen(torch, width)))
+        x = x if kind == "f32" else x.bfloat16()
+        out = Codes(torch, rows, width, pad)
+        R.quantize_rows(ptr(x), kind, ld, rows, width, *out.args, stream(torch))
+        equal_codes(*out.get(), x[:, :width].double().cpu().numpy())
+
+
+def test_quantize_rows_borders(torch):
+    """Values on and next to the borders between codes, for scales of many last bits."""
+    rng = np.random.RandomState(0)
+    s = (1 + rng.rand(600)).astype(np.float32)
+    top = (s.astype(np.float64) * 127).astype(np.float32)
+    scale = (top.astype(np.float64) / 127).astype(np.float32)
+    n = rng.randint(0, 127, (600, 400)) + 0.5
+    x = (n * scale.astype(np.float64)[:, None]).astype(np.float32)
+    x = np.where(rng.rand(*x.shape) < 0.5, x, np.nextafter(x, np.float32(rng.choice([0, 1e9])), dtype=np.float32))
+    x[:, 0] = top
+    x *= rng.choice([-1, 1], x.shape).astype(np.float32)
+    d = torch.from_numpy(x).cuda()
+    out = Codes(torch, 600, 400)
+    R.quantize_rows(ptr(d), "f32", 400, 600, 400, *out.args, stream(torch))
+    equal_codes(*out.get(), x.astype(np.float64))
+
+
+def test_quantize_rows_many(torch):
+    """More rows than one launch of a block each might take at once."""
+    x = torch.randn(70001, 16, device="cuda", generator=gen(torch, 1))
+    out = Codes(torch, 70001, 16)
+    R.quantize_rows(ptr(x), "f32", 16, 70001, 16, *out.args, stream(torch))
+    equal_codes(*out.get(), x.double().cpu().numpy())
+
+
+def test_quantize_rows_offsets_past_32_bits(torch):
+    """Strides that put the last rows' elements and codes behind 2^32 bytes."""
+    ld, rows = 1 << 28, 6
+    x = torch.zeros(rows, ld, dtype=torch.bfloat16, device="cuda")
+    codes, scales = torch.zeros(rows, (1 << 30), dtype=torch.int8, device="cuda"), torch.zeros(rows, device="cuda")
+    v = torch.randn(rows, 100, device="cuda", generator=gen(torch, 2)).bfloat16()
+    x[:, :100] = v
+    R.quantize_rows(ptr(x), "bf16", ld, rows, 100, ptr(codes), 1 << 30, ptr(scales), stream(torch))
+    equal_codes(codes[:, :100].cpu().numpy().astype(np.float64), scales.cpu().numpy().astype(np.float64), v.double().cpu().numpy())
+
+
+# ---------------------------------------------------------------------------
+# add_norm
+# ---------------------------------------------------------------------------
+def norm_value(h, w, eps=EPS):
+    h = h.astype(np.float64)
+    with np.errstate(invalid="ignore", over="ignore", divide="ignore"):
+        return h * w / np.sqrt((h * h).mean(-1, keepdims=True) + eps)
+
+
+def check_y(y, v):
+    with np.errstate(invalid="ignore", over="ignore"):
+        bad = ~np.isfinite(v.astype(np.float32))
+        assert np.array_equal(np.isnan(y), np.isnan(v))
+        fine = ~bad & np.isfinite(y)
+        assert (fine | bad).all()
+        assert (np.abs(y - v)[fine] <= np.maximum(np.abs(v[fine]) * (HALF + SLACK), 2.0 ** -150)).all()
+
+
+@pytest.mark.parametrize("kind,delta,total,y,codes", [
+    ("bf16", True, True, False, True), ("f32", True, True, True, True), ("bf16", False, False, True, False),
+    ("f32", True, False, False, True), ("bf16", False, False, True, True), ("bf16", True, True, True, False)])
+@pytest.mark.parametrize("width", WIDTHS)
+def test_add_norm(torch, width, kind, delta, total, y, codes):
+    rows, pad = rows_for(width), (width % 3)
+    ld = up(width, 4) + 4 * pad
+    g = gen(torch, width)
+    x = torch.full((rows, ld), float("nan"), device="cuda")
+    x[:, :width] = torch.randn(rows, width, device="cuda", generator=g)
+    if rows >= 9:
+        odd_rows(torch, x[:, :width])
+    d = torch.randn(rows, ld, device="cuda", generator=g) if delta else None
+    if delta and rows >= 4:
+        d[1] = 0
+        d[2] *= 1e-39
+    w = (1 + 0.3 * torch.randn(width, device="cuda", generator=g)).to(torch.bfloat16 if kind == "bf16" else torch.float32)
+    s = torch.full((rows + 1, ld), 77.0, device="cuda") if total else None
+    o = torch.full((rows + 1, ld), 77.0, device="cuda") if y else None
+    out = Codes(torch, rows, width, pad)
+    R.add_norm(ptr(x), ld, ptr(d), ld, rows, width, ptr(w), kind, EPS, ptr(s), ld, ptr(o), ld, *(out.args if codes else (None, 0, None)),
+               stream(torch))
+    h = (x + d if delta else x)[:, :width]
+    if total:
+        assert np.array_equal(s[:rows, :width].cpu().numpy(), h.cpu().numpy(), equal_nan=True)
+        assert (s[rows] == 77).all() and (s[:, width:] == 77).all()
+    v = norm_value(h.cpu().numpy(), w.double().cpu().numpy())
+    if y:
+        check_y(o[:rows, :width].double().cpu().numpy(), v)
+        assert (o[rows] == 77).all() and (o[:, width:] == 77).all()
+    if codes:
+        check_codes(*out.get(), v)
+
+
+@pytest.mark.parametrize("place", ["sum is x", "sum is delta", "y is x", "y is delta, sum is x", "y is x, no sum", "y is delta, no sum"])
+@pytest.mark.parametrize("width", [100, 3584, 18944, 70001])
+def test_add_norm_in_place(torch, width, place):
+    rows, ld = 5, up(width, 4)
+    g = gen(torch, 5)
+    x, d = (torch.randn(rows, ld, device="cuda", generator=g) for _ in range(2))
+    w = torch.randn(width, device="cuda", generator=g)
+    h = (x + d)[:, :width].cpu().numpy()
+    other = torch.zeros(rows, ld, device="cuda")
+    total, y = {"sum is x": (x, None), "sum is delta": (d, None), "y is x": (other, x), "y is delta, sum is x": (x, d),
+                "y is x, no sum": (None, x), "y is delta, no sum": (None, d)}[place]
+    out = Codes(torch, rows, width)
+    R.add_norm(ptr(x), ld, ptr(d), ld, rows, width, ptr(w), "f32", EPS, ptr(total), ld, ptr(y), ld, *out.args, stream(torch))
+    v = norm_value(h, w.double().cpu().numpy())
+    check_codes(*out.get(), v)
+    if total is not None:
+        assert np.array_equal(total[:, :width].cpu().numpy(), h)
+    if y is not None:
+        check_y(y[:, :width].double().cpu().numpy(), v)
+
+
+def test_add_norm_far_values(torch):
+    """Squares that leave f32, weights that do with the values, eps 0, weights of 0 and NaN."""
+    rows, width = 8, 1000
+    g = gen(torch, 6)
+    x = torch.randn(rows, width, device="cuda", generator=g) * torch.tensor([1e30, 1e-30, 1e38, 1e-38, 1, 1e20, 1e-20, 0.0], device="cuda")[:, None]
+    for w in (torch.randn(width, device="cuda", generator=g) * 1e25, torch.randn(width, device="cuda", generator=g) * 1e-30,
+              torch.zeros(width, device="cuda"), torch.full((width,), float("nan"), device="cuda")):
+        for eps in (EPS, 0.0):
+            y, out = torch.zeros_like(x), Codes(torch, rows, width)
+            R.add_norm(ptr(x), width, None, 0, rows, width, ptr(w), "f32", eps, None, 0, ptr(y), width, *out.args, stream(torch))
+            v = norm_value(x.cpu().numpy(), w.double().cpu().numpy(), eps)
+            check_y(y.double().cpu().numpy(), v)
+            check_codes(*out.get(), v)
+
+
+# ---------------------------------------------------------------------------
+# silu_mul
+# ---------------------------------------------------------------------------
+def gate_value(g, u):
+    g = g.astype(np.float64)
+    with np.errstate(invalid="ignore", over="ignore"):
+        return g / (1 + np.exp(-g)) * u
+
+
+@pytest.mark.parametrize("width", WIDTHS)
+def test_silu_mul(torch, width):
+    rows = rows_for(width)
+    for pad in (0, 5):
+        ld = up(width, 4) + 4 * pad
+        g = gen(torch, width + 1)
+        a = torch.full((rows, 2 * ld), float("nan"), device="cuda")
+        a[:, :width] = 3 * torch.randn(rows, width, device="cuda", generator=g)
+        a[:, ld:ld + width] = odd_rows(torch, torch.randn(rows, width, device="cuda", generator=g))
+        if rows >= 9:
+            a[0, :width] *= 60  # gates of -150 and less
+            a[8, : width // 2] = -300
+        out = Codes(torch, rows, width, pad)
+        R.silu_mul(ptr(a), 2 * ld, ptr(a) + 4 * ld, 2 * ld, rows, width, *out.args, stream(torch))
+        check_codes(*out.get(), gate_value(a[:, :width].cpu().numpy(), a[:, ld:ld + width].double().cpu().numpy()))
+
+
+@pytest.mark.parametrize("low,high,size", [(-120, -60, 1e30), (-104, -80, 1.0), (-95, -85, 3e38), (-700, -80, 1.0), (60, 120, 1e-38),
+                                           (-1e-30, 1e-30, 1e-10), (-20, 20, 1e38), (-800, -740, 1e38), (-90, 90, 1e13)])
+def test_silu_mul_far_values(torch, low, high, size):
+    """Gates whose exponential leaves f32, products that do: a row's codes follow the values all the same."""
+    rows, width = 6, 2000
+    g = gen(torch, 7)
+    gate = torch.empty(rows, width, device="cuda").uniform_(low, high, generator=g)
+    u = torch.randn(rows, width, device="cuda", generator=g).clamp_(-1, 1) * size
+    out = Codes(torch, rows, width)
+    R.silu_mul(ptr(gate), width, ptr(u), width, rows, width, *out.args, stream(torch))
+    check_codes(*out.get(), gate_value(gate.cpu().numpy(), u.double().cpu().numpy()))
+
+
+@pytest.mark.parametrize("g,u", [(float("-inf"), 1.0), (float("inf"), 1.0), (float("nan"), 1.0), (1.0, float("inf")), (-200.0, float("inf")),
+                                 (3e38, 3e38), (-1e4, float("nan"))])
+def test_silu_mul_not_finite(torch, g, u):
+    gate, up_ = torch.ones(3, 512, device="cuda"), torch.ones(3, 512, device="cuda")
+    gate[1, 300], up_[1, 300] = g, u
+    out = Codes(torch, 3, 512)
+    R.silu_mul(ptr(gate), 512, ptr(up_), 512, 3, 512, *out.args, stream(torch))
+    check_codes(*out.get(), gate_value(gate.cpu().numpy(), up_.double().cpu().numpy()))
+
+
+# ---------------------------------------------------------------------------
+# linear_i8
+# ---------------------------------------------------------------------------
+class Product:
+    def __init__(self, torch, M, N, K, bias=False, padw=0, padx=0, pady=0, seed=0, least=False, space=None):
+        g = gen(torch, seed * 1000 + M + N + K)
+        self.torch, self.sizes, self.strides = torch, (M, N, K), (K + 16 * padw, K + 16 * padx, N + pady)
+        r = lambda n, ld: torch.randint(-128 if least else -127, 128, (n, ld), dtype=torch.int8, device="cuda", generator=g)  # noqa: E731
+        self.W, self.X = r(N, self.strides[0]), r(M, self.strides[1])
+        if least:
+            self.W[:, ::2], self.X[:, ::2] = -128, -128
+        self.ws = torch.empty(N, device="cuda").uniform_(1e-4, 2e-3, generator=g)
+        self.xs = torch.empty(M, device="cuda").uniform_(1e-3, 1e-1, generator=g)
+        self.bias = torch.randn(N, device="cuda", generator=g).bfloat16() if bias else None
+        self.Y = torch.full((M + 1, self.strides[2]), 55.0, device="cuda")
+        self.space = torch.zeros(R.linear_i8_workspace(M, N, K), dtype=torch.uint8, device="cuda") if space is None else space
+
+    def run(self, stream_=None):
+        R.linear_i8(ptr(self.W), self.strides[0], ptr(self.ws), ptr(self.X), self.strides[1], ptr(self.xs), ptr(self.bias), ptr(self.Y),
+                    self.strides[2], *self.sizes, ptr(self.space), self.space.numel(), stream_ or stream(self.torch))
+
+    def want(self):
+        M, N, K = self.sizes
+        y = self.torch.empty(M, N, device="cuda")
+        w = self.W[:, :K].double().t().contiguous()
+        for m in range(0, M, 256):
+            y[m:m + 256] = (self.X[m:m + 256, :K].double() @ w).float()
+        y = (y * self.xs[:, None]) * self.ws
+        return y if self.bias is None else y + self.bias.float()
+
+    def check(self):
+        M, N, K = self.sizes
+        want, got = self.want().cpu().numpy(), self.Y.cpu().numpy()
+        bad = np.argwhere(~((got[:M, :N] == want) | (np.isnan(want) & np.isnan(got[:M, :N]))))
+        assert not len(bad), f"{len(bad)} of {M * N} differ, first at {bad[0]}: {got[tuple(bad[0])]} for {want[tuple(bad[0])]}"
+        assert (got[M:] == 55).all() and (got[:, N:] == 55).all(), "written behind the output"
+        self.Y.fill_(55.0)
+
+
+ROWS = [1, 2, 3, 4, 5, 7, 8, 9, 15, 16, 17, 31, 32, 33, 48, 63, 64, 65, 100, 127, 128, 129, 200, 255, 257, 333, 600]
+
+
+@pytest.mark.parametrize("N,K", [(1, 16), (3, 32), (15, 48), (16, 64), (17, 80), (33, 112), (64, 128), (65, 144), (130, 256), (256, 272),
+                                 (300, 1008), (896, 896), (1152, 4864), (2048, 2048)])
+def test_linear_i8(torch, N, K):
+    for i, M in enumerate(ROWS):
+        p = Product(torch, M, N, K, bias=i % 2 == 0, padw=i % 3, padx=i % 4, pady=i % 5)
+        p.run()
+        p.check()
+
+
+@pytest.mark.parametrize("M,N,K", [(1, 37888, 3584), (4, 4608, 3584), (2, 3584, 18944), (8, 2048, 8192), (48, 4608, 3584), (64, 3584, 18944),
+                                   (128, 16384, 2048), (200, 6144, 2048), (1, 16, 131056), (9, 40, 131056), (300, 64, 131056),
+                                   (1000, 1152, 896), (2049, 4608, 3584), (4096, 9728, 896), (777, 3584, 3600), (5000, 257, 528),
+                                   (70000, 16, 16), (1, 70001, 32)])
+def test_linear_i8_large(torch, M, N, K):
+    p = Product(torch, M, N, K, bias=N % 3 == 0, seed=1)
+    p.run()
+    p.check()
+
+
+@pytest.mark.parametrize("M", [1, 5, 20, 70, 300])
+def test_linear_i8_most_negative(torch, M):
+    """Codes of -128, and sums next to the ends of 32 bits."""
+    p = Product(torch, M, 40, 131056, least=True)
+    p.run()
+    p.check()
+    p.W.fill_(-128), p.X.fill_(-128)
+    p.run()
+    p.check()
+    p.X.fill_(127)
+    p.run()
+    p.check()
+
+
+@pytest.mark.parametrize("M", [1, 6, 40, 130, 700])
+def test_linear_i8_scales(torch, M):
+    """Rows whose scale is 0 or NaN, codes of zeros."""
+    p = Product(torch, M, 100, 640)
+    p.xs[0] = float("nan")
+    if M > 3:
+        p.xs[1], p.X[1] = 0, 0
+        p.xs[2] = float("inf")
+    p.ws[3], p.ws[5] = 0, float("nan")
+    p.run()
+    p.check()
+
+
+def test_linear_i8_one_workspace_for_all_sizes(torch):
+    """A workspace made for the largest call serves all others, in any order."""
+    sizes = [(300, 896, 4864), (1, 2048, 2048), (48, 1152, 8192), (5, 40, 131056), (64, 3584, 3584), (17, 16, 65536), (129, 300, 4096)]
+    space = torch.zeros(max(R.linear_i8_workspace(*s) for s in sizes), dtype=torch.uint8, device="cuda")
+    products = [Product(torch, *s, space=space, seed=i) for i, s in enumerate(sizes)]
+    for _ in range(3):
+        for p in products:
+            p.run()
+        torch.cuda.synchronize()
+        for p in products:
+            p.check()
+        products = products[3:] + products[:3]
+
+
+def test_linear_i8_two_streams(torch):
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    products = [Product(torch, 48, 2048, 8192, seed=3), Product(torch, 20, 1152, 18944, seed=4)]
+    torch.cuda.synchronize()
+    for _ in range(20):
+        for p, s in zip(products, streams):
+            p.run(s.cuda_stream)
+    torch.cuda.synchronize()
+    for p in products:
+        p.check()
+
+
+def test_linear_i8_unaligned_output(torch):
+    """Y at an address and with a stride that no vector store fits."""
+    for M, N in ((1, 33), (5, 64), (70, 130), (300, 257), (600, 512)):
+        p = Product(torch, M, N, 512, bias=True)
+        want = p.want()
+        flat = torch.full((M * (N + 1) + 9,), 55.0, device="cuda")
+        R.linear_i8(ptr(p.W), 512, ptr(p.ws), ptr(p.X), 512, ptr(p.xs), ptr(p.bias), ptr(flat) + 4, N + 1, M, N, 512, ptr(p.space),
+                    p.space.numel(), stream(torch))
+        got = flat[1:1 + M * (N + 1)].view(M, N + 1)
+        assert torch.equal(got[:, :N], want) and flat[0] == 55 and (got[:, N] == 55).all() and (flat[1 + M * (N + 1):] == 55).all()
+
+
+def test_linear_i8_offsets_past_32_bits(torch):
+    """W, X and Y of more than 2^32 bytes."""
+    N, K, ld = 5000, 64, 1 << 20
+    W = torch.zeros(N, ld, dtype=torch.int8, device="cuda")
+    for M in (3, 40, 300):
+        p = Product(torch, M, N, K)
+        W[:, :K] = p.W
+        p.W, p.strides = W, (ld, K, N)
+        p.run()
+        p.check()
+    X = W
+    for n in (20, 300):
+        p = Product(torch, N, n, K, seed=2)
+        X[:, :K] = p.X
+        p.X, p.strides = X, (K, ld, n)
+        p.run()
+        p.check()
+    del W, X, p
+    p = Product(torch, 5000, 300, 128, pady=(1 << 18))
+    p.run()
+    assert torch.equal(p.Y[:5000, :300], p.want())
+    assert (p.Y[:5000, 300:310] == 55).all() and (p.Y[5000] == 55).all()
+
+
+# ---------------------------------------------------------------------------
+# Together, as a program uses them
+# ---------------------------------------------------------------------------
+class Block:
+    """One transformer block with 8-bit products over a paged cache, on `most` rows."""
+
+    def __init__(self, torch, most, hidden=256, heads=4, kv=2, inter=672, seed=0):
+        self.torch, self.most, self.hidden, self.heads, self.kv, self.inter = torch, most, hidden, heads, kv, inter
+        self.hd = hd = hidden // heads
+        g = gen(torch, seed)
+        self.qkv_n = (heads + 2 * kv) * hd
+        self.weights = {}
+        self.plain = {}
+        for name, (n, k) in dict(qkv=(self.qkv_n, hidden), o=(hidden, hidden), gu=(2 * inter, hidden), down=(hidden, inter)).items():
+            w = (torch.randn(n, k, device="cuda", generator=g) * 0.05).bfloat16()
+            codes, scales = torch.zeros(n, k, dtype=torch.int8, device="cuda"), torch.zeros(n, device="cuda")
+            R.quantize_rows(ptr(w), "bf16", k, n, k, ptr(codes), k, ptr(scales), stream(torch))
+            self.weights[name] = (codes, scales)
+        self.bias = torch.randn(self.qkv_n, device="cuda", generator=g).bfloat16()
+        self.norms = [(1 + 0.1 * torch.randn(hidden, device="cuda", generator=g)).bfloat16() for _ in range(3)]
+        self.inv = (1e4 ** -(torch.arange(0, hd, 2, device="cuda", dtype=torch.float64) / hd)).float()
+        self.pages, self.ps, self.R = 64, 16, 3
+        self.k, self.v = (torch.zeros(self.pages * self.ps, kv, hd, device="cuda", dtype=torch.bfloat16) for _ in range(2))
+        self.cache = R.PagedCache(ptr(self.k), ptr(self.v), "bf16", kv, hd, self.ps, self.pages)
+        self.table = torch.arange(self.pages, device="cuda", dtype=torch.int32).view(4, 16)[:3].contiguous()
+        f = lambda *s: torch.zeros(*s, device="cuda")  # noqa: E731
+        b = lambda *s: torch.zeros(*s, dtype=torch.int8, device="cuda")  # noqa: E731
+        i = lambda n: torch.zeros(n, dtype=torch.int32, device="cuda")  # noqa: E731
+        self.x, self.qkv, self.att, self.o, self.gu, self.d, self.y = (f(most, n) for n in (
+            hidden, self.qkv_n, hidden, hidden, 2 * inter, hidden, hidden))
+        self.c1, self.c2, self.c3, self.c4 = b(most, hidden), b(most, hidden), b(most, hidden), b(most, inter)
+        self.s1, self.s2, self.s3, self.s4 = (f(most) for _ in range(4))
+        self.row_start, self.start, self.pos = i(4), i(3), i(most)
+        self.slots = torch.full((most,), -1, dtype=torch.int64, device="cuda")
+        wa = R.paged_attention_workspace(most, 3, heads, kv, hd)
+        self.wa = torch.zeros(wa, dtype=torch.uint8, device="cuda")
+        self.wl = torch.zeros(max(R.linear_i8_workspace(most, n, k) for n, k in ((self.qkv_n, hidden), (2 * inter, hidden), (hidden, inter))),
+                              dtype=torch.uint8, device="cuda")
+
+    def batch(self, past, add, seed):
+        torch = self.torch
+        rows = sum(add)
+        pos = np.concatenate([p + np.arange(a) for p, a in zip(past, add)] or [[]])
+        req = np.concatenate([np.full(a, r) for r, a in enumerate(add)] or [[]]).astype(int)
+        slots = np.full(self.most, -1, np.int64)
+        table = self.table.cpu().numpy()
+        slots[:rows] = table[req, pos.astype(int) // self.ps] * self.ps + pos.astype(int) % self.ps
+        full = np.zeros(self.most, np.int32)
+        full[:rows] = pos
+        self.row_start.copy_(torch.from_numpy(np.cumsum([0, *add]).astype(np.int32)))
+        self.start.copy_(torch.tensor(past, dtype=torch.int32))
+        self.pos.copy_(torch.from_numpy(full))
+        self.slots.copy_(torch.from_numpy(slots))
+        self.x.copy_(torch.randn(self.most, self.hidden, device="cuda", generator=gen(torch, seed)))
+        self.d.copy_(torch.randn(self.most, self.hidden, device="cuda", generator=gen(torch, seed + 1)))
+
+    def product(self, name, codes, scales, bias, out, s):
+        w, ws = self.weights[name]
+        n, k = w.shape
+        R.linear_i8(ptr(w), k, ptr(ws), ptr(codes), k, ptr(scales), ptr(bias), ptr(out), n, self.most, n, k, ptr(self.wl), self.wl.numel(), s)
+
+    def step(self):
+        s, T, h, H, K, hd = stream(self.torch), self.most, self.hidden, self.heads, self.kv, self.hd
+        # (x is the residual, d what the block before this adds to it)
+        R.add_norm(ptr(self.x), h, ptr(self.d), h, T, h, ptr(self.norms[0]), "bf16", EPS, ptr(self.x), h, None, 0, ptr(self.c1), h, ptr(self.s1), s)
+        self.product("qkv", self.c1, self.s1, self.bias, self.qkv, s)
+        ld, base = self.qkv_n, ptr(self.qkv)
+        R.norm_rope_append(self.cache, base, ld, base + 4 * H * hd, ld, base + 4 * (H + K) * hd, ld, T, H, base, ld, ptr(self.inv),
+                           ptr(self.pos), ptr(self.slots), "split_half", None, None, EPS, s)
+        R.paged_attention(self.cache, ptr(self.table), 16, ptr(self.row_start), ptr(self.start), 3, base, ld, ptr(self.att), h, T, H,
+                          hd ** -0.5, 0, ptr(self.wa), self.wa.numel(), s)
+        R.quantize_rows(ptr(self.att), "f32", h, T, h, ptr(self.c2), h, ptr(self.s2), s)
+        self.product("o", self.c2, self.s2, None, self.o, s)
+        R.add_norm(ptr(self.x), h, ptr(self.o), h, T, h, ptr(self.norms[1]), "bf16", EPS, ptr(self.x), h, None, 0, ptr(self.c3), h, ptr(self.s3), s)
+        self.product("gu", self.c3, self.s3, None, self.gu, s)
+        R.silu_mul(ptr(self.gu), 2 * self.inter, ptr(self.gu) + 4 * self.inter, 2 * self.inter, T, self.inter, ptr(self.c4), self.inter,
+                   ptr(self.s4), s)
+        self.product("down", self.c4, self.s4, None, self.d, s)
+        # the last norm, in f32 for the vocabulary's product in bf16
+        R.add_norm(ptr(self.x), h, ptr(self.d), h, T, h, ptr(self.norms[2]), "bf16", EPS, None, 0, ptr(self.y), h, None, 0, None, s)
+
+    def state(self):
+        return [t.clone() for t in (self.x, self.qkv, self.att, self.o, self.gu, self.d, self.y, self.c1, self.c2, self.c3, self.c4, self.s1,
+                                    self.s2, self.s3, self.s4, self.k, self.v)]
+
+    def check(self, x0, d0, rows):
+        """Every stage against 64 bits on what the stage before it left."""
+        n = lambda t: t.double().cpu().numpy()  # noqa: E731
+        h1 = n(x0 + d0)
+        check_codes(n(self.c1), n(self.s1), norm_value(h1, n(self.norms[0])))
+        check_codes(n(self.c2), n(self.s2), n(self.att))
+        assert self.torch.equal(self.x, (x0 + d0) + self.o)
+        check_codes(n(self.c3), n(self.s3), norm_value(n(self.x), n(self.norms[1])))
+        gu = self.gu.cpu().numpy()
+        check_codes(n(self.c4), n(self.s4), gate_value(gu[:, : self.inter], gu[:, self.inter:].astype(np.float64)))
+        for name, c, s, out in (("o", self.c2, self.s2, self.o), ("gu", self.c3, self.s3, self.gu), ("down", self.c4, self.s4, self.d)):
+            w, ws = self.weights[name]
+            want = ((c.double() @ w.double().t()).float() * s[:, None]) * ws
+            assert self.torch.equal(out, want), name
+        w, ws = self.weights["qkv"]
+        qkv = ((self.c1.double() @ w.double().t()).float() * self.s1[:, None]) * ws + self.bias.float()
+        kd = self.heads * self.hd
+        assert self.torch.equal(self.qkv[:, kd:], qkv[:, kd:])  # (q is turned in place)
+        v = qkv[:, kd + self.kv * self.hd:].view(self.most, self.kv, self.hd).bfloat16()
+        live = self.slots[:rows]
+        assert self.torch.equal(self.v[live], v[:rows])
+        check_y(n(self.y), norm_value((self.x + self.d).cpu().numpy(), n(self.norms[2])))
+
+
+BATCHES = [((0, 0, 0), (20, 7, 1)), ((20, 7, 1), (1, 1, 1)), ((21, 8, 2), (5, 0, 3)), ((26, 8, 5), (1, 30, 1))]
+
+
+def test_a_block_of_products(torch):
+    block = Block(torch, 40)
+    for i, (past, add) in enumerate(BATCHES):
+        block.batch(past, add, 10 * i)
+        x0, d0 = block.x.clone(), block.d.clone()
+        block.step()
+        block.check(x0, d0, sum(add))
+
+
+def test_a_captured_block_equals_an_eager_one(torch):
+    eager, captured = Block(torch, 40), Block(torch, 40)
+    for b in (eager, captured):  # what a first call sets up is set up outside of the capture
+        b.batch(*BATCHES[0], 0)
+        b.step()
+        b.k.zero_(), b.v.zero_()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        captured.step()
+    for i, (past, add) in enumerate(BATCHES + BATCHES[:1]):
+        for b in (eager, captured):
+            b.batch(past, add, 10 * i)
+        eager.step()
+        graph.replay()
+        torch.cuda.synchronize()
+        for a, b in zip(eager.state(), captured.state()):
+            assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("rows", [1, 5, 40, 300])
+def test_calls_repeat_to_the_bit(torch, rows):
+    block = Block(torch, rows, hidden=896, heads=14, kv=2, inter=4864)
+    add = (rows, 0, 0)
+    first = None
+    for _ in range(3):
+        block.batch((0, 0, 0), add if rows <= 256 else (256, 44, 0), 1)
+        block.step()
+        state = block.state()
+        first = first or state
+        for a, b in zip(first, state):
+            assert torch.equal(a, b)

@@ -1,0 +1,172 @@
+"""Ops around 8-bit products without a GPU: the refusals of their entry points
+and the arithmetic behind them."""
+import shutil
+import subprocess
+from pathlib import Path
+
+import numpy as np
+import pytest
+
+from vvli_amd import runtime as R
+from vvli_amd._lib import VvliError
+
+ROOT = Path(__file__).resolve().parents[1]
+P = 0x100000  # addresses that no refused call looks behind
+Q, S, T, U = 16 * P, 32 * P, 48 * P, 64 * P
+
+CONFIG, NULL = "InvalidConfig", "NullArgument"
+
+
+def refused(call, name, **kw):
+    with pytest.raises(VvliError) as e:
+        call(**kw)
+    assert e.value.name == name, str(e.value)
+
+
+def quantize(**kw):
+    a = dict(x=P, kind="f32", ldx=64, rows=3, width=50, codes=Q, ldc=64, scales=S)
+    a.update(kw)
+    R.quantize_rows(**a)
+
+
+def norm(**kw):
+    a = dict(x=P, ldx=64, delta=Q, ldd=64, rows=3, width=50, weight=S, weight_kind="f32", eps=1e-6, total=T, lds=64, y=None, ldy=0,
+             codes=U, ldc=64, scales=2 * U)
+    a.update(kw)
+    R.add_norm(**a)
+
+
+def gate(**kw):
+    a = dict(gate=P, ldg=128, up=P + 4 * 64, ldu=128, rows=3, width=50, codes=Q, ldc=64, scales=S)
+    a.update(kw)
+    R.silu_mul(**a)
+
+
+def linear(**kw):
+    a = dict(W=P, ldw=64, w_scales=Q, X=S, ldx=64, x_scales=T, bias=None, Y=U, ldy=40, M=5, N=40, K=64, workspace=2 * U,
+             workspace_bytes=1 << 30)
+    a.update(kw)
+    R.linear_i8(**a)
+
+
+CODES = [(dict(codes=None), NULL), (dict(scales=None), NULL), (dict(ldc=48), CONFIG), (dict(ldc=72), CONFIG), (dict(codes=Q + 8), CONFIG),
+         (dict(ldc=1 << 31), CONFIG), (dict(width=65), CONFIG)]
+SIZES = [(dict(rows=1 << 31), CONFIG), (dict(width=0), CONFIG), (dict(width=(1 << 31) - 1, ldx=1 << 31), CONFIG)]
+
+
+@pytest.mark.parametrize("bad,name", CODES + SIZES + [
+    (dict(x=None), NULL), (dict(x=P + 4), CONFIG), (dict(ldx=49), CONFIG), (dict(ldx=50), CONFIG), (dict(ldx=48), CONFIG),
+    (dict(ldx=60, kind="bf16"), CONFIG), (dict(ldx=1 << 31), CONFIG),
+    (dict(codes=P), CONFIG), (dict(codes=P + 3 * 256 - 64), CONFIG), (dict(scales=P + 4), CONFIG), (dict(scales=Q + 8), CONFIG),
+])
+def test_quantize_rows_refusals(bad, name):
+    refused(quantize, name, **bad)
+
+
+def test_quantize_rows_unknown_kind():
+    from vvli_amd import _lib
+
+    assert _lib.lib().vvli_gpu_quantize_rows(P, 2, 64, 3, 50, Q, 64, S, None) == 1
+
+
+@pytest.mark.parametrize("bad,name", CODES[:2] + CODES[2:4] + [(dict(codes=U + 8), CONFIG)] + SIZES[:2] + [
+    (dict(x=None), NULL), (dict(weight=None), NULL), (dict(weight=S + 8), CONFIG), (dict(x=P + 8), CONFIG), (dict(ldx=48), CONFIG),
+    (dict(ldd=54), CONFIG), (dict(delta=Q + 4), CONFIG), (dict(total=T + 4), CONFIG), (dict(lds=48), CONFIG), (dict(y=3 * U, ldy=48), CONFIG),
+    (dict(y=3 * U + 4, ldy=64), CONFIG), (dict(eps=-1e-6), CONFIG), (dict(eps=float("nan")), CONFIG), (dict(eps=float("inf")), CONFIG),
+    (dict(delta=None), CONFIG),                              # a sum without delta
+    (dict(codes=None, scales=None), NULL),                   # nothing to compute
+    (dict(y=3 * U, ldy=64, codes=None), NULL), (dict(y=3 * U, ldy=64, scales=None), NULL),
+    (dict(total=P, lds=128), CONFIG), (dict(total=Q, lds=128), CONFIG),       # in place with another stride
+    (dict(total=P + 16), CONFIG), (dict(y=P + 256, ldy=64), CONFIG),          # shifted
+    (dict(y=T, ldy=64), CONFIG), (dict(total=P, y=P, ldy=64), CONFIG),        # sum and y in one place
+    (dict(codes=P), CONFIG), (dict(codes=Q), CONFIG), (dict(codes=T), CONFIG), (dict(scales=P), CONFIG), (dict(codes=S), CONFIG),
+    (dict(total=S), CONFIG), (dict(scales=S + 100), CONFIG),
+])
+def test_add_norm_refusals(bad, name):
+    refused(norm, name, **bad)
+
+
+def test_add_norm_unknown_weight_kind():
+    from vvli_amd import _lib
+
+    assert _lib.lib().vvli_gpu_add_norm(P, 64, None, 0, 3, 50, S, 2, 1e-6, None, 0, None, 0, U, 64, 2 * U, None) == 1
+
+
+@pytest.mark.parametrize("bad,name", CODES[:6] + SIZES[:2] + [
+    (dict(gate=None), NULL), (dict(up=None), NULL), (dict(gate=P + 4), CONFIG), (dict(up=P + 8), CONFIG), (dict(ldg=48), CONFIG),
+    (dict(ldu=130), CONFIG), (dict(codes=P), CONFIG), (dict(codes=P + 256), CONFIG), (dict(scales=P), CONFIG),
+])
+def test_silu_mul_refusals(bad, name):
+    refused(gate, name, **bad)
+
+
+@pytest.mark.parametrize("bad,name", [
+    (dict(W=None), NULL), (dict(w_scales=None), NULL), (dict(X=None), NULL), (dict(x_scales=None), NULL), (dict(Y=None), NULL),
+    (dict(workspace=None), NULL), (dict(N=0), CONFIG), (dict(K=0), CONFIG), (dict(K=56), CONFIG), (dict(M=1 << 31), CONFIG),
+    (dict(K=131072, ldw=131072, ldx=131072), CONFIG), (dict(K=80), CONFIG), (dict(ldw=72), CONFIG), (dict(ldx=48), CONFIG),
+    (dict(ldw=1 << 31), CONFIG), (dict(W=P + 8), CONFIG), (dict(X=S + 4), CONFIG), (dict(ldy=39), CONFIG), (dict(ldy=1 << 31), CONFIG),
+    (dict(workspace=2 * U + 8), CONFIG), (dict(workspace_bytes=0), CONFIG), (dict(Y=P), CONFIG), (dict(Y=S + 64), CONFIG), (dict(Y=Q), CONFIG),
+    (dict(Y=T), CONFIG), (dict(bias=U + 8), CONFIG), (dict(Y=2 * U + 4), CONFIG), (dict(N=1 << 31, ldy=1 << 31), CONFIG),
+])
+def test_linear_i8_refusals(bad, name):
+    refused(linear, name, **bad)
+
+
+def test_linear_i8_workspace():
+    assert R.linear_i8_workspace(1, 16, 16) > 0
+    assert R.linear_i8_workspace(1, 0, 16) == R.linear_i8_workspace(1, 16, 24) == R.linear_i8_workspace(1, 16, 131072) == 0
+    for n, k in ((896, 4864), (2048, 2048), (40000, 16), (16, 131056)):
+        sizes = [R.linear_i8_workspace(m, n, k) for m in (1, 2, 5, 17, 64, 65, 300, 2000, 100000)]
+        assert sizes == sorted(sizes)  # up to M rows
+
+
+def test_no_rows_launch_nothing():
+    """(An address that nothing is behind: a launch would fail, here without a GPU and there with one.)"""
+    quantize(rows=0)
+    norm(rows=0)
+    gate(rows=0)
+    linear(M=0)
+
+
+HARNESS = """
+#include "row_bytes.hpp"
+#include <cstdio>
+int main() {
+    unsigned long long p, lp, wp, rp, q, lq, wq, rq;
+    while (scanf("%llu %llu %llu %llu %llu %llu %llu %llu", &p, &lp, &wp, &rp, &q, &lq, &wq, &rq) == 8)
+        printf("%d\\n", vvli::rows_meet(vvli::RowBytes{(void*)p, lp, wp, rp}, vvli::RowBytes{(void*)q, lq, wq, rq}));
+}
+"""
+
+
+@pytest.mark.skipif(not shutil.which("g++"), reason="no host compiler")
+def test_rows_that_share_bytes_are_found(tmp_path):
+    """Against sets of bytes: of one stride exactly, of two strides wherever the ranges meet."""
+    (tmp_path / "t.cpp").write_text(HARNESS)
+    subprocess.run(["g++", "-std=c++17", "-O1", f"-I{ROOT / 'vvli_amd' / 'csrc'}", "-o", tmp_path / "t", tmp_path / "t.cpp"], check=True)
+    rng = np.random.RandomState(3)
+    cases = []
+    for _ in range(4000):
+        la, lb = rng.randint(1, 12), rng.randint(1, 12)
+        lb = la if rng.rand() < 0.7 else lb
+        cases.append((100 + rng.randint(0, 60), la, rng.randint(1, la + 1), rng.randint(0, 5), 100 + rng.randint(0, 60), lb,
+                      rng.randint(1, lb + 1), rng.randint(0, 5)))
+    out = subprocess.run([tmp_path / "t"], input="\n".join(" ".join(map(str, c)) for c in cases), capture_output=True, text=True,
+                         check=True).stdout.split()
+    met = beside = 0
+    for (p, lp, wp, rp, q, lq, wq, rq), got in zip(cases, out):
+        a = {p + i * lp + e for i in range(rp) for e in range(wp)}
+        b = {q + i * lq + e for i in range(rq) for e in range(wq)}
+        ranges = bool(a and b) and max(min(a), min(b)) <= min(max(a), max(b))
+        want = bool(a & b)
+        if lp != lq:
+            assert int(got) == ranges
+        elif want:
+            assert int(got) == 1, (p, lp, wp, rp, q, lq, wq, rq)
+            met += 1
+        elif int(got):  # only where a row beyond the last would share one
+            a = {p + i * lp + e for i in range(-9, rp + 9) for e in range(wp)}
+            assert ranges and a & {q + i * lq + e for i in range(-9, rq + 9) for e in range(wq)}
+        else:
+            beside += ranges
+    assert met > 100 and beside > 50

@@ -200,6 +200,17 @@ PROTOTYPES = {
         c_int, [c_void_p, c_uint64, c_void_p, c_uint64, c_void_p, c_void_p, c_uint32, c_uint32, c_uint32, c_void_p,
                 c_void_p, c_void_p, c_void_p, c_void_p, c_size_t, c_void_p]),
     "vvli_gpu_verify_drafts_workspace": (c_size_t, [c_uint32, c_uint32]),
+    "vvli_gpu_quantize_rows": (
+        c_int, [c_void_p, c_uint32, c_uint64, c_uint32, c_uint32, c_void_p, c_uint64, c_void_p, c_void_p]),
+    "vvli_gpu_add_norm": (
+        c_int, [c_void_p, c_uint64, c_void_p, c_uint64, c_uint32, c_uint32, c_void_p, c_uint32, c_float, c_void_p, c_uint64,
+                c_void_p, c_uint64, c_void_p, c_uint64, c_void_p, c_void_p]),
+    "vvli_gpu_silu_mul": (
+        c_int, [c_void_p, c_uint64, c_void_p, c_uint64, c_uint32, c_uint32, c_void_p, c_uint64, c_void_p, c_void_p]),
+    "vvli_gpu_linear_i8": (
+        c_int, [c_void_p, c_uint64, c_void_p, c_void_p, c_uint64, c_void_p, c_void_p, c_void_p, c_uint64, c_uint32, c_uint32,
+                c_uint32, c_void_p, c_size_t, c_void_p]),
+    "vvli_gpu_linear_i8_workspace": (c_size_t, [c_uint32, c_uint32, c_uint32]),
     "vvli_host_fill_deterministic": (None, [c_void_p, c_size_t, c_uint32]),
     "vvli_host_fill_synthetic": (c_int, [POINTER(CConfig), c_uint64, c_float, c_void_p, c_size_t, c_uint32]),
     "vvli_host_synthetic_normal": (c_double, [c_uint64, c_uint64, c_uint64]),

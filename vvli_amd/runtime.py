@@ -497,3 +497,39 @@ def verify_drafts(target: int, ldt: int, draft: int | None, ldd: int, tokens: in
     """vvli_gpu_verify_drafts: drafted tokens against the target's probabilities."""
     _lib.check(_lib.lib().vvli_gpu_verify_drafts(target, ldt, draft, ldd, tokens, row_start, requests, rows, vocab, u_accept,
                                                  u_sample, accepted, out, workspace, workspace_bytes, stream))
+
+
+# ---- products in 8-bit integers and what stands between them (raw device pointers) ----
+ROW_KINDS = {"f32": WEIGHT_F32, "bf16": WEIGHT_BF16}
+
+
+def quantize_rows(x: int, kind: str, ldx: int, rows: int, width: int, codes: int, ldc: int, scales: int,
+                  stream: int | None = None) -> None:
+    """vvli_gpu_quantize_rows: rows of type ``kind`` ("f32" or "bf16") as 8-bit codes with a scale each."""
+    _lib.check(_lib.lib().vvli_gpu_quantize_rows(x, ROW_KINDS[kind], ldx, rows, width, codes, ldc, scales, stream))
+
+
+def add_norm(x: int, ldx: int, delta: int | None, ldd: int, rows: int, width: int, weight: int, weight_kind: str, eps: float,
+             total: int | None, lds: int, y: int | None, ldy: int, codes: int | None, ldc: int, scales: int | None,
+             stream: int | None = None) -> None:
+    """vvli_gpu_add_norm: x + delta (to ``total``), its RMS norm in f32 (to ``y``) and in 8 bits (to ``codes`` and ``scales``)."""
+    _lib.check(_lib.lib().vvli_gpu_add_norm(x, ldx, delta, ldd, rows, width, weight, ROW_KINDS[weight_kind], eps, total, lds, y,
+                                            ldy, codes, ldc, scales, stream))
+
+
+def silu_mul(gate: int, ldg: int, up: int, ldu: int, rows: int, width: int, codes: int, ldc: int, scales: int,
+             stream: int | None = None) -> None:
+    """vvli_gpu_silu_mul: silu(gate) * up in 8 bits."""
+    _lib.check(_lib.lib().vvli_gpu_silu_mul(gate, ldg, up, ldu, rows, width, codes, ldc, scales, stream))
+
+
+def linear_i8_workspace(M: int, N: int, K: int) -> int:
+    """Bytes of workspace (zeroed once) of ``linear_i8`` calls of up to M rows with these N and K."""
+    return _lib.lib().vvli_gpu_linear_i8_workspace(M, N, K)
+
+
+def linear_i8(W: int, ldw: int, w_scales: int, X: int, ldx: int, x_scales: int, bias: int | None, Y: int, ldy: int, M: int,
+              N: int, K: int, workspace: int | None, workspace_bytes: int, stream: int | None = None) -> None:
+    """vvli_gpu_linear_i8: the product of two matrices of 8-bit codes with a scale for each of their rows."""
+    _lib.check(_lib.lib().vvli_gpu_linear_i8(W, ldw, w_scales, X, ldx, x_scales, bias, Y, ldy, M, N, K, workspace,
+                                             workspace_bytes, stream))

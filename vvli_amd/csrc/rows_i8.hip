@@ -2,9 +2,24 @@
 // (vvli_gpu_quantize_rows), of a residual's sum behind its RMS norm
 // (vvli_gpu_add_norm) and of a gated activation (vvli_gpu_silu_mul).
 //
-// scale = f32(max |v| / 127), code = rint(v / scale). Which code a value near
-// a border between two gets follows its 64-bit value, so that codes do not
-// change with the order of a row's sums.
+// scale = f32(max |v| / 127), code = rint(v / scale), of v as it is in exact
+// arithmetic, so that codes do not change with the order of a row's sums.
+// Memory bounds all three, and 64-bit arithmetic on every value would be longer
+// than the memory's time (a block a row, all in f64: gate 2500 x 18944 385 us,
+// norm 6001 x 3584 314): values are formed in f32, whose error is known, and 64
+// bits settle what f32 cannot, which is
+//   * the largest value of a gated row: those whose f32 value is within that
+//     error of the largest one (mostly one of a row) are formed in f64 (a
+//     norm's are all: a product each);
+//   * a code whose f32 quotient is within the error of a border between two
+//     codes: its unit of 4 or 8 values is formed in f64 (of a wave's 64 units
+//     one in 30, gated one in 8).
+// Where f32's error is not the usual one (values that left its normal range) a
+// row is formed in f64 as a whole. Measured (inputs that no cache holds; a copy
+// of 1 GB moves 5.06 TB/s): weights 18944 x 3584 bf16 46 us (4.4 TB/s), f32 rows
+// 6001 x 3584 21.5 (5.0), their norm with the sum 62 (4.5), gate 2500 x 18944 100
+// (4.3; the products, exponentials and packing beside the loads are as long).
+// One row of 2048: 4.2, 4.8 and 5.2 us, of which 4.1 is a launch.
 #include <algorithm>
 
 #include "device_common.hpp"
@@ -27,91 +42,386 @@ struct RowsArgs {
     float eps;
 };
 
-__device__ __forceinline__ float bf16_at(const void* p, size_t i) {
-    return __uint_as_float(static_cast<uint32_t>(static_cast<const uint16_t*>(p)[i]) << 16);
+__device__ __forceinline__ float bf16_bits(uint32_t u) { return __uint_as_float(u << 16); }
+__device__ __forceinline__ float bf16_at(const void* p, size_t i) { return bf16_bits(static_cast<const uint16_t*>(p)[i]); }
+
+// ---- reductions: within a wave by DPP, between waves through LDS -----------
+// (quad_perm, row_half_mirror and row_mirror leave every lane of 16 with their total; four totals by readlane)
+template <int CTRL>
+__device__ __forceinline__ uint32_t dpp(uint32_t v) {
+    return __builtin_amdgcn_update_dpp(0, v, CTRL, 0xF, 0xF, false);
 }
-
-constexpr int kThreads = 1024, kWaves = kThreads / 64;
-
-// The sum of a block's values, in an order that does not change.
-__device__ __forceinline__ double block_sum(double v, double (&part)[kWaves]) {
-    for (int o = 32; o; o >>= 1) v += __shfl_xor(v, o, 64);
-    __syncthreads();
-    if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = v;
-    __syncthreads();
-    v = 0;
-    for (int i = 0; i < kWaves; ++i) v += part[i];
+template <int CTRL>
+__device__ __forceinline__ double dpp(double v) {
+    const uint64_t u = __builtin_bit_cast(uint64_t, v);
+    return __builtin_bit_cast(double, static_cast<uint64_t>(dpp<CTRL>(static_cast<uint32_t>(u >> 32))) << 32 |
+                                          dpp<CTRL>(static_cast<uint32_t>(u)));
+}
+template <int CTRL>
+__device__ __forceinline__ float dpp(float v) {
+    return __uint_as_float(dpp<CTRL>(__float_as_uint(v)));
+}
+__device__ __forceinline__ uint32_t lane_of(uint32_t v, int lane) { return __builtin_amdgcn_readlane(v, lane); }
+__device__ __forceinline__ double lane_of(double v, int lane) {
+    const uint64_t u = __builtin_bit_cast(uint64_t, v);
+    return __builtin_bit_cast(double, static_cast<uint64_t>(lane_of(static_cast<uint32_t>(u >> 32), lane)) << 32 |
+                                          lane_of(static_cast<uint32_t>(u), lane));
+}
+__device__ __forceinline__ float lane_of(float v, int lane) { return __uint_as_float(lane_of(__float_as_uint(v), lane)); }
+struct Add {
+    template <typename T>
+    __device__ __forceinline__ T operator()(T a, T b) const { return a + b; }
+};
+struct Max {  // (of doubles: NaN if one is NaN)
+    __device__ __forceinline__ float operator()(float a, float b) const { return fmaxf(a, b); }
+    __device__ __forceinline__ double operator()(double a, double b) const { return a >= b || a != a ? a : b; }
+};
+template <typename T, typename F>
+__device__ __forceinline__ T reduce_wave(T v, F f) {
+    v = f(v, dpp<0xB1>(v)), v = f(v, dpp<0x4E>(v)), v = f(v, dpp<0x141>(v)), v = f(v, dpp<0x140>(v));
+    return f(f(lane_of(v, 0), lane_of(v, 16)), f(lane_of(v, 32), lane_of(v, 48)));
+}
+// Two values of a row's WAVES waves at once; part: 2 WAVES values.
+template <int WAVES, typename T, typename F, typename H>
+__device__ __forceinline__ void reduce(T& v, F f, T& w, H h, T* part) {
+    v = reduce_wave(v, f), w = reduce_wave(w, h);
+    if constexpr (WAVES > 1) {
+        __syncthreads();
+        if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = v, part[WAVES + (threadIdx.x >> 6)] = w;
+        __syncthreads();
+        v = part[0], w = part[WAVES];
+#pragma unroll
+        for (int i = 1; i < WAVES; ++i) v = f(v, part[i]), w = h(w, part[WAVES + i]);
+    }
+}
+template <int WAVES, typename T, typename F>
+__device__ __forceinline__ T reduce(T v, F f, T* part) {
+    v = reduce_wave(v, f);
+    if constexpr (WAVES > 1) {
+        __syncthreads();
+        if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = v;
+        __syncthreads();
+        v = part[0];
+#pragma unroll
+        for (int i = 1; i < WAVES; ++i) v = f(v, part[i]);
+    }
     return v;
 }
-// The largest; NaN if a value is NaN.
-__device__ __forceinline__ double larger(double a, double b) { return a >= b || a != a ? a : b; }
-__device__ __forceinline__ double block_max(double v, double (&part)[kWaves]) {
-    for (int o = 32; o; o >>= 1) v = larger(v, __shfl_xor(v, o, 64));
-    __syncthreads();
-    if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = v;
-    __syncthreads();
-    v = part[0];
-    for (int i = 1; i < kWaves; ++i) v = larger(v, part[i]);
-    return v;
-}
 
-// A block a row, two passes over it.
+// ---- a row's values ---------------------------------------------------------
+// In f64, as the definition has them (norm: without the factor of its row).
 template <int OP>
-__global__ __launch_bounds__(kThreads) void rows_i8_kernel(RowsArgs a) {
-    __shared__ double part[kWaves];
+struct Row {
+    const RowsArgs& a;
+    const float *x, *b;
+    uint32_t row;
+    const float* h;  // where the sum is stored (in x's or delta's place, it may be): read there from then on
+    __device__ __forceinline__ Row(const RowsArgs& a_, uint32_t r)
+        : a(a_), x(static_cast<const float*>(a_.x) + r * a_.ldx), b(a_.b ? a_.b + r * a_.ldb : nullptr), row(r),
+          h(a_.sum ? a_.sum + r * a_.lds : nullptr) {}
+    __device__ __forceinline__ float hidden(uint32_t e) const { return h ? h[e] : b ? x[e] + b[e] : x[e]; }
+    __device__ __forceinline__ float weight(uint32_t e) const {
+        return a.weight_bf16 ? bf16_at(a.weight, e) : static_cast<const float*>(a.weight)[e];
+    }
+    __device__ __forceinline__ double operator()(uint32_t e) const {
+        if constexpr (OP == kRowsF32) return x[e];
+        if constexpr (OP == kRowsBf16) return bf16_at(a.x, row * a.ldx + e);
+        if constexpr (OP == kRowsNorm) return static_cast<double>(hidden(e)) * static_cast<double>(weight(e));
+        const double g = x[e];
+        return g / (1.0 + exp(-g)) * static_cast<double>(b[e]);
+    }
+};
+
+__device__ __forceinline__ float scale_of(double top) {
+    const float s = static_cast<float>(top / 127.0);
+    return s < INFINITY ? s : NAN;
+}
+__device__ __forceinline__ int code_of(double v, float scale) {
+    return scale > 0 ? static_cast<int>(fmin(fmax(rint(v / static_cast<double>(scale)), -127.0), 127.0)) : 0;
+}
+
+// ---- any width: a block a row, two passes over it, all in f64 ----------------
+constexpr int kAnyThreads = 1024, kAnyWaves = kAnyThreads / 64;
+
+template <int OP>
+__global__ __launch_bounds__(kAnyThreads) void rows_any_kernel(RowsArgs a) {
+    __shared__ double part[kAnyWaves];
     for (uint32_t row = blockIdx.x; row < a.rows; row += gridDim.x) {
-        const float* x = static_cast<const float*>(a.x) + row * a.ldx;
-        const float* b = a.b ? a.b + row * a.ldb : nullptr;
-        auto weight = [&](uint32_t e) { return a.weight_bf16 ? bf16_at(a.weight, e) : static_cast<const float*>(a.weight)[e]; };
-        auto hidden = [&](uint32_t e) { return b ? x[e] + b[e] : x[e]; };
-        auto value = [&](uint32_t e) -> double {  // norm: without the factor of its row
-            if constexpr (OP == kRowsF32) return x[e];
-            if constexpr (OP == kRowsBf16) return bf16_at(a.x, row * a.ldx + e);
-            if constexpr (OP == kRowsNorm) return static_cast<double>(hidden(e)) * static_cast<double>(weight(e));
-            const double g = x[e];
-            return g / (1.0 + exp(-g)) * static_cast<double>(b[e]);
-        };
+        const Row<OP> value(a, row);
         double top = 0, square = 0;
-        for (uint32_t e = threadIdx.x; e < a.width; e += kThreads) {
-            top = larger(top, fabs(value(e)));
+        for (uint32_t e = threadIdx.x; e < a.width; e += kAnyThreads) {
             if constexpr (OP == kRowsNorm) {
-                const double h = hidden(e);
+                if (a.sum) a.sum[row * a.lds + e] = value.x[e] + value.b[e];
+            }
+            top = Max()(top, fabs(value(e)));
+            if constexpr (OP == kRowsNorm) {
+                const double h = value.hidden(e);
                 square = fma(h, h, square);
             }
         }
-        top = block_max(top, part);
+        top = reduce<kAnyWaves>(top, Max(), part);
         double factor = 1;
         if constexpr (OP == kRowsNorm) {
-            factor = 1.0 / sqrt(block_sum(square, part) / a.width + static_cast<double>(a.eps));
+            factor = 1.0 / sqrt(reduce<kAnyWaves>(square, Add(), part) / a.width + static_cast<double>(a.eps));
             top *= factor;
         }
-        float scale = static_cast<float>(top / 127.0);
-        if (!(scale < INFINITY)) scale = NAN;
-        for (uint32_t e = threadIdx.x; e < a.width; e += kThreads) {
+        const float scale = scale_of(top);
+        for (uint32_t e = threadIdx.x; e < a.width; e += kAnyThreads) {
             double v = value(e);
             if constexpr (OP == kRowsNorm) {
-                const float h = hidden(e);
                 v *= factor;
-                if (a.sum) a.sum[row * a.lds + e] = h;
                 if (a.y) a.y[row * a.ldy + e] = static_cast<float>(v);
             }
-            if (a.codes) {
-                const double t = rint(v / static_cast<double>(scale));
-                a.codes[row * a.ldc + e] = scale > 0 ? static_cast<int8_t>(fmin(fmax(t, -127.0), 127.0)) : 0;
-            }
+            if (a.codes) a.codes[row * a.ldc + e] = static_cast<int8_t>(code_of(v, scale));
         }
         if (a.codes) {
             const uint32_t end = (a.width + kCodesPerUnit - 1) / kCodesPerUnit * kCodesPerUnit;
-            for (uint32_t e = a.width + threadIdx.x; e < end; e += kThreads) a.codes[row * a.ldc + e] = 0;
+            for (uint32_t e = a.width + threadIdx.x; e < end; e += kAnyThreads) a.codes[row * a.ldc + e] = 0;
             if (threadIdx.x == 0) a.scales[row] = scale;
         }
     }
 }
 
+// ---- rows that registers hold: WAVES waves a row, one pass -------------------
+// A lane holds units of E values (4 of f32, 8 of bf16: 16 bytes), unit lane + 64
+// WAVES j of the row for j < V, so that a load of a wave is 1 KiB in a row; what
+// it keeps are the f32 values that the codes are made of (of bf16 the units as
+// they come). What f64 settles is read again.
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+
+// f32's silu(g) u, for g >= -16 off by less than 1.3e-6 < 2^-19.5 of the value: the exponent's product with log2 e is off by
+// 2^-20 and 2.3e-7 where it is largest (of a value between 16 and 32), v_exp_f32 and v_rcp_f32 by one last bit, the rest
+// by half of one each. Below -16 it is off by 2^-16 of a value that is under 1.9e-6 |u|: rows where that could be a
+// larger part of the row's largest value than 2^-9 are not usual ones.
+__device__ __forceinline__ float gated32(float g, float u) {
+    const float p = __builtin_amdgcn_exp2f(g * -1.44269502f);
+    return g * u * __builtin_amdgcn_rcpf(1.f + p);
+}
+constexpr float kMostUp = 0x1p10f;  // of a usual row: max |u| over the largest value
+// How far |t - rint(t)| may be from 1/2 for f32 to tell the code of t = value / scale, |t| <= 127: off by 127 halves of a
+// last bit of f32 for the product and for the quotient each (2^-16), and of a norm's value (2^-17); a gated value by
+// 127 * 1.3e-6 more (1.7e-4).
 template <int OP>
-int launch(RowsArgs& a, hipStream_t s) {
-    const uint32_t blocks = std::min(a.rows, 1u << 20);
-    PAGED_TRY(vlaunch(rows_i8_kernel<OP>, dim3(blocks), dim3(kThreads), 0, s, a));
+constexpr float band() { return OP == kRowsGate ? 0x1p-12f : 0x1p-14f; }
+// Last bits of f32 by which two gated values may be off (2 * 1.3e-6 * 2^24 = 44).
+constexpr uint32_t kTopBits = 48;
+
+// Keeps the compiler from reading ahead over all of a row's units, and from keeping each unit's address and bound from
+// one use to the next: either takes more registers than there are.
+__device__ __forceinline__ void in_turn(uint32_t& id) { asm volatile("" : "+v"(id)::"memory"); }
+
+// The weights of unit u, whole.
+__device__ __forceinline__ f32x4 weights4(const RowsArgs& a, uint32_t u) {
+    if (!a.weight_bf16) return *as_global(static_cast<const f32x4*>(a.weight) + u);
+    const uint2 t = load_u32x2(static_cast<const uint2*>(a.weight) + u);
+    return f32x4{bf16_bits(t.x), __uint_as_float(t.x & 0xffff0000u), bf16_bits(t.y), __uint_as_float(t.y & 0xffff0000u)};
+}
+
+template <int OP, int WAVES, int V>
+__global__ __launch_bounds__(WAVES == 1 ? 256 : WAVES * 64, 4) void rows_i8_kernel(RowsArgs a) {
+    constexpr int G = WAVES * 64, E = OP == kRowsBf16 ? 8 : 4, ROWS = WAVES == 1 ? 4 : 1;  // rows of a block
+    constexpr int N = V % 4 == 0 ? 4 : V % 3 == 0 ? 3 : 2;  // units in flight
+    static_assert(V % N == 0, "whole turns");
+    __shared__ double part_d[2 * WAVES];
+    __shared__ float part_f[2 * WAVES];
+    uint32_t id = WAVES == 1 ? threadIdx.x & 63 : threadIdx.x;
+    // Whole units, and those behind them up to the padded width: the first may hold the row's last values, lane i has
+    // the i-th of them as its unit V.
+    const uint32_t full = a.width / E, units = (a.width + kCodesPerUnit - 1) / kCodesPerUnit * (kCodesPerUnit / E);
+    const uint32_t first = blockIdx.x * ROWS + (WAVES == 1 ? __builtin_amdgcn_readfirstlane(threadIdx.x / 64) : 0);
+    for (uint32_t row = first; row < a.rows; row += gridDim.x * ROWS) {
+        const Row<OP> value(a, row);
+        f32x4 v[V + 1];
+        float top = 0, most_u = 0, odd32 = 0;
+        double square = 0, exact = 0, odd = 0;  // odd: NaN if a value is not finite
+        auto norm_value = [&](float h, float w) {
+            const double x = h, y = x * static_cast<double>(w);
+            square = fma(x, x, square), exact = fmax(exact, fabs(y)), odd = fma(y, 0.0, odd);
+            return h * w;
+        };
+#pragma unroll
+        for (int j0 = 0; j0 < V; j0 += N) {
+            in_turn(id);
+#pragma unroll
+            for (int j = j0; j < j0 + N; ++j) v[j] = f32x4{0, 0, 0, 0};
+            if (static_cast<uint32_t>(j0) * G >= full) continue;  // (the same for all)
+#pragma unroll
+            for (int j = j0; j < j0 + N; ++j) {
+                const uint32_t at = id + j * G, u = min(at, full - 1);
+                const bool in = at < full;
+                if constexpr (OP == kRowsBf16) {
+                    v[j] = *as_global(reinterpret_cast<const f32x4*>(static_cast<const uint16_t*>(a.x) + row * a.ldx) + u);
+                } else if constexpr (OP == kRowsGate) {
+                    const f32x4 g = *as_global(reinterpret_cast<const f32x4*>(value.x) + u), b = *as_global(reinterpret_cast<const f32x4*>(value.b) + u);
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) v[j][e] = gated32(g[e], b[e]), most_u = fmaxf(most_u, fabsf(b[e]));
+                } else {
+                    v[j] = *as_global(reinterpret_cast<const f32x4*>(value.x) + u);
+                    if constexpr (OP == kRowsNorm) {
+                        const f32x4 w = weights4(a, u);
+                        if (value.b) v[j] += *as_global(reinterpret_cast<const f32x4*>(value.b) + u);
+                        if (a.sum && in) *as_global(reinterpret_cast<f32x4*>(a.sum + row * a.lds) + u) = v[j];
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) v[j][e] = norm_value(in ? v[j][e] : 0.f, in ? w[e] : 0.f);
+                    }
+                }
+            }
+        }
+        v[V] = f32x4{0, 0, 0, 0};
+        if (units > full && id == 0) {
+#pragma unroll
+            for (uint32_t e = 0; e < E; ++e) {
+                const uint32_t at = full * E + e;
+                if (at >= a.width) continue;
+                if constexpr (OP == kRowsBf16) {
+                    const uint32_t w = static_cast<const uint16_t*>(a.x)[row * a.ldx + at];
+                    v[V][e / 2] = __uint_as_float(__float_as_uint(v[V][e / 2]) | w << (e % 2 * 16));
+                } else if constexpr (OP == kRowsGate) {
+                    v[V][e] = gated32(value.x[at], value.b[at]), most_u = fmaxf(most_u, fabsf(value.b[at]));
+                } else if constexpr (OP == kRowsNorm) {
+                    const float h = value.b ? value.x[at] + value.b[at] : value.x[at];
+                    if (a.sum) a.sum[row * a.lds + at] = h;
+                    v[V][e] = norm_value(h, value.weight(at));
+                } else {
+                    v[V][e] = value.x[at];
+                }
+            }
+        }
+        in_turn(id);
+        double factor = 1;
+        bool usual = true;  // (of the whole row)
+        auto unit_of = [&](int j) { return j < V ? id + j * G : full + id; };
+        if constexpr (OP == kRowsNorm) {
+            if (!(odd == 0)) exact = odd;
+            reduce<WAVES>(exact, Max(), square, Add(), part_d);
+            factor = 1.0 / sqrt(square / a.width + static_cast<double>(a.eps));
+            usual = exact >= 0x1p-100 && exact <= 0x1p100;
+            exact *= factor;
+        } else {
+#pragma unroll
+            for (int j = 0; j <= V; ++j) {
+                f32x4 t = v[j], o = v[j];
+                if constexpr (OP == kRowsBf16) {
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        const uint32_t w = __float_as_uint(t[e]);
+                        t[e] = bf16_bits(w), o[e] = __uint_as_float(w & 0xffff0000u);
+                        top = fmaxf(fmaxf(fabsf(t[e]), fabsf(o[e])), top), odd32 = fmaf(t[e], 0.f, odd32), odd32 = fmaf(o[e], 0.f, odd32);
+                    }
+                } else {
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) top = fmaxf(top, fabsf(t[e])), odd32 = fmaf(t[e], 0.f, odd32);
+                }
+            }
+            float largest = odd32 == 0 ? top : INFINITY;  // (of the thread's)
+            if constexpr (OP == kRowsGate) reduce<WAVES>(largest, Max(), most_u, Max(), part_f);
+            else largest = reduce<WAVES>(largest, Max(), part_f);
+            exact = top = largest;
+        }
+        if constexpr (OP == kRowsGate) {
+            usual = top >= 0x1p-40f && top <= 0x1p100f && most_u <= kMostUp * top;
+            const uint32_t least = __float_as_uint(top) - kTopBits;
+            uint32_t near = 0;  // units that may hold the largest
+#pragma unroll
+            for (int j = 0; j <= V; ++j) {
+                const float most = fmaxf(fmaxf(fabsf(v[j][0]), fabsf(v[j][1])), fmaxf(fabsf(v[j][2]), fabsf(v[j][3])));
+                if (most >= __uint_as_float(least)) near |= 1u << j;
+            }
+            if (!usual) near = (2u << V) - 1;
+            exact = 0;
+            for (; near; near &= near - 1) {
+                const uint32_t u = unit_of(__builtin_ctz(near));
+                for (uint32_t e = u * 4; e < min(u * 4 + 4, a.width); ++e) exact = Max()(exact, fabs(value(e)));
+            }
+            exact = reduce<WAVES>(exact, Max(), part_d);
+        }
+        const float scale = scale_of(exact), quotient = static_cast<float>(factor / static_cast<double>(scale));
+        usual = usual && scale >= 0x1p-126f;
+        int8_t* const codes = a.codes ? a.codes + row * a.ldc : nullptr;
+        if (codes) {
+            if (id == 0) a.scales[row] = scale;
+            uint32_t doubt = 0;
+#pragma unroll
+            for (int j = 0; j <= V; ++j) {
+                if (j % N == 0) in_turn(id);
+                const uint32_t u = unit_of(j);
+                uint32_t word[E / 4];
+                float far = 0;
+#pragma unroll
+                for (int q = 0; q < E / 4; ++q) {
+                    uint32_t bits[4];
+                    float off[4];
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        float x = v[j][e];
+                        if constexpr (OP == kRowsBf16) {
+                            const uint32_t two = __float_as_uint(v[j][q * 2 + e / 2]);
+                            x = e % 2 ? __uint_as_float(two & 0xffff0000u) : bf16_bits(two);
+                        }
+                        const float near = fmaf(x, quotient, 0x1.8p23f);  // rint of the product in the last bits
+                        off[e] = fmaf(x, quotient, 0x1.8p23f - near), bits[e] = __float_as_uint(near);
+                    }
+                    far = fmaxf(fmaxf(far, fmaxf(fabsf(off[0]), fabsf(off[1]))), fmaxf(fabsf(off[2]), fabsf(off[3])));
+                    // (v_perm_b32: bytes 0-3 of the second operand, 4-7 of the first)
+                    word[q] = __builtin_amdgcn_perm(__builtin_amdgcn_perm(bits[3], bits[2], 0x0c0c0400),
+                                                    __builtin_amdgcn_perm(bits[1], bits[0], 0x0c0c0400), 0x05040100);
+                }
+                if (u < (j < V ? full : units)) {
+                    if (!usual || far > 0.5f - band<OP>()) doubt |= 1u << j;
+                    if constexpr (E == 8) *as_global(reinterpret_cast<vvli_u32x2*>(codes) + u) = vvli_u32x2{word[0], word[1]};
+                    else *as_global(reinterpret_cast<uint32_t*>(codes) + u) = word[0];
+                }
+            }
+            for (; doubt; doubt &= doubt - 1) {
+                const uint32_t u = unit_of(__builtin_ctz(doubt));
+                uint64_t word = 0;
+                for (uint32_t e = u * E; e < min(u * E + E, a.width); ++e)
+                    word |= static_cast<uint64_t>(code_of(value(e) * factor, scale) & 0xff) << (e - u * E) * 8;
+                if constexpr (E == 8) *reinterpret_cast<uint64_t*>(codes + u * 8) = word;
+                else *reinterpret_cast<uint32_t*>(codes + u * 4) = static_cast<uint32_t>(word);
+            }
+        }
+        if constexpr (OP == kRowsNorm) {
+            if (a.y) {  // (may be x or delta: behind all that reads them)
+                float* y = a.y + row * a.ldy;
+                for (uint32_t u = id; u < full; u += G) {
+                    f32x4 o;
+                    const f32x4 w = weights4(a, u);
+#pragma unroll
+                    for (uint32_t e = 0; e < 4; ++e)
+                        o[e] = static_cast<float>(static_cast<double>(value.hidden(u * 4 + e)) * static_cast<double>(w[e]) * factor);
+                    *as_global(reinterpret_cast<f32x4*>(y) + u) = o;
+                }
+                if (const uint32_t e = full * 4 + id; e < a.width) y[e] = static_cast<float>(value(e) * factor);
+            }
+        }
+    }
+}
+
+template <int OP, int WAVES, int V>
+hipError_t launch_rows(const RowsArgs& a, hipStream_t s) {
+    constexpr uint32_t ROWS = WAVES == 1 ? 4 : 1, THREADS = WAVES == 1 ? 256 : WAVES * 64;
+    const uint32_t blocks = std::min((a.rows - 1) / ROWS + 1, 1u << 20);
+    return vlaunch(rows_i8_kernel<OP, WAVES, OP == kRowsBf16 ? V / 2 : V>, dim3(blocks), dim3(THREADS), 0, s, a);
+}
+
+template <int OP>
+int launch(const RowsArgs& a, hipStream_t s) {
+    // By the width alone: the fewest waves that hold a row in 4 to 12 units a lane, so that several rows' blocks share a
+    // CU and one's loads run beside another's codes. Norm, us, of waves x units (6001 x 3584: 4 x 4 62, 2 x 8 66, 16 x 4
+    // 165; 2500 x 8192: 4 x 8 57, 8 x 4 60, 16 x 4 94; 300 x 8192: 14.4, 12.0, 17.6; 2500 x 18944: 8 x 12 147, 16 x 8 174;
+    // 75 x 3584: 4 x 4 6.0, 2 x 8 7.5, 8 x 4 6.5; 1 x 2048: 4.8 from 2 waves on, 1 x 8 6.2).
+    const uint32_t w = a.width;
+    hipError_t e;
+    if (w <= 1024) e = launch_rows<OP, 1, 4>(a, s);
+    else if (w <= 2048) e = launch_rows<OP, 2, 4>(a, s);
+    else if (w <= 4096) e = launch_rows<OP, 4, 4>(a, s);
+    else if (w <= 8192) e = launch_rows<OP, 4, 8>(a, s);
+    else if (w <= 16384) e = launch_rows<OP, 8, 8>(a, s);
+    else if (w <= 24576) e = launch_rows<OP, 8, 12>(a, s);
+    else if (w <= 32768) e = launch_rows<OP, 16, 8>(a, s);
+    else e = vlaunch(rows_any_kernel<OP>, dim3(std::min(a.rows, 1u << 20)), dim3(kAnyThreads), 0, s, a);
+    PAGED_TRY(e);
     return VVLI_OK;
 }
 

@@ -4,6 +4,8 @@
 //
 // The sums are exact in 32 bits, so no split or order of them changes a result.
 #include <algorithm>
+#include <type_traits>
+#include <utility>
 
 #include "device_common.hpp"
 #include "rows_i8.hpp"
@@ -22,6 +24,8 @@ struct LinearI8Args {
     float* Y;
     uint64_t ldw, ldx, ldy;
     uint32_t M, N, K;
+    uint32_t split_steps;  // steps of 128 codes of a part of K
+    int* parts;            // [part][M][N]
     bool vector;  // Y's rows and w_scales at 16-byte addresses
 };
 
@@ -198,184 +202,258 @@ hipError_t launch_stream(const LinearI8Args& a, hipStream_t s) {
     return vlaunch(linear_i8_stream_kernel<R, XG, ST, WV>, dim3(static_cast<uint32_t>((tn + 7) / 8 * 8 * tm)), dim3(WV * 64), LDS, s, a);
 }
 
-// ---- many rows: 256 x 256 ------------------------------------------------------
-// A block of four waves per CU, one on each SIMD, 128 x 128 each: the fewest
-// fragment bytes a product that the registers hold (256 of sums, 64 for each of
-// two sets of fragments). LDS takes 64 KiB of copies and gives 128 KiB of fragments
-// in a step of 128 codes, 1536 cycles of its 128 bytes a cycle, for 2048 cycles of
-// products; eight waves of 128 x 64 read 192 KiB, which with the copies is all of
-// them (4096 x 3584 x 18944: 271 us).
+// ---- more rows: tiles ----------------------------------------------------------
+// A block of four waves, 2 over rows of W x 2 over rows of X, 32 RN x 32 RM each.
+//
+// 4 x 4 (a tile of 256 x 256, one wave on each SIMD of a CU) moves the fewest
+// fragment bytes a product that the registers hold (256 of sums, 64 for each of two
+// sets of fragments): LDS takes 64 KiB of copies and gives 128 KiB of fragments in
+// a step of 128 codes, 1536 cycles of its 128 bytes a cycle, for 2048 cycles of
+// products. (Eight waves of 128 x 64 read 192 KiB, which with the copies is all that
+// LDS gives: 4096 x 3584 x 18944 271 us, four waves 238.) Smaller ones are for
+// launches whose large tiles would leave CUs idle.
 //
 // A step has two halves of 64 codes. While the products of a half run, the next
-// half's fragments come out of LDS, a read behind every other product. In the
-// middle of a step stands its one barrier: every wave has read all of the step's
-// stages, and the next step's have arrived; copies into the stages just read are
-// issued behind the first products after it.
+// half's fragments come out of LDS and copies for later steps are issued, both
+// spread evenly: a wave that has its SIMD to itself must not wait to issue (all of a
+// step's copies in one half took 246 us). In the middle of a step stands its one
+// barrier: every wave has read all of the step's stages, and the next step's have
+// arrived.
 //
-// LDS: three stages of W and two of X, 32 KiB each (160 KiB in all), rows of 128
-// bytes with 16-byte unit c of row r at c ^ (r & 7). X's copies are for the step
-// after next, W's for the third from there.
-constexpr int kTile = 256, kTileStage = kTile * 128, kTileLds = 5 * kTileStage, kTileThreads = 256;
-constexpr uint32_t kTileBytes = 1u << 31;  // 256 rows are below it: where copies of zeros point
+// LDS: ST stages of X and one more of W, rows of 128 bytes with 16-byte unit c of
+// row r at c ^ (r & 7). X's copies are issued in a step's second half, into the
+// stage just read, W's in the first half of the step after it. 256 x 256 leaves room
+// for two stages; smaller tiles take more, since their steps are shorter and what is
+// on its way lasts as long.
+//
+// SPLIT: a block has a part of K and leaves its sums, 32-bit integers, for
+// linear_i8_join_kernel.
+constexpr int kTileThreads = 256;
+constexpr uint32_t kBufferBytes = 1u << 31;  // a tile's rows are below it: copies of zeros point behind it
 
 typedef int i32x16 __attribute__((ext_vector_type(16)));
 
-// (No wait: whoever uses v waits for it with fragments_done, which nothing that uses it can be moved ahead of.)
+template <typename F, int... I>
+__device__ __forceinline__ void each(F f, std::integer_sequence<int, I...>) {
+    (f(std::integral_constant<int, I>{}), ...);
+}
+template <int N, typename F>
+__device__ __forceinline__ void each(F f) {
+    each(f, std::make_integer_sequence<int, N>{});
+}
+
+// (No wait: whoever uses v calls fragments_done first, and nothing that uses it can be moved ahead of that.)
 template <int OFF>
 __device__ __forceinline__ void read_fragment(i32x4& v, uint32_t from) {
     asm volatile("ds_read_b128 %0, %1 offset:%2" : "=&v"(v) : "v"(from), "n"(OFF) : "memory");
 }
-__device__ __forceinline__ void fragments_done(i32x4 (&w)[2][4], i32x4 (&x)[2][4]) {
-    asm volatile("s_waitcnt lgkmcnt(0)"
-                 : "+v"(w[0][0]), "+v"(w[0][1]), "+v"(w[0][2]), "+v"(w[0][3]), "+v"(w[1][0]), "+v"(w[1][1]), "+v"(w[1][2]), "+v"(w[1][3])
-                 :
-                 : "memory");
-    asm volatile(""
-                 : "+v"(x[0][0]), "+v"(x[0][1]), "+v"(x[0][2]), "+v"(x[0][3]), "+v"(x[1][0]), "+v"(x[1][1]), "+v"(x[1][2]), "+v"(x[1][3])
-                 :
-                 : "memory");
+template <int RN, int RM>
+__device__ __forceinline__ void fragments_done(i32x4 (&w)[2][RN], i32x4 (&x)[2][RM]) {
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+#pragma unroll
+        for (int r = 0; r < RN; ++r) asm volatile("" : "+v"(w[k][r]));
+#pragma unroll
+        for (int c = 0; c < RM; ++c) asm volatile("" : "+v"(x[k][c]));
+    }
 }
-// 1 KiB into LDS from a buffer of kTileBytes bytes: 16 bytes a lane, zeros for lanes behind its end.
+// 1 KiB into LDS from a buffer of kBufferBytes: 16 bytes a lane, zeros for lanes behind its end.
 __device__ __forceinline__ void copy_buffer16(__amdgpu_buffer_rsrc_t from, uint32_t at, uint32_t k, char* to) {
     __builtin_amdgcn_raw_ptr_buffer_load_lds(from, (lds_void*)to, 16, at, k, 0, 0);
 }
 
-__global__ __launch_bounds__(kTileThreads, 1) void linear_i8_tile_kernel(LinearI8Args a) {
-    extern __shared__ __attribute__((aligned(1024))) char tile_lds[];  // W [3] | X [2]
+template <int RN, int RM, int ST>
+struct TileShape {
+    static constexpr int N = 64 * RN, M = 64 * RM, WStage = N * 128, XStage = M * 128, Lds = (ST + 1) * WStage + ST * XStage;
+    static_assert(Lds <= 160 * 1024, "stages fit");
+};
+
+template <int RN, int RM, int ST, bool SPLIT>
+__global__ __launch_bounds__(kTileThreads, RN * RM == 16 ? 1 : 2) void linear_i8_tile_kernel(LinearI8Args a) {
+    using S = TileShape<RN, RM, ST>;
+    constexpr int WG = 2 * RN, XG = 2 * RM;  // copies of a wave a step
+    extern __shared__ __attribute__((aligned(1024))) char tile_lds[];  // W [ST + 1] | X [ST]
     const uint32_t lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const uint32_t wn = wave / 2, wm = wave % 2;
     uint32_t m0, n0;
     {  // blocks of one XCD (b % 8) take tiles that follow one another: panels of 8 tiles of W by all of X
-        const uint32_t tn = (a.N + kTile - 1) / kTile, tm = (a.M + kTile - 1) / kTile, tiles = tn * tm;
+        const uint32_t tn = (a.N + S::N - 1) / S::N, tm = (a.M + S::M - 1) / S::M, tiles = tn * tm;
         const uint32_t xcd = blockIdx.x % 8, per = tiles / 8, rem = tiles % 8;
         const uint32_t u = xcd * per + min(xcd, rem) + blockIdx.x / 8;
         const uint32_t panel = u / (tm * 8), wide = min(8u, tn - 8 * panel), within = u - panel * tm * 8;
-        m0 = within / wide * kTile, n0 = (8 * panel + within % wide) * kTile;
+        m0 = within / wide * S::M, n0 = (8 * panel + within % wide) * S::N;
     }
-    const __amdgpu_buffer_rsrc_t W = __builtin_amdgcn_make_buffer_rsrc(const_cast<int8_t*>(a.W) + n0 * a.ldw, 0, kTileBytes, 0x20000);
-    const __amdgpu_buffer_rsrc_t X = __builtin_amdgcn_make_buffer_rsrc(const_cast<int8_t*>(a.X) + m0 * a.ldx, 0, kTileBytes, 0x20000);
+    const __amdgpu_buffer_rsrc_t W = __builtin_amdgcn_make_buffer_rsrc(const_cast<int8_t*>(a.W) + n0 * a.ldw, 0, kBufferBytes, 0x20000);
+    const __amdgpu_buffer_rsrc_t X = __builtin_amdgcn_make_buffer_rsrc(const_cast<int8_t*>(a.X) + m0 * a.ldx, 0, kBufferBytes, 0x20000);
     const uint32_t unit = (lane % 8 ^ lane / 8) * 16;  // of a row's 128 codes, what this lane copies
-    uint32_t w_at[8], x_at[8];
+    uint32_t w_at[WG], x_at[XG];
 #pragma unroll
-    for (int g = 0; g < 8; ++g) {
-        const uint32_t row = wave * 64 + g * 8 + lane / 8;
-        w_at[g] = min(row, a.N - 1 - n0) * static_cast<uint32_t>(a.ldw) + unit;
-        x_at[g] = min(row, a.M - 1 - m0) * static_cast<uint32_t>(a.ldx) + unit;
-    }
-    const int steps = static_cast<int>((a.K + 127) / 128);
+    for (int g = 0; g < WG; ++g) w_at[g] = min((wave * WG + g) * 8 + lane / 8, a.N - 1 - n0) * static_cast<uint32_t>(a.ldw) + unit;
+#pragma unroll
+    for (int g = 0; g < XG; ++g) x_at[g] = min((wave * XG + g) * 8 + lane / 8, a.M - 1 - m0) * static_cast<uint32_t>(a.ldx) + unit;
+    const int all_steps = static_cast<int>((a.K + 127) / 128);
+    const int first = SPLIT ? static_cast<int>(blockIdx.y * a.split_steps) : 0, steps = SPLIT ? min(static_cast<int>(a.split_steps), all_steps - first) : all_steps;
+    const uint32_t k_first = first * 128, k_end = min(k_first + steps * 128, a.K);
+    // Each XCD starts at another eighth of the steps and goes round. All blocks at the same columns of rows that are an even
+    // number of 256 bytes apart would meet in few of the memory's channels (512 x 4608 x 14336: 73 us).
+    const int turn = steps * static_cast<int>((blockIdx.x + blockIdx.y * gridDim.x) % 8) / 8;
+    // (Copies of steps that there are none of are zeros, and what is read of them is never used: no branch is in the way.)
+    auto k_of = [&](int step) { return k_first + (step + turn < steps ? step + turn : step + turn - steps) * 128; };
+    auto end_of = [&](int step) { return step < steps ? k_end : 0; };
     auto copy_w = [&](int step, int g) {
-        const uint32_t k = step * 128;
-        copy_buffer16(W, k + unit < a.K ? w_at[g] : kTileBytes, k, tile_lds + step % 3 * kTileStage + wave * 8192 + g * 1024);
+        const uint32_t k = k_of(step);
+        copy_buffer16(W, k + unit < end_of(step) ? w_at[g] : kBufferBytes, k, tile_lds + step % (ST + 1) * S::WStage + (wave * WG + g) * 1024);
     };
     auto copy_x = [&](int step, int g) {
-        const uint32_t k = step * 128;
-        copy_buffer16(X, k + unit < a.K ? x_at[g] : kTileBytes, k, tile_lds + (3 + step % 2) * kTileStage + wave * 8192 + g * 1024);
+        const uint32_t k = k_of(step);
+        copy_buffer16(X, k + unit < end_of(step) ? x_at[g] : kBufferBytes, k,
+                      tile_lds + (ST + 1) * S::WStage + step % ST * S::XStage + (wave * XG + g) * 1024);
     };
-    // (Copies of steps that there are none of are zeros, and what is read of them is never used: no branch is in the way.)
+    for (int t = 0; t < ST; ++t) {
 #pragma unroll
-    for (int t = 0; t < 2; ++t) {
+        for (int g = 0; g < WG; ++g) copy_w(t, g);
 #pragma unroll
-        for (int g = 0; g < 8; ++g) copy_w(t, g);
-#pragma unroll
-        for (int g = 0; g < 8; ++g) copy_x(t, g);
+        for (int g = 0; g < XG; ++g) copy_x(t, g);
     }
-    i32x16 sum[4][4];
+    i32x16 sum[RN][RM];
 #pragma unroll
-    for (int r = 0; r < 4; ++r)
+    for (int r = 0; r < RN; ++r)
 #pragma unroll
-        for (int t = 0; t < 4; ++t)
+        for (int c = 0; c < RM; ++c)
 #pragma unroll
-            for (int e = 0; e < 16; ++e) sum[r][t][e] = 0;
-    // Fragments [half of 64][32 codes][tile of 32 rows]: lane l row l % 32, codes 16 (l / 32) .. + 15.
-    i32x4 fw[2][2][4], fx[2][2][4];
+            for (int e = 0; e < 16; ++e) sum[r][c][e] = 0;
+    // Fragments [half of 64][32 codes][32 rows]: lane l row l % 32, codes 16 (l / 32) .. + 15.
+    i32x4 fw[2][2][RN], fx[2][2][RM];
     const uint32_t at = lane % 32 * 128 + (lane / 32 ^ lane % 8) * 16;
-    const uint32_t w_lds = lds_address(tile_lds) + wn * 128 * 128 + at, x_lds = lds_address(tile_lds) + 3 * kTileStage + wm * 128 * 128 + at;
-#define TILE_READ(h, i, ws, xs)                                                                        \
-    do {                                                                                               \
-        constexpr int kk = (i) / 8, what = (i) % 8, tile = what % 4;                                   \
-        if constexpr (what < 4) read_fragment<tile * 4096>(fw[h][kk][tile], (ws) ^ ((h) * 64 + kk * 32)); \
-        else read_fragment<tile * 4096>(fx[h][kk][tile], (xs) ^ ((h) * 64 + kk * 32));                 \
-    } while (0)
-#define TILE_PAIR(h, p)                                                                                \
-    do {                                                                                               \
-        constexpr int kk = (p) / 8, r = (p) % 8 / 2, c = (p) % 2 * 2;                                  \
-        sum[r][c] = __builtin_amdgcn_mfma_i32_32x32x32_i8(fx[h][kk][c], fw[h][kk][r], sum[r][c], 0, 0, 0);             \
-        sum[r][c + 1] = __builtin_amdgcn_mfma_i32_32x32x32_i8(fx[h][kk][c + 1], fw[h][kk][r], sum[r][c + 1], 0, 0, 0); \
-        __builtin_amdgcn_sched_barrier(0);                                                             \
-    } while (0)
-#define TILE_ALL(X) X(0) X(1) X(2) X(3) X(4) X(5) X(6) X(7) X(8) X(9) X(10) X(11) X(12) X(13) X(14) X(15)
-    wait_copies<16>();
+    const uint32_t w_lds = lds_address(tile_lds) + wn * (RN * 4096) + at;
+    const uint32_t x_lds = lds_address(tile_lds) + (ST + 1) * S::WStage + wm * (RM * 4096) + at;
+    constexpr int P = 2 * RN * RM, R = 2 * (RN + RM);  // products and reads of a half
+    auto read = [&](auto half, auto i, uint32_t ws, uint32_t xs) {
+        constexpr int h = half, k = i / (RN + RM), what = i % (RN + RM);
+        if constexpr (what < RN) read_fragment<what * 4096>(fw[h][k][what], ws ^ (h * 64 + k * 32));
+        else read_fragment<(what - RN) * 4096>(fx[h][k][what - RN], xs ^ (h * 64 + k * 32));
+    };
+    // The products of half h with reads and copies spread among them.
+    auto half = [&](auto h, uint32_t ws, uint32_t xs, int step) {
+        constexpr int C = h ? XG : WG;
+        each<P>([&](auto p) {
+            constexpr int k = p / (RN * RM), r = p / RM % RN, c = p % RM;
+            sum[r][c] = __builtin_amdgcn_mfma_i32_32x32x32_i8(fx[h][k][c], fw[h][k][r], sum[r][c], 0, 0, 0);
+            __builtin_amdgcn_sched_barrier(0);
+            constexpr int r0 = p * R / P, r1 = (p + 1) * R / P, c0 = p * C / P, c1 = (p + 1) * C / P;
+            each<r1 - r0>([&](auto i) { read(std::integral_constant<int, 1 - h>{}, std::integral_constant<int, r0 + i>{}, ws, xs); });
+            each<c1 - c0>([&](auto i) {
+                if constexpr (h) copy_x(step, c0 + i);
+                else copy_w(step, c0 + i);
+            });
+            __builtin_amdgcn_sched_barrier(0);
+        });
+        fragments_done(fw[1 - h], fx[1 - h]);
+    };
+    using Zero = std::integral_constant<int, 0>;
+    using One = std::integral_constant<int, 1>;
+    wait_copies<(ST - 1) * (WG + XG)>();
     __builtin_amdgcn_s_barrier();
-#define FIRST(i) TILE_READ(0, i, w_lds, x_lds);
-    TILE_ALL(FIRST)
+    each<R>([&](auto i) { read(Zero{}, i, w_lds, x_lds); });
     fragments_done(fw[0], fx[0]);
     for (int t = 0; t < steps; ++t) {
-        const uint32_t ws = w_lds + t % 3 * kTileStage, xs = x_lds + t % 2 * kTileStage;
-#define HALF0(i)                                                          \
-    TILE_PAIR(0, i);                                                      \
-    TILE_READ(1, i, ws, xs);                                              \
-    if ((i) % 2 == 0) copy_w(t + 2, (i) / 2);                             \
-    __builtin_amdgcn_sched_barrier(0);
-        TILE_ALL(HALF0)
-        fragments_done(fw[1], fx[1]);
-        wait_copies<8>();  // (W's for t + 2 may be in flight)
+        half(Zero{}, w_lds + t % (ST + 1) * S::WStage, x_lds + t % ST * S::XStage, t + ST);
+        wait_copies<(ST - 1) * WG + (ST - 2) * XG>();  // (those for t + 2 and later may be in flight)
         __builtin_amdgcn_sched_barrier(0);
         __builtin_amdgcn_s_barrier();
         __builtin_amdgcn_sched_barrier(0);
-        const uint32_t wt = w_lds + (t + 1) % 3 * kTileStage, xt = x_lds + (t + 1) % 2 * kTileStage;
-#define HALF1(i)                                                          \
-    TILE_PAIR(1, i);                                                      \
-    TILE_READ(0, i, wt, xt);                                              \
-    if ((i) % 2 == 0) copy_x(t + 2, (i) / 2);                             \
-    __builtin_amdgcn_sched_barrier(0);
-        TILE_ALL(HALF1)
-        fragments_done(fw[0], fx[0]);
+        half(One{}, w_lds + (t + 1) % (ST + 1) * S::WStage, x_lds + (t + 1) % ST * S::XStage, t + ST);
     }
     wait_copies<0>();  // (LDS is not given back with copies on their way)
-#undef FIRST
-#undef HALF0
-#undef HALF1
-#undef TILE_ALL
-#undef TILE_PAIR
-#undef TILE_READ
     // A lane's results are of one row of W (l % 32) for each of r and of the rows 8 e + 4 (l / 32) .. + 3 of X for each of c
     // and e, so that half a wave stores 128 bytes in a row. (As 32 bytes of each of 32 rows, scales read between the
     // stores, a tile's end took 20 us.) All scales are read before the first store: stores count among the loads.
-    const uint32_t n = n0 + wn * 128 + lane % 32, m = m0 + wm * 128 + lane / 32 * 4;
-    float w_scale[4], bias[4], x_scale[4][16];
+    const uint32_t n = n0 + wn * (32 * RN) + lane % 32, m = m0 + wm * (32 * RM) + lane / 32 * 4;
+    // Y (or the part's sums) from this tile on: rows behind M are behind the buffer's end, columns behind N are sent there.
+    // What differs between a lane's results is the same for all lanes, so that a store takes no address arithmetic of its
+    // own (with it, and a branch for each row, the end of a tile of 256 x 256 took 9 us more).
+    const uint32_t rows = min(a.M - m0, S::M + 0u), pitch = SPLIT ? a.N * 4 : static_cast<uint32_t>(a.ldy) * 4;
+    void* const out = SPLIT ? static_cast<void*>(a.parts + (static_cast<size_t>(blockIdx.y) * a.M + m0) * a.N + n0) : a.Y + m0 * a.ldy + n0;
+    const __amdgpu_buffer_rsrc_t Y = __builtin_amdgcn_make_buffer_rsrc(out, 0, (rows - 1) * pitch + min(a.N - n0, S::N + 0u) * 4, 0x20000);
+    const __amdgpu_buffer_rsrc_t x_scales = __builtin_amdgcn_make_buffer_rsrc(const_cast<float*>(a.x_scales) + m0, 0, rows * 4, 0x20000);
+    float w_scale[RN], bias[RN];
+    f32x4 x_scale[RM][4];
+    uint32_t y_at[RN];
 #pragma unroll
-    for (int r = 0; r < 4; ++r) {
-        const uint32_t at = min(n + r * 32, a.N - 1);
-        w_scale[r] = a.w_scales[at], bias[r] = bias_at(a.bias, at);
+    for (int r = 0; r < RN; ++r) {
+        const uint32_t row = min(n + r * 32, a.N - 1);
+        y_at[r] = n + r * 32 < a.N ? (m - m0) * pitch + (n - n0 + r * 32) * 4 : kBufferBytes;
+        if constexpr (!SPLIT) w_scale[r] = a.w_scales[row], bias[r] = bias_at(a.bias, row);
+    }
+    if constexpr (!SPLIT) {
+#pragma unroll
+        for (int c = 0; c < RM; ++c)
+#pragma unroll
+            for (int q = 0; q < 4; ++q)
+                x_scale[c][q] = __builtin_bit_cast(f32x4, __builtin_amdgcn_raw_buffer_load_b128(x_scales, (m - m0 + c * 32 + q * 8) * 4, 0, 0));
     }
 #pragma unroll
-    for (int c = 0; c < 4; ++c)
-#pragma unroll
-        for (int e = 0; e < 16; ++e) x_scale[c][e] = a.x_scales[min(m + c * 32 + e / 4 * 8 + e % 4, a.M - 1)];
-#pragma unroll
-    for (int c = 0; c < 4; ++c)
+    for (int c = 0; c < RM; ++c)
 #pragma unroll
         for (int e = 0; e < 16; ++e) {
-            const uint32_t row = m + c * 32 + e / 4 * 8 + e % 4;
-            if (row >= a.M) continue;
-            float* y = a.Y + row * a.ldy + n;
+            const uint32_t down = (c * 32 + e / 4 * 8 + e % 4) * pitch;
 #pragma unroll
-            for (int r = 0; r < 4; ++r)
-                if (n + r * 32 < a.N) y[r * 32] = finish(sum[r][c][e], x_scale[c][e], w_scale[r], bias[r]);
+            for (int r = 0; r < RN; ++r) {
+                uint32_t value = sum[r][c][e];
+                if constexpr (!SPLIT) value = __float_as_uint(finish(sum[r][c][e], x_scale[c][e / 4][e % 4], w_scale[r], bias[r]));
+                __builtin_amdgcn_raw_buffer_store_b32(value, Y, y_at[r], down, 0);
+            }
         }
 }
 
+// Adds the parts of a split K and finishes them, four results of a row of Y a thread.
+__global__ __launch_bounds__(256) void linear_i8_join_kernel(LinearI8Args a, uint32_t splits) {
+    const uint32_t quads = (a.N + 3) / 4;
+    const size_t size = static_cast<size_t>(a.M) * a.N;
+    for (uint32_t i = blockIdx.x * 256 + threadIdx.x; i < quads * a.M; i += gridDim.x * 256) {
+        const uint32_t m = i / quads, n = i % quads * 4;
+        const int* p = a.parts + static_cast<size_t>(m) * a.N + n;
+        i32x4 v = {0, 0, 0, 0};
+        if (a.N % 4 == 0) {
+            for (uint32_t z = 0; z < splits; ++z) v += *reinterpret_cast<const i32x4*>(p + z * size);
+        } else {
+            for (uint32_t z = 0; z < splits; ++z)
+                for (int j = 0; j < 4; ++j)
+                    if (n + j < a.N) v[j] += p[z * size + j];
+        }
+        store4(a, m, n, v);
+    }
+}
+
+template <int RN, int RM, int ST>
 hipError_t launch_tile(const LinearI8Args& a, hipStream_t s) {
-    const uint64_t tiles = ((uint64_t{a.N} + kTile - 1) / kTile) * ((uint64_t{a.M} + kTile - 1) / kTile);
-    static const hipError_t ready = hipFuncSetAttribute(reinterpret_cast<const void*>(linear_i8_tile_kernel),
-                                                        hipFuncAttributeMaxDynamicSharedMemorySize, kTileLds);
+    using S = TileShape<RN, RM, ST>;
+    const uint64_t tiles = ((uint64_t{a.N} + S::N - 1) / S::N) * ((uint64_t{a.M} + S::M - 1) / S::M);
+    static const hipError_t ready = hipFuncSetAttribute(reinterpret_cast<const void*>(linear_i8_tile_kernel<RN, RM, ST, false>),
+                                                        hipFuncAttributeMaxDynamicSharedMemorySize, S::Lds);
     if (ready != hipSuccess) return ready;
-    return vlaunch(linear_i8_tile_kernel, dim3(static_cast<uint32_t>(tiles)), dim3(kTileThreads), kTileLds, s, a);
+    return vlaunch(linear_i8_tile_kernel<RN, RM, ST, false>, dim3(static_cast<uint32_t>(tiles)), dim3(kTileThreads), S::Lds, s, a);
+}
+// K in `splits` parts (at most; each has steps), their sums in the workspace.
+template <int RN, int RM, int ST>
+hipError_t launch_tile_split(LinearI8Args a, uint32_t splits, hipStream_t s) {
+    using S = TileShape<RN, RM, ST>;
+    const uint32_t tiles = ((a.N + S::N - 1) / S::N) * ((a.M + S::M - 1) / S::M), steps = (a.K + 127) / 128;
+    static const hipError_t ready = hipFuncSetAttribute(reinterpret_cast<const void*>(linear_i8_tile_kernel<RN, RM, ST, true>),
+                                                        hipFuncAttributeMaxDynamicSharedMemorySize, S::Lds);
+    if (ready != hipSuccess) return ready;
+    a.split_steps = (steps + splits - 1) / splits;
+    splits = (steps + a.split_steps - 1) / a.split_steps;
+    const hipError_t e = vlaunch(linear_i8_tile_kernel<RN, RM, ST, true>, dim3(tiles, splits), dim3(kTileThreads), S::Lds, s, a);
+    if (e != hipSuccess) return e;
+    const uint32_t quads = (a.N + 3) / 4 * a.M;
+    return vlaunch(linear_i8_join_kernel, dim3(std::min((quads + 255) / 256, 2048u)), dim3(256), 0, s, a, splits);
 }
 
 hipError_t launch_linear(const LinearI8Args& a, hipStream_t s) {
     const uint64_t stride = std::max(a.ldw, a.ldx);
-    if (a.M >= 256 && stride * kTile <= kTileBytes / 2) return launch_tile(a, s);
+    if (a.M >= 256 && std::max(stride, a.ldy * 4) * 256 <= kBufferBytes / 2) return launch_tile<4, 4, 2>(a, s);
     if (a.M <= 8) return launch_stream<1, 1, 4, 4>(a, s);
     if (a.M <= 16) return launch_stream<1, 2, 4, 4>(a, s);
     if (a.M <= 32) return launch_stream<2, 4, 3, 4>(a, s);
@@ -390,7 +468,7 @@ bool sizes_ok(uint32_t M, uint32_t N, uint32_t K) {
 
 extern "C" {
 
-size_t vvli_gpu_linear_i8_workspace(uint32_t M, uint32_t N, uint32_t K) { return sizes_ok(M, N, K) ? 16 : 0; }
+size_t vvli_gpu_linear_i8_workspace(uint32_t M, uint32_t N, uint32_t K) { return sizes_ok(M, N, K) ? size_t{64} << 20 : 0; }
 
 int vvli_gpu_linear_i8(const int8_t* W, uint64_t ldw, const float* w_scales, const int8_t* X, uint64_t ldx,
                        const float* x_scales, const uint16_t* bias, float* Y, uint64_t ldy, uint32_t M, uint32_t N,
@@ -414,6 +492,7 @@ int vvli_gpu_linear_i8(const int8_t* W, uint64_t ldw, const float* w_scales, con
     LinearI8Args a{};
     a.W = W, a.X = X, a.w_scales = w_scales, a.x_scales = x_scales, a.bias = bias, a.Y = Y;
     a.ldw = ldw, a.ldx = ldx, a.ldy = ldy, a.M = M, a.N = N, a.K = K;
+    a.parts = static_cast<int*>(workspace);
     a.vector = aligned16(Y) && ldy % 4 == 0 && aligned16(w_scales);
     const hipStream_t st = static_cast<hipStream_t>(stream);
     PAGED_TRY(launch_linear(a, st));

@@ -619,16 +619,15 @@ int vvli_gpu_silu_mul(const float* gate, uint64_t ldg, const float* up, uint64_t
  * of N f32 (ldy >= N, any alignment of f32). W and X at 16-byte addresses,
  * their strides and K multiples of 16, K <= 131056 (so that no sum leaves 32
  * bits, whatever the codes, -128 too). M = 0 is no error.
- * workspace: at least vvli_gpu_linear_i8_workspace bytes, at a 16-byte
- * address, zeroed once, when it is allocated (a call leaves its counters
- * zeroed). It belongs to one call at a time, so calls or replays that may
- * overlap need one each, and to this op alone; it serves calls of any sizes up
- * to its own. */
+ * workspace: at least vvli_gpu_linear_i8_workspace bytes, at a 16-byte address
+ * (NULL where that is 0). What it holds means nothing between calls. It belongs
+ * to one call at a time, so calls or replays that may overlap need one each; it
+ * serves calls of any sizes up to its own. */
 int vvli_gpu_linear_i8(const int8_t* W, uint64_t ldw, const float* w_scales, const int8_t* X, uint64_t ldx,
                        const float* x_scales, const uint16_t* bias, float* Y, uint64_t ldy, uint32_t M, uint32_t N,
                        uint32_t K, void* workspace, size_t workspace_bytes, void* stream);
-/* Bytes of workspace that calls of up to M rows with these N and K need; 0 for
- * sizes that a call refuses. */
+/* Bytes of workspace that calls of up to M rows with up to these N and K need
+ * (0 for few rows, which need none, and for sizes that a call refuses). */
 size_t vvli_gpu_linear_i8_workspace(uint32_t M, uint32_t N, uint32_t K);
 
 #ifdef __cplusplus

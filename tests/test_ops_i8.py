@@ -43,7 +43,7 @@ def gate(**kw):
 
 
 def linear(**kw):
-    a = dict(W=P, ldw=64, w_scales=Q, X=S, ldx=64, x_scales=T, bias=None, Y=U, ldy=40, M=5, N=40, K=64, workspace=2 * U,
+    a = dict(W=P, ldw=1024, w_scales=Q, X=S, ldx=1024, x_scales=T, bias=None, Y=U, ldy=40, M=50, N=40, K=1024, workspace=2 * U,
              workspace_bytes=1 << 30)
     a.update(kw)
     R.linear_i8(**a)
@@ -103,7 +103,7 @@ def test_silu_mul_refusals(bad, name):
 @pytest.mark.parametrize("bad,name", [
     (dict(W=None), NULL), (dict(w_scales=None), NULL), (dict(X=None), NULL), (dict(x_scales=None), NULL), (dict(Y=None), NULL),
     (dict(workspace=None), NULL), (dict(N=0), CONFIG), (dict(K=0), CONFIG), (dict(K=56), CONFIG), (dict(M=1 << 31), CONFIG),
-    (dict(K=131072, ldw=131072, ldx=131072), CONFIG), (dict(K=80), CONFIG), (dict(ldw=72), CONFIG), (dict(ldx=48), CONFIG),
+    (dict(K=131072, ldw=131072, ldx=131072), CONFIG), (dict(K=1040), CONFIG), (dict(ldw=1032), CONFIG), (dict(ldx=1008), CONFIG),
     (dict(ldw=1 << 31), CONFIG), (dict(W=P + 8), CONFIG), (dict(X=S + 4), CONFIG), (dict(ldy=39), CONFIG), (dict(ldy=1 << 31), CONFIG),
     (dict(workspace=2 * U + 8), CONFIG), (dict(workspace_bytes=0), CONFIG), (dict(Y=P), CONFIG), (dict(Y=S + 64), CONFIG), (dict(Y=Q), CONFIG),
     (dict(Y=T), CONFIG), (dict(bias=U + 8), CONFIG), (dict(Y=2 * U + 4), CONFIG), (dict(N=1 << 31, ldy=1 << 31), CONFIG),
@@ -113,11 +113,78 @@ def test_linear_i8_refusals(bad, name):
 
 
 def test_linear_i8_workspace():
-    assert R.linear_i8_workspace(1, 16, 16) > 0
-    assert R.linear_i8_workspace(1, 0, 16) == R.linear_i8_workspace(1, 16, 24) == R.linear_i8_workspace(1, 16, 131072) == 0
-    for n, k in ((896, 4864), (2048, 2048), (40000, 16), (16, 131056)):
-        sizes = [R.linear_i8_workspace(m, n, k) for m in (1, 2, 5, 17, 64, 65, 300, 2000, 100000)]
-        assert sizes == sorted(sizes)  # up to M rows
+    assert R.linear_i8_workspace(1, 16, 16) == R.linear_i8_workspace(32, 16, 131056) == R.linear_i8_workspace(5000, 16, 512) == 0
+    assert R.linear_i8_workspace(300, 0, 4096) == R.linear_i8_workspace(300, 16, 4104) == R.linear_i8_workspace(300, 16, 131072) == 0
+    assert R.linear_i8_workspace(300, 16, 4096) > 0
+    ms, ns, ks = (1, 32, 33, 64, 65, 300, 2000, 100000), (1, 16, 896, 3584, 40000, 200000), (16, 1008, 1024, 4096, 131056)
+    for n in ns:  # it serves calls of any sizes up to its own
+        for k in ks:
+            sizes = [R.linear_i8_workspace(m, n, k) for m in ms]
+            assert sizes == sorted(sizes) and max(sizes) <= 64 << 20
+            assert all(R.linear_i8_workspace(m, n, k) <= R.linear_i8_workspace(m, 2 * n, k) for m in ms)
+    for m in ms:
+        sizes = [R.linear_i8_workspace(m, 896, k) for k in ks]
+        assert sizes == sorted(sizes)
+
+
+PLAN = """
+#include "linear_i8_plan.hpp"
+#include <cstdio>
+int main() {
+    unsigned long long m, n, k, ld;
+    unsigned cus;
+    while (scanf("%llu %llu %llu %llu %u", &m, &n, &k, &ld, &cus) == 5) {
+        const vvli::I8Plan p = vvli::i8_plan(m, n, k, ld, cus);
+        const vvli::I8Kernel& x = vvli::kI8Kernels[p.kernel];
+        printf("%u %u %llu %d %d %d %d %llu %u\\n", p.kernel, p.splits, (unsigned long long)p.blocks, (int)x.kind, x.r, x.m, x.split,
+               (unsigned long long)vvli::i8_part_bytes(m, n, k), vvli::kI8KernelCount);
+    }
+}
+"""
+
+
+@pytest.fixture(scope="module")
+def plan(tmp_path_factory):
+    if not shutil.which("g++"):
+        pytest.skip("no host compiler")
+    d = tmp_path_factory.mktemp("plan")
+    (d / "t.cpp").write_text(PLAN)
+    subprocess.run(["g++", "-std=c++17", "-O1", f"-I{ROOT / 'vvli_amd' / 'csrc'}", "-o", d / "t", d / "t.cpp"], check=True)
+
+    def ask(sizes):
+        text = "\n".join(" ".join(map(str, s)) for s in sizes)
+        out = subprocess.run([d / "t"], input=text, capture_output=True, text=True, check=True).stdout.split("\n")
+        return [tuple(map(int, line.split())) for line in out if line]
+
+    return ask
+
+
+def test_every_kernel_is_taken_somewhere(plan):
+    ms = [1, 2, 5, 8, 9, 16, 17, 24, 32, 33, 48, 64, 96, 128, 192, 256, 384, 512, 768, 1024, 1536, 2048, 4096]
+    shapes = [(1152, 896), (896, 4864), (9728, 896), (2048, 2048), (2048, 8192), (16384, 2048), (4608, 3584), (3584, 18944), (37888, 3584),
+              (128, 1024), (40, 131056), (128256, 2048)]
+    got = plan([(m, n, k, max(k, 4 * n), 256) for m in ms for n, k in shapes])
+    assert {g[0] for g in got} == set(range(got[0][8]))
+
+
+def test_plans_fit_their_calls(plan):
+    """Parts fit the workspace, parts have steps, tiles only where their buffers reach, few rows need nothing."""
+    rng = np.random.RandomState(1)
+    sizes = []
+    for _ in range(4000):
+        m, n = (int(np.exp(rng.uniform(0, np.log(200000)))) for _ in range(2))
+        k = 16 * int(np.exp(rng.uniform(0, np.log(8191))))
+        ld = max(k, 4 * n, int(np.exp(rng.uniform(0, np.log(2 ** 30)))))
+        sizes.append((m, n, k, ld, int(rng.choice([256, 64, 304]))))
+    for (m, n, k, ld, cus), (kernel, splits, blocks, kind, r, c, split, room, _) in zip(sizes, plan(sizes)):
+        assert blocks > 0 and (splits > 1) == bool(split)
+        if split:
+            assert splits * m * n * 4 <= room and k >= 512 * splits and m > 32
+        if kind == 1:
+            assert ld * 256 <= 1 << 30 and m > 32
+            assert blocks == splits * -(-n // (64 * r)) * -(-m // (64 * c))
+        else:
+            assert blocks == -(-(-(-n // (16 * r))) // 8) * 8 * -(-m // (8 * c))
 
 
 def test_no_rows_launch_nothing():

@@ -8,6 +8,7 @@
 #include <utility>
 
 #include "device_common.hpp"
+#include "linear_i8_plan.hpp"
 #include "rows_i8.hpp"
 
 using namespace vvli;
@@ -451,13 +452,35 @@ hipError_t launch_tile_split(LinearI8Args a, uint32_t splits, hipStream_t s) {
     return vlaunch(linear_i8_join_kernel, dim3(std::min((quads + 255) / 256, 2048u)), dim3(256), 0, s, a, splits);
 }
 
-hipError_t launch_linear(const LinearI8Args& a, hipStream_t s) {
-    const uint64_t stride = std::max(a.ldw, a.ldx);
-    if (a.M >= 256 && std::max(stride, a.ldy * 4) * 256 <= kBufferBytes / 2) return launch_tile<4, 4, 2>(a, s);
-    if (a.M <= 8) return launch_stream<1, 1, 4, 4>(a, s);
-    if (a.M <= 16) return launch_stream<1, 2, 4, 4>(a, s);
-    if (a.M <= 32) return launch_stream<2, 4, 3, 4>(a, s);
-    return launch_stream<2, 8, 2, 4>(a, s);
+template <uint32_t I>
+hipError_t launch_kernel(const LinearI8Args& a, const I8Plan& plan, hipStream_t s) {
+    constexpr I8Kernel k = kI8Kernels[I];
+    if constexpr (k.kind == kI8Stream) return launch_stream<k.r, k.m, k.stages, k.waves>(a, s);
+    else if constexpr (k.split) return launch_tile_split<k.r, k.m, k.stages>(a, plan.splits, s);
+    else return launch_tile<k.r, k.m, k.stages>(a, s);
+}
+template <uint32_t... I>
+hipError_t launch_plan(const LinearI8Args& a, const I8Plan& plan, hipStream_t s, std::integer_sequence<uint32_t, I...>) {
+    hipError_t e = hipErrorInvalidValue;
+    (void)((plan.kernel == I && (e = launch_kernel<I>(a, plan, s), true)) || ...);
+    return e;
+}
+
+hipError_t launch_linear(LinearI8Args a, hipStream_t s) {
+    const I8Plan plan = i8_plan(a.M, a.N, a.K, std::max(std::max(a.ldw, a.ldx), a.ldy * 4), gemm_cus());
+    if (plan.blocks * 512 < (uint64_t{1} << 32)) return launch_plan(a, plan, s, std::make_integer_sequence<uint32_t, kI8KernelCount>{});
+    // More threads than a launch takes: the longer side in halves.
+    LinearI8Args b = a;
+    if (a.M >= a.N) {
+        a.M = (a.M / 2 + 255) / 256 * 256, b.M -= a.M;
+        b.X += a.M * a.ldx, b.x_scales += a.M, b.Y += a.M * a.ldy;
+    } else {
+        a.N = (a.N / 2 + 255) / 256 * 256, b.N -= a.N;
+        b.W += a.N * a.ldw, b.w_scales += a.N, b.Y += a.N;
+        if (b.bias) b.bias += a.N;
+    }
+    const hipError_t e = launch_linear(a, s);
+    return e != hipSuccess ? e : launch_linear(b, s);
 }
 
 bool sizes_ok(uint32_t M, uint32_t N, uint32_t K) {
@@ -468,25 +491,27 @@ bool sizes_ok(uint32_t M, uint32_t N, uint32_t K) {
 
 extern "C" {
 
-size_t vvli_gpu_linear_i8_workspace(uint32_t M, uint32_t N, uint32_t K) { return sizes_ok(M, N, K) ? size_t{64} << 20 : 0; }
+size_t vvli_gpu_linear_i8_workspace(uint32_t M, uint32_t N, uint32_t K) { return sizes_ok(M, N, K) ? i8_part_bytes(M, N, K) : 0; }
 
 int vvli_gpu_linear_i8(const int8_t* W, uint64_t ldw, const float* w_scales, const int8_t* X, uint64_t ldx,
                        const float* x_scales, const uint16_t* bias, float* Y, uint64_t ldy, uint32_t M, uint32_t N,
                        uint32_t K, void* workspace, size_t workspace_bytes, void* stream) {
     const char* who = "vvli_gpu_linear_i8";
-    if (!W || !w_scales || !X || !x_scales || !Y || !workspace) return set_error(VVLI_NULL_ARG, "NULL argument to %s", who);
+    if (!W || !w_scales || !X || !x_scales || !Y) return set_error(VVLI_NULL_ARG, "NULL argument to %s", who);
     if (!sizes_ok(M, N, K))
         return set_error(VVLI_INVALID_CONFIG, "%s: bad sizes M=%u N=%u K=%u (K: whole 16s up to %u)", who, M, N, K, kMostK);
     int rc;
     if ((rc = check_row_units(W, ldw, K, 1, "W", who)) || (rc = check_row_units(X, ldx, K, 1, "X", who))) return rc;
     if (ldy < N || ldy >= kPagedMost)
         return set_error(VVLI_INVALID_CONFIG, "%s: rows of Y of %u (stride %llu)", who, N, static_cast<unsigned long long>(ldy));
-    if (!aligned16(workspace) || workspace_bytes < vvli_gpu_linear_i8_workspace(M, N, K))
+    const size_t need = vvli_gpu_linear_i8_workspace(M, N, K);
+    if (need && !workspace) return set_error(VVLI_NULL_ARG, "%s: NULL workspace", who);
+    if (need && (!aligned16(workspace) || workspace_bytes < need))
         return set_error(VVLI_INVALID_CONFIG, "%s: workspace of %zu bytes", who, workspace_bytes);
     const RowBytes y{Y, ldy * 4, uint64_t{N} * 4, M};
     if (rows_meet(y, RowBytes{W, ldw, K, N}) || rows_meet(y, RowBytes{X, ldx, K, M}) || rows_meet(y, RowBytes{w_scales, 4, 4, N}) ||
         rows_meet(y, RowBytes{x_scales, 4, 4, M}) || rows_meet(y, RowBytes{bias, 2, 2, N}) ||
-        rows_meet(y, RowBytes{workspace, workspace_bytes, workspace_bytes, 1}))
+        rows_meet(y, RowBytes{workspace, need, need, 1}))
         return set_error(VVLI_INVALID_CONFIG, "%s: Y overlaps another argument", who);
     if (M == 0) return VVLI_OK;
     LinearI8Args a{};

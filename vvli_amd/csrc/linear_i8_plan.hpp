@@ -1,0 +1,114 @@
+// linear_i8_plan.hpp -- which kernel a product of 8-bit codes takes: host
+// arithmetic on its sizes.
+#pragma once
+
+#include <stdint.h>
+
+namespace vvli {
+
+enum I8Kind { kI8Stream, kI8Tile };
+
+// A kernel, and what a call of it takes, in us:
+//   base + turn * turns + round * rounds * work + fill * blocks / CUs * work + w * (W in MB) + y * (Y in MB) + part * (parts in MB)
+// rounds: blocks that a CU gets. Streams: work is what a block copies, in units of
+// 1024 copies, turns the chunks that a wave takes one after the other. Tiles: work
+// is the steps of a block, turns the rounds.
+//
+// The numbers are fits (nonnegative, of relative errors; 2 to 17 % rms) to 223
+// sizes, M = 1 to 4096 with (N, K) of nine projections, W in no cache. Choosing by
+// them costs 1.4 % over the fastest of some hundred measured variants on the
+// geometric mean, 18 % where it costs most (48 x 2048 x 8192: 10.3 us, four groups
+// of X 8.8).
+struct I8Kernel {
+    I8Kind kind;
+    uint8_t r, m, stages, waves;  // stream: tiles of 16 rows of W, groups of 8 of X; tile: 64s of rows of either
+    bool split;                   // tile: K in parts
+    float base, turn, round, fill, w, y, part;
+};
+constexpr I8Kernel kI8Kernels[] = {
+    {kI8Stream, 1, 1, 2, 8, false, 3.24f, 0.f, 9.84f, 6.50f, 0.0471f, 0.f, 0.f},
+    {kI8Stream, 1, 2, 2, 8, false, 3.34f, 0.f, 7.81f, 10.8f, 0.0195f, 0.f, 0.f},
+    {kI8Stream, 1, 4, 2, 8, false, 3.27f, 0.416f, 0.f, 10.5f, 0.0273f, 0.f, 0.f},
+    {kI8Stream, 1, 8, 2, 8, false, 3.39f, 0.756f, 0.f, 8.38f, 0.0136f, 0.f, 0.f},
+    {kI8Stream, 2, 1, 2, 4, false, 3.03f, 0.0782f, 13.6f, 0.f, 0.0583f, 0.f, 0.f},
+    {kI8Stream, 2, 2, 2, 4, false, 3.03f, 0.0531f, 14.0f, 1.98f, 0.0382f, 0.f, 0.f},
+    {kI8Stream, 2, 4, 2, 4, false, 3.16f, 0.f, 14.2f, 4.11f, 0.0197f, 0.f, 0.f},
+    {kI8Stream, 2, 8, 1, 8, false, 3.46f, 1.11f, 0.f, 6.36f, 0.0534f, 0.f, 0.f},
+    {kI8Tile, 1, 1, 4, 4, false, 3.08f, 0.11f, 0.209f, 0.f, 0.0836f, 0.182f, 0.f},
+    {kI8Tile, 2, 1, 3, 4, false, 1.71f, 1.55f, 0.287f, 0.0791f, 0.1f, 0.0759f, 0.f},
+    {kI8Tile, 2, 2, 2, 4, false, 4.13f, 0.765f, 0.202f, 0.258f, 0.0964f, 0.137f, 0.f},
+    {kI8Tile, 2, 2, 4, 4, false, 0.f, 3.96f, 0.341f, 0.26f, 0.0685f, 0.0889f, 0.f},
+    {kI8Tile, 4, 2, 2, 4, false, 3.68f, 0.699f, 0.616f, 0.258f, 0.0666f, 0.2f, 0.f},
+    {kI8Tile, 4, 4, 2, 4, false, 2.02f, 6.84f, 0.979f, 0.372f, 0.0231f, 0.143f, 0.f},
+    {kI8Tile, 1, 1, 4, 4, true, 6.9f, 0.0599f, 0.167f, 0.00552f, 0.0902f, 0.f, 0.423f},
+    {kI8Tile, 2, 2, 2, 4, true, 7.34f, 0.f, 0.363f, 0.161f, 0.0699f, 0.0576f, 0.27f},
+    {kI8Tile, 4, 4, 2, 4, true, 9.29f, 1.79f, 0.879f, 0.374f, 0.0377f, 0.131f, 0.27f},
+};
+constexpr uint32_t kI8KernelCount = sizeof(kI8Kernels) / sizeof(kI8Kernels[0]);
+
+constexpr uint32_t kI8MostSplits = 8, kI8SplitCodes = 512, kI8SplitTiles = 128;  // parts of K, codes of a part at least, tiles at most
+constexpr uint64_t kI8PartBytes = uint64_t{64} << 20;                           // of all parts together
+constexpr uint64_t kI8TileBytes = uint64_t{1} << 30;                            // 256 rows of W, X or Y for a tile kernel
+
+// Bytes of parts that calls of up to M rows may take (it does not fall where M, N or K grow).
+inline uint64_t i8_part_bytes(uint64_t M, uint64_t N, uint64_t K) {
+    if (M <= 32 || K < 2 * kI8SplitCodes) return 0;
+    return M * N >= kI8PartBytes / 4 / kI8MostSplits ? kI8PartBytes : M * N * 4 * kI8MostSplits;
+}
+
+struct I8Plan {
+    uint32_t kernel, splits;  // of kI8Kernels
+    uint64_t blocks;
+};
+
+inline uint64_t i8_up(uint64_t n, uint64_t d) { return (n + d - 1) / d; }
+
+// Blocks of a call without a split.
+inline uint64_t i8_blocks(const I8Kernel& k, uint64_t M, uint64_t N) {
+    return k.kind == kI8Stream ? i8_up(i8_up(N, 16 * k.r), 8) * 8 * i8_up(M, 8 * k.m) : i8_up(N, 64 * k.r) * i8_up(M, 64 * k.m);
+}
+
+inline double i8_time(const I8Kernel& k, uint64_t M, uint64_t N, uint64_t K, uint64_t splits, uint32_t cus) {
+    const uint64_t steps = i8_up(K, 128);
+    const double w = static_cast<double>(N) * K / 1e6, y = 4.0 * M * N / 1e6;
+    if (k.kind == kI8Stream) {
+        const uint64_t blocks = i8_up(N, 16 * k.r) * i8_up(M, 8 * k.m), copies = 2 * k.r + k.m;
+        const uint64_t fit = 160 / (k.waves * k.stages * copies);  // of a CU's LDS
+        const double work = static_cast<double>(copies) * steps / 1024.0;
+        return k.base + k.turn * i8_up(blocks, cus * (fit ? fit : 1)) * i8_up(steps, k.waves) + k.round * i8_up(blocks, cus) * work +
+               k.fill * work * blocks / cus + k.w * w + k.y * y;
+    }
+    const uint64_t blocks = i8_blocks(k, M, N) * splits, work = i8_up(steps, splits), rounds = i8_up(blocks, cus);
+    return k.base + k.turn * rounds + k.round * rounds * work + k.fill * static_cast<double>(blocks) * work / cus + k.w * w + k.y * y +
+           k.part * splits * y;
+}
+
+// Whether k takes the call at all: streams hold whatever they are given, but are slow from a few groups of X on; tiles are
+// for more rows than a stream's group, and their rows have to fit a buffer's 32-bit offsets (ld: of W, X, Y in bytes, the
+// largest).
+inline bool i8_takes(const I8Kernel& k, uint64_t M, uint64_t N, uint64_t K, uint64_t ld, uint32_t cus) {
+    const bool tiles = M > 32 && ld * 256 <= kI8TileBytes;
+    if (k.kind == kI8Stream) return !tiles ? k.m == (M <= 8 ? 1 : M <= 16 ? 2 : M <= 32 ? 4 : 8) || (M <= 32 && M > 8u * k.m && M <= 32u * k.m) : i8_up(M, 8 * k.m) <= (k.m == 1 ? 4u : 8u);
+    if (!tiles) return false;
+    const uint64_t blocks = i8_blocks(k, M, N);
+    if (k.split) return blocks <= kI8SplitTiles && K >= 2 * kI8SplitCodes;
+    // 128 x 128: two blocks of a CU where there are as many, else deeper stages.
+    return !(k.r == 2 && k.m == 2) || (blocks <= cus) == (k.stages == 4);
+}
+
+inline I8Plan i8_plan(uint64_t M, uint64_t N, uint64_t K, uint64_t ld, uint32_t cus) {
+    I8Plan best{0, 1, 0};
+    double least = 0;
+    for (uint32_t i = 0; i < kI8KernelCount; ++i) {
+        const I8Kernel& k = kI8Kernels[i];
+        if (!i8_takes(k, M, N, K, ld, cus)) continue;
+        for (uint64_t s = k.split ? 2 : 1; s <= (k.split ? kI8MostSplits : 1); ++s) {
+            if (k.split && (K < s * kI8SplitCodes || s * M * N * 4 > kI8PartBytes)) break;
+            const double t = i8_time(k, M, N, K, s, cus);
+            if (best.blocks == 0 || t < least) least = t, best = I8Plan{i, static_cast<uint32_t>(s), i8_blocks(k, M, N) * s};
+        }
+    }
+    return best;
+}
+
+}  // namespace vvli

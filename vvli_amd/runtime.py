@@ -524,7 +524,7 @@ def silu_mul(gate: int, ldg: int, up: int, ldu: int, rows: int, width: int, code
 
 
 def linear_i8_workspace(M: int, N: int, K: int) -> int:
-    """Bytes of workspace (zeroed once) of ``linear_i8`` calls of up to M rows with these N and K."""
+    """Bytes of workspace of ``linear_i8`` calls of up to M rows with up to these N and K (0: none)."""
     return _lib.lib().vvli_gpu_linear_i8_workspace(M, N, K)
 
 

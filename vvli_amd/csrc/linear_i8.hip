@@ -4,6 +4,7 @@
 //
 // The sums are exact in 32 bits, so no split or order of them changes a result.
 #include <algorithm>
+#include <atomic>
 #include <type_traits>
 #include <utility>
 
@@ -192,14 +193,26 @@ __global__ __launch_bounds__(WV * 64) void linear_i8_stream_kernel(LinearI8Args 
     }
 }
 
+// Lets a kernel have `bytes` of dynamic LDS, once on each device.
+hipError_t allow_lds(const void* kernel, int bytes, std::atomic<uint64_t>& done) {
+    int device = 0;
+    hipError_t e = hipGetDevice(&device);
+    if (e != hipSuccess) return e;
+    const uint64_t bit = uint64_t{1} << (device & 63);
+    if (done.load(std::memory_order_relaxed) & bit) return hipSuccess;
+    e = hipFuncSetAttribute(kernel, hipFuncAttributeMaxDynamicSharedMemorySize, bytes);
+    if (e == hipSuccess) done.fetch_or(bit, std::memory_order_relaxed);
+    return e;
+}
+
 template <int R, int XG, int ST, int WV>
 hipError_t launch_stream(const LinearI8Args& a, hipStream_t s) {
     constexpr int MT = (XG + 1) / 2, LDS = WV * ST * (2 * R + XG) * 1024;
     static_assert(LDS <= 160 * 1024 && R * MT <= ST * (2 * R + XG) && ST <= 4, "stages, sums and waits fit");
     const uint64_t tn = (uint64_t{a.N} + 16 * R - 1) / (16 * R), tm = (uint64_t{a.M} + 8 * XG - 1) / (8 * XG);
-    static const hipError_t ready = hipFuncSetAttribute(reinterpret_cast<const void*>(linear_i8_stream_kernel<R, XG, ST, WV>),
-                                                        hipFuncAttributeMaxDynamicSharedMemorySize, LDS);
-    if (ready != hipSuccess) return ready;
+    static std::atomic<uint64_t> ready{0};
+    const hipError_t set = allow_lds(reinterpret_cast<const void*>(linear_i8_stream_kernel<R, XG, ST, WV>), LDS, ready);
+    if (set != hipSuccess) return set;
     return vlaunch(linear_i8_stream_kernel<R, XG, ST, WV>, dim3(static_cast<uint32_t>((tn + 7) / 8 * 8 * tm)), dim3(WV * 64), LDS, s, a);
 }
 
@@ -431,9 +444,9 @@ template <int RN, int RM, int ST>
 hipError_t launch_tile(const LinearI8Args& a, hipStream_t s) {
     using S = TileShape<RN, RM, ST>;
     const uint64_t tiles = ((uint64_t{a.N} + S::N - 1) / S::N) * ((uint64_t{a.M} + S::M - 1) / S::M);
-    static const hipError_t ready = hipFuncSetAttribute(reinterpret_cast<const void*>(linear_i8_tile_kernel<RN, RM, ST, false>),
-                                                        hipFuncAttributeMaxDynamicSharedMemorySize, S::Lds);
-    if (ready != hipSuccess) return ready;
+    static std::atomic<uint64_t> ready{0};
+    const hipError_t set = allow_lds(reinterpret_cast<const void*>(linear_i8_tile_kernel<RN, RM, ST, false>), S::Lds, ready);
+    if (set != hipSuccess) return set;
     return vlaunch(linear_i8_tile_kernel<RN, RM, ST, false>, dim3(static_cast<uint32_t>(tiles)), dim3(kTileThreads), S::Lds, s, a);
 }
 // K in `splits` parts (at most; each has steps), their sums in the workspace.
@@ -441,9 +454,9 @@ template <int RN, int RM, int ST>
 hipError_t launch_tile_split(LinearI8Args a, uint32_t splits, hipStream_t s) {
     using S = TileShape<RN, RM, ST>;
     const uint32_t tiles = ((a.N + S::N - 1) / S::N) * ((a.M + S::M - 1) / S::M), steps = (a.K + 127) / 128;
-    static const hipError_t ready = hipFuncSetAttribute(reinterpret_cast<const void*>(linear_i8_tile_kernel<RN, RM, ST, true>),
-                                                        hipFuncAttributeMaxDynamicSharedMemorySize, S::Lds);
-    if (ready != hipSuccess) return ready;
+    static std::atomic<uint64_t> ready{0};
+    const hipError_t set = allow_lds(reinterpret_cast<const void*>(linear_i8_tile_kernel<RN, RM, ST, true>), S::Lds, ready);
+    if (set != hipSuccess) return set;
     a.split_steps = (steps + splits - 1) / splits;
     splits = (steps + a.split_steps - 1) / a.split_steps;
     const hipError_t e = vlaunch(linear_i8_tile_kernel<RN, RM, ST, true>, dim3(tiles, splits), dim3(kTileThreads), S::Lds, s, a);

@@ -17,8 +17,8 @@ with n <= 70000 under 2^-36 relative, so that
 """
 import numpy as np
 import pytest
+from test_ops_i8 import ODD
 
-from vvli_amd import config as C
 from vvli_amd import runtime as R
 
 pytestmark = pytest.mark.gpu
@@ -371,6 +371,15 @@ def test_linear_i8_large(torch, M, N, K):
     p = Product(torch, M, N, K, bias=N % 3 == 0, seed=1)
     p.run()
     p.check()
+
+
+@pytest.mark.parametrize("M,N,K", ODD)
+def test_linear_i8_every_kernel(torch, M, N, K):
+    for pad in ((0, 0, 0), (1, 3, 5)):
+        p = Product(torch, M, N, K, True, *pad, seed=2)
+        for _ in range(2):
+            p.run()
+            p.check()
 
 
 @pytest.mark.parametrize("M", [1, 5, 20, 70, 300])

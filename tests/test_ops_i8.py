@@ -159,6 +159,20 @@ def plan(tmp_path_factory):
     return ask
 
 
+# (M, N, K) of two calls for each kernel: odd sizes, K that ends inside a step, an odd number of tiles.
+ODD = [(1, 33, 432), (5, 413, 2672), (35, 39, 624), (109, 365, 1120), (153, 43, 752), (161, 189, 3904), (1, 24713, 16),
+       (1, 29723, 912), (1, 31, 16), (65, 169, 48), (173, 95, 16), (67, 32037, 16), (441, 41, 848), (209, 1751, 992),
+       (261, 41, 480), (217, 725, 832), (323, 5905, 16), (129, 2383, 1936), (263, 43, 288), (861, 475, 832),
+       (33, 24827, 16), (55, 32197, 208), (857, 9191, 16), (1371, 3365, 2800), (145, 41, 16), (311, 1461, 32),
+       (461, 14459, 144), (295, 18253, 928), (189, 39433, 656), (395, 18565, 2480), (61, 33, 18576), (311, 401, 6768),
+       (3017, 75, 10976), (687, 875, 14512), (181, 5555, 10272), (623, 3541, 16112)]
+
+
+def test_odd_sizes_reach_every_kernel(plan):
+    got = plan([(m, n, k, max(k, 4 * n), 256) for m, n, k in ODD])
+    assert {g[0] for g in got} == set(range(got[0][8]))
+
+
 def test_every_kernel_is_taken_somewhere(plan):
     ms = [1, 2, 5, 8, 9, 16, 17, 24, 32, 33, 48, 64, 96, 128, 192, 256, 384, 512, 768, 1024, 1536, 2048, 4096]
     shapes = [(1152, 896), (896, 4864), (9728, 896), (2048, 2048), (2048, 8192), (16384, 2048), (4608, 3584), (3584, 18944), (37888, 3584),

@@ -80,7 +80,7 @@ __device__ __forceinline__ void wait_copies() {
 // block: nothing can come between the reads and it.
 template <int R, int MT>
 __device__ __forceinline__ void read_fragments(i32x4 (&w)[R], i32x4 (&x)[MT], uint32_t wa, uint32_t xa) {
-    static_assert((R == 1 || R == 2 || R == 4) && (MT == 1 || MT == 2 || MT == 4), "as written");
+    static_assert((R == 1 || R == 2) && (MT >= 1 && MT <= 4), "as written");
 #define LDS_W(i, at) "ds_read_b128 %" #i ", %[wa] offset:" #at "\n\t"
 #define LDS_X(i, at) "ds_read_b128 %" #i ", %[xa] offset:" #at "\n\t"
 #define LDS_END "s_waitcnt lgkmcnt(0)"
@@ -100,15 +100,12 @@ __device__ __forceinline__ void read_fragments(i32x4 (&w)[R], i32x4 (&x)[MT], ui
     if constexpr (R == 2 && MT == 4)
         asm volatile(LDS_W(0, 0) LDS_W(1, 2048) LDS_X(2, 0) LDS_X(3, 2048) LDS_X(4, 4096) LDS_X(5, 6144) LDS_END
                      : "=&v"(w[0]), "=&v"(w[1]), "=&v"(x[0]), "=&v"(x[1]), "=&v"(x[2]), "=&v"(x[3]) LDS_IN);
-    if constexpr (R == 4 && MT == 1)
-        asm volatile(LDS_W(0, 0) LDS_W(1, 2048) LDS_W(2, 4096) LDS_W(3, 6144) LDS_X(4, 0) LDS_END
-                     : "=&v"(w[0]), "=&v"(w[1]), "=&v"(w[2]), "=&v"(w[3]), "=&v"(x[0]) LDS_IN);
-    if constexpr (R == 4 && MT == 2)
-        asm volatile(LDS_W(0, 0) LDS_W(1, 2048) LDS_W(2, 4096) LDS_W(3, 6144) LDS_X(4, 0) LDS_X(5, 2048) LDS_END
-                     : "=&v"(w[0]), "=&v"(w[1]), "=&v"(w[2]), "=&v"(w[3]), "=&v"(x[0]), "=&v"(x[1]) LDS_IN);
-    if constexpr (R == 4 && MT == 4)
-        asm volatile(LDS_W(0, 0) LDS_W(1, 2048) LDS_W(2, 4096) LDS_W(3, 6144) LDS_X(4, 0) LDS_X(5, 2048) LDS_X(6, 4096) LDS_X(7, 6144) LDS_END
-                     : "=&v"(w[0]), "=&v"(w[1]), "=&v"(w[2]), "=&v"(w[3]), "=&v"(x[0]), "=&v"(x[1]), "=&v"(x[2]), "=&v"(x[3]) LDS_IN);
+    if constexpr (R == 1 && MT == 3)
+        asm volatile(LDS_W(0, 0) LDS_X(1, 0) LDS_X(2, 2048) LDS_X(3, 4096) LDS_END
+                     : "=&v"(w[0]), "=&v"(x[0]), "=&v"(x[1]), "=&v"(x[2]) LDS_IN);
+    if constexpr (R == 2 && MT == 3)
+        asm volatile(LDS_W(0, 0) LDS_W(1, 2048) LDS_X(2, 0) LDS_X(3, 2048) LDS_X(4, 4096) LDS_END
+                     : "=&v"(w[0]), "=&v"(w[1]), "=&v"(x[0]), "=&v"(x[1]), "=&v"(x[2]) LDS_IN);
 #undef LDS_W
 #undef LDS_X
 #undef LDS_END
@@ -124,6 +121,7 @@ __device__ __forceinline__ void read_fragments(i32x4 (&w)[R], i32x4 (&x)[MT], ui
 // before the sums of all meet at the end.
 template <int R, int XG, int ST, int WV>
 __global__ __launch_bounds__(WV * 64) void linear_i8_stream_kernel(LinearI8Args a) {
+    static_assert(XG == 1 || XG % 2 == 0, "X tiles of 16 rows, or one of 8 twice over");
     constexpr int MT = (XG + 1) / 2, D = 2 * R + XG, STAGE = D * 1024;  // X tiles of 16 rows, copies and bytes of a stage
     extern __shared__ __attribute__((aligned(1024))) char stream_lds[];  // [WV][ST][W: R * 2 KiB | X: XG KiB]
     const uint32_t lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);

@@ -14,11 +14,11 @@ enum I8Kind { kI8Stream, kI8Tile };
 // 1024 copies, turns the chunks that a wave takes one after the other. Tiles: work
 // is the steps of a block, turns the rounds.
 //
-// The numbers are fits (nonnegative, of relative errors; 2 to 17 % rms) to 223
-// sizes, M = 1 to 4096 with (N, K) of nine projections, W in no cache. Choosing by
-// them costs 1.4 % over the fastest of some hundred measured variants on the
-// geometric mean, 18 % where it costs most (48 x 2048 x 8192: 10.3 us, four groups
-// of X 8.8).
+// The numbers are fits (nonnegative, of relative errors, sizes where the kernel is
+// near the fastest weighing most) to 286 sizes, M = 1 to 4096 with (N, K) of nine
+// projections, W in no cache. Choosing by them costs 1.0 % over the fastest of some
+// hundred measured variants on the geometric mean, 11 % where it costs most (768 x
+// 3584 x 18944: K in six parts 75 us, in four 67).
 struct I8Kernel {
     I8Kind kind;
     uint8_t r, m, stages, waves;  // stream: tiles of 16 rows of W, groups of 8 of X; tile: 64s of rows of either
@@ -26,23 +26,24 @@ struct I8Kernel {
     float base, turn, round, fill, w, y, part;
 };
 constexpr I8Kernel kI8Kernels[] = {
-    {kI8Stream, 1, 1, 2, 8, false, 3.24f, 0.f, 9.84f, 6.50f, 0.0471f, 0.f, 0.f},
-    {kI8Stream, 1, 2, 2, 8, false, 3.34f, 0.f, 7.81f, 10.8f, 0.0195f, 0.f, 0.f},
-    {kI8Stream, 1, 4, 2, 8, false, 3.27f, 0.416f, 0.f, 10.5f, 0.0273f, 0.f, 0.f},
-    {kI8Stream, 1, 8, 2, 8, false, 3.39f, 0.756f, 0.f, 8.38f, 0.0136f, 0.f, 0.f},
-    {kI8Stream, 2, 1, 2, 4, false, 3.03f, 0.0782f, 13.6f, 0.f, 0.0583f, 0.f, 0.f},
-    {kI8Stream, 2, 2, 2, 4, false, 3.03f, 0.0531f, 14.0f, 1.98f, 0.0382f, 0.f, 0.f},
-    {kI8Stream, 2, 4, 2, 4, false, 3.16f, 0.f, 14.2f, 4.11f, 0.0197f, 0.f, 0.f},
-    {kI8Stream, 2, 8, 1, 8, false, 3.46f, 1.11f, 0.f, 6.36f, 0.0534f, 0.f, 0.f},
-    {kI8Tile, 1, 1, 4, 4, false, 3.08f, 0.11f, 0.209f, 0.f, 0.0836f, 0.182f, 0.f},
-    {kI8Tile, 2, 1, 3, 4, false, 1.71f, 1.55f, 0.287f, 0.0791f, 0.1f, 0.0759f, 0.f},
-    {kI8Tile, 2, 2, 2, 4, false, 4.13f, 0.765f, 0.202f, 0.258f, 0.0964f, 0.137f, 0.f},
-    {kI8Tile, 2, 2, 4, 4, false, 0.f, 3.96f, 0.341f, 0.26f, 0.0685f, 0.0889f, 0.f},
-    {kI8Tile, 4, 2, 2, 4, false, 3.68f, 0.699f, 0.616f, 0.258f, 0.0666f, 0.2f, 0.f},
-    {kI8Tile, 4, 4, 2, 4, false, 2.02f, 6.84f, 0.979f, 0.372f, 0.0231f, 0.143f, 0.f},
-    {kI8Tile, 1, 1, 4, 4, true, 6.9f, 0.0599f, 0.167f, 0.00552f, 0.0902f, 0.f, 0.423f},
-    {kI8Tile, 2, 2, 2, 4, true, 7.34f, 0.f, 0.363f, 0.161f, 0.0699f, 0.0576f, 0.27f},
-    {kI8Tile, 4, 4, 2, 4, true, 9.29f, 1.79f, 0.879f, 0.374f, 0.0377f, 0.131f, 0.27f},
+    {kI8Stream, 1, 1, 2, 8, false, 3.28f, 0.f, 10.8f, 0.607f, 0.0681f, 0.f, 0.f},
+    {kI8Stream, 1, 2, 2, 8, false, 3.32f, 0.f, 9.32f, 3.76f, 0.0481f, 0.f, 0.f},
+    {kI8Stream, 1, 4, 2, 8, false, 3.13f, 0.561f, 0.f, 1.65f, 0.0355f, 0.f, 0.f},
+    {kI8Stream, 2, 1, 2, 4, false, 3.17f, 0.0757f, 11.2f, 0.f, 0.0711f, 0.f, 0.f},
+    {kI8Stream, 2, 2, 2, 4, false, 3.09f, 0.0625f, 12.5f, 1.45f, 0.0484f, 0.f, 0.f},
+    {kI8Stream, 2, 4, 2, 4, false, 3.12f, 0.0114f, 13.6f, 1.13f, 0.0477f, 0.f, 0.f},
+    {kI8Stream, 2, 8, 1, 8, false, 3.35f, 0.689f, 3.24f, 4.12f, 0.081f, 0.f, 0.f},
+    {kI8Stream, 1, 6, 2, 8, false, 3.f, 0.856f, 0.f, 0.824f, 0.0326f, 0.f, 0.f},
+    {kI8Stream, 2, 6, 2, 4, false, 3.79f, 0.f, 11.8f, 2.63f, 0.0542f, 0.f, 0.f},
+    {kI8Tile, 1, 1, 4, 4, false, 3.34f, 0.f, 0.144f, 0.0667f, 0.0843f, 0.168f, 0.f},
+    {kI8Tile, 2, 1, 3, 4, false, 1.53f, 1.73f, 0.248f, 0.119f, 0.0851f, 0.0917f, 0.f},
+    {kI8Tile, 2, 2, 2, 4, false, 3.59f, 2.36f, 0.126f, 0.343f, 0.0931f, 0.0322f, 0.f},
+    {kI8Tile, 2, 2, 4, 4, false, 2.83f, 0.f, 0.395f, 0.157f, 0.109f, 0.183f, 0.f},
+    {kI8Tile, 4, 2, 2, 4, false, 4.06f, 0.f, 0.581f, 0.31f, 0.0694f, 0.192f, 0.f},
+    {kI8Tile, 4, 4, 2, 4, false, 3.4f, 2.62f, 0.832f, 0.591f, 0.0438f, 0.192f, 0.f},
+    {kI8Tile, 1, 1, 4, 4, true, 5.88f, 0.f, 0.144f, 0.0408f, 0.102f, 0.f, 0.484f},
+    {kI8Tile, 2, 2, 2, 4, true, 7.09f, 0.f, 0.275f, 0.258f, 0.094f, 0.241f, 0.192f},
+    {kI8Tile, 4, 4, 2, 4, true, 7.04f, 3.19f, 0.63f, 0.899f, 0.0267f, 0.0752f, 0.261f},
 };
 constexpr uint32_t kI8KernelCount = sizeof(kI8Kernels) / sizeof(kI8Kernels[0]);
 
@@ -88,7 +89,7 @@ inline double i8_time(const I8Kernel& k, uint64_t M, uint64_t N, uint64_t K, uin
 // largest).
 inline bool i8_takes(const I8Kernel& k, uint64_t M, uint64_t N, uint64_t K, uint64_t ld, uint32_t cus) {
     const bool tiles = M > 32 && ld * 256 <= kI8TileBytes;
-    if (k.kind == kI8Stream) return !tiles ? k.m == (M <= 8 ? 1 : M <= 16 ? 2 : M <= 32 ? 4 : 8) || (M <= 32 && M > 8u * k.m && M <= 32u * k.m) : i8_up(M, 8 * k.m) <= (k.m == 1 ? 4u : 8u);
+    if (k.kind == kI8Stream) return M > 32 && !tiles ? k.m == 8 : i8_up(M, 8 * k.m) <= (k.m == 1 ? 4u : 8u) && (k.m == 1 || 4u * k.m < M + 8);
     if (!tiles) return false;
     const uint64_t blocks = i8_blocks(k, M, N);
     if (k.split) return blocks <= kI8SplitTiles && K >= 2 * kI8SplitCodes;

@@ -164,6 +164,21 @@ def test_quantize_rows_many(torch):
     equal_codes(*out.get(), x.double().cpu().numpy())
 
 
+@pytest.mark.parametrize("rows,width", [((1 << 22) + 5, 4), ((1 << 20) + 3, 1028)])
+def test_quantize_rows_more_than_a_launch_has_blocks(torch, rows, width):
+    """Blocks that take a row after the other (four of them at a time up to 1024 values)."""
+    x = torch.zeros(rows, width + width % 8, dtype=torch.bfloat16, device="cuda")
+    x.uniform_(-1, 1, generator=gen(torch, 3))
+    codes, scales = torch.full((rows + 1, up(width, 16)), 99, dtype=torch.int8, device="cuda"), torch.full((rows + 1,), -5.0, device="cuda")
+    R.quantize_rows(ptr(x), "bf16", x.shape[1], rows, width, ptr(codes), codes.shape[1], ptr(scales), stream(torch))
+    want = (x[:, :width].abs().amax(-1).double() / 127).float()
+    assert torch.equal(scales[:rows], want) and scales[rows] == -5 and (codes[rows] == 99).all()
+    assert (codes[:rows, width:] == 0).all()
+    for part in (slice(0, 400), slice(rows - 400, rows)):
+        equal_codes(codes[part, :width].cpu().numpy().astype(np.float64), scales[part].cpu().numpy().astype(np.float64),
+                    x[part, :width].double().cpu().numpy())
+
+
 def test_quantize_rows_offsets_past_32_bits(torch):
     """Strides that put the last rows' elements and codes behind 2^32 bytes."""
     ld, rows = 1 << 28, 6
@@ -445,6 +460,70 @@ def test_linear_i8_unaligned_output(torch):
                     p.space.numel(), stream(torch))
         got = flat[1:1 + M * (N + 1)].view(M, N + 1)
         assert torch.equal(got[:, :N], want) and flat[0] == 55 and (got[:, N] == 55).all() and (flat[1 + M * (N + 1):] == 55).all()
+
+
+@pytest.mark.parametrize("M", [33, 65, 129, 193, 257, 300, 513])
+@pytest.mark.parametrize("N,K", [(40, 96), (333, 1536), (8200, 256)])
+def test_linear_i8_rows_behind_the_last(torch, M, N, K):
+    """A tile's rows that there are none of lie in memory that is not Y's."""
+    p = Product(torch, M, N, K, True, pady=3)
+    p.Y = torch.full((M + 300, N + 3), 55.0, device="cuda")
+    p.run()
+    p.check()
+
+
+@pytest.mark.parametrize("M,N,K", [(1, 33, 64), (20, 50, 256), (70, 130, 144), (300, 270, 512), (311, 401, 6768)])
+def test_linear_i8_scales_at_any_address(torch, M, N, K):
+    p = Product(torch, M, N, K, True)
+    for name, t in (("xs", p.xs), ("ws", p.ws), ("bias", p.bias)):
+        setattr(p, name, torch.cat([t[:1], t])[1:])
+        assert ptr(getattr(p, name)) % 16
+    p.run()
+    p.check()
+
+
+@pytest.mark.parametrize("M", [1, 9, 50, 300])
+@pytest.mark.parametrize("width", [1, 100, 897, 2030])
+def test_products_of_odd_widths(torch, M, width):
+    """Rows of a width that is no multiple of 16 multiply as the next one: the codes behind them are 0."""
+    N, K = 70, up(width, 16)
+    g = gen(torch, 9)
+    rows = lambda n: torch.randn(n, up(width, 4), device="cuda", generator=g)  # noqa: E731
+    x, w = rows(M), rows(N)
+    c, s, cw, sw = (torch.full(size, 99, dtype=t, device="cuda")
+                    for n in (M, N) for size, t in (((n, K), torch.int8), ((n,), torch.float32)))
+    for a, b, d in ((x, c, s), (w, cw, sw)):
+        R.quantize_rows(ptr(a), "f32", a.shape[1], len(a), width, ptr(b), K, ptr(d), stream(torch))
+    y, space = torch.zeros(M, N, device="cuda"), torch.zeros(R.linear_i8_workspace(M, N, K), dtype=torch.uint8, device="cuda")
+    R.linear_i8(ptr(cw), K, ptr(sw), ptr(c), K, ptr(s), None, ptr(y), N, M, N, K, ptr(space), space.numel(), stream(torch))
+    want = ((c[:, :width].double() @ cw[:, :width].double().t().contiguous()).float() * s[:, None]) * sw
+    assert torch.equal(y, want)
+    # (each value is off by half a step of its row's scale at most, the products by what that makes of a sum)
+    v, vw, h, hw = x[:, :width].double(), w[:, :width].double(), s.double()[:, None] / 2, sw.double()[:, None] / 2
+    off = h * vw.abs().sum(-1)[None] + v.abs().sum(-1, keepdim=True) * hw.t() + width * h * hw.t()
+    assert ((y.double() - v @ vw.t().contiguous()).abs() <= off * (1 + 1e-4) + 1e-30).all()
+
+
+def test_linear_i8_captured(torch):
+    """Products of every kind of kernel in one graph and one workspace, replayed with eager calls in between."""
+    sizes = [(1, 300, 640), (20, 896, 896), (311, 401, 6768), (70, 130, 1040), (300, 1152, 896), (687, 875, 14512)]
+    space = torch.zeros(max(R.linear_i8_workspace(*s) for s in sizes), dtype=torch.uint8, device="cuda")
+    products = [Product(torch, *s, bias=True, space=space, seed=i) for i, s in enumerate(sizes)]
+    other = Product(torch, 311, 401, 6768, seed=11)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        for p in products:
+            p.run()
+    for i in range(4):
+        for p in products:
+            p.X.copy_(p.X.roll(i, 0))
+            p.Y.fill_(55.0)
+        space.fill_(i)
+        graph.replay()
+        other.run()
+        torch.cuda.synchronize()
+        for p in products + [other]:
+            p.check()
 
 
 def test_linear_i8_offsets_past_32_bits(torch):

@@ -107,6 +107,8 @@ def test_silu_mul_refusals(bad, name):
     (dict(ldw=1 << 31), CONFIG), (dict(W=P + 8), CONFIG), (dict(X=S + 4), CONFIG), (dict(ldy=39), CONFIG), (dict(ldy=1 << 31), CONFIG),
     (dict(workspace=2 * U + 8), CONFIG), (dict(workspace_bytes=0), CONFIG), (dict(Y=P), CONFIG), (dict(Y=S + 64), CONFIG), (dict(Y=Q), CONFIG),
     (dict(Y=T), CONFIG), (dict(bias=U + 8), CONFIG), (dict(Y=2 * U + 4), CONFIG), (dict(N=1 << 31, ldy=1 << 31), CONFIG),
+    (dict(workspace=P), CONFIG), (dict(workspace=S - 16), CONFIG), (dict(workspace=Q), CONFIG), (dict(workspace=T), CONFIG),
+    (dict(bias=2 * U + 2), CONFIG),
 ])
 def test_linear_i8_refusals(bad, name):
     refused(linear, name, **bad)

@@ -519,11 +519,11 @@ int vvli_gpu_linear_i8(const int8_t* W, uint64_t ldw, const float* w_scales, con
     if (need && !workspace) return set_error(VVLI_NULL_ARG, "%s: NULL workspace", who);
     if (need && (!aligned16(workspace) || workspace_bytes < need))
         return set_error(VVLI_INVALID_CONFIG, "%s: workspace of %zu bytes", who, workspace_bytes);
-    const RowBytes y{Y, ldy * 4, uint64_t{N} * 4, M};
-    if (rows_meet(y, RowBytes{W, ldw, K, N}) || rows_meet(y, RowBytes{X, ldx, K, M}) || rows_meet(y, RowBytes{w_scales, 4, 4, N}) ||
-        rows_meet(y, RowBytes{x_scales, 4, 4, M}) || rows_meet(y, RowBytes{bias, 2, 2, N}) ||
-        rows_meet(y, RowBytes{workspace, need, need, 1}))
-        return set_error(VVLI_INVALID_CONFIG, "%s: Y overlaps another argument", who);
+    const RowBytes y{Y, ldy * 4, uint64_t{N} * 4, M}, space{workspace, need, need, 1};
+    const RowBytes inputs[] = {{W, ldw, K, N}, {X, ldx, K, M}, {w_scales, 4, 4, N}, {x_scales, 4, 4, M}, {bias, 2, 2, N}};
+    for (const RowBytes& in : inputs)
+        if (rows_meet(y, in) || rows_meet(space, in)) return set_error(VVLI_INVALID_CONFIG, "%s: Y or the workspace overlaps an input", who);
+    if (rows_meet(y, space)) return set_error(VVLI_INVALID_CONFIG, "%s: Y overlaps the workspace", who);
     if (M == 0) return VVLI_OK;
     LinearI8Args a{};
     a.W = W, a.X = X, a.w_scales = w_scales, a.x_scales = x_scales, a.bias = bias, a.Y = Y;

@@ -17,7 +17,7 @@ with n <= 70000 under 2^-36 relative, so that
 """
 import numpy as np
 import pytest
-from test_ops_i8 import ODD
+from test_ops_i8 import CUT, ODD
 
 from vvli_amd import runtime as R
 
@@ -388,7 +388,7 @@ def test_linear_i8_large(torch, M, N, K):
     p.check()
 
 
-@pytest.mark.parametrize("M,N,K", ODD)
+@pytest.mark.parametrize("M,N,K", ODD + CUT)
 def test_linear_i8_every_kernel(torch, M, N, K):
     for pad in ((0, 0, 0), (1, 3, 5)):
         p = Product(torch, M, N, K, True, *pad, seed=2)

@@ -138,8 +138,9 @@ int main() {
     while (scanf("%llu %llu %llu %llu %u", &m, &n, &k, &ld, &cus) == 5) {
         const vvli::I8Plan p = vvli::i8_plan(m, n, k, ld, cus);
         const vvli::I8Kernel& x = vvli::kI8Kernels[p.kernel];
-        printf("%u %u %llu %d %d %d %d %llu %u\\n", p.kernel, p.splits, (unsigned long long)p.blocks, (int)x.kind, x.r, x.m, x.split,
-               (unsigned long long)vvli::i8_part_bytes(m, n, k), vvli::kI8KernelCount);
+        printf("%u %u %llu %d %d %d %d %llu %u %llu\\n", p.kernel, p.splits, (unsigned long long)p.blocks, (int)x.kind, x.r, x.m, x.split,
+               (unsigned long long)vvli::i8_part_bytes(m, n, k), vvli::kI8KernelCount,
+               (unsigned long long)p.cut);
     }
 }
 """
@@ -169,10 +170,14 @@ ODD = [(1, 33, 432), (5, 413, 2672), (35, 39, 624), (109, 365, 1120), (153, 43, 
        (461, 14459, 144), (295, 18253, 928), (189, 39433, 656), (395, 18565, 2480), (61, 33, 18576), (311, 401, 6768),
        (3017, 75, 10976), (687, 875, 14512), (181, 5555, 10272), (623, 3541, 16112)]
 
+# Two launches of columns, the second of small tiles, a stream, a split K and large tiles.
+CUT = [(411, 34783, 752), (475, 33565, 880), (393, 32779, 3616), (917, 21673, 1808)]
+
 
 def test_odd_sizes_reach_every_kernel(plan):
     got = plan([(m, n, k, max(k, 4 * n), 256) for m, n, k in ODD])
-    assert {g[0] for g in got} == set(range(got[0][8]))
+    assert {g[0] for g in got} == set(range(got[0][8])) and not any(g[9] for g in got)
+    assert all(g[9] for g in plan([(m, n, k, 4 * n, 256) for m, n, k in CUT]))
 
 
 def test_every_kernel_is_taken_somewhere(plan):
@@ -192,7 +197,11 @@ def test_plans_fit_their_calls(plan):
         k = 16 * int(np.exp(rng.uniform(0, np.log(8191))))
         ld = max(k, 4 * n, int(np.exp(rng.uniform(0, np.log(2 ** 30)))))
         sizes.append((m, n, k, ld, int(rng.choice([256, 64, 304]))))
-    for (m, n, k, ld, cus), (kernel, splits, blocks, kind, r, c, split, room, _) in zip(sizes, plan(sizes)):
+    cuts = 0
+    for (m, n, k, ld, cus), (kernel, splits, blocks, kind, r, c, split, room, _, cut) in zip(sizes, plan(sizes)):
+        if cut:  # whole rounds of large tiles, columns left for the next launch
+            assert kind == 1 and not split and 0 < cut < n and cut % (64 * r) == 0 and blocks <= -(-n // (64 * r)) * -(-m // (64 * c)) // cus * cus
+            n, cuts = cut, cuts + 1
         assert blocks > 0 and (splits > 1) == bool(split)
         if split:
             assert splits * m * n * 4 <= room and k >= 512 * splits and m > 32
@@ -201,6 +210,7 @@ def test_plans_fit_their_calls(plan):
             assert blocks == splits * -(-n // (64 * r)) * -(-m // (64 * c))
         else:
             assert blocks == -(-(-(-n // (16 * r))) // 8) * 8 * -(-m // (8 * c))
+    assert cuts > 20
 
 
 def test_no_rows_launch_nothing():

@@ -479,18 +479,19 @@ hipError_t launch_plan(const LinearI8Args& a, const I8Plan& plan, hipStream_t s,
 
 hipError_t launch_linear(LinearI8Args a, hipStream_t s) {
     const I8Plan plan = i8_plan(a.M, a.N, a.K, std::max(std::max(a.ldw, a.ldx), a.ldy * 4), gemm_cus());
-    if (plan.blocks * 512 < (uint64_t{1} << 32)) return launch_plan(a, plan, s, std::make_integer_sequence<uint32_t, kI8KernelCount>{});
-    // More threads than a launch takes: the longer side in halves.
+    const bool fits = plan.blocks * 512 < (uint64_t{1} << 32);  // (else more threads than a launch takes: the longer side in halves)
+    const auto kernels = std::make_integer_sequence<uint32_t, kI8KernelCount>{};
+    if (fits && !plan.cut) return launch_plan(a, plan, s, kernels);
     LinearI8Args b = a;
-    if (a.M >= a.N) {
+    if (!fits && a.M >= a.N) {
         a.M = (a.M / 2 + 255) / 256 * 256, b.M -= a.M;
         b.X += a.M * a.ldx, b.x_scales += a.M, b.Y += a.M * a.ldy;
     } else {
-        a.N = (a.N / 2 + 255) / 256 * 256, b.N -= a.N;
+        a.N = fits ? static_cast<uint32_t>(plan.cut) : (a.N / 2 + 255) / 256 * 256, b.N -= a.N;
         b.W += a.N * a.ldw, b.w_scales += a.N, b.Y += a.N;
         if (b.bias) b.bias += a.N;
     }
-    const hipError_t e = launch_linear(a, s);
+    const hipError_t e = fits ? launch_plan(a, plan, s, kernels) : launch_linear(a, s);
     return e != hipSuccess ? e : launch_linear(b, s);
 }
 

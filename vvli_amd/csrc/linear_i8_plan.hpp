@@ -46,6 +46,8 @@ constexpr I8Kernel kI8Kernels[] = {
     {kI8Tile, 4, 4, 2, 4, true, 7.04f, 3.19f, 0.63f, 0.899f, 0.0267f, 0.0752f, 0.261f},
 };
 constexpr uint32_t kI8KernelCount = sizeof(kI8Kernels) / sizeof(kI8Kernels[0]);
+constexpr uint32_t kI8Largest = 14;  // tiles of 256 x 256, the fastest a product where they fill the CUs
+static_assert(kI8Kernels[kI8Largest].r == 4 && kI8Kernels[kI8Largest].m == 4 && !kI8Kernels[kI8Largest].split, "256 x 256");
 
 constexpr uint32_t kI8MostSplits = 8, kI8SplitCodes = 512, kI8SplitTiles = 128;  // parts of K, codes of a part at least, tiles at most
 constexpr uint64_t kI8PartBytes = uint64_t{64} << 20;                           // of all parts together
@@ -60,6 +62,7 @@ inline uint64_t i8_part_bytes(uint64_t M, uint64_t N, uint64_t K) {
 struct I8Plan {
     uint32_t kernel, splits;  // of kI8Kernels
     uint64_t blocks;
+    uint64_t cut;  // columns of Y of this launch (0: all); a call of the others follows
 };
 
 inline uint64_t i8_up(uint64_t n, uint64_t d) { return (n + d - 1) / d; }
@@ -97,18 +100,35 @@ inline bool i8_takes(const I8Kernel& k, uint64_t M, uint64_t N, uint64_t K, uint
     return !(k.r == 2 && k.m == 2) || (blocks <= cus) == (k.stages == 4);
 }
 
-inline I8Plan i8_plan(uint64_t M, uint64_t N, uint64_t K, uint64_t ld, uint32_t cus) {
-    I8Plan best{0, 1, 0};
-    double least = 0;
+// The kernel that takes least, and what it takes.
+inline I8Plan i8_one(uint64_t M, uint64_t N, uint64_t K, uint64_t ld, uint32_t cus, double& least) {
+    I8Plan best{0, 1, 0, 0};
     for (uint32_t i = 0; i < kI8KernelCount; ++i) {
         const I8Kernel& k = kI8Kernels[i];
         if (!i8_takes(k, M, N, K, ld, cus)) continue;
         for (uint64_t s = k.split ? 2 : 1; s <= (k.split ? kI8MostSplits : 1); ++s) {
             if (k.split && (K < s * kI8SplitCodes || s * M * N * 4 > kI8PartBytes)) break;
             const double t = i8_time(k, M, N, K, s, cus);
-            if (best.blocks == 0 || t < least) least = t, best = I8Plan{i, static_cast<uint32_t>(s), i8_blocks(k, M, N) * s};
+            if (best.blocks == 0 || t < least) least = t, best = I8Plan{i, static_cast<uint32_t>(s), i8_blocks(k, M, N) * s, 0};
         }
     }
+    return best;
+}
+
+// Where 256 x 256 tiles leave a last round that few CUs have a tile of, the whole rounds are a launch of their own and the
+// other columns one of smaller tiles (us, all in one launch and so, 256 CUs: 4096 x 4608 x 3584 83 -> 73, 1024 x 37888 x
+// 3584 158 -> 145, 4096 x 37888 x 3584 550 -> 532, 4096 x 6144 x 2048 64.7 -> 62.4). The fits' `base` stands for what the
+// second launch costs.
+inline I8Plan i8_plan(uint64_t M, uint64_t N, uint64_t K, uint64_t ld, uint32_t cus) {
+    double least = 0;
+    I8Plan best = i8_one(M, N, K, ld, cus, least);
+    const I8Kernel& k = kI8Kernels[kI8Largest];
+    if (!i8_takes(k, M, N, K, ld, cus)) return best;
+    const uint64_t tm = i8_up(M, 64 * k.m), tiles = i8_blocks(k, M, N), first = tiles / cus * cus / tm * 64 * k.r;
+    if (tiles <= cus || first == 0 || first >= N) return best;
+    double rest = 0;
+    i8_one(M, N - first, K, ld, cus, rest);
+    if (i8_time(k, M, first, K, 1, cus) + rest < least) best = I8Plan{kI8Largest, 1, first / (64 * k.r) * tm, first};
     return best;
 }
 

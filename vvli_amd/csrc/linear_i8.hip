@@ -233,7 +233,9 @@ hipError_t launch_stream(const LinearI8Args& a, hipStream_t s) {
 // arrived.
 //
 // LDS: ST stages of X and one more of W, rows of 128 bytes with 16-byte unit c of
-// row r at c ^ (r & 7). X's copies are issued in a step's second half, into the
+// row r at c ^ (r / 2 & 7): the 16 lanes that a cycle of 256 bytes serves (0-3,
+// 12-15, 20-23 and 24-27, and so on) read the same unit of 16 rows, two rows of
+// which are as long as all banks (r & 7 had two lanes at each bank). X's copies are issued in a step's second half, into the
 // stage just read, W's in the first half of the step after it. 256 x 256 leaves room
 // for two stages; smaller tiles take more, since their steps are shorter and what is
 // on its way lasts as long.
@@ -298,12 +300,13 @@ __global__ __launch_bounds__(kTileThreads, RN * RM == 16 ? 1 : 2) void linear_i8
     }
     const __amdgpu_buffer_rsrc_t W = __builtin_amdgcn_make_buffer_rsrc(const_cast<int8_t*>(a.W) + n0 * a.ldw, 0, kBufferBytes, 0x20000);
     const __amdgpu_buffer_rsrc_t X = __builtin_amdgcn_make_buffer_rsrc(const_cast<int8_t*>(a.X) + m0 * a.ldx, 0, kBufferBytes, 0x20000);
-    const uint32_t unit = (lane % 8 ^ lane / 8) * 16;  // of a row's 128 codes, what this lane copies
+    // Of a row's 128 codes, what this lane copies (g: of 8 rows, odd and even ones alternate, WG and XG being even).
+    auto unit = [&](int g) { return (lane % 8 ^ lane / 16 ^ g % 2 * 4) * 16; };
     uint32_t w_at[WG], x_at[XG];
 #pragma unroll
-    for (int g = 0; g < WG; ++g) w_at[g] = min((wave * WG + g) * 8 + lane / 8, a.N - 1 - n0) * static_cast<uint32_t>(a.ldw) + unit;
+    for (int g = 0; g < WG; ++g) w_at[g] = min((wave * WG + g) * 8 + lane / 8, a.N - 1 - n0) * static_cast<uint32_t>(a.ldw) + unit(g);
 #pragma unroll
-    for (int g = 0; g < XG; ++g) x_at[g] = min((wave * XG + g) * 8 + lane / 8, a.M - 1 - m0) * static_cast<uint32_t>(a.ldx) + unit;
+    for (int g = 0; g < XG; ++g) x_at[g] = min((wave * XG + g) * 8 + lane / 8, a.M - 1 - m0) * static_cast<uint32_t>(a.ldx) + unit(g);
     const int all_steps = static_cast<int>((a.K + 127) / 128);
     const int first = SPLIT ? static_cast<int>(blockIdx.y * a.split_steps) : 0, steps = SPLIT ? min(static_cast<int>(a.split_steps), all_steps - first) : all_steps;
     const uint32_t k_first = first * 128, k_end = min(k_first + steps * 128, a.K);
@@ -315,11 +318,11 @@ __global__ __launch_bounds__(kTileThreads, RN * RM == 16 ? 1 : 2) void linear_i8
     auto end_of = [&](int step) { return step < steps ? k_end : 0; };
     auto copy_w = [&](int step, int g) {
         const uint32_t k = k_of(step);
-        copy_buffer16(W, k + unit < end_of(step) ? w_at[g] : kBufferBytes, k, tile_lds + step % (ST + 1) * S::WStage + (wave * WG + g) * 1024);
+        copy_buffer16(W, k + unit(g) < end_of(step) ? w_at[g] : kBufferBytes, k, tile_lds + step % (ST + 1) * S::WStage + (wave * WG + g) * 1024);
     };
     auto copy_x = [&](int step, int g) {
         const uint32_t k = k_of(step);
-        copy_buffer16(X, k + unit < end_of(step) ? x_at[g] : kBufferBytes, k,
+        copy_buffer16(X, k + unit(g) < end_of(step) ? x_at[g] : kBufferBytes, k,
                       tile_lds + (ST + 1) * S::WStage + step % ST * S::XStage + (wave * XG + g) * 1024);
     };
     for (int t = 0; t < ST; ++t) {
@@ -337,7 +340,7 @@ __global__ __launch_bounds__(kTileThreads, RN * RM == 16 ? 1 : 2) void linear_i8
             for (int e = 0; e < 16; ++e) sum[r][c][e] = 0;
     // Fragments [half of 64][32 codes][32 rows]: lane l row l % 32, codes 16 (l / 32) .. + 15.
     i32x4 fw[2][2][RN], fx[2][2][RM];
-    const uint32_t at = lane % 32 * 128 + (lane / 32 ^ lane % 8) * 16;
+    const uint32_t at = lane % 32 * 128 + (lane / 32 ^ lane / 2 % 8) * 16;
     const uint32_t w_lds = lds_address(tile_lds) + wn * (RN * 4096) + at;
     const uint32_t x_lds = lds_address(tile_lds) + (ST + 1) * S::WStage + wm * (RM * 4096) + at;
     constexpr int P = 2 * RN * RM, R = 2 * (RN + RM);  // products and reads of a half

@@ -168,10 +168,12 @@ ODD = [(1, 33, 432), (5, 413, 2672), (35, 39, 624), (109, 365, 1120), (153, 43, 
        (261, 41, 480), (217, 725, 832), (323, 5905, 16), (129, 2383, 1936), (263, 43, 288), (861, 475, 832),
        (33, 24827, 16), (55, 32197, 208), (857, 9191, 16), (1371, 3365, 2800), (145, 41, 16), (311, 1461, 32),
        (461, 14459, 144), (295, 18253, 928), (189, 39433, 656), (395, 18565, 2480), (61, 33, 18576), (311, 401, 6768),
-       (3017, 75, 10976), (687, 875, 14512), (181, 5555, 10272), (623, 3541, 16112)]
+       (3017, 75, 10976), (687, 875, 14512), (181, 5555, 10272), (623, 3541, 16112),
+       (1207, 6409, 608), (847, 2359, 1504), (395, 27229, 512), (1393, 9401, 1472), (65, 16505, 592), (133, 17291, 576),
+       (131, 34373, 672), (155, 33383, 576), (133, 21, 9328), (149, 179, 16128), (73, 2793, 9920), (139, 5585, 8944)]
 
-# Two launches of columns, the second of small tiles, a stream, a split K and large tiles.
-CUT = [(411, 34783, 752), (475, 33565, 880), (393, 32779, 3616), (917, 21673, 1808)]
+# Two launches of columns, the second a stream, large and small tiles and a split K.
+CUT = [(475, 33565, 880), (393, 32779, 3616), (921, 28579, 688), (963, 36935, 720), (537, 21815, 4688)]
 
 
 def test_odd_sizes_reach_every_kernel(plan):

@@ -3,6 +3,14 @@
 //   Y[m,n] = f32(sum_k W[n,k] X[m,k]) * x_scales[m] * w_scales[n] + bias[n].
 //
 // The sums are exact in 32 bits, so no split or order of them changes a result.
+//
+// Up to some 100 rows W's bytes bound it, above them the products, in between what a
+// launch and a block's chain of copies, products and stores cost (3.8 us is a launch
+// and a block that ends at once). Measured, us (W in no cache; a copy of 256 MB
+// moves 5.4 TB/s, a library product of 8192 cubed 2466 TOP/s): 1 x 37888 x 3584 22.0
+// (6.2 TB/s), 5 x 2048 x 8192 6.2, 48 x 4608 x 3584 8.4, 128 x 37888 x 3584 37 (4.2
+// TB/s), 333 x 896 x 4864 9.7, 2048 x 4608 x 3584 41 (1640 TOP/s), 4096 x 3584 x
+// 18944 238 (2330), 4096 x 37888 x 3584 516 (2150).
 #include <algorithm>
 #include <atomic>
 #include <type_traits>
@@ -118,7 +126,10 @@ __device__ __forceinline__ void read_fragments(i32x4 (&w)[R], i32x4 (&x)[MT], ui
 // its chunks into its own ST stages of LDS (copies of 1 KiB, 8 rows of 128 bytes
 // each) and reads them back in the order of the products' lanes (16-byte unit c of
 // row r at c ^ (r & 7): no bank conflicts), so that no wave waits for another
-// before the sums of all meet at the end.
+// before the sums of all meet at the end. Loads into registers instead of copies
+// hold as much in flight only with registers that leave fewer waves: 1 x 37888 x
+// 3584 32 us, so 22.0. W is read once and passes the caches (nontemporal), X, which
+// all blocks read, stays in them.
 template <int R, int XG, int ST, int WV>
 __global__ __launch_bounds__(WV * 64) void linear_i8_stream_kernel(LinearI8Args a) {
     static_assert(XG == 1 || XG % 2 == 0, "X tiles of 16 rows, or one of 8 twice over");
@@ -219,11 +230,16 @@ hipError_t launch_stream(const LinearI8Args& a, hipStream_t s) {
 //
 // 4 x 4 (a tile of 256 x 256, one wave on each SIMD of a CU) moves the fewest
 // fragment bytes a product that the registers hold (256 of sums, 64 for each of two
-// sets of fragments): LDS takes 64 KiB of copies and gives 128 KiB of fragments in
-// a step of 128 codes, 1536 cycles of its 128 bytes a cycle, for 2048 cycles of
-// products. (Eight waves of 128 x 64 read 192 KiB, which with the copies is all that
-// LDS gives: 4096 x 3584 x 18944 271 us, four waves 238.) Smaller ones are for
-// launches whose large tiles would leave CUs idle.
+// sets of fragments): of a step of 128 codes, 2048 cycles of products, LDS takes 64
+// KiB of copies and gives 128 KiB of fragments (eight waves of 128 x 64 read 192
+// KiB: 4096 x 3584 x 18944 271 us, four waves 238). Others are for launches whose
+// large tiles would leave CUs idle.
+//
+// What bounds large calls is the card's power: 4096 x 3584 x 18944 runs at 2330 to
+// 2390 TOP/s and 4096 x 37888 x 3584, with 620 MB of Y behind its products, at 2130,
+// the products busy 61 % of the cycles at a clock of 1.75 of 2.4 GHz. A loop of
+// nothing but these products runs at 3400 TOP/s on random codes (4700 on zeros,
+// which take no power), with its fragments read from LDS at 2700 to 3000.
 //
 // A step has two halves of 64 codes. While the products of a half run, the next
 // half's fragments come out of LDS and copies for later steps are issued, both
@@ -233,12 +249,13 @@ hipError_t launch_stream(const LinearI8Args& a, hipStream_t s) {
 // arrived.
 //
 // LDS: ST stages of X and one more of W, rows of 128 bytes with 16-byte unit c of
-// row r at c ^ (r / 2 & 7): the 16 lanes that a cycle of 256 bytes serves (0-3,
-// 12-15, 20-23 and 24-27, and so on) read the same unit of 16 rows, two rows of
-// which are as long as all banks (r & 7 had two lanes at each bank). X's copies are issued in a step's second half, into the
-// stage just read, W's in the first half of the step after it. 256 x 256 leaves room
-// for two stages; smaller tiles take more, since their steps are shorter and what is
-// on its way lasts as long.
+// row r at c ^ (r / 2 & 7): what 16 rows hold of one unit lies at 16 places of the
+// 256 bytes that a cycle gives. (At c ^ (r & 7), SQ_LDS_BANK_CONFLICT was half of
+// SQ_LDS_IDX_ACTIVE, now it is 0: 256 x 3584 x 3584 10.5 us then, 9.9 now, large
+// calls the same.) X's copies are issued in a step's second half, into the stage
+// just read, W's in the first half of the step after it. 256 x 256 leaves room for
+// two stages; smaller tiles take more, since their steps are shorter and what is on
+// its way lasts as long.
 //
 // SPLIT: a block has a part of K and leaves its sums, 32-bit integers, for
 // linear_i8_join_kernel.
@@ -284,7 +301,7 @@ struct TileShape {
 };
 
 template <int RN, int RM, int ST, bool SPLIT>
-__global__ __launch_bounds__(kTileThreads, RN * RM == 16 ? 1 : 2) void linear_i8_tile_kernel(LinearI8Args a) {
+__global__ __launch_bounds__(kTileThreads, RN * RM >= 9 ? 1 : 2) void linear_i8_tile_kernel(LinearI8Args a) {
     using S = TileShape<RN, RM, ST>;
     constexpr int WG = 2 * RN, XG = 2 * RM;  // copies of a wave a step
     extern __shared__ __attribute__((aligned(1024))) char tile_lds[];  // W [ST + 1] | X [ST]

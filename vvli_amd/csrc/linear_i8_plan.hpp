@@ -15,10 +15,14 @@ enum I8Kind { kI8Stream, kI8Tile };
 // is the steps of a block, turns the rounds.
 //
 // The numbers are fits (nonnegative, of relative errors, sizes where the kernel is
-// near the fastest weighing most) to 286 sizes, M = 1 to 4096 with (N, K) of nine
-// projections, W in no cache. Choosing by them costs 1.0 % over the fastest of some
-// hundred measured variants on the geometric mean, 11 % where it costs most (768 x
-// 3584 x 18944: K in six parts 75 us, in four 67).
+// near the fastest weighing most) to 365 sizes, M = 1 to 4096 with (N, K) of nine
+// projections, W in no cache. On the geometric mean, choosing by them costs 0.3 %
+// over the fastest kernel here and 1.2 % over that of 126 measured variants; 15 %
+// where it costs most (448 x 3584 x 18944: 58 us, in parts by 128 x 128 tiles of
+// four stages 51). Sides of 192 fill the CUs where those of 128 and 256 leave a
+// third of them idle (us without and with them: 2048 x 4608 x 3584 49 and 41, 1536 x
+// 16384 x 2048 72 and 65, 896 x 9728 x 896 20.9 and 18.5, 131 x 37888 x 3584 48 and
+// 43).
 struct I8Kernel {
     I8Kind kind;
     uint8_t r, m, stages, waves;  // stream: tiles of 16 rows of W, groups of 8 of X; tile: 64s of rows of either
@@ -29,24 +33,27 @@ constexpr I8Kernel kI8Kernels[] = {
     {kI8Stream, 1, 1, 2, 8, false, 3.28f, 0.f, 10.8f, 0.607f, 0.0681f, 0.f, 0.f},
     {kI8Stream, 1, 2, 2, 8, false, 3.32f, 0.f, 9.32f, 3.76f, 0.0481f, 0.f, 0.f},
     {kI8Stream, 1, 4, 2, 8, false, 3.13f, 0.561f, 0.f, 1.65f, 0.0355f, 0.f, 0.f},
+    {kI8Stream, 1, 6, 2, 8, false, 3.f, 0.856f, 0.f, 0.824f, 0.0326f, 0.f, 0.f},
     {kI8Stream, 2, 1, 2, 4, false, 3.17f, 0.0757f, 11.2f, 0.f, 0.0711f, 0.f, 0.f},
     {kI8Stream, 2, 2, 2, 4, false, 3.09f, 0.0625f, 12.5f, 1.45f, 0.0484f, 0.f, 0.f},
     {kI8Stream, 2, 4, 2, 4, false, 3.12f, 0.0114f, 13.6f, 1.13f, 0.0477f, 0.f, 0.f},
-    {kI8Stream, 2, 8, 1, 8, false, 3.35f, 0.689f, 3.24f, 4.12f, 0.081f, 0.f, 0.f},
-    {kI8Stream, 1, 6, 2, 8, false, 3.f, 0.856f, 0.f, 0.824f, 0.0326f, 0.f, 0.f},
     {kI8Stream, 2, 6, 2, 4, false, 3.79f, 0.f, 11.8f, 2.63f, 0.0542f, 0.f, 0.f},
+    {kI8Stream, 2, 8, 1, 8, false, 3.35f, 0.689f, 3.24f, 4.12f, 0.081f, 0.f, 0.f},
     {kI8Tile, 1, 1, 4, 4, false, 3.34f, 0.f, 0.144f, 0.0667f, 0.0843f, 0.168f, 0.f},
     {kI8Tile, 2, 1, 3, 4, false, 1.53f, 1.73f, 0.248f, 0.119f, 0.0851f, 0.0917f, 0.f},
     {kI8Tile, 2, 2, 2, 4, false, 3.59f, 2.36f, 0.126f, 0.343f, 0.0931f, 0.0322f, 0.f},
     {kI8Tile, 2, 2, 4, 4, false, 2.83f, 0.f, 0.395f, 0.157f, 0.109f, 0.183f, 0.f},
+    {kI8Tile, 3, 2, 2, 4, false, 2.98f, 0.f, 0.521f, 0.194f, 0.08f, 0.199f, 0.f},
     {kI8Tile, 4, 2, 2, 4, false, 4.06f, 0.f, 0.581f, 0.31f, 0.0694f, 0.192f, 0.f},
+    {kI8Tile, 3, 4, 2, 4, false, 3.32f, 1.64f, 0.696f, 0.452f, 0.0435f, 0.19f, 0.f},
+    {kI8Tile, 4, 3, 2, 4, false, 2.47f, 1.7f, 0.768f, 0.379f, 0.0577f, 0.19f, 0.f},
     {kI8Tile, 4, 4, 2, 4, false, 3.4f, 2.62f, 0.832f, 0.591f, 0.0438f, 0.192f, 0.f},
     {kI8Tile, 1, 1, 4, 4, true, 5.88f, 0.f, 0.144f, 0.0408f, 0.102f, 0.f, 0.484f},
     {kI8Tile, 2, 2, 2, 4, true, 7.09f, 0.f, 0.275f, 0.258f, 0.094f, 0.241f, 0.192f},
     {kI8Tile, 4, 4, 2, 4, true, 7.04f, 3.19f, 0.63f, 0.899f, 0.0267f, 0.0752f, 0.261f},
 };
 constexpr uint32_t kI8KernelCount = sizeof(kI8Kernels) / sizeof(kI8Kernels[0]);
-constexpr uint32_t kI8Largest = 14;  // tiles of 256 x 256, the fastest a product where they fill the CUs
+constexpr uint32_t kI8Largest = 17;  // tiles of 256 x 256, the fastest a product where they fill the CUs
 static_assert(kI8Kernels[kI8Largest].r == 4 && kI8Kernels[kI8Largest].m == 4 && !kI8Kernels[kI8Largest].split, "256 x 256");
 
 constexpr uint32_t kI8MostSplits = 8, kI8SplitCodes = 512, kI8SplitTiles = 128;  // parts of K, codes of a part at least, tiles at most

@@ -172,8 +172,8 @@ ODD = [(1, 33, 432), (5, 413, 2672), (35, 39, 624), (109, 365, 1120), (153, 43, 
        (1207, 6409, 608), (847, 2359, 1504), (395, 27229, 512), (1393, 9401, 1472), (65, 16505, 592), (133, 17291, 576),
        (131, 34373, 672), (155, 33383, 576), (133, 21, 9328), (149, 179, 16128), (73, 2793, 9920), (139, 5585, 8944)]
 
-# Two launches of columns, the second a stream, large and small tiles and a split K.
-CUT = [(475, 33565, 880), (393, 32779, 3616), (921, 28579, 688), (963, 36935, 720), (537, 21815, 4688)]
+# Two launches of columns, the second a split K, a stream and small tiles.
+CUT = [(393, 32779, 3616), (537, 21815, 4688), (409, 33031, 1728), (431, 37029, 1072), (387, 33589, 1296)]
 
 
 def test_odd_sizes_reach_every_kernel(plan):

@@ -12,14 +12,16 @@
 //     error of the largest one (mostly one of a row) are formed in f64 (a
 //     norm's are all: a product each);
 //   * a code whose f32 quotient is within the error of a border between two
-//     codes: its unit of 4 or 8 values is formed in f64 (of a wave's 64 units
-//     one in 30, gated one in 8).
+//     codes. Its unit of 16 bytes is read again, at once, and f64 forms the values
+//     that are in doubt alone (of a wave's 64 units one in 30 holds one, gated one
+//     in 8; of bf16, whose few bits make ties, nine of ten waves do. Read and
+//     formed one after the other, weights took 59 us, gate 100).
 // Where f32's error is not the usual one (values that left its normal range) a
 // row is formed in f64 as a whole. Measured (inputs that no cache holds; a copy
-// of 1 GB moves 5.06 TB/s): weights 18944 x 3584 bf16 46 us (4.4 TB/s), f32 rows
-// 6001 x 3584 21.5 (5.0), their norm with the sum 62 (4.5), gate 2500 x 18944 100
-// (4.3; the products, exponentials and packing beside the loads are as long).
-// One row of 2048: 4.2, 4.8 and 5.2 us, of which 4.1 is a launch.
+// of 1 GB moves 5.06 TB/s): weights 18944 x 3584 bf16 41.6 us (4.9 TB/s), f32 rows
+// 6001 x 3584 21.3 (5.0), their norm with the sum 61.5 (4.5), gate 2500 x 18944 90.5
+// (4.7; the products, exponentials and packing beside the loads are near as long).
+// One row of 2048: 4.2, 4.6 and 4.8 us, of which 3.8 is a launch.
 #include <algorithm>
 
 #include "device_common.hpp"
@@ -41,6 +43,9 @@ struct RowsArgs {
     bool weight_bf16;
     float eps;
 };
+
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef uint16_t u16x2 __attribute__((ext_vector_type(2)));
 
 __device__ __forceinline__ float bf16_bits(uint32_t u) { return __uint_as_float(u << 16); }
 __device__ __forceinline__ float bf16_at(const void* p, size_t i) { return bf16_bits(static_cast<const uint16_t*>(p)[i]); }
@@ -108,10 +113,27 @@ __device__ __forceinline__ T reduce(T v, F f, T* part) {
     return v;
 }
 
+// f32's silu(g) u, for g >= -16 off by less than 1.3e-6 < 2^-19.5 of the value: the exponent's product with log2 e is off by
+// 2^-20 and 2.3e-7 where it is largest (of a value between 16 and 32), v_exp_f32 and v_rcp_f32 by one last bit, the rest
+// by half of one each. Below -16 it is off by 2^-16 of a value that is under 1.9e-6 |u|: rows where that could be a
+// larger part of the row's largest value than 2^-9 are not usual ones.
+__device__ __forceinline__ float gated32(float g, float u) {
+    const float p = __builtin_amdgcn_exp2f(g * -1.44269502f);
+    return g * u * __builtin_amdgcn_rcpf(1.f + p);
+}
+
+// The weights of unit u, whole.
+__device__ __forceinline__ f32x4 weights4(const RowsArgs& a, uint32_t u) {
+    if (!a.weight_bf16) return *as_global(static_cast<const f32x4*>(a.weight) + u);
+    const uint2 t = load_u32x2(static_cast<const uint2*>(a.weight) + u);
+    return f32x4{bf16_bits(t.x), __uint_as_float(t.x & 0xffff0000u), bf16_bits(t.y), __uint_as_float(t.y & 0xffff0000u)};
+}
+
 // ---- a row's values ---------------------------------------------------------
-// In f64, as the definition has them (norm: without the factor of its row).
+// A value is made of one or two others: of a row's, a hidden value and its weight, or gate and up.
 template <int OP>
 struct Row {
+    static constexpr int E = OP == kRowsBf16 ? 8 : 4;  // values of 16 bytes
     const RowsArgs& a;
     const float *x, *b;
     uint32_t row;
@@ -119,18 +141,58 @@ struct Row {
     __device__ __forceinline__ Row(const RowsArgs& a_, uint32_t r)
         : a(a_), x(static_cast<const float*>(a_.x) + r * a_.ldx), b(a_.b ? a_.b + r * a_.ldb : nullptr), row(r),
           h(a_.sum ? a_.sum + r * a_.lds : nullptr) {}
-    __device__ __forceinline__ float hidden(uint32_t e) const { return h ? h[e] : b ? x[e] + b[e] : x[e]; }
     __device__ __forceinline__ float weight(uint32_t e) const {
         return a.weight_bf16 ? bf16_at(a.weight, e) : static_cast<const float*>(a.weight)[e];
     }
-    __device__ __forceinline__ double operator()(uint32_t e) const {
-        if constexpr (OP == kRowsF32) return x[e];
+    __device__ __forceinline__ float first(uint32_t e) const {
         if constexpr (OP == kRowsBf16) return bf16_at(a.x, row * a.ldx + e);
-        if constexpr (OP == kRowsNorm) return static_cast<double>(hidden(e)) * static_cast<double>(weight(e));
-        const double g = x[e];
-        return g / (1.0 + exp(-g)) * static_cast<double>(b[e]);
+        if constexpr (OP == kRowsNorm) return h ? h[e] : b ? x[e] + b[e] : x[e];
+        return x[e];
     }
+    __device__ __forceinline__ float second(uint32_t e) const {
+        return OP == kRowsNorm ? weight(e) : OP == kRowsGate ? b[e] : 0.f;
+    }
+    typedef float Unit __attribute__((ext_vector_type(E)));
+    // The E values of unit u, 0 behind the width (whole: none is).
+    __device__ __forceinline__ void unit(uint32_t u, bool whole, Unit& p, Unit& q) const {
+        if (!whole) {
+#pragma unroll
+            for (uint32_t e = 0; e < E; ++e) {
+                const bool in = u * E + e < a.width;
+                p[e] = in ? first(u * E + e) : 0.f, q[e] = in ? second(u * E + e) : 0.f;
+            }
+            return;
+        }
+        const void* at = OP == kRowsBf16 ? static_cast<const void*>(static_cast<const uint16_t*>(a.x) + row * a.ldx) : OP == kRowsNorm && h ? h : x;
+        f32x4 v = *as_global(static_cast<const f32x4*>(at) + u), w = {0, 0, 0, 0};
+        if constexpr (OP == kRowsNorm) {
+            w = weights4(a, u);
+            if (!h && b) v += *as_global(reinterpret_cast<const f32x4*>(b) + u);
+        }
+        if constexpr (OP == kRowsGate) w = *as_global(reinterpret_cast<const f32x4*>(b) + u);
+#pragma unroll
+        for (int e = 0; e < E; ++e) {
+            const uint32_t two = __float_as_uint(v[e * 4 / E]);
+            p[e] = OP != kRowsBf16 ? v[e * 4 / E] : e % 2 ? __uint_as_float(two & 0xffff0000u) : bf16_bits(two), q[e] = w[e * 4 / E];
+        }
+    }
+    // As the definition has it (norm: without the factor of its row), and as f32 has it.
+    static __device__ __forceinline__ double f64(float p, float q) {
+        if constexpr (OP == kRowsNorm) return static_cast<double>(p) * static_cast<double>(q);
+        const double g = p;
+        if constexpr (OP == kRowsGate) return g / (1.0 + exp(-g)) * static_cast<double>(q);
+        return g;
+    }
+    static __device__ __forceinline__ float f32(float p, float q) { return OP == kRowsNorm ? p * q : OP == kRowsGate ? gated32(p, q) : p; }
+    __device__ __forceinline__ double operator()(uint32_t e) const { return f64(first(e), second(e)); }
 };
+template <typename U>
+__device__ __forceinline__ float pick(U v, uint32_t i) {
+    float r = v[0];
+#pragma unroll
+    for (uint32_t e = 1; e < sizeof(U) / 4; ++e) r = i == e ? v[e] : r;
+    return r;
+}
 
 __device__ __forceinline__ float scale_of(double top) {
     const float s = static_cast<float>(top / 127.0);
@@ -155,7 +217,7 @@ __global__ __launch_bounds__(kAnyThreads) void rows_any_kernel(RowsArgs a) {
             }
             top = Max()(top, fabs(value(e)));
             if constexpr (OP == kRowsNorm) {
-                const double h = value.hidden(e);
+                const double h = value.first(e);
                 square = fma(h, h, square);
             }
         }
@@ -187,16 +249,7 @@ __global__ __launch_bounds__(kAnyThreads) void rows_any_kernel(RowsArgs a) {
 // WAVES j of the row for j < V, so that a load of a wave is 1 KiB in a row; what
 // it keeps are the f32 values that the codes are made of (of bf16 the units as
 // they come). What f64 settles is read again.
-typedef float f32x4 __attribute__((ext_vector_type(4)));
 
-// f32's silu(g) u, for g >= -16 off by less than 1.3e-6 < 2^-19.5 of the value: the exponent's product with log2 e is off by
-// 2^-20 and 2.3e-7 where it is largest (of a value between 16 and 32), v_exp_f32 and v_rcp_f32 by one last bit, the rest
-// by half of one each. Below -16 it is off by 2^-16 of a value that is under 1.9e-6 |u|: rows where that could be a
-// larger part of the row's largest value than 2^-9 are not usual ones.
-__device__ __forceinline__ float gated32(float g, float u) {
-    const float p = __builtin_amdgcn_exp2f(g * -1.44269502f);
-    return g * u * __builtin_amdgcn_rcpf(1.f + p);
-}
 constexpr float kMostUp = 0x1p10f;  // of a usual row: max |u| over the largest value
 // How far |t - rint(t)| may be from 1/2 for f32 to tell the code of t = value / scale, |t| <= 127: off by 127 halves of a
 // last bit of f32 for the product and for the quotient each (2^-16), and of a norm's value (2^-17); a gated value by
@@ -210,16 +263,9 @@ constexpr uint32_t kTopBits = 48;
 // one use to the next: either takes more registers than there are.
 __device__ __forceinline__ void in_turn(uint32_t& id) { asm volatile("" : "+v"(id)::"memory"); }
 
-// The weights of unit u, whole.
-__device__ __forceinline__ f32x4 weights4(const RowsArgs& a, uint32_t u) {
-    if (!a.weight_bf16) return *as_global(static_cast<const f32x4*>(a.weight) + u);
-    const uint2 t = load_u32x2(static_cast<const uint2*>(a.weight) + u);
-    return f32x4{bf16_bits(t.x), __uint_as_float(t.x & 0xffff0000u), bf16_bits(t.y), __uint_as_float(t.y & 0xffff0000u)};
-}
-
 template <int OP, int WAVES, int V>
 __global__ __launch_bounds__(WAVES == 1 ? 256 : WAVES * 64, 4) void rows_i8_kernel(RowsArgs a) {
-    constexpr int G = WAVES * 64, E = OP == kRowsBf16 ? 8 : 4, ROWS = WAVES == 1 ? 4 : 1;  // rows of a block
+    constexpr int G = WAVES * 64, E = Row<OP>::E, ROWS = WAVES == 1 ? 4 : 1;  // rows of a block
     constexpr int N = V % 4 == 0 ? 4 : V % 3 == 0 ? 3 : 2;  // units in flight
     static_assert(V % N == 0, "whole turns");
     __shared__ double part_d[2 * WAVES];
@@ -228,6 +274,7 @@ __global__ __launch_bounds__(WAVES == 1 ? 256 : WAVES * 64, 4) void rows_i8_kern
     // Whole units, and those behind them up to the padded width: the first may hold the row's last values, lane i has
     // the i-th of them as its unit V.
     const uint32_t full = a.width / E, units = (a.width + kCodesPerUnit - 1) / kCodesPerUnit * (kCodesPerUnit / E);
+    const bool tail = units > full;  // (the same for all, as a width is: whole units mostly)
     const uint32_t first = blockIdx.x * ROWS + (WAVES == 1 ? __builtin_amdgcn_readfirstlane(threadIdx.x / 64) : 0);
     for (uint32_t row = first; row < a.rows; row += gridDim.x * ROWS) {
         const Row<OP> value(a, row);
@@ -268,7 +315,7 @@ __global__ __launch_bounds__(WAVES == 1 ? 256 : WAVES * 64, 4) void rows_i8_kern
             }
         }
         v[V] = f32x4{0, 0, 0, 0};
-        if (units > full && id == 0) {
+        if (tail && id == 0) {
 #pragma unroll
             for (uint32_t e = 0; e < E; ++e) {
                 const uint32_t at = full * E + e;
@@ -298,19 +345,23 @@ __global__ __launch_bounds__(WAVES == 1 ? 256 : WAVES * 64, 4) void rows_i8_kern
             usual = exact >= 0x1p-100 && exact <= 0x1p100;
             exact *= factor;
         } else {
+            if constexpr (OP == kRowsBf16) {  // (two values at a time: without their signs, bits are ordered as values are)
+                u16x2 most = {0, 0};
 #pragma unroll
-            for (int j = 0; j <= V; ++j) {
-                f32x4 t = v[j], o = v[j];
-                if constexpr (OP == kRowsBf16) {
+                for (int j = 0; j <= V; ++j) {
+                    if (j == V && !tail) continue;
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        const uint32_t w = __float_as_uint(t[e]);
-                        t[e] = bf16_bits(w), o[e] = __uint_as_float(w & 0xffff0000u);
-                        top = fmaxf(fmaxf(fabsf(t[e]), fabsf(o[e])), top), odd32 = fmaf(t[e], 0.f, odd32), odd32 = fmaf(o[e], 0.f, odd32);
-                    }
-                } else {
+                    for (int e = 0; e < 4; ++e)
+                        most = __builtin_elementwise_max(most, __builtin_bit_cast(u16x2, __float_as_uint(v[j][e]) & 0x7fff7fffu));
+                }
+                const uint32_t m = max(most[0], most[1]);
+                top = bf16_bits(m), odd32 = m < 0x7f80u ? 0.f : NAN;
+            } else {
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) top = fmaxf(top, fabsf(t[e])), odd32 = fmaf(t[e], 0.f, odd32);
+                for (int j = 0; j <= V; ++j) {
+                    if (j == V && !tail) continue;
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) top = fmaxf(top, fabsf(v[j][e])), odd32 = fmaf(v[j][e], 0.f, odd32);
                 }
             }
             float largest = odd32 == 0 ? top : INFINITY;  // (of the thread's)
@@ -324,19 +375,27 @@ __global__ __launch_bounds__(WAVES == 1 ? 256 : WAVES * 64, 4) void rows_i8_kern
             uint32_t near = 0;  // units that may hold the largest
 #pragma unroll
             for (int j = 0; j <= V; ++j) {
+                if (j == V && !tail) continue;
                 const float most = fmaxf(fmaxf(fabsf(v[j][0]), fabsf(v[j][1])), fmaxf(fabsf(v[j][2]), fabsf(v[j][3])));
                 if (most >= __uint_as_float(least)) near |= 1u << j;
             }
-            if (!usual) near = (2u << V) - 1;
+            if (!usual) near = (2u << V) - 1;  // (unit V too: there are no values in it where there is no tail)
             exact = 0;
             for (; near; near &= near - 1) {
                 const uint32_t u = unit_of(__builtin_ctz(near));
-                for (uint32_t e = u * 4; e < min(u * 4 + 4, a.width); ++e) exact = Max()(exact, fabs(value(e)));
+                typename Row<OP>::Unit p, q;
+                value.unit(u, u < full, p, q);
+                uint32_t some = 0;
+#pragma unroll
+                for (uint32_t e = 0; e < E; ++e)
+                    if (u * E + e < a.width && (!usual || fabsf(gated32(p[e], q[e])) >= __uint_as_float(least - 1))) some |= 1u << e;
+                for (; some; some &= some - 1) exact = Max()(exact, fabs(value.f64(pick(p, __builtin_ctz(some)), pick(q, __builtin_ctz(some)))));
             }
             exact = reduce<WAVES>(exact, Max(), part_d);
         }
-        const float scale = scale_of(exact), quotient = static_cast<float>(factor / static_cast<double>(scale));
-        usual = usual && scale >= 0x1p-126f;
+        const float scale = scale_of(exact), quotient = scale == 0 ? 0.f : static_cast<float>(factor / static_cast<double>(scale));
+        // (Rows of zeros, padding mostly, have no codes to settle: f32's values are finite there, a norm's below 2^-15.)
+        usual = scale == 0 ? OP == kRowsNorm || top < INFINITY : usual && scale >= 0x1p-126f;
         int8_t* const codes = a.codes ? a.codes + row * a.ldc : nullptr;
         if (codes) {
             if (id == 0) a.scales[row] = scale;
@@ -344,6 +403,7 @@ __global__ __launch_bounds__(WAVES == 1 ? 256 : WAVES * 64, 4) void rows_i8_kern
 #pragma unroll
             for (int j = 0; j <= V; ++j) {
                 if (j % N == 0) in_turn(id);
+                if (j == V && !tail) continue;
                 const uint32_t u = unit_of(j);
                 uint32_t word[E / 4];
                 float far = 0;
@@ -372,25 +432,41 @@ __global__ __launch_bounds__(WAVES == 1 ? 256 : WAVES * 64, 4) void rows_i8_kern
                     else *as_global(reinterpret_cast<uint32_t*>(codes) + u) = word[0];
                 }
             }
+            // (Of a unit in doubt, only the values that are, mostly one. The bound is a little wider than the one above.)
             for (; doubt; doubt &= doubt - 1) {
                 const uint32_t u = unit_of(__builtin_ctz(doubt));
-                uint64_t word = 0;
-                for (uint32_t e = u * E; e < min(u * E + E, a.width); ++e)
-                    word |= static_cast<uint64_t>(code_of(value(e) * factor, scale) & 0xff) << (e - u * E) * 8;
-                if constexpr (E == 8) *reinterpret_cast<uint64_t*>(codes + u * 8) = word;
-                else *reinterpret_cast<uint32_t*>(codes + u * 4) = static_cast<uint32_t>(word);
+                typename Row<OP>::Unit p, q;
+                value.unit(u, u < full, p, q);
+                uint32_t some = 0;
+#pragma unroll
+                for (uint32_t e = 0; e < E; ++e) {
+                    const float x = value.f32(p[e], q[e]), near = fmaf(x, quotient, 0x1.8p23f), off = fmaf(x, quotient, 0x1.8p23f - near);
+                    if (u * E + e < a.width && (!usual || fabsf(off) > 0.5f - 1.0625f * band<OP>())) some |= 1u << e;
+                }
+                for (; some; some &= some - 1) {
+                    const uint32_t e = __builtin_ctz(some);
+                    codes[u * E + e] = static_cast<int8_t>(code_of(value.f64(pick(p, e), pick(q, e)) * factor, scale));
+                }
             }
         }
         if constexpr (OP == kRowsNorm) {
             if (a.y) {  // (may be x or delta: behind all that reads them)
                 float* y = a.y + row * a.ldy;
-                for (uint32_t u = id; u < full; u += G) {
-                    f32x4 o;
-                    const f32x4 w = weights4(a, u);
 #pragma unroll
-                    for (uint32_t e = 0; e < 4; ++e)
-                        o[e] = static_cast<float>(static_cast<double>(value.hidden(u * 4 + e)) * static_cast<double>(w[e]) * factor);
-                    *as_global(reinterpret_cast<f32x4*>(y) + u) = o;
+                for (int j0 = 0; j0 < V; j0 += N) {
+                    in_turn(id);
+                    if (static_cast<uint32_t>(j0) * G >= full) continue;
+                    typename Row<OP>::Unit p[N], q[N];
+#pragma unroll
+                    for (int j = 0; j < N; ++j) value.unit(min(id + (j0 + j) * G, full - 1), true, p[j], q[j]);
+#pragma unroll
+                    for (int j = 0; j < N; ++j) {
+                        const uint32_t u = id + (j0 + j) * G;
+                        f32x4 o;
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) o[e] = static_cast<float>(value.f64(p[j][e], q[j][e]) * factor);
+                        if (u < full) *as_global(reinterpret_cast<f32x4*>(y) + u) = o;
+                    }
                 }
                 if (const uint32_t e = full * 4 + id; e < a.width) y[e] = static_cast<float>(value(e) * factor);
             }

@@ -156,6 +156,23 @@ def test_quantize_rows_borders(torch):
     equal_codes(*out.get(), x.astype(np.float64))
 
 
+@pytest.mark.parametrize("width", [7, 401, 896, 3584, 18950])
+def test_quantize_rows_ties(torch, width):
+    """Rows of bf16 whose quotients fall on borders by the hundred (127 / 254 of 8-bit values is one half)."""
+    rng = np.random.RandomState(width)
+    m = rng.randint(-255, 256, (40, width)).astype(np.float64)
+    top = np.array([254, 254, 255, 128, 192, 160, 224, 250] * 5, np.float64)
+    m = np.clip(m * np.exp2(-rng.randint(0, 4, m.shape)), -top[:, None], top[:, None])
+    m[:, width // 2] = top
+    x = torch.from_numpy((m * np.exp2(rng.randint(-20, 20, (40, 1)))).astype(np.float32)).cuda().bfloat16()
+    ld = up(width, 8)
+    d = torch.full((40, ld), float("nan"), dtype=torch.bfloat16, device="cuda")
+    d[:, :width] = x
+    out = Codes(torch, 40, width)
+    R.quantize_rows(ptr(d), "bf16", ld, 40, width, *out.args, stream(torch))
+    equal_codes(*out.get(), x.double().cpu().numpy())
+
+
 def test_quantize_rows_many(torch):
     """More rows than one launch of a block each might take at once."""
     x = torch.randn(70001, 16, device="cuda", generator=gen(torch, 1))
@@ -315,6 +332,38 @@ def test_silu_mul_far_values(torch, low, high, size):
     out = Codes(torch, rows, width)
     R.silu_mul(ptr(gate), width, ptr(u), width, rows, width, *out.args, stream(torch))
     check_codes(*out.get(), gate_value(gate.cpu().numpy(), u.double().cpu().numpy()))
+
+
+@pytest.mark.parametrize("width", [5, 16, 2050, 18944, 40000])
+def test_silu_mul_rows_without_values(torch, width):
+    """Rows of zeros, of products that are 0 where f32's are none, and below what a scale holds."""
+    ld = up(width, 4)
+    gate, u = torch.ones(6, ld, device="cuda"), torch.ones(6, ld, device="cuda")
+    gate[0] = 0
+    u[1] = 0
+    gate[2], u[2] = -1e4, 3e38
+    gate[3], u[3] = -1e4, -3e38
+    gate[3, 0], u[3, 0] = 1, 1e-30
+    gate[4], u[4] = -80, 1e-20
+    out = Codes(torch, 6, width)
+    R.silu_mul(ptr(gate), ld, ptr(u), ld, 6, width, *out.args, stream(torch))
+    codes, scales = out.get()
+    check_codes(codes, scales, gate_value(gate[:, :width].cpu().numpy(), u[:, :width].double().cpu().numpy()))
+    assert (scales[:3] == 0).all() and (codes[:3] == 0).all() and scales[4] == 0 and scales[5] > 0
+
+
+def test_add_norm_weights_not_finite(torch):
+    """A weight of infinity makes a row of zeros NaN, and any other."""
+    x, w = torch.zeros(4, 700, device="cuda"), torch.ones(700, device="cuda")
+    x[1:] = torch.randn(3, 700, device="cuda", generator=gen(torch, 8))
+    for bad in (float("inf"), float("-inf")):
+        w[333] = bad
+        y, out = torch.zeros_like(x), Codes(torch, 4, 700)
+        R.add_norm(ptr(x), 700, None, 0, 4, 700, ptr(w), "f32", EPS, None, 0, ptr(y), 700, *out.args, stream(torch))
+        v = norm_value(x.cpu().numpy(), w.double().cpu().numpy())
+        codes, scales = out.get()
+        check_codes(codes, scales, v)
+        assert np.isnan(scales).all() and np.isnan(y[0, 333].item()) and np.isinf(y[1:, 333].cpu().numpy()).all()
 
 
 @pytest.mark.parametrize("g,u", [(float("-inf"), 1.0), (float("inf"), 1.0), (float("nan"), 1.0), (1.0, float("inf")), (-200.0, float("inf")),

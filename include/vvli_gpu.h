@@ -563,7 +563,8 @@ size_t vvli_gpu_verify_drafts_workspace(uint32_t requests, uint32_t vocab);
 /* No counterpart in the reference, whose products take bf16 or f32 weights.
  * For programs with a loop of their own around products: W and X as 8-bit
  * codes with one f32 scale for each row (W: each output channel, X: each
- * token), half of bf16's bytes for few rows and twice its rate for many.
+ * token), half of bf16's bytes where few rows stand, and where many do one
+ * product of integers where vvli_gpu_linear has two of bf16 (it splits X).
  * vvli_gpu_quantize_rows makes codes of any rows (weights, once; attention's
  * output), vvli_gpu_add_norm and vvli_gpu_silu_mul make them of what a
  * transformer block computes in front of its products, vvli_gpu_linear_i8

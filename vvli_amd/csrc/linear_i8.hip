@@ -88,7 +88,7 @@ __device__ __forceinline__ void wait_copies() {
 // block: nothing can come between the reads and it.
 template <int R, int MT>
 __device__ __forceinline__ void read_fragments(i32x4 (&w)[R], i32x4 (&x)[MT], uint32_t wa, uint32_t xa) {
-    static_assert((R == 1 || R == 2) && (MT >= 1 && MT <= 4), "as written");
+    static_assert(MT >= 1 && ((R == 1 && MT <= 3) || (R == 2 && MT <= 4)), "as written");
 #define LDS_W(i, at) "ds_read_b128 %" #i ", %[wa] offset:" #at "\n\t"
 #define LDS_X(i, at) "ds_read_b128 %" #i ", %[xa] offset:" #at "\n\t"
 #define LDS_END "s_waitcnt lgkmcnt(0)"
@@ -97,9 +97,6 @@ __device__ __forceinline__ void read_fragments(i32x4 (&w)[R], i32x4 (&x)[MT], ui
         asm volatile(LDS_W(0, 0) LDS_X(1, 0) LDS_END : "=&v"(w[0]), "=&v"(x[0]) LDS_IN);
     if constexpr (R == 1 && MT == 2)
         asm volatile(LDS_W(0, 0) LDS_X(1, 0) LDS_X(2, 2048) LDS_END : "=&v"(w[0]), "=&v"(x[0]), "=&v"(x[1]) LDS_IN);
-    if constexpr (R == 1 && MT == 4)
-        asm volatile(LDS_W(0, 0) LDS_X(1, 0) LDS_X(2, 2048) LDS_X(3, 4096) LDS_X(4, 6144) LDS_END
-                     : "=&v"(w[0]), "=&v"(x[0]), "=&v"(x[1]), "=&v"(x[2]), "=&v"(x[3]) LDS_IN);
     if constexpr (R == 2 && MT == 1)
         asm volatile(LDS_W(0, 0) LDS_W(1, 2048) LDS_X(2, 0) LDS_END : "=&v"(w[0]), "=&v"(w[1]), "=&v"(x[0]) LDS_IN);
     if constexpr (R == 2 && MT == 2)
@@ -169,10 +166,7 @@ __global__ __launch_bounds__(WV * 64) void linear_i8_stream_kernel(LinearI8Args 
     const uint32_t at = (lane / 16 ^ lane % 8) * 16, ring0 = lds_address(ring);
     const uint32_t wa = lane % 16 * 128 + at, xa = R * 2048 + (XG == 1 ? lane % 8 : lane % 16) * 128 + at;
     for (uint32_t i = 0; i < mine; ++i) {
-        const uint32_t newer = min(mine - 1 - i, static_cast<uint32_t>(ST - 1));
-        if (newer == ST - 1) wait_copies<(ST - 1) * D>();
-        else if (ST > 2 && newer == ST - 2) wait_copies<(ST > 2 ? ST - 2 : 0) * D>();
-        else if (ST > 3 && newer == ST - 3) wait_copies<(ST > 3 ? ST - 3 : 0) * D>();
+        if (i + 1 < mine) wait_copies<(ST - 1) * D>();  // (the next chunk's may be in flight)
         else wait_copies<0>();
         const uint32_t stage = ring0 + i % ST * STAGE;
         i32x4 fw[2][R], fx[2][MT];
@@ -217,7 +211,7 @@ hipError_t allow_lds(const void* kernel, int bytes, std::atomic<uint64_t>& done)
 template <int R, int XG, int ST, int WV>
 hipError_t launch_stream(const LinearI8Args& a, hipStream_t s) {
     constexpr int MT = (XG + 1) / 2, LDS = WV * ST * (2 * R + XG) * 1024;
-    static_assert(LDS <= 160 * 1024 && R * MT <= ST * (2 * R + XG) && ST <= 4, "stages, sums and waits fit");
+    static_assert(LDS <= 160 * 1024 && R * MT <= ST * (2 * R + XG) && ST <= 2, "stages, sums and waits fit");
     const uint64_t tn = (uint64_t{a.N} + 16 * R - 1) / (16 * R), tm = (uint64_t{a.M} + 8 * XG - 1) / (8 * XG);
     static std::atomic<uint64_t> ready{0};
     const hipError_t set = allow_lds(reinterpret_cast<const void*>(linear_i8_stream_kernel<R, XG, ST, WV>), LDS, ready);

@@ -15,13 +15,13 @@
 //     codes. Its unit of 16 bytes is read again, at once, and f64 forms the values
 //     that are in doubt alone (of a wave's 64 units one in 30 holds one, gated one
 //     in 8; of bf16, whose few bits make ties, nine of ten waves do. Read and
-//     formed one after the other, weights took 59 us, gate 100).
+//     formed one after the other, weights took 59 us, gate 10 more).
 // Where f32's error is not the usual one (values that left its normal range) a
 // row is formed in f64 as a whole. Measured (inputs that no cache holds; a copy
 // of 1 GB moves 5.06 TB/s): weights 18944 x 3584 bf16 41.6 us (4.9 TB/s), f32 rows
-// 6001 x 3584 21.3 (5.0), their norm with the sum 61.5 (4.5), gate 2500 x 18944 90.5
-// (4.7; the products, exponentials and packing beside the loads are near as long).
-// One row of 2048: 4.2, 4.6 and 4.8 us, of which 3.8 is a launch.
+// 6001 x 3584 19.4 (5.5), their norm with the sum 55.2 (5.1), gate 2500 x 18944 86.8
+// (4.9; the products, exponentials and packing beside the loads are near as long).
+// One row of 2048: 4.2, 4.5 and 4.4 us, of which 3.8 is a launch.
 #include <algorithm>
 
 #include "device_common.hpp"
@@ -130,6 +130,17 @@ __device__ __forceinline__ f32x4 weights4(const RowsArgs& a, uint32_t u) {
 }
 
 // ---- a row's values ---------------------------------------------------------
+// Rows that are mostly not read again pass the caches, which leaves them to what is stored (norm, us: 6001 x 3584 58.0, so
+// 55.2; 2500 x 18944 128, 114; f32 rows 6001 x 3584 21.3, 19.4). Units in doubt are read again: of bf16 and gated rows
+// they are many (gate 300 x 4864 8.5, with rows so 9.8). Codes stay in the caches for whoever reads them next.
+template <int OP>
+constexpr bool kOnce = OP == kRowsF32 || OP == kRowsNorm;
+template <bool ONCE>
+__device__ __forceinline__ f32x4 read16(const void* p, uint32_t u) {
+    const auto at = as_global(static_cast<const f32x4*>(p) + u);
+    return ONCE ? __builtin_nontemporal_load(at) : *at;
+}
+
 // A value is made of one or two others: of a row's, a hidden value and its weight, or gate and up.
 template <int OP>
 struct Row {
@@ -292,25 +303,29 @@ __global__ __launch_bounds__(WAVES == 1 ? 256 : WAVES * 64, 4) void rows_i8_kern
 #pragma unroll
             for (int j = j0; j < j0 + N; ++j) v[j] = f32x4{0, 0, 0, 0};
             if (static_cast<uint32_t>(j0) * G >= full) continue;  // (the same for all)
+            f32x4 p[N], q[N];
+#pragma unroll
+            for (int j = 0; j < N; ++j) {
+                const uint32_t u = min(id + (j0 + j) * G, full - 1);
+                if constexpr (OP == kRowsBf16) p[j] = read16<false>(static_cast<const uint16_t*>(a.x) + row * a.ldx, u);
+                else p[j] = read16<kOnce<OP>>(value.x, u);
+                if constexpr (OP == kRowsGate || OP == kRowsNorm) q[j] = value.b ? read16<kOnce<OP>>(value.b, u) : f32x4{0, 0, 0, 0};
+            }
 #pragma unroll
             for (int j = j0; j < j0 + N; ++j) {
-                const uint32_t at = id + j * G, u = min(at, full - 1);
-                const bool in = at < full;
-                if constexpr (OP == kRowsBf16) {
-                    v[j] = *as_global(reinterpret_cast<const f32x4*>(static_cast<const uint16_t*>(a.x) + row * a.ldx) + u);
-                } else if constexpr (OP == kRowsGate) {
-                    const f32x4 g = *as_global(reinterpret_cast<const f32x4*>(value.x) + u), b = *as_global(reinterpret_cast<const f32x4*>(value.b) + u);
+                const uint32_t at = id + j * G;
+                v[j] = p[j - j0];
+                if constexpr (OP == kRowsGate) {
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) v[j][e] = gated32(g[e], b[e]), most_u = fmaxf(most_u, fabsf(b[e]));
-                } else {
-                    v[j] = *as_global(reinterpret_cast<const f32x4*>(value.x) + u);
-                    if constexpr (OP == kRowsNorm) {
-                        const f32x4 w = weights4(a, u);
-                        if (value.b) v[j] += *as_global(reinterpret_cast<const f32x4*>(value.b) + u);
-                        if (a.sum && in) *as_global(reinterpret_cast<f32x4*>(a.sum + row * a.lds) + u) = v[j];
+                    for (int e = 0; e < 4; ++e) v[j][e] = gated32(v[j][e], q[j - j0][e]), most_u = fmaxf(most_u, fabsf(q[j - j0][e]));
+                }
+                if constexpr (OP == kRowsNorm) {
+                    const bool in = at < full;
+                    const f32x4 w = weights4(a, min(at, full - 1));
+                    if (value.b) v[j] += q[j - j0];
+                    if (a.sum && in) *as_global(reinterpret_cast<f32x4*>(a.sum + row * a.lds) + at) = v[j];
 #pragma unroll
-                        for (int e = 0; e < 4; ++e) v[j][e] = norm_value(in ? v[j][e] : 0.f, in ? w[e] : 0.f);
-                    }
+                    for (int e = 0; e < 4; ++e) v[j][e] = norm_value(in ? v[j][e] : 0.f, in ? w[e] : 0.f);
                 }
             }
         }
@@ -484,9 +499,9 @@ hipError_t launch_rows(const RowsArgs& a, hipStream_t s) {
 template <int OP>
 int launch(const RowsArgs& a, hipStream_t s) {
     // By the width alone: the fewest waves that hold a row in 4 to 12 units a lane, so that several rows' blocks share a
-    // CU and one's loads run beside another's codes. Norm, us, of waves x units (6001 x 3584: 4 x 4 62, 2 x 8 66, 16 x 4
-    // 165; 2500 x 8192: 4 x 8 57, 8 x 4 60, 16 x 4 94; 300 x 8192: 14.4, 12.0, 17.6; 2500 x 18944: 8 x 12 147, 16 x 8 174;
-    // 75 x 3584: 4 x 4 6.0, 2 x 8 7.5, 8 x 4 6.5; 1 x 2048: 4.8 from 2 waves on, 1 x 8 6.2).
+    // CU and one's loads run beside another's codes. Norm, us, of waves x units (6001 x 3584: 4 x 4 55, 2 x 8 58, 8 x 4
+    // 70; 2500 x 8192: 4 x 8 51, 8 x 4 52, 16 x 4 81; 300 x 8192: 12.7, 12.1, 17.1; 2500 x 18944: 8 x 12 114, 16 x 8 146;
+    // 75 x 3584: 4 x 4 5.6, 2 x 8 6.8, 8 x 4 6.1; 1 x 2048: 4.8 from 2 waves on, 1 x 8 5.8).
     const uint32_t w = a.width;
     hipError_t e;
     if (w <= 1024) e = launch_rows<OP, 1, 4>(a, s);

@@ -321,6 +321,17 @@ def test_silu_mul(torch, width):
         check_codes(*out.get(), gate_value(a[:, :width].cpu().numpy(), a[:, ld:ld + width].double().cpu().numpy()))
 
 
+def test_silu_mul_longer_than_the_caches(torch):
+    """More than 128 MiB of gate and up, of an odd width."""
+    rows, width, ld = 900, 18950, 2 * 18952
+    g = gen(torch, 12)
+    a = torch.randn(rows, ld, device="cuda", generator=g)
+    a[5], a[6, :18952], a[7, 3] = 0, -60, float("inf")
+    out = Codes(torch, rows, width)
+    R.silu_mul(ptr(a), ld, ptr(a) + 4 * 18952, ld, rows, width, *out.args, stream(torch))
+    check_codes(*out.get(), gate_value(a[:, :width].cpu().numpy(), a[:, 18952:18952 + width].double().cpu().numpy()))
+
+
 @pytest.mark.parametrize("low,high,size", [(-120, -60, 1e30), (-104, -80, 1.0), (-95, -85, 3e38), (-700, -80, 1.0), (60, 120, 1e-38),
                                            (-1e-30, 1e-30, 1e-10), (-20, 20, 1e38), (-800, -740, 1e38), (-90, 90, 1e13)])
 def test_silu_mul_far_values(torch, low, high, size):

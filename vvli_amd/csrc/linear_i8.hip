@@ -231,7 +231,7 @@ hipError_t launch_stream(const LinearI8Args& a, hipStream_t s) {
 //
 // What bounds large calls is the card's power: 4096 x 3584 x 18944 runs at 2330 to
 // 2390 TOP/s and 4096 x 37888 x 3584, with 620 MB of Y behind its products, at 2130,
-// the products busy 61 % of the cycles at a clock of 1.75 of 2.4 GHz. A loop of
+// the products busy 60 % of the cycles at a clock of 1.75 to 1.8 of 2.4 GHz. A loop of
 // nothing but these products runs at 3400 TOP/s on random codes (4700 on zeros,
 // which take no power), with its fragments read from LDS at 2700 to 3000.
 //

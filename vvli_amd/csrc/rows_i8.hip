@@ -19,10 +19,11 @@
 // Where f32's error is not the usual one (values that left its normal range) a
 // row is formed in f64 as a whole. Measured (inputs that no cache holds; a copy
 // of 1 GB moves 5.06 TB/s): weights 18944 x 3584 bf16 41.6 us (4.9 TB/s), f32 rows
-// 6001 x 3584 19.4 (5.5), their norm with the sum 55.2 (5.1), gate 2500 x 18944 86.8
-// (4.9; the products, exponentials and packing beside the loads are near as long).
+// 6001 x 3584 19.4 (5.5), their norm with the sum 55.2 (5.1), gate 2500 x 18944 80.1
+// (5.3).
 // One row of 2048: 4.2, 4.5 and 4.4 us, of which 3.8 is a launch.
 #include <algorithm>
+#include <type_traits>
 
 #include "device_common.hpp"
 #include "rows_i8.hpp"
@@ -41,6 +42,7 @@ struct RowsArgs {
     uint64_t ldx, ldb, lds, ldy, ldc;  // elements
     uint32_t rows, width;
     bool weight_bf16;
+    bool once;  // gate and up pass the caches
     float eps;
 };
 
@@ -131,10 +133,11 @@ __device__ __forceinline__ f32x4 weights4(const RowsArgs& a, uint32_t u) {
 
 // ---- a row's values ---------------------------------------------------------
 // Rows that are mostly not read again pass the caches, which leaves them to what is stored (norm, us: 6001 x 3584 58.0, so
-// 55.2; 2500 x 18944 128, 114; f32 rows 6001 x 3584 21.3, 19.4). Units in doubt are read again: of bf16 and gated rows
-// they are many (gate 300 x 4864 8.5, with rows so 9.8). Codes stay in the caches for whoever reads them next.
-template <int OP>
-constexpr bool kOnce = OP == kRowsF32 || OP == kRowsNorm;
+// 55.2; 2500 x 18944 128, 114; f32 rows 6001 x 3584 21.3, 19.4). Units in doubt are read again. Of bf16 rows they are many
+// (18944 x 3584 41.6, so 43.6), and of gated ones, which pass the caches only where they are too long for them to hold
+// (300 x 4864 8.5, so 9.8; 3000 x 4864 31.7, 34.3; 4096 x 8192 58.2, 53.1; 2500 x 18944 86.7, 80.1). Codes stay in the
+// caches for whoever reads them next.
+constexpr uint64_t kOnceBytes = uint64_t{128} << 20;
 template <bool ONCE>
 __device__ __forceinline__ f32x4 read16(const void* p, uint32_t u) {
     const auto at = as_global(static_cast<const f32x4*>(p) + u);
@@ -304,12 +307,22 @@ __global__ __launch_bounds__(WAVES == 1 ? 256 : WAVES * 64, 4) void rows_i8_kern
             for (int j = j0; j < j0 + N; ++j) v[j] = f32x4{0, 0, 0, 0};
             if (static_cast<uint32_t>(j0) * G >= full) continue;  // (the same for all)
             f32x4 p[N], q[N];
+            auto load = [&](auto once) {
 #pragma unroll
-            for (int j = 0; j < N; ++j) {
-                const uint32_t u = min(id + (j0 + j) * G, full - 1);
-                if constexpr (OP == kRowsBf16) p[j] = read16<false>(static_cast<const uint16_t*>(a.x) + row * a.ldx, u);
-                else p[j] = read16<kOnce<OP>>(value.x, u);
-                if constexpr (OP == kRowsGate || OP == kRowsNorm) q[j] = value.b ? read16<kOnce<OP>>(value.b, u) : f32x4{0, 0, 0, 0};
+                for (int j = 0; j < N; ++j) {
+                    const uint32_t u = min(id + (j0 + j) * G, full - 1);
+                    if constexpr (OP == kRowsBf16) p[j] = read16<once>(static_cast<const uint16_t*>(a.x) + row * a.ldx, u);
+                    else p[j] = read16<once>(value.x, u);
+                    if constexpr (OP == kRowsGate || OP == kRowsNorm) q[j] = value.b ? read16<once>(value.b, u) : f32x4{0, 0, 0, 0};
+                }
+            };
+            if constexpr (OP != kRowsGate) {
+                load(std::bool_constant<OP != kRowsBf16>{});
+            } else if (a.once) {
+                load(std::true_type{});
+                in_turn(id);  // (else the compiler makes both branches one)
+            } else {
+                load(std::false_type{});
             }
 #pragma unroll
             for (int j = j0; j < j0 + N; ++j) {
@@ -497,7 +510,8 @@ hipError_t launch_rows(const RowsArgs& a, hipStream_t s) {
 }
 
 template <int OP>
-int launch(const RowsArgs& a, hipStream_t s) {
+int launch(RowsArgs a, hipStream_t s) {
+    a.once = uint64_t{a.rows} * a.width * 8 > kOnceBytes;
     // By the width alone: the fewest waves that hold a row in 4 to 12 units a lane, so that several rows' blocks share a
     // CU and one's loads run beside another's codes. Norm, us, of waves x units (6001 x 3584: 4 x 4 55, 2 x 8 58, 8 x 4
     // 70; 2500 x 8192: 4 x 8 51, 8 x 4 52, 16 x 4 81; 300 x 8192: 12.7, 12.1, 17.1; 2500 x 18944: 8 x 12 114, 16 x 8 146;

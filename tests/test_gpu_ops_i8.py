@@ -17,7 +17,7 @@ with n <= 70000 under 2^-36 relative, so that
 """
 import numpy as np
 import pytest
-from test_ops_i8 import CUT, ODD
+from test_ops_i8 import CUT, LONG, ODD
 
 from vvli_amd import runtime as R
 
@@ -455,6 +455,16 @@ def test_linear_i8_every_kernel(torch, M, N, K):
         for _ in range(2):
             p.run()
             p.check()
+
+
+@pytest.mark.parametrize("M,N,K", LONG)
+def test_linear_i8_long_results(torch, M, N, K):
+    p = Product(torch, M, N, K, True, pady=3, seed=6)
+    want = p.want()
+    for _ in range(2):
+        p.run()
+        assert torch.equal(p.Y[:M, :N], want) and (p.Y[M:] == 55).all() and (p.Y[:, N:] == 55).all()
+        p.Y.fill_(55.0)
 
 
 @pytest.mark.parametrize("M", [1, 5, 20, 70, 300])

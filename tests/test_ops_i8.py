@@ -175,11 +175,18 @@ ODD = [(1, 33, 432), (5, 413, 2672), (35, 39, 624), (109, 365, 1120), (153, 43, 
 # Two launches of columns, the second a split K, a stream and small tiles.
 CUT = [(393, 32779, 3616), (537, 21815, 4688), (409, 33031, 1728), (431, 37029, 1072), (387, 33589, 1296)]
 
+# Results of more than 128 MiB by each of the large tiles (the last two: in two launches).
+LONG = [(3551, 9743, 112), (37293, 909, 192), (683, 49517, 224), (13293, 2641, 928), (11015, 3213, 880), (645, 54647, 912),
+        (1161, 29417, 1232), (669, 51443, 1168)]
+
 
 def test_odd_sizes_reach_every_kernel(plan):
     got = plan([(m, n, k, max(k, 4 * n), 256) for m, n, k in ODD])
     assert {g[0] for g in got} == set(range(got[0][8])) and not any(g[9] for g in got)
-    assert all(g[9] for g in plan([(m, n, k, 4 * n, 256) for m, n, k in CUT]))
+    assert all(g[9] for g in plan([(m, n, k, 4 * n, 256) for m, n, k in CUT + LONG[-2:]]))
+    assert all(m * n * 4 > 128 << 20 for m, n, _ in LONG)
+    tiles = {(g[4], g[5]) for g in plan([(m, n, k, 4 * n, 256) for m, n, k in LONG])}
+    assert tiles == {(2, 2), (3, 2), (4, 2), (3, 4), (4, 3), (4, 4)}
 
 
 def test_every_kernel_is_taken_somewhere(plan):

@@ -37,9 +37,14 @@ struct LinearI8Args {
     uint32_t split_steps;  // steps of 128 codes of a part of K
     int* parts;            // [part][M][N]
     bool vector;  // Y's rows and w_scales at 16-byte addresses
+    bool long_y;  // Y passes the caches
 };
 
-constexpr int kOnce = 2;  // cache policy of copies of what is read once: nontemporal
+constexpr int kOnce = 2;  // cache policy of what passes the caches: nontemporal
+// Y that they would not hold till it is read leaves them to W and X (us: 4096 x 37888 x 3584 523, so 507; 2048 x 37888 x
+// 3584 270, 265; 4096 x 9728 x 896 72.6, 55.1). Shorter ones are read next out of them (a layer's five calls on 64 rows
+// 67.4, so 69.7; on 4096 rows, whose Y is longer, the same either way).
+constexpr uint64_t kLongY = uint64_t{128} << 20;
 constexpr uint32_t kMostK = 131056;  // 131056 * 128 * 128 < 2^31
 
 __device__ __forceinline__ float finish(int sum, float x_scale, float w_scale, float bias) {
@@ -252,7 +257,7 @@ hipError_t launch_stream(const LinearI8Args& a, hipStream_t s) {
 // its way lasts as long.
 //
 // SPLIT: a block has a part of K and leaves its sums, 32-bit integers, for
-// linear_i8_join_kernel.
+// linear_i8_join_kernel. LONG: Y passes the caches.
 constexpr int kTileThreads = 256;
 constexpr uint32_t kBufferBytes = 1u << 31;  // a tile's rows are below it: copies of zeros point behind it
 
@@ -294,7 +299,7 @@ struct TileShape {
     static_assert(Lds <= 160 * 1024, "stages fit");
 };
 
-template <int RN, int RM, int ST, bool SPLIT>
+template <int RN, int RM, int ST, bool SPLIT, bool LONG>
 __global__ __launch_bounds__(kTileThreads, RN * RM >= 9 ? 1 : 2) void linear_i8_tile_kernel(LinearI8Args a) {
     using S = TileShape<RN, RM, ST>;
     constexpr int WG = 2 * RN, XG = 2 * RM;  // copies of a wave a step
@@ -428,7 +433,7 @@ __global__ __launch_bounds__(kTileThreads, RN * RM >= 9 ? 1 : 2) void linear_i8_
             for (int r = 0; r < RN; ++r) {
                 uint32_t value = sum[r][c][e];
                 if constexpr (!SPLIT) value = __float_as_uint(finish(sum[r][c][e], x_scale[c][e / 4][e % 4], w_scale[r], bias[r]));
-                __builtin_amdgcn_raw_buffer_store_b32(value, Y, y_at[r], down, 0);
+                __builtin_amdgcn_raw_buffer_store_b32(value, Y, y_at[r], down, LONG ? kOnce : 0);
             }
         }
 }
@@ -452,14 +457,18 @@ __global__ __launch_bounds__(256) void linear_i8_join_kernel(LinearI8Args a, uin
     }
 }
 
-template <int RN, int RM, int ST>
+template <int RN, int RM, int ST, bool LONG = false>
 hipError_t launch_tile(const LinearI8Args& a, hipStream_t s) {
     using S = TileShape<RN, RM, ST>;
+    if constexpr (!LONG && RN * RM >= 4 && ST == 2) {  // (others hardly ever have a long Y)
+        if (a.long_y) return launch_tile<RN, RM, ST, true>(a, s);
+    }
     const uint64_t tiles = ((uint64_t{a.N} + S::N - 1) / S::N) * ((uint64_t{a.M} + S::M - 1) / S::M);
     static std::atomic<uint64_t> ready{0};
-    const hipError_t set = allow_lds(reinterpret_cast<const void*>(linear_i8_tile_kernel<RN, RM, ST, false>), S::Lds, ready);
+    const auto kernel = linear_i8_tile_kernel<RN, RM, ST, false, LONG>;
+    const hipError_t set = allow_lds(reinterpret_cast<const void*>(kernel), S::Lds, ready);
     if (set != hipSuccess) return set;
-    return vlaunch(linear_i8_tile_kernel<RN, RM, ST, false>, dim3(static_cast<uint32_t>(tiles)), dim3(kTileThreads), S::Lds, s, a);
+    return vlaunch(kernel, dim3(static_cast<uint32_t>(tiles)), dim3(kTileThreads), S::Lds, s, a);
 }
 // K in `splits` parts (at most; each has steps), their sums in the workspace.
 template <int RN, int RM, int ST>
@@ -467,11 +476,11 @@ hipError_t launch_tile_split(LinearI8Args a, uint32_t splits, hipStream_t s) {
     using S = TileShape<RN, RM, ST>;
     const uint32_t tiles = ((a.N + S::N - 1) / S::N) * ((a.M + S::M - 1) / S::M), steps = (a.K + 127) / 128;
     static std::atomic<uint64_t> ready{0};
-    const hipError_t set = allow_lds(reinterpret_cast<const void*>(linear_i8_tile_kernel<RN, RM, ST, true>), S::Lds, ready);
+    const hipError_t set = allow_lds(reinterpret_cast<const void*>(linear_i8_tile_kernel<RN, RM, ST, true, false>), S::Lds, ready);
     if (set != hipSuccess) return set;
     a.split_steps = (steps + splits - 1) / splits;
     splits = (steps + a.split_steps - 1) / a.split_steps;
-    const hipError_t e = vlaunch(linear_i8_tile_kernel<RN, RM, ST, true>, dim3(tiles, splits), dim3(kTileThreads), S::Lds, s, a);
+    const hipError_t e = vlaunch(linear_i8_tile_kernel<RN, RM, ST, true, false>, dim3(tiles, splits), dim3(kTileThreads), S::Lds, s, a);
     if (e != hipSuccess) return e;
     const uint32_t quads = (a.N + 3) / 4 * a.M;
     return vlaunch(linear_i8_join_kernel, dim3(std::min((quads + 255) / 256, 2048u)), dim3(256), 0, s, a, splits);
@@ -544,7 +553,7 @@ int vvli_gpu_linear_i8(const int8_t* W, uint64_t ldw, const float* w_scales, con
     a.W = W, a.X = X, a.w_scales = w_scales, a.x_scales = x_scales, a.bias = bias, a.Y = Y;
     a.ldw = ldw, a.ldx = ldx, a.ldy = ldy, a.M = M, a.N = N, a.K = K;
     a.parts = static_cast<int*>(workspace);
-    a.vector = aligned16(Y) && ldy % 4 == 0 && aligned16(w_scales);
+    a.vector = aligned16(Y) && ldy % 4 == 0 && aligned16(w_scales), a.long_y = uint64_t{M} * N * 4 > kLongY;
     const hipStream_t st = static_cast<hipStream_t>(stream);
     PAGED_TRY(launch_linear(a, st));
     return VVLI_OK;

@@ -10,7 +10,7 @@
 // moves 5.4 TB/s, a library product of 8192 cubed 2466 TOP/s): 1 x 37888 x 3584 22.0
 // (6.2 TB/s), 5 x 2048 x 8192 6.2, 48 x 4608 x 3584 8.4, 128 x 37888 x 3584 37 (4.2
 // TB/s), 333 x 896 x 4864 9.7, 2048 x 4608 x 3584 41 (1640 TOP/s), 4096 x 3584 x
-// 18944 238 (2330), 4096 x 37888 x 3584 516 (2150).
+// 18944 230 to 238 (2340 to 2420), 4096 x 37888 x 3584 507 (2190).
 #include <algorithm>
 #include <atomic>
 #include <type_traits>
@@ -235,7 +235,7 @@ hipError_t launch_stream(const LinearI8Args& a, hipStream_t s) {
 // large tiles would leave CUs idle.
 //
 // What bounds large calls is the card's power: 4096 x 3584 x 18944 runs at 2330 to
-// 2390 TOP/s and 4096 x 37888 x 3584, with 620 MB of Y behind its products, at 2130,
+// 2390 TOP/s and 4096 x 37888 x 3584, with 620 MB of Y behind its products, at 2190,
 // the products busy 60 % of the cycles at a clock of 1.75 to 1.8 of 2.4 GHz. A loop of
 // nothing but these products runs at 3400 TOP/s on random codes (4700 on zeros,
 // which take no power), with its fragments read from LDS at 2700 to 3000.

@@ -86,6 +86,16 @@ def test_add_norm_refusals(bad, name):
     refused(norm, name, **bad)
 
 
+@pytest.mark.parametrize("place", [P, Q], ids=["x", "delta"])
+@pytest.mark.parametrize("rows", [1, 3])
+@pytest.mark.parametrize("others", [dict(total=None), dict(), dict(total=None, y=3 * U, ldy=64), dict(y=3 * U, ldy=64)],
+                         ids=["codes alone", "sum", "y", "sum and y"])
+def test_add_norm_refuses_codes_in_place(place, rows, others):
+    """sum and y may lie where x or delta does, codes may not, whatever their stride."""
+    for ldc in (64, 128, 256, 512):
+        refused(norm, CONFIG, codes=place, ldc=ldc, rows=rows, **others)
+
+
 def test_add_norm_unknown_weight_kind():
     from vvli_amd import _lib
 

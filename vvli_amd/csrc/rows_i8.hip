@@ -548,9 +548,11 @@ int check_sizes(uint32_t rows, uint32_t width, const char* who) {
 struct Outputs {  // what a call writes, and whether an input meets it
     RowBytes at[4];
     const char* name[4];
+    bool in_place[4];
     int n = 0;
-    void add(const void* p, uint64_t ld, uint64_t width, uint64_t rows, const char* what) {
-        if (p) at[n] = RowBytes{p, ld, width, rows}, name[n++] = what;
+    // may: the output may be an input itself, with its stride (each value is read before its place is written)
+    void add(const void* p, uint64_t ld, uint64_t width, uint64_t rows, const char* what, bool may = false) {
+        if (p) at[n] = RowBytes{p, ld, width, rows}, in_place[n] = may, name[n++] = what;
     }
     int each_other(const char* who) const {
         for (int i = 0; i < n; ++i)
@@ -558,10 +560,9 @@ struct Outputs {  // what a call writes, and whether an input meets it
                 if (rows_meet(at[i], at[j])) return set_error(VVLI_INVALID_CONFIG, "%s: %s overlaps %s", who, name[i], name[j]);
         return VVLI_OK;
     }
-    // same: an output that is the input itself, with its stride, is fine (each value is read before its place is written)
-    int input(const RowBytes& in, bool same, const char* what, const char* who) const {
+    int input(const RowBytes& in, const char* what, const char* who) const {
         for (int i = 0; i < n; ++i)
-            if (rows_meet(at[i], in) && !(same && at[i].p == in.p && at[i].ld == in.ld))
+            if (rows_meet(at[i], in) && !(in_place[i] && at[i].p == in.p && at[i].ld == in.ld))
                 return set_error(VVLI_INVALID_CONFIG, "%s: %s overlaps %s", who, name[i], what);
         return VVLI_OK;
     }
@@ -582,7 +583,7 @@ int vvli_gpu_quantize_rows(const void* x, uint32_t kind, uint64_t ldx, uint32_t 
         return rc;
     Outputs out;
     out.add(codes, ldc, padded(width), rows, "codes"), out.add(scales, 4, 4, rows, "scales");
-    if ((rc = out.each_other(who)) || (rc = out.input(RowBytes{x, ldx * e, uint64_t{width} * e, rows}, false, "x", who))) return rc;
+    if ((rc = out.each_other(who)) || (rc = out.input(RowBytes{x, ldx * e, uint64_t{width} * e, rows}, "x", who))) return rc;
     if (rows == 0) return VVLI_OK;
     RowsArgs a{};
     a.x = x, a.scales = scales, a.codes = codes, a.ldx = ldx, a.ldc = ldc, a.rows = rows, a.width = width;
@@ -610,12 +611,12 @@ int vvli_gpu_add_norm(const float* x, uint64_t ldx, const float* delta, uint64_t
     }
     const uint64_t w = uint64_t{width} * 4;
     Outputs out;
-    out.add(sum, lds * 4, w, rows, "sum"), out.add(y, ldy * 4, w, rows, "y");
+    out.add(sum, lds * 4, w, rows, "sum", true), out.add(y, ldy * 4, w, rows, "y", true);
     out.add(codes, ldc, padded(width), rows, "codes"), out.add(scales, 4, 4, rows, "scales");
     const uint64_t wb = uint64_t{width} * (weight_kind == VVLI_WEIGHT_BF16 ? 2 : 4);
-    if ((rc = out.each_other(who)) || (rc = out.input(RowBytes{x, ldx * 4, w, rows}, true, "x", who)) ||
-        (rc = out.input(RowBytes{delta, ldd * 4, w, rows}, true, "delta", who)) ||
-        (rc = out.input(RowBytes{weight, wb, wb, 1}, false, "weight", who)))
+    if ((rc = out.each_other(who)) || (rc = out.input(RowBytes{x, ldx * 4, w, rows}, "x", who)) ||
+        (rc = out.input(RowBytes{delta, ldd * 4, w, rows}, "delta", who)) ||
+        (rc = out.input(RowBytes{weight, wb, wb, 1}, "weight", who)))
         return rc;
     if (rows == 0) return VVLI_OK;
     RowsArgs a{};
@@ -635,8 +636,8 @@ int vvli_gpu_silu_mul(const float* gate, uint64_t ldg, const float* up, uint64_t
     const uint64_t w = uint64_t{width} * 4;
     Outputs out;
     out.add(codes, ldc, padded(width), rows, "codes"), out.add(scales, 4, 4, rows, "scales");
-    if ((rc = out.each_other(who)) || (rc = out.input(RowBytes{gate, ldg * 4, w, rows}, false, "gate", who)) ||
-        (rc = out.input(RowBytes{up, ldu * 4, w, rows}, false, "up", who)))
+    if ((rc = out.each_other(who)) || (rc = out.input(RowBytes{gate, ldg * 4, w, rows}, "gate", who)) ||
+        (rc = out.input(RowBytes{up, ldu * 4, w, rows}, "up", who)))
         return rc;
     if (rows == 0) return VVLI_OK;
     RowsArgs a{};

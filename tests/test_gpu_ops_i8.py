@@ -387,6 +387,53 @@ def test_silu_mul_not_finite(torch, g, u):
     check_codes(*out.get(), gate_value(gate.cpu().numpy(), up_.double().cpu().numpy()))
 
 
+# Bits of NaN other than those that arithmetic makes: low bits set, a sign, signaling ones.
+NANS = [0x7FC000A5, 0xFFC0FFFF, 0x7F8000A5, 0x7FFFFFFF]
+
+
+def nan_of(torch, bits):
+    return torch.tensor([bits - (1 << 32) if bits >> 31 else bits], dtype=torch.int32, device="cuda").view(torch.float32)
+
+
+@pytest.mark.parametrize("bits", NANS, ids=hex)
+@pytest.mark.parametrize("width", [1, 5, 17, 1025, 2047, 4099, 18945, 40001])
+def test_nans_of_any_bits(torch, width, bits):
+    """A row with a NaN has scale NaN and codes 0, zeros behind its width among them, whatever the NaN's bits."""
+    rows, ld, nan = 4, up(width, 8), nan_of(torch, bits)
+    g = gen(torch, width + 2)
+    x, d = (torch.randn(rows, ld, device="cuda", generator=g) for _ in range(2))
+    bad = x.clone()
+    bad.view(torch.int32)[1, width // 2] = nan.view(torch.int32)
+    bad.view(torch.int32)[2, width - 1] = nan.view(torch.int32)
+    half = bad.bfloat16()
+    half.view(torch.int16)[1:3, width // 2] = nan.view(torch.int32).item() >> 16 | 1  # (a signaling one's low bits are cut off)
+    w = torch.randn(ld, device="cuda", generator=g)
+    w_nan, w_half = w.clone(), w.bfloat16()
+    w_nan.view(torch.int32)[width // 2] = nan.view(torch.int32)
+    w_half.view(torch.int16)[width // 2] = nan.view(torch.int32).item() >> 16 | 1
+
+    def looked_at(call, want):
+        out = Codes(torch, rows, width, 1)
+        call(out)
+        codes, scales = out.get()
+        assert np.array_equal(np.isnan(scales), want), scales
+        assert (codes[want] == 0).all()
+
+    some, every = np.array([False, True, True, False]), np.ones(rows, bool)
+    s = stream(torch)
+    looked_at(lambda o: R.quantize_rows(ptr(bad), "f32", ld, rows, width, *o.args, s), some)
+    looked_at(lambda o: R.quantize_rows(ptr(half), "bf16", ld, rows, width, *o.args, s), some)
+    looked_at(lambda o: R.silu_mul(ptr(bad), ld, ptr(x), ld, rows, width, *o.args, s), some)
+    looked_at(lambda o: R.silu_mul(ptr(x), ld, ptr(bad), ld, rows, width, *o.args, s), some)
+    total, y = torch.zeros(rows, ld, device="cuda"), torch.zeros(rows, ld, device="cuda")
+    for a, b in ((bad, None), (bad, d), (x, bad), (bad, bad)):
+        looked_at(lambda o: R.add_norm(ptr(a), ld, ptr(b), ld, rows, width, ptr(w), "f32", EPS, ptr(total) if b is not None else None, ld,
+                                       ptr(y), ld, *o.args, s), some)
+        assert torch.isnan(y[1:3, :width]).all() and torch.isfinite(y[[0, 3]]).all()
+    for kind, t in (("f32", w_nan), ("bf16", w_half)):
+        looked_at(lambda o: R.add_norm(ptr(x), ld, None, 0, rows, width, ptr(t), kind, EPS, None, 0, None, 0, *o.args, s), every)
+
+
 # ---------------------------------------------------------------------------
 # linear_i8
 # ---------------------------------------------------------------------------

@@ -421,7 +421,9 @@ __global__ __launch_bounds__(WAVES == 1 ? 256 : WAVES * 64, 4) void rows_i8_kern
             }
             exact = reduce<WAVES>(exact, Max(), part_d);
         }
-        const float scale = scale_of(exact), quotient = scale == 0 ? 0.f : static_cast<float>(factor / static_cast<double>(scale));
+        // (0 beside a scale of 0 or NaN: the zeros behind the width are stored as they come, and a norm's NaN would bring
+        // its bits into them.)
+        const float scale = scale_of(exact), quotient = scale > 0 ? static_cast<float>(factor / static_cast<double>(scale)) : 0.f;
         // (Rows of zeros, padding mostly, have no codes to settle: f32's values are finite there, a norm's below 2^-15.)
         usual = scale == 0 ? OP == kRowsNorm || top < INFINITY : usual && scale >= 0x1p-126f;
         int8_t* const codes = a.codes ? a.codes + row * a.ldc : nullptr;

@@ -820,3 +820,64 @@ def test_calls_repeat_to_the_bit(torch, rows):
         first = first or state
         for a, b in zip(first, state):
             assert torch.equal(a, b)
+
+
+# ---------------------------------------------------------------------------
+# The ends of each kernel's widths, up to the widest rows that registers hold
+# ---------------------------------------------------------------------------
+EDGES = [2048, 2049, 4097, 8193, 16385, 24571, 24576, 24577, 24592, 28001, 32765, 32768, 32769, 32784]
+
+
+def far_rows(torch, width, ld, seed):
+    """Rows whose largest value is one of the last, another one of each (so that a value that is dropped shows in all)."""
+    x = torch.randn(5, ld, device="cuda", generator=gen(torch, seed))
+    x[:, width:] = float("nan")
+    for r in range(5):
+        x[r, max(0, width - 1 - 3 * r)] = 20.0 + r
+    return x
+
+
+@pytest.mark.parametrize("kind", ["f32", "bf16"])
+@pytest.mark.parametrize("width", EDGES)
+def test_quantize_rows_at_the_ends_of_widths(torch, width, kind):
+    ld = up(width, 8) + 8
+    x = far_rows(torch, width, ld, width)
+    x = x if kind == "f32" else x.bfloat16()
+    out = Codes(torch, 5, width, 1)
+    R.quantize_rows(ptr(x), kind, ld, 5, width, *out.args, stream(torch))
+    equal_codes(*out.get(), x[:, :width].double().cpu().numpy())
+
+
+@pytest.mark.parametrize("place", ["apart", "sum is x", "y is x", "y is delta, sum is x", "y is x, no sum", "y is delta, no sum"])
+@pytest.mark.parametrize("width", EDGES)
+def test_add_norm_at_the_ends_of_widths(torch, width, place):
+    ld = up(width, 4) + 4
+    g = gen(torch, width + 3)
+    x, d = far_rows(torch, width, ld, width + 1), torch.randn(5, ld, device="cuda", generator=g)
+    w = (1 + 0.3 * torch.randn(width, device="cuda", generator=g)).to(torch.bfloat16 if width % 2 else torch.float32)
+    h = (x + d)[:, :width].cpu().numpy()
+    other, more = torch.full((5, ld), 77.0, device="cuda"), torch.full((5, ld), 77.0, device="cuda")
+    total, y = {"apart": (other, more), "sum is x": (x, None), "y is x": (other, x), "y is delta, sum is x": (x, d),
+                "y is x, no sum": (None, x), "y is delta, no sum": (None, d)}[place]
+    behind = [None if t is None else t[:, width:].cpu().numpy() for t in (total, y)]
+    out = Codes(torch, 5, width, 1)
+    R.add_norm(ptr(x), ld, ptr(d), ld, 5, width, ptr(w), "bf16" if width % 2 else "f32", EPS, ptr(total), ld, ptr(y), ld, *out.args,
+               stream(torch))
+    v = norm_value(h, w.double().cpu().numpy())
+    check_codes(*out.get(), v)
+    if total is not None:
+        assert np.array_equal(total[:, :width].cpu().numpy(), h)
+    if y is not None:
+        check_y(y[:, :width].double().cpu().numpy(), v)
+    for t, b in zip((total, y), behind):
+        assert t is None or np.array_equal(t[:, width:].cpu().numpy(), b, equal_nan=True)
+
+
+@pytest.mark.parametrize("width", EDGES)
+def test_silu_mul_at_the_ends_of_widths(torch, width):
+    ld = up(width, 4) + 4
+    gate, u = far_rows(torch, width, ld, width + 4), far_rows(torch, width, ld, width + 5)
+    gate[4, :width] *= 60  # gates of -150 and less
+    out = Codes(torch, 5, width, 1)
+    R.silu_mul(ptr(gate), ld, ptr(u), ld, 5, width, *out.args, stream(torch))
+    check_codes(*out.get(), gate_value(gate[:, :width].cpu().numpy(), u[:, :width].double().cpu().numpy()))

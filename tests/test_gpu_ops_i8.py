@@ -17,7 +17,7 @@ with n <= 70000 under 2^-36 relative, so that
 """
 import numpy as np
 import pytest
-from test_ops_i8 import CUT, LONG, ODD
+from test_ops_i8 import CUT, LONG, ODD, SPLIT
 
 from vvli_amd import runtime as R
 
@@ -881,3 +881,85 @@ def test_silu_mul_at_the_ends_of_widths(torch, width):
     out = Codes(torch, 5, width, 1)
     R.silu_mul(ptr(gate), ld, ptr(u), ld, 5, width, *out.args, stream(torch))
     check_codes(*out.get(), gate_value(gate[:, :width].cpu().numpy(), u[:, :width].double().cpu().numpy()))
+
+
+# ---------------------------------------------------------------------------
+# Workspaces that calls leave parts of K in
+# ---------------------------------------------------------------------------
+class Space:
+    """A workspace of what calls of these sizes ask for, with marks behind it."""
+
+    def __init__(self, torch, sizes):
+        self.bytes = max(R.linear_i8_workspace(*s) for s in sizes)
+        self.all = torch.full((self.bytes + 4096,), 7, dtype=torch.uint8, device="cuda")
+        self.part = self.all[: self.bytes]
+
+    def fill(self, torch, seed):
+        self.part.random_(0, 256, generator=gen(torch, seed))
+
+    def check(self):
+        assert (self.all[self.bytes:] == 7).all(), "written behind the workspace"
+
+
+@pytest.mark.parametrize("size", SPLIT)
+def test_linear_i8_writes_no_more_than_its_workspace(torch, size):
+    space = Space(torch, [size])
+    p = Product(torch, *size, bias=True, space=space.part, seed=7)
+    for i in range(2):
+        space.fill(torch, i)
+        p.run()
+        p.check()
+    space.check()
+
+
+def test_linear_i8_one_workspace_for_parts_of_all_sizes(torch):
+    """A workspace made for the largest call serves calls with parts and without, in any order, whatever is in it."""
+    sizes = [s for pair in zip(SPLIT, [(1, 2048, 2048), (5, 40, 131056), (48, 1152, 8192), (129, 300, 4096)] * 3) for s in pair]
+    space = Space(torch, sizes)
+    products = [Product(torch, *s, bias=i % 3 == 0, pady=i % 2, space=space.part, seed=i) for i, s in enumerate(sizes)]
+    for turn in range(3):
+        space.fill(torch, turn)
+        for p in products:
+            p.run()
+        torch.cuda.synchronize()
+        for p in products:
+            p.check()
+        products = products[::-1] if turn else products[7:] + products[:7]
+    space.check()
+
+
+@pytest.mark.parametrize("first,second", [(0, 1), (2, 4), (3, 5), (6, 0), (7, 8)])
+def test_linear_i8_parts_on_two_streams(torch, first, second):
+    """Calls with parts that overlap, a workspace each."""
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    products = [Product(torch, *SPLIT[i], seed=8) for i in (first, second)]
+    torch.cuda.synchronize()
+    for _ in range(10):
+        for p, s in zip(products, streams):
+            p.run(s.cuda_stream)
+    torch.cuda.synchronize()
+    for p in products:
+        p.check()
+
+
+def test_linear_i8_two_graphs_with_one_workspace(torch):
+    """Graphs that are replayed one after the other may share it, with eager calls on it in between."""
+    sizes = [SPLIT[0], SPLIT[1], SPLIT[4], SPLIT[5]]
+    space = Space(torch, sizes)
+    products = [Product(torch, *s, bias=True, space=space.part, seed=20 + i) for i, s in enumerate(sizes)]
+    graphs = [torch.cuda.CUDAGraph() for _ in range(2)]
+    for graph, part in zip(graphs, (products[:2], products[2:])):
+        with torch.cuda.graph(graph):
+            for p in part:
+                p.run()
+    eager = Product(torch, *SPLIT[6], space=space.part, seed=30)
+    for i in range(4):
+        for p in products:
+            p.X.copy_(p.X.roll(i, 0))
+        for graph in graphs[:: 1 if i % 2 else -1]:
+            graph.replay()
+            eager.run()
+        torch.cuda.synchronize()
+        for p in products + [eager]:
+            p.check()
+    space.check()

@@ -282,3 +282,18 @@ def test_rows_that_share_bytes_are_found(tmp_path):
         else:
             beside += ranges
     assert met > 100 and beside > 50
+
+
+# Calls that leave parts of K in their workspace: tiles of each of the three sizes that have them, rows of results that are
+# whole units and not.
+SPLIT = [(311, 401, 6768), (687, 875, 14512), (300, 64, 131056), (623, 3541, 16112), (133, 21, 9328), (181, 5555, 10272),
+         (61, 33, 18576), (448, 3584, 18944), (256, 3584, 18944)]
+
+
+def test_split_sizes_leave_parts(plan):
+    got = plan([(m, n, k, max(k, 4 * n), 256) for m, n, k in SPLIT])
+    assert all(g[1] > 1 and g[6] for g in got)
+    assert {(g[4], g[5]) for g in got} == {(1, 1), (2, 2), (4, 4)}
+    assert {n % 4 == 0 for _, n, _ in SPLIT} == {True, False}
+    for (m, n, k), g in zip(SPLIT, got):
+        assert 0 < g[1] * m * n * 4 <= R.linear_i8_workspace(m, n, k)

@@ -17,7 +17,7 @@ with n <= 70000 under 2^-36 relative, so that
 """
 import numpy as np
 import pytest
-from test_ops_i8 import CUT, LONG, ODD, SPLIT
+from test_ops_i8 import CUT, FAR, FAR_STRIDE, LONG, ODD, SPLIT
 
 from vvli_amd import runtime as R
 
@@ -963,3 +963,25 @@ def test_linear_i8_two_graphs_with_one_workspace(torch):
         for p in products + [eager]:
             p.check()
     space.check()
+
+
+# ---------------------------------------------------------------------------
+# Rows far apart, and more of them than a launch takes
+# ---------------------------------------------------------------------------
+@pytest.mark.parametrize("which", ["W", "X", "Y"])
+@pytest.mark.parametrize("M,N,K", FAR)
+def test_linear_i8_strides_over_4_MiB(torch, M, N, K, which):
+    p = Product(torch, M, N, K, bias=True, pady=FAR_STRIDE // 4 - N if which == "Y" else 0, seed=9)
+    if which != "Y":
+        tight = getattr(p, which)
+        far = torch.zeros(len(tight), FAR_STRIDE, dtype=torch.int8, device="cuda")
+        far[:, :K] = tight
+        far[:, K:K + 64] = 99
+        setattr(p, which, far)
+        p.strides = tuple(FAR_STRIDE if n == which else s for n, s in zip("WXY", p.strides))
+    want = p.want()
+    for _ in range(2):
+        p.run()
+        assert torch.equal(p.Y[:M, :N], want)
+        assert (p.Y[:M, N:] == 55).all() and (p.Y[M:] == 55).all()
+        p.Y.fill_(55.0)

@@ -297,3 +297,13 @@ def test_split_sizes_leave_parts(plan):
     assert {n % 4 == 0 for _, n, _ in SPLIT} == {True, False}
     for (m, n, k), g in zip(SPLIT, got):
         assert 0 < g[1] * m * n * 4 <= R.linear_i8_workspace(m, n, k)
+
+
+# Sizes (M, N, K) with a stride of more than 4 MiB of W, X or Y, whose rows of a tile are behind what a tile's offsets reach.
+FAR_STRIDE = (1 << 22) + 16  # bytes
+FAR = [(33, 300, 64), (40, 65, 1040), (300, 40, 64), (300, 300, 1040), (1000, 33, 272)]
+
+
+def test_far_strides_take_streams(plan):
+    for ld, kinds in ((FAR_STRIDE, {0}), (1 << 22, {0, 1})):
+        assert {g[3] for g in plan([(m, n, k, ld, 256) for m, n, k in FAR])} == kinds

@@ -17,7 +17,7 @@ with n <= 70000 under 2^-36 relative, so that
 """
 import numpy as np
 import pytest
-from test_ops_i8 import CUT, FAR, FAR_STRIDE, LONG, ODD, SPLIT
+from test_ops_i8 import CUT, FAR, FAR_STRIDE, HUGE, LONG, ODD, SPLIT
 
 from vvli_amd import runtime as R
 
@@ -985,3 +985,18 @@ def test_linear_i8_strides_over_4_MiB(torch, M, N, K, which):
         assert torch.equal(p.Y[:M, :N], want)
         assert (p.Y[:M, N:] == 55).all() and (p.Y[M:] == 55).all()
         p.Y.fill_(55.0)
+
+
+@pytest.mark.parametrize("M,N,K", HUGE)
+def test_linear_i8_more_blocks_than_a_launch_takes(torch, M, N, K):
+    p = Product(torch, M, N, K, bias=True, seed=10)
+    p.run()
+    part = 1 << 24
+    for m in range(0, M, part):
+        for n in range(0, N, part):
+            rows, cols = slice(m, min(m + part, M)), slice(n, min(n + part, N))
+            # (whole numbers below 2^24; one side has one row)
+            y = (p.X[rows].float() * p.W[cols].float()).sum(-1).view(rows.stop - m, cols.stop - n)
+            want = (y * p.xs[rows, None]) * p.ws[cols] + p.bias[cols].float()
+            assert torch.equal(p.Y[rows, cols], want), (m, n)
+    assert (p.Y[M:] == 55).all()

@@ -307,3 +307,54 @@ FAR = [(33, 300, 64), (40, 65, 1040), (300, 40, 64), (300, 300, 1040), (1000, 33
 def test_far_strides_take_streams(plan):
     for ld, kinds in ((FAR_STRIDE, {0}), (1 << 22, {0, 1})):
         assert {g[3] for g in plan([(m, n, k, ld, 256) for m, n, k in FAR])} == kinds
+
+
+LAUNCHES = """
+#include "linear_i8_plan.hpp"
+#include <cstdio>
+int main() {
+    unsigned long long m, n, k, ld;
+    unsigned cus;
+    int stop;
+    while (scanf("%llu %llu %llu %llu %u %d", &m, &n, &k, &ld, &cus, &stop) == 6) {
+        auto f = [&](const vvli::I8Plan& p, uint64_t m0, uint64_t M, uint64_t n0, uint64_t N) {
+            printf("%u,%u,%llu,%llu,%llu,%llu,%llu ", p.kernel, p.splits, (unsigned long long)p.blocks, (unsigned long long)m0,
+                   (unsigned long long)M, (unsigned long long)n0, (unsigned long long)N);
+            return --stop != 0;
+        };
+        printf("%d\\n", (int)vvli::i8_launches(m, n, k, ld, cus, f));
+    }
+}
+"""
+
+# More columns, or rows, than one launch has blocks for.
+HUGE = [(1, (1 << 27) + 21, 16), (1, (1 << 27) + 24, 32), ((1 << 29) + 5, 1, 16)]
+
+
+def test_launches_cover_their_call_once(tmp_path):
+    if not shutil.which("g++"):
+        pytest.skip("no host compiler")
+    (tmp_path / "t.cpp").write_text(LAUNCHES)
+    subprocess.run(["g++", "-std=c++17", "-O1", f"-I{ROOT / 'vvli_amd' / 'csrc'}", "-o", tmp_path / "t", tmp_path / "t.cpp"], check=True)
+    rng = np.random.RandomState(5)
+    most = (1 << 31) - 1
+    calls = HUGE + CUT + LONG + ODD + SPLIT + [(1, most, 16), (most, 1, 16), (40, most, 16), (most, 40, 16)]
+    while len(calls) < 1000:
+        m, n = (int(np.exp(rng.uniform(0, np.log(most)))) for _ in range(2))
+        if m * n < 1 << 42:
+            calls.append((m, n, 16 * int(np.exp(rng.uniform(0, np.log(8191))))))
+
+    def ask(calls, stop):
+        text = "\n".join(f"{m} {n} {k} {max(k, 4 * n)} 256 {stop}" for m, n, k in calls)
+        out = subprocess.run([tmp_path / "t"], input=text, capture_output=True, text=True, check=True).stdout.split("\n")
+        return [([tuple(map(int, x.split(","))) for x in line.split()[:-1]], line.split()[-1] == "1") for line in out if line]
+
+    for (m, n, k), (got, whole) in zip(calls, ask(calls, 0)):
+        assert whole and all(blocks < 1 << 23 for _, _, blocks, *_ in got)
+        assert all(M and N and m0 % 256 == 0 and n0 % 64 == 0 and m0 + M <= m and n0 + N <= n for *_, m0, M, n0, N in got)
+        assert sum(M * N for *_, M, _, N in got) == m * n
+        for i, (*_, m0, M, n0, N) in enumerate(got):
+            assert all(m0 + M <= m1 or m1 + M1 <= m0 or n0 + N <= n1 or n1 + N1 <= n0 for *_, m1, M1, n1, N1 in got[:i])
+        assert len(got) > 1 or (m, n, k) not in HUGE + CUT
+    for got, whole in ask(HUGE + CUT, 1):  # a launch that fails is the last
+        assert len(got) == 1 and not whole

@@ -500,22 +500,18 @@ hipError_t launch_plan(const LinearI8Args& a, const I8Plan& plan, hipStream_t s,
     return e;
 }
 
-hipError_t launch_linear(LinearI8Args a, hipStream_t s) {
-    const I8Plan plan = i8_plan(a.M, a.N, a.K, std::max(std::max(a.ldw, a.ldx), a.ldy * 4), gemm_cus());
-    const bool fits = plan.blocks * 512 < (uint64_t{1} << 32);  // (else more threads than a launch takes: the longer side in halves)
-    const auto kernels = std::make_integer_sequence<uint32_t, kI8KernelCount>{};
-    if (fits && !plan.cut) return launch_plan(a, plan, s, kernels);
-    LinearI8Args b = a;
-    if (!fits && a.M >= a.N) {
-        a.M = (a.M / 2 + 255) / 256 * 256, b.M -= a.M;
-        b.X += a.M * a.ldx, b.x_scales += a.M, b.Y += a.M * a.ldy;
-    } else {
-        a.N = fits ? static_cast<uint32_t>(plan.cut) : (a.N / 2 + 255) / 256 * 256, b.N -= a.N;
-        b.W += a.N * a.ldw, b.w_scales += a.N, b.Y += a.N;
-        if (b.bias) b.bias += a.N;
-    }
-    const hipError_t e = fits ? launch_plan(a, plan, s, kernels) : launch_linear(a, s);
-    return e != hipSuccess ? e : launch_linear(b, s);
+hipError_t launch_linear(const LinearI8Args& a, hipStream_t s) {
+    hipError_t e = hipSuccess;
+    auto launch = [&](const I8Plan& plan, uint64_t m0, uint64_t M, uint64_t n0, uint64_t N) {
+        LinearI8Args b = a;
+        b.M = static_cast<uint32_t>(M), b.N = static_cast<uint32_t>(N);
+        b.W += n0 * a.ldw, b.w_scales += n0, b.X += m0 * a.ldx, b.x_scales += m0, b.Y += m0 * a.ldy + n0;
+        if (b.bias) b.bias += n0;
+        e = launch_plan(b, plan, s, std::make_integer_sequence<uint32_t, kI8KernelCount>{});
+        return e == hipSuccess;
+    };
+    i8_launches(a.M, a.N, a.K, std::max(std::max(a.ldw, a.ldx), a.ldy * 4), gemm_cus(), launch);
+    return e;
 }
 
 bool sizes_ok(uint32_t M, uint32_t N, uint32_t K) {

@@ -139,4 +139,20 @@ inline I8Plan i8_plan(uint64_t M, uint64_t N, uint64_t K, uint64_t ld, uint32_t 
     return best;
 }
 
+constexpr uint64_t kI8MostBlocks = (uint64_t{1} << 32) / 512;  // a launch has fewer than 2^32 threads
+
+// The launches of a call, in order: f(plan, m0, M, n0, N) for the rows m0 .. m0 + M - 1 and columns n0 .. n0 + N - 1 of Y of
+// each, until one returns false. A launch with too many blocks is two of half the longer side.
+template <typename F>
+bool i8_launches(uint64_t M, uint64_t N, uint64_t K, uint64_t ld, uint32_t cus, F& f, uint64_t m0 = 0, uint64_t n0 = 0) {
+    const I8Plan plan = i8_plan(M, N, K, ld, cus);
+    if (plan.blocks < kI8MostBlocks) {
+        if (!plan.cut) return f(plan, m0, M, n0, N);
+        return f(plan, m0, M, n0, plan.cut) && i8_launches(M, N - plan.cut, K, ld, cus, f, m0, n0 + plan.cut);
+    }
+    const uint64_t half = i8_up((M >= N ? M : N) / 2, 256) * 256;
+    if (M >= N) return i8_launches(half, N, K, ld, cus, f, m0, n0) && i8_launches(M - half, N, K, ld, cus, f, m0 + half, n0);
+    return i8_launches(M, half, K, ld, cus, f, m0, n0) && i8_launches(M, N - half, K, ld, cus, f, m0, n0 + half);
+}
+
 }  // namespace vvli

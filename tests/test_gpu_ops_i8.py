@@ -1000,3 +1000,117 @@ def test_linear_i8_more_blocks_than_a_launch_takes(torch, M, N, K):
             want = (y * p.xs[rows, None]) * p.ws[cols] + p.bias[cols].float()
             assert torch.equal(p.Y[rows, cols], want), (m, n)
     assert (p.Y[M:] == 55).all()
+
+
+# ---------------------------------------------------------------------------
+# Calls that share inputs, rows by the million, rows far apart, the least scales
+# ---------------------------------------------------------------------------
+@pytest.mark.parametrize("width", [5, 401, 2050, 18944, 33000])
+@pytest.mark.parametrize("place", ["apart", "sum is both", "y is both"])
+def test_add_norm_of_rows_and_themselves(torch, width, place):
+    ld = up(width, 4)
+    x, w = torch.randn(4, ld, device="cuda", generator=gen(torch, 13)), torch.randn(width, device="cuda", generator=gen(torch, 14))
+    h = (x + x)[:, :width].cpu().numpy()
+    total, y = {"apart": (torch.zeros_like(x), torch.zeros_like(x)), "sum is both": (x, torch.zeros_like(x)), "y is both": (None, x)}[place]
+    out = Codes(torch, 4, width)
+    R.add_norm(ptr(x), ld, ptr(x), ld, 4, width, ptr(w), "f32", EPS, ptr(total), ld, ptr(y), ld, *out.args, stream(torch))
+    v = norm_value(h, w.double().cpu().numpy())
+    check_codes(*out.get(), v)
+    check_y(y[:, :width].double().cpu().numpy(), v)
+    assert total is None or np.array_equal(total[:, :width].cpu().numpy(), h)
+
+
+@pytest.mark.parametrize("width", [5, 401, 2050, 18944, 33000])
+def test_silu_mul_of_rows_and_themselves(torch, width):
+    ld = up(width, 4)
+    x, out = torch.randn(4, ld, device="cuda", generator=gen(torch, 15)), Codes(torch, 4, width)
+    R.silu_mul(ptr(x), ld, ptr(x), ld, 4, width, *out.args, stream(torch))
+    v = x[:, :width].cpu().numpy()
+    check_codes(*out.get(), gate_value(v, v.astype(np.float64)))
+
+
+@pytest.mark.parametrize("n,K", [(1, 64), (20, 640), (300, 1040), (311, 6768)])
+def test_linear_i8_of_rows_and_themselves(torch, n, K):
+    p = Product(torch, n, n, K)
+    p.W, p.ws = p.X, p.xs
+    p.run()
+    p.check()
+
+
+@pytest.mark.parametrize("rows,width", [((1 << 22) + 5, 20), ((1 << 20) + 3, 1028)])
+def test_norm_and_gate_of_more_rows_than_a_launch_has_blocks(torch, rows, width):
+    g = gen(torch, 16)
+    x, d = (torch.empty(rows, width, device="cuda").uniform_(-2, 2, generator=g) for _ in range(2))
+    w = torch.randn(width, device="cuda", generator=g)
+    some = torch.cat([torch.arange(200), torch.randint(0, rows, (200,)), torch.arange(rows - 200, rows)]).cuda()
+    n = lambda t: t.double().cpu().numpy()  # noqa: E731
+
+    def outputs():
+        codes = torch.full((rows + 1, up(width, 16)), 99, dtype=torch.int8, device="cuda")
+        return codes, torch.full((rows + 1,), -5.0, device="cuda")
+
+    def check(codes, scales, v):
+        assert (codes[rows] == 99).all() and scales[rows] == -5 and (codes[:rows, width:] == 0).all()
+        assert (scales[:rows] > 0).all() and (codes[:rows].abs().amax(-1) == 127).all()  # (every row was formed)
+        check_codes(n(codes[some, :width]), n(scales[some]), v)
+
+    codes, scales = outputs()
+    R.silu_mul(ptr(x), width, ptr(d), width, rows, width, ptr(codes), codes.shape[1], ptr(scales), stream(torch))
+    check(codes, scales, gate_value(x[some].cpu().numpy(), n(d[some])))
+    h = x + d
+    codes, scales = outputs()
+    R.add_norm(ptr(x), width, ptr(d), width, rows, width, ptr(w), "f32", EPS, ptr(x), width, ptr(d), width, ptr(codes), codes.shape[1],
+               ptr(scales), stream(torch))
+    v = norm_value(h[some].cpu().numpy(), n(w))
+    check(codes, scales, v)
+    check_y(n(d[some]), v)
+    assert torch.equal(x, h)
+
+
+def test_norm_and_gate_offsets_past_32_bits(torch):
+    """Strides that put the last rows' values and codes behind 2^32 bytes."""
+    ld, rows, width = 1 << 28, 6, 1000
+    g = gen(torch, 17)
+    x, d = (torch.zeros(rows, ld, device="cuda") for _ in range(2))
+    for t in (x, d):
+        t[:, :width] = torch.randn(rows, width, device="cuda", generator=g)
+    w = torch.randn(width, device="cuda", generator=g)
+    codes, scales = torch.zeros(rows, 1 << 30, dtype=torch.int8, device="cuda"), torch.zeros(rows, device="cuda")
+    n = lambda t: t.double().cpu().numpy()  # noqa: E731
+    v = gate_value(x[:, :width].cpu().numpy(), n(d[:, :width]))
+    R.silu_mul(ptr(x), ld, ptr(d), ld, rows, width, ptr(codes), 1 << 30, ptr(scales), stream(torch))
+    check_codes(n(codes[:, :width]), n(scales), v)
+    h = (x[:, :width] + d[:, :width]).cpu().numpy()
+    R.add_norm(ptr(x), ld, ptr(d), ld, rows, width, ptr(w), "f32", EPS, ptr(x), ld, ptr(d), ld, ptr(codes), 1 << 30, ptr(scales), stream(torch))
+    v = norm_value(h, n(w))
+    check_codes(n(codes[:, :width]), n(scales), v)
+    check_y(n(d[:, :width]), v)
+    assert np.array_equal(x[:, :width].cpu().numpy(), h) and not x[:, width:width + 64].any() and not d[:, width:width + 64].any()
+
+
+def test_products_from_two_threads(torch):
+    """Calls at once from two threads of the host, a stream and a workspace each."""
+    import threading
+
+    products = [Product(torch, *SPLIT[i], bias=True, seed=40 + i) for i in (0, 1)] + [Product(torch, *s, seed=43) for s in ((5, 413, 2672), (300, 896, 896))]
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    torch.cuda.synchronize()
+    failed = []
+
+    def work(k):
+        try:
+            for _ in range(10):
+                for p in products[k::2]:
+                    p.run(streams[k].cuda_stream)
+        except Exception as e:
+            failed.append(e)
+
+    threads = [threading.Thread(target=work, args=(k,)) for k in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    torch.cuda.synchronize()
+    assert not failed
+    for p in products:
+        p.check()

@@ -572,11 +572,12 @@ size_t vvli_gpu_verify_drafts_workspace(uint32_t requests, uint32_t vocab);
  *
  * Rows in 8 bits: of a row y of real numbers, scale = f32(max |y| / 127) and
  * code = the integer nearest to y / scale (a tie: the even one), -127 .. 127,
- * so that code * scale is within half a scale of y. Both are those of exact
- * arithmetic wherever 64 bits tell a value from the border between two codes:
- * they depend neither on a call's other rows nor on its sizes. A row of zeros,
- * and one whose scale is below f32's range, has scale 0 and codes 0. A row
- * with a value that is not finite, or whose scale is over f32's range, has
+ * so that code * scale is within half a scale of y (not so where the scale is
+ * a denormal: it has few bits, and values beyond 127 of it have codes of 127
+ * and -127). Both are those of exact arithmetic wherever 64 bits tell a value
+ * from the border between two codes: they depend neither on a call's other
+ * rows nor on its sizes. A row of zeros, and one whose scale is below f32's
+ * range, has scale 0 and codes 0. A row with a value that is not finite, or whose scale is over f32's range, has
  * scale NaN and codes 0: products with it are NaN. Codes of a row start at a
  * multiple of 16 bytes (ldc % 16 == 0), and behind its last code up to the
  * next multiple of 16 stand zeros (ldc holds them too), so that a width that
@@ -588,8 +589,9 @@ size_t vvli_gpu_verify_drafts_workspace(uint32_t requests, uint32_t vocab);
  * elements) of f32 and bf16 start at 16-byte addresses (ld a multiple of 4 or
  * 8). Nothing behind a row's width is read or, but for the codes' zeros,
  * written. Outputs do not overlap inputs or each other, but that a call says
- * so; sizes and overlaps that a call does not take return VVLI_INVALID_CONFIG
- * before any launch. rows 0 is no error: nothing is launched. Results do not
+ * so (rows may lie beside rows of the same stride; those of different strides
+ * overlap where their ranges do, gaps included); sizes and overlaps that a call
+ * does not take return VVLI_INVALID_CONFIG before any launch. rows 0 is no error: nothing is launched. Results do not
  * change from run to run. */
 
 /* Rows x (type kind: VVLI_WEIGHT_F32 or VVLI_WEIGHT_BF16) in 8 bits. */

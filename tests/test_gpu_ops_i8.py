@@ -1088,6 +1088,38 @@ def test_norm_and_gate_offsets_past_32_bits(torch):
     assert np.array_equal(x[:, :width].cpu().numpy(), h) and not x[:, width:width + 64].any() and not d[:, width:width + 64].any()
 
 
+@pytest.mark.parametrize("width", [33, 2000, 33000])
+def test_least_scales(torch, width):
+    """Scales of few bits: the codes of values that 127 of them do not reach are 127 and -127."""
+    rows, ld, least = 12, up(width, 8), 2.0 ** -149
+    rng = np.random.RandomState(width)
+    tops = np.array([63, 64, 127, 190, 191, 254, 300, 1000, 5000, 100000, 1 << 20, 1 << 24])  # (in steps of the denormals)
+    m = rng.randint(-tops[:, None], tops[:, None] + 1, (rows, width)).astype(np.float64)
+    m[:, width // 2] = tops
+    x = torch.zeros(rows, ld, device="cuda")
+    x[:, :width] = torch.from_numpy((m * least).astype(np.float32)).cuda()
+    assert np.array_equal(x[:, :width].double().cpu().numpy(), m * least)
+    out = Codes(torch, rows, width)
+    R.quantize_rows(ptr(x), "f32", ld, rows, width, *out.args, stream(torch))
+    codes, scales = out.get()
+    equal_codes(codes, scales, m * least)
+    assert scales[0] == 0 and scales[3] == least and codes[3, width // 2] == 127 and abs(m[3, width // 2] - 127) > 60
+    half = (x * 2.0 ** 16).bfloat16()  # (whole steps of bf16's denormals, or its 8 bits)
+    out = Codes(torch, rows, width)
+    R.quantize_rows(ptr(half), "bf16", ld, rows, width, *out.args, stream(torch))
+    equal_codes(*out.get(), half[:, :width].double().cpu().numpy())
+    gate = torch.randn(rows, ld, device="cuda", generator=gen(torch, 18))
+    out = Codes(torch, rows, width)
+    R.silu_mul(ptr(gate), ld, ptr(x), ld, rows, width, *out.args, stream(torch))
+    check_codes(*out.get(), gate_value(gate[:, :width].cpu().numpy(), m * least))
+    for t in x[[3, 6, 8]]:
+        y, out = torch.zeros(rows, ld, device="cuda"), Codes(torch, rows, width)
+        R.add_norm(ptr(gate), ld, None, 0, rows, width, ptr(t), "f32", EPS, None, 0, ptr(y), ld, *out.args, stream(torch))
+        v = norm_value(gate[:, :width].cpu().numpy(), t[:width].double().cpu().numpy())
+        check_codes(*out.get(), v)
+        check_y(y[:, :width].double().cpu().numpy(), v)
+
+
 def test_products_from_two_threads(torch):
     """Calls at once from two threads of the host, a stream and a workspace each."""
     import threading

@@ -577,11 +577,12 @@ size_t vvli_gpu_verify_drafts_workspace(uint32_t requests, uint32_t vocab);
  * and -127). Both are those of exact arithmetic wherever 64 bits tell a value
  * from the border between two codes: they depend neither on a call's other
  * rows nor on its sizes. A row of zeros, and one whose scale is below f32's
- * range, has scale 0 and codes 0. A row with a value that is not finite, or whose scale is over f32's range, has
- * scale NaN and codes 0: products with it are NaN. Codes of a row start at a
- * multiple of 16 bytes (ldc % 16 == 0), and behind its last code up to the
- * next multiple of 16 stand zeros (ldc holds them too), so that a width that
- * is no multiple of 16 multiplies as K = the next one.
+ * range, has scale 0 and codes 0. A row with a value that is not finite, or
+ * whose scale is over f32's range, has scale NaN and codes 0: products with it
+ * are NaN. Codes of a row start at a multiple of 16 bytes (ldc % 16 == 0), and
+ * behind its last code up to the next multiple of 16 stand zeros (ldc holds
+ * them too), so that a width that is no multiple of 16 multiplies as K = the
+ * next one.
  *
  * As above, every pointer is device memory, aligned to its elements, of the
  * current device, to which `stream` belongs; the calls are asynchronous,
@@ -591,8 +592,8 @@ size_t vvli_gpu_verify_drafts_workspace(uint32_t requests, uint32_t vocab);
  * written. Outputs do not overlap inputs or each other, but that a call says
  * so (rows may lie beside rows of the same stride; those of different strides
  * overlap where their ranges do, gaps included); sizes and overlaps that a call
- * does not take return VVLI_INVALID_CONFIG before any launch. rows 0 is no error: nothing is launched. Results do not
- * change from run to run. */
+ * does not take return VVLI_INVALID_CONFIG before any launch. rows 0 is no
+ * error: nothing is launched. Results do not change from run to run. */
 
 /* Rows x (type kind: VVLI_WEIGHT_F32 or VVLI_WEIGHT_BF16) in 8 bits. */
 int vvli_gpu_quantize_rows(const void* x, uint32_t kind, uint64_t ldx, uint32_t rows, uint32_t width, int8_t* codes,

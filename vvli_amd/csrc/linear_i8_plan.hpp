@@ -16,13 +16,14 @@ enum I8Kind { kI8Stream, kI8Tile };
 //
 // The numbers are fits (nonnegative, of relative errors, sizes where the kernel is
 // near the fastest weighing most) to 365 sizes, M = 1 to 4096 with (N, K) of nine
-// projections, W in no cache. On the geometric mean, choosing by them costs 0.3 %
-// over the fastest kernel here and 1.2 % over that of 126 measured variants; 15 %
-// where it costs most (448 x 3584 x 18944: 58 us, in parts by 128 x 128 tiles of
-// four stages 51). Sides of 192 fill the CUs where those of 128 and 256 leave a
-// third of them idle (us without and with them: 2048 x 4608 x 3584 49 and 41, 1536 x
-// 16384 x 2048 72 and 65, 896 x 9728 x 896 20.9 and 18.5, 131 x 37888 x 3584 48 and
-// 43).
+// projections, W in no cache, before results of more than 128 MiB passed the caches
+// (4096 x 9728 x 896: 64.8 by the fit, 55 measured). On the geometric mean, choosing
+// by them cost 0.3 % over the fastest kernel here and 1.2 % over that of 126
+// measured variants then; 15 % where it cost most (448 x 3584 x 18944: 58 us, in
+// parts by 128 x 128 tiles of four stages 51). Sides of 192 fill the CUs where those
+// of 128 and 256 leave a third of them idle (us without and with them: 2048 x 4608 x
+// 3584 49 and 41, 1536 x 16384 x 2048 72 and 65, 896 x 9728 x 896 20.9 and 18.5, 131
+// x 37888 x 3584 48 and 43).
 struct I8Kernel {
     I8Kind kind;
     uint8_t r, m, stages, waves;  // stream: tiles of 16 rows of W, groups of 8 of X; tile: 64s of rows of either
@@ -124,7 +125,7 @@ inline I8Plan i8_one(uint64_t M, uint64_t N, uint64_t K, uint64_t ld, uint32_t c
 
 // Where 256 x 256 tiles leave a last round that few CUs have a tile of, the whole rounds are a launch of their own and the
 // other columns one of smaller tiles (us, all in one launch and so, 256 CUs: 4096 x 4608 x 3584 83 -> 73, 1024 x 37888 x
-// 3584 158 -> 145, 4096 x 37888 x 3584 550 -> 532, 4096 x 6144 x 2048 64.7 -> 62.4). The fits' `base` stands for what the
+// 3584 158 -> 145, 4096 x 37888 x 3584 529 -> 516, 4096 x 6144 x 2048 64.7 -> 62.4). The fits' `base` stands for what the
 // second launch costs.
 inline I8Plan i8_plan(uint64_t M, uint64_t N, uint64_t K, uint64_t ld, uint32_t cus) {
     double least = 0;

@@ -17,10 +17,11 @@
 //     in 8; of bf16, whose few bits make ties, nine of ten waves do. Read and
 //     formed one after the other, weights took 59 us, gate 10 more).
 // Where f32's error is not the usual one (values that left its normal range) a
-// row is formed in f64 as a whole. Measured (inputs that no cache holds; a copy
-// of 1 GB moves 5.06 TB/s): weights 18944 x 3584 bf16 41.6 us (4.9 TB/s), f32 rows
-// 6001 x 3584 19.4 (5.5), their norm with the sum 55.2 (5.1), gate 2500 x 18944 80.1
-// (5.3).
+// row is formed in f64 as a whole. Measured (calls that follow one another over
+// inputs that no cache holds; a copy of 1 GB moves 5.06 TB/s): weights 18944 x 3584
+// bf16 41.6 us (4.9 TB/s), f32 rows 6001 x 3584 19.4 (5.5), their norm with the sum
+// 55.2 (5.1), gate 2500 x 18944 80.1 (5.3). Behind a fill of 300 MB, whose lines the
+// caches have yet to write: weights 55.7, norm 56.0, gate 101.8.
 // One row of 2048: 4.2, 4.5 and 4.4 us, of which 3.8 is a launch.
 #include <algorithm>
 #include <type_traits>

@@ -10,7 +10,7 @@
 // moves 5.4 TB/s, a library product of 8192 cubed 2466 TOP/s): 1 x 37888 x 3584 22.0
 // (6.2 TB/s), 5 x 2048 x 8192 6.2, 48 x 4608 x 3584 8.4, 128 x 37888 x 3584 37 (4.2
 // TB/s), 333 x 896 x 4864 9.7 to 10.1, 2048 x 4608 x 3584 41 (1640 TOP/s), 4096 x 3584 x
-// 18944 230 to 238 (2340 to 2420), 4096 x 37888 x 3584 507 (2190).
+// 18944 230 to 238 (2340 to 2420), 4096 x 37888 x 3584 507 to 522 (2130 to 2190).
 #include <algorithm>
 #include <atomic>
 #include <type_traits>
